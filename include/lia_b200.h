@@ -642,6 +642,52 @@ int lia_rglru_scan(const float* u, const float* z, const float* z_bias, const fl
 int lia_router_topk_grouped(const float* logits, int ldl, const float* correction, int renorm, int sigmoid, int groups, int keep, int* idx,
                             float* wt, int M, int E, int top, lia_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Serving with drafted tokens: caches of 8 bits, attention of several new tokens behind a history, log probabilities.
+ * (Not in the reference, which caches bf16 and decodes one token per sequence.)
+ * ---------------------------------------------------------------------------------------------------------------- */
+enum { LIA_CACHE_BF16 = 0, LIA_CACHE_INT8 = 1, LIA_CACHE_E4M3 = 2 };
+
+/* One side (keys or values) of a cache of heads of `dim` channels: the number of (slot, position, head, channel) lies at
+ * data[slot * slot_stride + position * pos_stride + head * head_stride + channel], strides in numbers; with 8 bits the numbers of a
+ * (slot, position, head) stand for themselves times scale[slot * scale_slot_stride + head * scale_head_stride + position].  data and all its
+ * strides: whole 16-byte vectors (8 bytes for lia_kv_store_8bit and lia_kv_load_8bit). */
+typedef struct LiaCacheView {
+  void* data;
+  float* scale;                  /* NULL with bf16 */
+  int64_t slot_stride, pos_stride, head_stride, scale_slot_stride, scale_head_stride;
+  int32_t slots, capacity, type, dim;
+} LiaCacheView;
+
+/* Rows' keys k [M, G * dim] and values v [M, G * vdim] (bf16 or fp32, ldk and ldv apart) into 8-bit caches at meta[row] = (slot, position); a row whose slot or position
+ * the caches do not have is left out.  int8: scale = a / 127, code = rint(127 x / a) with a the largest magnitude of the head's numbers (counted as 2^-100 at least);
+ * e4m3: scale = the least power of two with a / scale <= 448, code = x / scale rounded to nearest even
+ * (what would read back as 2^128: to the code below).  A head with an infinity or NaN gets scale NaN and codes 0.
+ * norm_values: values are first divided by sqrt(mean of their head's squares + eps).  Two rows of one call must not share a place. */
+int lia_kv_store_8bit(const void* k, long long ldk, const void* v, long long ldv, int act_f32, const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, int M, int G,
+                      float eps, int norm_values, lia_stream_t stream);
+/* The reverse: code * scale of the rows at meta into k [M, G * dim] and v [M, G * vdim]; NaN for a row whose slot or position the caches do not have */
+int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, void* k, long long ldk, void* v, long long ldv, int out_f32, int M, int G,
+                     lia_stream_t stream);
+
+/* Attention of portions of new tokens behind their histories.  segs[i] = (slot, p0, row, n): the n tokens of rows row .. row + n - 1 have their keys and values at positions
+ * p0 .. p0 + n - 1 of the slot, behind p0 cached positions.  Row i of a portion sees the history -- with window > 0 its positions above p0 + depth_i - window -- and of the n new
+ * tokens: without mask those up to its own (under the same window), else those whose bits are set in its `words` 64-bit words of mask (bit j: the portion's token j).  depth_i:
+ * depth[row + i], or i where depth is NULL.  A score is temp[h] * scale * (q . k), then softcap * tanh(score / softcap) if softcap > 0; query head h reads key/value head
+ * h / (H / G).  A row that sees nothing is 0; what it does not see has no effect, whatever its bits.  Rows of no portion stay as they are; a portion that its slot, the M rows, the mask's
+ * words or `rows` cannot hold gives NaN rows.  rows: the most rows of a portion; max_ctx: about the longest p0 + n (it decides how many blocks share a history, no more).
+ * q and out: bf16, ldq apart and [M, H * vdim].  Heads of 64 or 128 channels.  ws: lia_tree_attn_workspace_floats() floats (0: NULL will do). */
+size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx, int M, int H, int G, int dim, int vdim, int window, int type);
+int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
+                  const float* temp, void* out, float* ws, size_t ws_floats, int M, int H, int G, int rows, int max_ctx, int window, float scale, float softcap, lia_stream_t stream);
+
+/* Of every row of logits [M, V] (bf16 or fp32, ld apart): logp[n] of the n given tokens (an id outside [0, V) has NaN), the entropy of the distribution in nats, and the `top` <= 32
+ * largest logits' ids (int64; of equal ones the lowest first, NaN counts as -inf) and log probabilities.  Rows that hold NaN or +inf, or -inf alone, have NaN for all but the ids.
+ * ws: lia_token_logprobs_workspace_floats() floats (0: NULL will do). */
+size_t lia_token_logprobs_workspace_floats(int M, int V, int act_f32);
+int lia_token_logprobs(const void* logits, int act_f32, long long ld, int M, int V, const int64_t* tokens, int n, float* logp, float* entropy, int top, float* top_logp, int64_t* top_ids,
+                       float* ws, size_t ws_floats, lia_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(_HERE, "libliab200.so")
 
 EPI_BIAS, EPI_BIAS_RELU, EPI_BIAS_RESIDUAL, EPI_QKV = 0, 1, 2, 3
 ABI_VERSION = 11
+CACHE_BF16, CACHE_INT8, CACHE_E4M3 = 0, 1, 2
 TP_MAX_WORLD = 8
 P2P_HANDLE_BYTES = 64
 
@@ -27,6 +28,11 @@ class LiaTpArgs(ctypes.Structure):
     _fields_ = [("rank", c_int32), ("world", c_int32), ("arena", c_void_p * TP_MAX_WORLD),
                 ("ctl_off", ctypes.c_uint64), ("recv_off", ctypes.c_uint64), ("recv_bytes", ctypes.c_uint64),
                 ("out_off", ctypes.c_uint64), ("mc_arena", c_void_p)]
+
+
+class LiaCacheView(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("scale", c_void_p), ("slot_stride", c_int64), ("pos_stride", c_int64), ("head_stride", c_int64),
+                ("scale_slot_stride", c_int64), ("scale_head_stride", c_int64), ("slots", c_int32), ("capacity", c_int32), ("type", c_int32), ("dim", c_int32)]
 
 
 class LiaError(RuntimeError):
@@ -228,6 +234,15 @@ _PROTOTYPES = {
     "lia_rglru_scan": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                c_void_p, c_void_p]),
     "lia_router_topk_grouped": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    # serving with drafted tokens: caches of 8 bits, attention of several new tokens behind a history, log probabilities
+    "lia_kv_store_8bit": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_int, c_int, c_float, c_int,
+                                  c_void_p]),
+    "lia_kv_load_8bit": (c_int, [c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p]),
+    "lia_tree_attn_workspace_floats": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "lia_tree_attn": (c_int, [c_void_p, c_longlong, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                              c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p]),
+    "lia_token_logprobs_workspace_floats": (c_size_t, [c_int, c_int, c_int]),
+    "lia_token_logprobs": (c_int, [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 EXPORTS = tuple(_PROTOTYPES)

@@ -1,0 +1,467 @@
+// Attention of portions of new tokens -- a decoded token, a chain or a tree of drafted ones, a part of a prompt -- behind their cached histories, over caches of bf16, int8 or e4m3.
+//
+//   s_ij = cap tanh(temp_h scale ks_j (q_i . k_j) / cap),   o_i = sum_j p_ij vs_j v_j / sum_j p_ij,   p_ij = e^(s_ij - max) over the j that row i sees
+//
+// Few rows see a long history: what counts is that the history is read once, whatever the number of rows and of query heads that share a key head.  So a block has up to 32 of the
+// portion's (token, head) rows of one key head, its four warps take 16 keys each in turn, and the history is split over as many blocks as fill the GPU.  Keys and values go
+// from memory to the lanes that multiply them, without shared memory between: a product sums over channels in any order, so a lane's 16 neighbouring bytes of a key
+// are four steps' operands, and a product's columns may be any channels, so the 16 neighbouring bytes of four values are its operands for 16 (bf16: 8) products.
+//
+// 8-bit codes are exact in fp16 and so are multiplied there: q goes to fp16 by a power of two of its own for each row (its 8 bits fit; what is 2^-29 of the row's largest is
+// less exact), a key's scale is multiplied into its scores, and a value's into its weight -- in the exponent, s + log2 vs, so that the running maximum bounds the product and no scale is
+// too large or small: weights are 2^(s + log2 vs - max + 14) in fp16, 11 bits, and their sum takes p = weight / vs in fp32.  With bf16 caches weights are two bf16 parts: 16 bits.
+#include <cuda_fp16.h>
+
+#include "mma.cuh"
+#include "tree_attn.cuh"
+
+namespace {
+
+constexpr int WARPS = 4, THREADS = WARPS * 32, MAX_SPLITS = 64;
+
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// two codes as fp16: e4m3 in the low 16 bits
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t u) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)u, __NV_E4M3);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t int8x2(uint32_t u) {           // bytes 0x64, code + 128 of two numbers: 1024 + 128 + code
+  const uint32_t off = 0x64806480u;                                // 1152
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int DIM, int VDIM, int KIND, int RT>
+struct Shape {
+  static constexpr bool BITS8 = KIND != LIA_CACHE_BF16;
+  static constexpr int STEPS = DIM / 16;                           // products of a block of 16 keys with q
+  static constexpr int NT = VDIM / 8;                              // products' columns of 8 channels
+  static constexpr int KV = DIM * (BITS8 ? 1 : 2) / 64;            // 16-byte vectors of a key in a lane
+  static constexpr int VB = VDIM * (BITS8 ? 1 : 2) / 8;            // bytes of a value in a lane
+  static constexpr int ROWS = 16 * RT;
+  static constexpr int Q_BYTES = RT * STEPS * 32 * 16, O_BYTES = WARPS * ROWS * VDIM * 4, SMEM = (Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES) + 3 * WARPS * ROWS * 4;
+  // the channel of column `col` of the nt-th product with the values
+  static __device__ __forceinline__ int channel(int nt, int col) { return BITS8 ? col * (VDIM / 8) + nt : (nt >> 3) * 64 + col * 8 + (nt & 7); }
+};
+
+template <int DIM, int VDIM, int KIND, int RT>
+__global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(const TreeArgs a) {
+  using S = Shape<DIM, VDIM, KIND, RT>;
+  constexpr bool BITS8 = S::BITS8;
+  extern __shared__ uint4 smem[];
+  float* row_f = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + (S::Q_BYTES > S::O_BYTES ? S::Q_BYTES : S::O_BYTES));   // [ROWS] what a row's products with keys are multiplied by
+  float2* part = reinterpret_cast<float2*>(row_f + S::ROWS);       // [WARPS][ROWS] maximum, sum
+  pdl_launch_dependents();
+  pdl_wait();
+  const Portion p = portion_of(a, blockIdx.z);
+  if (!p.held) {
+    if (a.splits == 1 && blockIdx.y == 0) nan_rows<VDIM>(a, p);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t4 = lane & 3;
+  const int tile = blockIdx.y / a.G, g = blockIdx.y - tile * a.G, r0 = tile * S::ROWS, R = p.n * a.rep;
+  if (r0 >= R) return;
+
+  // ---- queries: rows (token, head) in the order of the products' operands
+  for (int r = warp; r < S::ROWS; r += WARPS) {
+    const bool there = r0 + r < R;
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    uint2 u = make_uint2(0u, 0u);
+    if (there && lane < DIM / 4) {
+      const bf16* src = a.q + (p.row + i) * a.ldq + h * DIM + lane * 4;
+      u = *reinterpret_cast<const uint2*>(src);
+    }
+    float f = a.scale * (a.temp != nullptr && there ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
+    uint2 w = u;
+    if constexpr (BITS8) {
+      uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int e = min(max((int)(top >> 7), 27), 253);            // the largest's exponent; its row becomes 2^14 and less
+      const float down = __uint_as_float((uint32_t)(254 + 14 - max(e, 15)) << 23);
+      float x[4];
+      unpack_bf16x2(u.x, x[0], x[1]);
+      unpack_bf16x2(u.y, x[2], x[3]);
+      w = make_uint2(pack_f16x2(x[0] * down, x[1] * down), pack_f16x2(x[2] * down, x[3] * down));
+      f /= down;
+    }
+    if (lane < DIM / 4) {
+      const int c = lane * 4, t = BITS8 ? (c >> 4) & 3 : (c >> 3) & 3, step = BITS8 ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
+      uint32_t* dst = reinterpret_cast<uint32_t*>(smem + ((r >> 4) * S::STEPS + step) * 32 + (r & 7) * 4 + t) + ((r >> 3) & 1);
+      dst[0] = w.x;
+      dst[2] = w.y;
+    }
+    if (lane == 0) row_f[r] = f;
+  }
+  __syncthreads();
+  uint32_t qa[RT == 1 ? S::STEPS : 1][4];                          // 16 rows' queries stay in registers, those of 32 in shared memory
+  if constexpr (RT == 1) {
+#pragma unroll
+    for (int s = 0; s < S::STEPS; ++s) *reinterpret_cast<uint4*>(qa[s]) = smem[s * 32 + lane];
+  }
+
+  // ---- which keys
+  const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + S::ROWS - 1) / a.rep);
+  int near = i0, far = i1;                                         // depths of the block's tokens
+  if (a.depth != nullptr) {
+    near = 1 << 29;
+    far = 0;
+    for (int i = i0 + lane; i <= i1; i += 32) {
+      const int d = depth_of(a, p, i);
+      near = min(near, d);
+      far = max(far, d);
+    }
+    near = __reduce_min_sync(0xffffffffu, near);
+    far = __reduce_max_sync(0xffffffffu, far);
+  }
+  const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = a.mask != nullptr ? p.p0 : p.p0 + i0 + 1;
+  const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
+
+  int ri[RT][2], rd[RT][2];                                        // of the lane's rows gq and gq + 8: token and depth
+  float rf[RT][2], m[RT][2], l[RT][2];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = rt * 16 + e * 8 + gq;
+      ri[rt][e] = min((r0 + r) / a.rep, p.n - 1);
+      rd[rt][e] = depth_of(a, p, ri[rt][e]);
+      rf[rt][e] = row_f[r];
+      m[rt][e] = -INFINITY;
+      l[rt][e] = 0.f;
+    }
+  float o[RT][S::NT][4];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int n = 0; n < S::NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[rt][n][e] = 0.f;
+
+  const uint8_t *kbase = a.k.at(p.slot, 0, g) + t4 * 16, *vbase = a.v.at(p.slot, 0, g) + gq * (BITS8 ? S::VB : 16);
+  const float *ksc = BITS8 ? a.k.scale_at(p.slot, g) : nullptr, *vsc = BITS8 ? a.v.scale_at(p.slot, g) : nullptr;
+  uint4 kr[2][S::KV];
+  uint32_t vr[4][S::VB / 4];
+  float ks[4], vs[4];
+  auto key_of = [&](int b, int c) { return min(lo + b * 16 + ((c >> 1) * 8 + t4 * 2 + (c & 1)), hi - 1); };   // of the lane's columns of scores
+  auto load_k = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint8_t* src = kbase + (long long)min(lo + b * 16 + j * 8 + gq, hi - 1) * a.k.pos;
+#pragma unroll
+      for (int c = 0; c < S::KV; ++c) kr[j][c] = ldg_act(src + c * 64);
+    }
+    if constexpr (BITS8) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        ks[c] = __ldcg(ksc + key_of(b, c));
+        vs[c] = __ldcg(vsc + key_of(b, c));
+      }
+    }
+  };
+  auto load_v = [&](int b) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint8_t* src = vbase + (long long)key_of(b, c) * a.v.pos;
+      if constexpr (S::VB == 8) {
+        const uint2 u = __ldcg(reinterpret_cast<const uint2*>(src));
+        vr[c][0] = u.x;
+        vr[c][1] = u.y;
+      } else {
+#pragma unroll
+        for (int w = 0; w < S::VB / 16; ++w) *reinterpret_cast<uint4*>(&vr[c][w * 4]) = ldg_act(src + w * 128);
+      }
+    }
+  };
+
+  if (b0 + warp < b1) {
+    load_k(b0 + warp);
+    load_v(b0 + warp);
+  }
+  const float two_by_cap = a.softcap > 0.f ? 2.f * LOG2E / a.softcap : 0.f;
+  for (int b = b0 + warp; b < b1; b += WARPS) {
+    // ---- scores of 16 keys
+    float s[RT][2][4];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[rt][j][e] = 0.f;
+#pragma unroll
+    for (int st = 0; st < S::STEPS; ++st) {
+      uint32_t kb[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (BITS8) {
+          const uint4& u = kr[j][st >> 2];
+          uint32_t w = (st & 3) == 0 ? u.x : (st & 3) == 1 ? u.y : (st & 3) == 2 ? u.z : u.w;
+          if constexpr (KIND == LIA_CACHE_INT8) {
+            w ^= 0x80808080u;
+            kb[j][0] = int8x2(__byte_perm(w, 0x64646464u, 0x4140));
+            kb[j][1] = int8x2(__byte_perm(w, 0x64646464u, 0x4342));
+          } else {
+            kb[j][0] = e4m3x2(w & 0xffffu);
+            kb[j][1] = e4m3x2(w >> 16);
+          }
+        } else {
+          const uint4& u = kr[j][st >> 1];
+          kb[j][0] = st & 1 ? u.z : u.x;
+          kb[j][1] = st & 1 ? u.w : u.y;
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        uint32_t qf[4];
+        if constexpr (RT == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[e] = qa[st][e];
+        } else {
+          *reinterpret_cast<uint4*>(qf) = smem[(rt * S::STEPS + st) * 32 + lane];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if constexpr (BITS8) mma_f16(s[rt][j], qf, kb[j][0], kb[j][1]);
+          else mma_bf16(s[rt][j], qf, kb[j][0], kb[j][1]);
+        }
+      }
+    }
+    float kf[4], lv[4], rv[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      kf[c] = BITS8 ? ks[c] : 1.f;
+      if constexpr (BITS8) vs[c] = max_nan(vs[c], 0x1p-120f);      // (a scale of 0 weighs nothing, and its score still counts)
+      lv[c] = BITS8 ? lg2(vs[c]) : 0.f;
+      rv[c] = BITS8 ? __fdividef(1.f, vs[c]) : 1.f;
+    }
+    if (b + WARPS < b1) load_k(b + WARPS);
+    // ---- weights
+    const int key0 = lo + b * 16;
+    const bool every = key0 >= all_lo && key0 + 16 <= min(all_hi, hi);
+    uint32_t pa[RT][BITS8 ? 1 : 2][4];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float& x = s[rt][c >> 1][e * 2 + (c & 1)];
+          x *= rf[rt][e];
+          if constexpr (BITS8) x *= kf[c];
+          if (a.softcap > 0.f) x = capped(x, a.softcap, two_by_cap) * LOG2E;
+          if constexpr (BITS8) x += lv[c];
+          if (!every) {
+            const int t = key0 + (c >> 1) * 8 + t4 * 2 + (c & 1);
+            if (t >= hi || !sees(a, p, ri[rt][e], rd[rt][e], t)) x = -INFINITY;
+          }
+          top = fmaxf(top, x);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m[rt][e], top), base = mn == -INFINITY ? 0.f : mn, keep = ex2(m[rt][e] - base);
+        m[rt][e] = mn;
+        l[rt][e] *= keep;
+        if (__any_sync(0xffffffffu, keep != 1.f)) {
+#pragma unroll
+          for (int n = 0; n < S::NT; ++n) {
+            o[rt][n][e * 2] *= keep;
+            o[rt][n][e * 2 + 1] *= keep;
+          }
+        }
+        float w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x = s[rt][c >> 1][e * 2 + (c & 1)];
+          w[c] = ex2(x - base + (BITS8 ? 14.f : 0.f));
+          l[rt][e] = BITS8 ? (x == -INFINITY ? l[rt][e] : fmaf(w[c], rv[c], l[rt][e])) : l[rt][e] + w[c];
+        }
+        if constexpr (BITS8) {
+          pa[rt][0][e] = pack_f16x2(w[0], w[1]);
+          pa[rt][0][2 + e] = pack_f16x2(w[2], w[3]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t top2 = pack_bf16x2(w[2 * c], w[2 * c + 1]);
+            float x, y;
+            unpack_bf16x2(top2, x, y);
+            pa[rt][0][c * 2 + e] = top2;
+            pa[rt][BITS8 ? 0 : 1][c * 2 + e] = pack_bf16x2(w[2 * c] - x, w[2 * c + 1] - y);
+          }
+        }
+      }
+    }
+    // ---- weighted values
+#pragma unroll
+    for (int w = 0; w < S::VB / 4; ++w) {
+      constexpr int PER = BITS8 ? 4 : 2;                           // channels of a word
+      uint32_t vb[PER][2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t u0 = vr[2 * c][w], u1 = vr[2 * c + 1][w];
+        if constexpr (BITS8) {
+          uint32_t x = __byte_perm(u0, u1, 0x5140), y = __byte_perm(u0, u1, 0x7362);
+          if constexpr (KIND == LIA_CACHE_INT8) {
+            x ^= 0x80808080u;
+            y ^= 0x80808080u;
+            vb[0][c] = int8x2(__byte_perm(x, 0x64646464u, 0x4140));
+            vb[1][c] = int8x2(__byte_perm(x, 0x64646464u, 0x4342));
+            vb[2][c] = int8x2(__byte_perm(y, 0x64646464u, 0x4140));
+            vb[3][c] = int8x2(__byte_perm(y, 0x64646464u, 0x4342));
+          } else {
+            vb[0][c] = e4m3x2(x & 0xffffu);
+            vb[1][c] = e4m3x2(x >> 16);
+            vb[2][c] = e4m3x2(y & 0xffffu);
+            vb[3][c] = e4m3x2(y >> 16);
+          }
+        } else {
+          vb[0][c] = __byte_perm(u0, u1, 0x5410);
+          vb[1][c] = __byte_perm(u0, u1, 0x7632);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < PER; ++c)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          if constexpr (BITS8) {
+            mma_f16(o[rt][w * 4 + c], pa[rt][0], vb[c][0], vb[c][1]);
+          } else {
+            mma_bf16(o[rt][w * 2 + c], pa[rt][0], vb[c][0], vb[c][1]);
+            mma_bf16(o[rt][w * 2 + c], pa[rt][BITS8 ? 0 : 1], vb[c][0], vb[c][1]);
+          }
+        }
+    }
+    if (b + WARPS < b1) load_v(b + WARPS);
+  }
+
+  // ---- the warps' parts meet in shared memory
+  __syncthreads();                                                 // (queries have been read)
+  float* os = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[rt][e];
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      const int r = warp * S::ROWS + rt * 16 + e * 8 + gq;
+      if (t4 == 0) part[r] = make_float2(m[rt][e], x);
+#pragma unroll
+      for (int n = 0; n < S::NT; n += 4)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<float4*>(os + r * VDIM + S::channel(n, t4 * 2 + c)) =
+              make_float4(o[rt][n][e * 2 + c], o[rt][n + 1][e * 2 + c], o[rt][n + 2][e * 2 + c], o[rt][n + 3][e * 2 + c]);
+    }
+  __syncthreads();
+  constexpr int N = VDIM / 32;
+  const long long rows = (long long)a.M * a.H;
+  for (int r = warp; r < S::ROWS && r0 + r < R; r += WARPS) {
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    float top = -INFINITY, sum = 0.f, y[N] = {};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w * S::ROWS + r].x);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 x = part[w * S::ROWS + r];
+      const float f = ex2(x.x - base);
+      sum = fmaf(x.y, f, sum);
+#pragma unroll
+      for (int c = 0; c < N; ++c) y[c] = fmaf(os[(w * S::ROWS + r) * VDIM + lane * N + c], f, y[c]);
+    }
+    if (a.splits == 1) {
+      put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
+    } else {
+      const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;
+#pragma unroll
+      for (int c = 0; c < N; ++c) a.ws[at * VDIM + lane * N + c] = y[c];
+      if (lane == 0) reinterpret_cast<float2*>(a.ws + a.splits * rows * VDIM)[at] = make_float2(top, sum);
+    }
+  }
+}
+
+// How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history
+struct Plan {
+  int rt, tiles, splits;
+};
+Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window) {
+  const long long R = (long long)rows * (H / G);
+  Plan p;
+  p.rt = R <= 16 ? 1 : 2;
+  p.tiles = (int)((R + 16 * p.rt - 1) / (16 * p.rt));
+  const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.rt == 1 ? 3 : 2);
+  const long long span = window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx;
+  long long s = room / blocks, most = (span + 255) / 256;          // (16 blocks of keys a block of threads at least)
+  if (s > most) s = most;
+  if (s > MAX_SPLITS) s = MAX_SPLITS;
+  p.splits = s < 1 ? 1 : (int)s;
+  return p;
+}
+size_t floats_of(const Plan& p, int M, int H, int vdim) { return p.splits > 1 ? (size_t)p.splits * M * H * (vdim + 2) : 0; }
+
+template <int DIM, int VDIM, int KIND, int RT> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
+  using S = Shape<DIM, VDIM, KIND, RT>;
+  static bool configured[64] = {};                                 // per device
+  int dev = 0;
+  LIA_CUDA(cudaGetDevice(&dev));
+  if (S::SMEM > 48 * 1024 && (dev >= 64 || !configured[dev])) {
+    LIA_CUDA(cudaFuncSetAttribute(tree_attn_kernel<DIM, VDIM, KIND, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    if (dev < 64) configured[dev] = true;
+  }
+  LIA_CUDA(lia_launch(tree_attn_kernel<DIM, VDIM, KIND, RT>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), S::SMEM, stream, a));
+  if (a.splits > 1) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
+  return LIA_OK;
+}
+template <int DIM, int VDIM, int KIND> int launch_rt(const TreeArgs& a, int rt, int nseg, cudaStream_t stream) {
+  return rt == 1 ? launch<DIM, VDIM, KIND, 1>(a, nseg, stream) : launch<DIM, VDIM, KIND, 2>(a, nseg, stream);
+}
+template <int KIND> int launch_dims(const TreeArgs& a, int rt, int nseg, cudaStream_t stream) {
+  if (a.k.dim == 128) return a.v.dim == 128 ? launch_rt<128, 128, KIND>(a, rt, nseg, stream) : launch_rt<128, 64, KIND>(a, rt, nseg, stream);
+  return a.v.dim == 128 ? launch_rt<64, 128, KIND>(a, rt, nseg, stream) : launch_rt<64, 64, KIND>(a, rt, nseg, stream);
+}
+
+}  // namespace
+
+extern "C" size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx, int M, int H, int G, int dim, int vdim, int window, int type) {
+  (void)dim; (void)type;
+  if (nseg <= 0 || rows <= 0 || M <= 0 || G <= 0 || H <= 0 || H % G || vdim <= 0) return 0;
+  return floats_of(plan_of(nseg, rows, max_ctx, H, G, window), M, H, vdim);
+}
+
+extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
+                             const float* temp, void* out, float* ws, size_t ws_floats, int M, int H, int G, int rows, int max_ctx, int window, float scale, float softcap, lia_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const char* wrong;
+  LIA_CHECK_ARG(!(wrong = cache8_wrong(kc, 16)) && !(wrong = cache8_wrong(vc, 16)), "lia_tree_attn: %s", wrong);
+  LIA_CHECK_ARG((kc->dim == 64 || kc->dim == 128) && (vc->dim == 64 || vc->dim == 128), "lia_tree_attn: heads have 64 or 128 channels, not %d and %d", kc->dim, vc->dim);
+  LIA_CHECK_ARG(kc->type == vc->type && kc->slots == vc->slots && kc->capacity == vc->capacity, "lia_tree_attn: caches of different types or sizes");
+  LIA_CHECK_ARG(M >= 0 && nseg >= 0 && rows >= 0 && max_ctx >= 0 && G > 0 && H > 0 && H % G == 0, "lia_tree_attn: bad sizes");
+  if (M == 0 || nseg == 0 || rows == 0) return LIA_OK;
+  LIA_CHECK_ARG(q && segs && out && (mask == nullptr || words > 0), "lia_tree_attn: null pointer");
+  LIA_CHECK_ARG(ldq >= (long long)H * kc->dim && ldq % 4 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0, "lia_tree_attn: queries and outputs have to be whole 8-byte vectors");
+  LIA_CHECK_ARG(mask == nullptr || rows <= 64 * words, "lia_tree_attn: %d words of mask do not hold %d tokens", words, rows);
+  const Plan plan = plan_of(nseg, rows, max_ctx, H, G, window);
+  LIA_CHECK_ARG(nseg <= 65535 && (long long)plan.tiles * G <= 65535, "lia_tree_attn: too many portions, or rows of one");
+  LIA_CHECK_ARG(plan.splits == 1 || (ws && ws_floats >= floats_of(plan, M, H, vc->dim) && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_tree_attn: needs a workspace of %zu floats",
+                floats_of(plan, M, H, vc->dim));
+  const TreeArgs a{reinterpret_cast<const bf16*>(q), ldq, cache8(kc), cache8(vc), segs, reinterpret_cast<const unsigned long long*>(mask), words, depth, temp,
+                   reinterpret_cast<bf16*>(out), ws, M, H, G, H / G, rows, window > 0 ? window : 1 << 30, plan.splits, plan.tiles, scale, softcap};
+  switch (kc->type) {
+    case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, plan.rt, nseg, stream);
+    case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, plan.rt, nseg, stream);
+    default: return launch_dims<LIA_CACHE_E4M3>(a, plan.rt, nseg, stream);
+  }
+}

@@ -38,6 +38,15 @@ class SlotState:
         self.rows.append(t)
         return t
 
+    def add_rows_8bit(self, heads, dim, dtype):
+        """A row cache of ``heads`` heads in int8 or float8_e4m3fn for ``ops.kv_store_8bit``: (codes [n_slots, capacity, heads * dim], scales [n_slots, heads, capacity])."""
+        if dtype not in (torch.int8, torch.float8_e4m3fn):
+            raise ValueError(f"8-bit rows are int8 or float8_e4m3fn, not {dtype}")
+        codes = torch.zeros(self.n_slots, self.capacity, int(heads) * int(dim), dtype=torch.uint8, device=self.device).view(dtype)
+        scales = torch.zeros(self.n_slots, int(heads), self.capacity, dtype=torch.float32, device=self.device)
+        self.rows += [codes, scales]
+        return codes, scales
+
     # ---- requests (scheduler side)
     def slot_of(self, req_id):
         return self.by_id.get(req_id)

@@ -1,0 +1,110 @@
+"""What the operators of drafted tokens refuse, and their state's shapes: no GPU, no launch."""
+import ctypes
+
+import pytest
+import torch
+
+BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import __graft_entry__ as g
+    g.build()
+    import lia_b200
+    from lia_b200 import _lib
+    return _lib
+
+
+def view(_lib, **change):
+    v = dict(data=1 << 20, scale=1 << 21, slot_stride=1 << 16, pos_stride=1024, head_stride=128, scale_slot_stride=512, scale_head_stride=64, slots=2, capacity=64, type=_lib.CACHE_INT8, dim=128)
+    return _lib.LiaCacheView(**(v | change))
+
+
+def test_view_layout(lib):
+    assert ctypes.sizeof(lib.LiaCacheView) == 72 and lib.LiaCacheView.slots.offset == 56
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"data": None}, "null cache"), ({"scale": None}, "scales"), ({"type": 7}, "type"), ({"type": 0, "scale": None}, "int8"), ({"slots": 0}, "empty"), ({"capacity": 0}, "empty"),
+    ({"data": (1 << 20) + 4}, "vectors"), ({"pos_stride": 1028}, "vectors"), ({"head_stride": 132}, "vectors"), ({"dim": 100}, "multiples of 8"), ({"dim": 2048}, "1024"),
+    ({"capacity": 65}, "different sizes"), ({"type": 2}, "both")])
+def test_store_and_load_refuse(lib, change, message):
+    L = lib.load()
+    good, bad = view(lib), view(lib, **change)
+    for kc, vc in ((bad, good), (good, bad)):
+        assert L.lia_kv_store_8bit(16, 1024, 16, 1024, 0, 16, kc, vc, 4, 8, 0.0, 0, None) == -1 and message in lib.last_error()
+        assert L.lia_kv_load_8bit(16, kc, vc, 16, 1024, 16, 1024, 0, 4, 8, None) == -1 and message in lib.last_error()
+
+
+def test_store_refuses_short_rows_and_null_pointers(lib):
+    L, v = lib.load(), view(lib)
+    assert L.lia_kv_store_8bit(16, 1023, 16, 1024, 0, 16, v, v, 4, 8, 0.0, 0, None) == -1 and "shorter" in lib.last_error()
+    assert L.lia_kv_store_8bit(None, 1024, 16, 1024, 0, 16, v, v, 4, 8, 0.0, 0, None) == -1
+    assert L.lia_kv_store_8bit(16, 1024, 16, 1024, 0, None, v, v, 4, 8, 0.0, 0, None) == -1
+    assert L.lia_kv_store_8bit(16, 1024, 16, 1024, 0, 16, v, v, -1, 8, 0.0, 0, None) == -1
+    assert L.lia_kv_store_8bit(16, 1 << 20, 16, 1 << 20, 0, 16, v, v, 1 << 28, 8, 0.0, 0, None) == -1 and "too many" in lib.last_error()
+    assert L.lia_kv_store_8bit(16, 1024, 16, 1024, 0, 16, v, v, 0, 8, 0.0, 0, None) == 0           # no rows, no launch
+
+
+def attn(lib, kc, vc, q=256, ldq=2048, segs=256, nseg=2, mask=None, words=0, out=256, ws=None, floats=0, M=8, H=16, G=8, rows=4, max_ctx=40, window=0):
+    return lib.load().lia_tree_attn(q, ldq, kc, vc, segs, nseg, mask, words, None, None, out, ws, floats, M, H, G, rows, max_ctx, window, 1.0, 0.0, None)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"data": (1 << 20) + 8}, "vectors"), ({"dim": 96}, "64 or 128"), ({"dim": 256}, "64 or 128"), ({"type": 2}, "different types"), ({"slots": 3}, "different types or sizes"),
+    ({"scale": None}, "scales")])
+def test_attention_refuses_caches(lib, change, message):
+    good, bad = view(lib), view(lib, **change)
+    assert attn(lib, bad, good) == -1 and message in lib.last_error()
+    assert attn(lib, good, bad) == -1 and message in lib.last_error()
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"q": None}, "null"), ({"segs": None}, "null"), ({"out": None}, "null"), ({"H": 15}, "sizes"), ({"G": 0}, "sizes"), ({"M": -1}, "sizes"), ({"ldq": 2047}, "vectors"), ({"ldq": 1024}, "vectors"),
+    ({"q": 260}, "vectors"), ({"mask": 256, "words": 0}, "null"), ({"mask": 256, "words": 1, "rows": 65}, "words"), ({"nseg": 70000}, "too many"),
+    ({"max_ctx": 100000, "nseg": 1}, "workspace"), ({"max_ctx": 100000, "nseg": 1, "ws": 256, "floats": 10}, "workspace")])
+def test_attention_refuses(lib, change, message):
+    v = view(lib)
+    assert attn(lib, v, v, **change) == -1 and message in lib.last_error()
+
+
+def test_attention_of_nothing(lib):
+    v = view(lib)
+    assert attn(lib, v, v, nseg=0) == attn(lib, v, v, M=0) == attn(lib, v, v, rows=0) == 0
+    assert lib.load().lia_tree_attn_workspace_floats(0, 4, 40, 8, 16, 8, 128, 128, 0, 1) == 0
+    assert lib.load().lia_tree_attn_workspace_floats(1, 4, 100000, 8, 16, 8, 128, 128, 0, 1) % (8 * 16 * 130) == 0
+
+
+@pytest.mark.parametrize("args,message", [
+    (dict(V=0), "sizes"), (dict(top=33), "sizes"), (dict(V=4, top=5), "sizes"), (dict(ld=99), "sizes"), (dict(n=-1), "sizes"), (dict(logits=None), "null"), (dict(logits=2), "misaligned"),
+    (dict(top=3, ids=None), "null"), (dict(n=1, tokens=None), "null"), (dict(V=50000, ld=50000), "workspace")])
+def test_logprobs_refuse(lib, args, message):
+    a = dict(logits=16, f32=1, ld=100, M=2, V=100, tokens=16, n=1, logp=16, entropy=16, top=0, best=16, ids=16, ws=None, floats=0) | args
+    rc = lib.load().lia_token_logprobs(a["logits"], a["f32"], a["ld"], a["M"], a["V"], a["tokens"], a["n"], a["logp"], a["entropy"], a["top"], a["best"], a["ids"], a["ws"], a["floats"], None)
+    assert rc == -1 and message in lib.last_error()
+
+
+def test_wrappers_refuse(lib):
+    """Tensors of the wrong shape, type or place raise before anything is launched."""
+    from lia_b200 import ops
+    E = lib.LiaError
+    z = torch.zeros
+    with pytest.raises(E):
+        ops.kv_store_8bit(z(2, 128, dtype=BF16), z(2, 128, dtype=BF16), z(2, 2, dtype=torch.int32), z(1, 4, 128, dtype=torch.int8), z(1, 4, 128, dtype=torch.int8), z(1, 1, 4), z(1, 1, 4), 1, 128, 128)
+    with pytest.raises(E):
+        ops.tree_attn(z(2, 128, dtype=BF16), z(1, 4, 128, dtype=BF16), z(1, 4, 128, dtype=BF16), z(1, 4, dtype=torch.int32), z(2, 128, dtype=BF16), 1, 1, 128, 128, 1.0, rows=2, max_ctx=2)
+    with pytest.raises(E):
+        ops.token_logprobs(z(2, 10))
+    with pytest.raises(E, match="float8_e4m3fn"):
+        ops._cache_view("x", "kcache", z(1, 4, 128), None, 1, 128)
+
+
+def test_slots_of_8_bit_rows():
+    from lia_b200.seq_state import SlotState
+    s = SlotState(3, 17, "cpu")
+    for dtype in (torch.int8, E4M3):
+        codes, scales = s.add_rows_8bit(4, 64, dtype)
+        assert codes.shape == (3, 17, 256) and codes.dtype == dtype and scales.shape == (3, 4, 17) and scales.dtype == F32
+    with pytest.raises(ValueError):
+        s.add_rows_8bit(4, 64, BF16)
