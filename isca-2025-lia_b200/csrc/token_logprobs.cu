@@ -2,10 +2,10 @@
 //
 //   with m = max x, L = sum e^(x - m), A = sum e^(x - m) (x - m):   log p(t) = x_t - m - ln L,   entropy = ln L - A / L
 //
-// One pass over the logits: every thread keeps a running maximum with its L and A (a larger maximum multiplies both by a power and moves A by L times the step), and every warp the 32
-// largest logits that it has met, sorted, one a lane, as whole numbers that order by value and then by lower id.  A logit that is not above the `top`-th of them costs one comparison (and
-// most blocks of 512 one vote); the others are gathered in shared memory, 32 at a time sorted across the warp's lanes and merged with the list.  The first block would have the list take
-// all of its logits; instead the top-th largest of its lanes' maxima is a bound that at most some dozens reach.
+// One pass over the logits: every thread keeps a running maximum with its L and A (a larger maximum multiplies both by a power and moves A by L times the step).  The largest ones are
+// found from what that leaves: the top-th largest of the 256 threads' maxima is reached by at least `top` logits and, as the largest ones seldom share a thread, by few more; the threads
+// that have one are known by their maxima, so that only their logits are read again (a tenth of the row, from L2), by all lanes of their warps.  What reaches the bound is sorted across a warp's lanes,
+// as whole numbers that order by value and then by lower id.  (A list of the largest ones kept by every warp through the pass took 34 instructions a logit instead of 7.)
 // Few rows share out a row's blocks over several blocks of threads, and a second kernel joins the parts (in the same order each time).
 //
 // Memory bounds it for many rows (a logit is read once, eight instructions each), the latency of one block of logits and two launches for few.
@@ -17,9 +17,34 @@ constexpr int WARPS = 8, THREADS = WARPS * 32, MAX_TOP = 32;
 constexpr float LOG2E = 1.4426950408889634f;
 typedef unsigned long long u64;
 
+// pairs of numbers, in one instruction each
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f32x2 both(float x) { return pack2(x, x); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));            // (below 2^-126 of the largest: 0)
   return y;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -57,11 +82,6 @@ __device__ __forceinline__ u64 key_of(float x, int id) {
   return (u64)o << 32 | (uint32_t)~id;
 }
 __device__ __forceinline__ int id_of(u64 k) { return ~(int)(uint32_t)k; }
-__device__ __forceinline__ float logit_of(u64 k) {
-  const uint32_t o = (uint32_t)(k >> 32);
-  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
-}
-
 // neighbours o lanes apart put the larger one first where `first_larger`
 __device__ __forceinline__ u64 exchange(u64 v, int o, bool keep_larger) {
   const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
@@ -74,6 +94,7 @@ __device__ __forceinline__ u64 sort_up(u64 v, int lane) {
     for (int o = k >> 1; o > 0; o >>= 1) v = exchange(v, o, ((lane & k) == 0) == ((lane & o) != 0));
   return v;
 }
+__device__ __forceinline__ u64 sort_down(u64 v, int lane) { return sort_up(v, lane ^ 31); }
 // list falls with the lane, more rises: the 32 largest of both, falling
 __device__ __forceinline__ u64 merge_down(u64 list, u64 more, int lane) {
   u64 v = list > more ? list : more;
@@ -123,62 +144,56 @@ template <typename T> __device__ __forceinline__ void finish(const Args& a, int 
   }
 }
 
+// The lists of a block's W warps (each in lists[warp], falling; a power of two of them) become one, in warp 0's hands
+template <int W> __device__ __forceinline__ u64 join_lists(u64 list, u64 (*lists)[32], int warp, int lane) {
+#pragma unroll
+  for (int half = W / 2; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) lists[warp][31 - lane] = list;                 // rising
+    __syncthreads();
+    if (warp < half) list = merge_down(list, lists[warp + half][lane], lane);
+  }
+  return list;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a) {
-  constexpr int N = Vec<T>::N, U = Vec<T>::U, SHARE = N * U;
-  __shared__ u64 gathered[WARPS][64];
+  constexpr int N = Vec<T>::N, U = Vec<T>::U, SHARE = N * U, ROOM = 1024;
+  __shared__ u64 found[ROOM];                                      // the logits that reach the bound
+  __shared__ u64 lists[WARPS][32];
+  __shared__ int count;
+  __shared__ uint32_t bound;
+  __shared__ uint8_t hot[WARPS][32];
   __shared__ Sums warp_sums[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
   const T* x = reinterpret_cast<const T*>(a.logits) + row * a.ld;
   const int skew = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));            // the row begins inside a 16-byte vector
   const uint4* vecs = reinterpret_cast<const uint4*>(x - skew);
   const int nv = (a.V + skew + N - 1) / N, blocks = (nv + 32 * U - 1) / (32 * U);
   const int b0 = (int)((long long)blocks * split / a.splits), b1 = (int)((long long)blocks * (split + 1) / a.splits);
 
+  auto vector = [&](int v) {                                       // what is not the row's own counts as -inf
+    const int e = v * N - skew;
+    if (v < nv && e >= 0 && e + N <= a.V) return ldg_act(vecs + v);
+    T t[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) t[j] = e + j >= 0 && e + j < a.V ? x[e + j] : (T)(-INFINITY);
+    return *reinterpret_cast<const uint4*>(t);
+  };
   auto load = [&](int b, uint4* u) {
+    if (b < b1 && (b > 0 || skew == 0) && (b + 1) * 32 * SHARE - skew <= a.V) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int v = b * 32 * U + i * 32 + lane, e = v * N - skew;
-      if (b < b1 && v < nv) {
-        if (e >= 0 && e + N <= a.V) {
-          u[i] = ldg_act(vecs + v);
-        } else {                                                   // the row's ends: what is not its own counts as -inf
-          T t[N];
+      for (int i = 0; i < U; ++i) u[i] = ldg_act(vecs + b * 32 * U + i * 32 + lane);
+    } else {
 #pragma unroll
-          for (int j = 0; j < N; ++j) t[j] = e + j >= 0 && e + j < a.V ? x[e + j] : (T)(-INFINITY);
-          u[i] = *reinterpret_cast<const uint4*>(t);
-        }
-      } else {
-        const T low = (T)(-INFINITY);
-        T t[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) t[j] = low;
-        u[i] = *reinterpret_cast<const uint4*>(t);
-      }
+      for (int i = 0; i < U; ++i) u[i] = vector((b < b1 ? b * 32 * U : nv) + i * 32 + lane);
     }
   };
 
+  // ---- sums, and every thread's maximum
   Sums s{-INFINITY, 0.f, 0.f};
-  u64 list = 0;
-  int held = 0;                                                    // gathered logits
-  float bound = __uint_as_float(0x7fc00000u);                      // the top-th of the list; NaN: it has not that many
-  u64* mine = gathered[warp];
-  auto take = [&](int n) {                                         // the first n <= 32 gathered ones join the list
-    __syncwarp();
-    list = merge_down(list, sort_up(lane < n ? mine[lane] : 0, lane), lane);
-    const u64 rest = lane + 32 < held ? mine[lane + 32] : 0;
-    __syncwarp();
-    mine[lane] = rest;
-    held -= n;
-    const u64 last = __shfl_sync(0xffffffffu, list, a.top - 1);
-    bound = last ? logit_of(last) : __uint_as_float(0x7fc00000u);
-    __syncwarp();
-  };
-
   uint4 u[U], next[U];
-  bool first = true;
   load(b0 + warp, u);
   for (int b = b0 + warp; b < b1; b += WARPS) {
     load(b + WARPS, next);
@@ -189,83 +204,139 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
     for (int i = 0; i < SHARE; ++i) m = fmaxf(m, f[i]);
     if (m > s.m) raise_to(s, m);
     const float base = s.m == -INFINITY ? 0.f : s.m;
-    float L[2] = {0.f, 0.f}, A[2] = {0.f, 0.f};
+    f32x2 L = 0ull, A = 0ull;
 #pragma unroll
-    for (int i = 0; i < SHARE; ++i) {
-      const float y = max_nan(f[i] - base, -200.f), e = ex2(y * LOG2E);                 // (e^-200 is 0; -inf would make 0 * inf of A)
-      L[i & 1] += e;
-      A[i & 1] = fmaf(e, y, A[i & 1]);
+    for (int i = 0; i < SHARE; i += 2) {
+      float y0, y1;
+      unpack2(add2(pack2(f[i], f[i + 1]), both(-base)), y0, y1);
+      const f32x2 y = pack2(max_nan(y0, -200.f), max_nan(y1, -200.f));                  // (e^-200 is 0; -inf would make 0 * inf of A)
+      unpack2(mul2(y, both(LOG2E)), y0, y1);
+      const f32x2 e = pack2(ex2(y0), ex2(y1));
+      L = add2(L, e);
+      A = fma2(e, y, A);
     }
-    s.L += L[0] + L[1];
-    s.A += A[0] + A[1];
-    if (a.top > 0) {
-      float least = bound;
-      bool equal = false;                                          // the first block's bound is not in the list yet
-      if (first) {
-        const u64 best = sort_up(key_of(m, 0), lane);              // (rising: the top-th largest is top from the end)
-        least = logit_of(__shfl_sync(0xffffffffu, best, 32 - a.top));
-        equal = true;
-        first = false;
-      }
-      if (__any_sync(0xffffffffu, equal || !(m <= least))) {
+    float p0, p1;
+    unpack2(L, p0, p1);
+    s.L += p0 + p1;
+    unpack2(A, p0, p1);
+    s.A += p0 + p1;
 #pragma unroll
-        for (int i = 0; i < SHARE; ++i) {
-          const int id = (b * 32 * U + (i / N) * 32 + lane) * N - skew + i % N;
-          const bool in = (equal ? !(f[i] < least) : !(f[i] <= least)) && id >= 0 && id < a.V;
-          const unsigned who = __ballot_sync(0xffffffffu, in);
-          if (who) {
-            if (in) mine[held + __popc(who & ((1u << lane) - 1u))] = key_of(f[i], id);
-            held += __popc(who);
-            if (held >= 32) {
-              take(32);
-              if (!equal) least = bound;
-            }
+    for (int i = 0; i < U; ++i) u[i] = next[i];
+  }
+
+  u64 list = 0;
+  if (a.top > 0) {
+    // ---- the top-th largest of the threads' maxima bounds what can be among the top
+    if (threadIdx.x == 0) count = 0;
+    const uint32_t most = (uint32_t)(key_of(s.m, 0) >> 32);
+    list = join_lists<WARPS>(sort_down((u64)most << 32 | 1u, lane), lists, warp, lane);
+    if (threadIdx.x == a.top - 1) bound = (uint32_t)(list >> 32);
+    __syncthreads();
+    // ---- the threads that have something that reaches it: their vectors once more, by all lanes of their warp
+    const unsigned who = __ballot_sync(0xffffffffu, most >= bound);
+    if (most >= bound) hot[warp][__popc(who & ((1u << lane) - 1u))] = (uint8_t)lane;
+    __syncwarp();
+    const int mine = b0 + warp < b1 ? (b1 - b0 - warp + WARPS - 1) / WARPS * U : 0, items = __popc(who) * mine;
+    for (int t0 = lane; t0 < items; t0 += 128) {
+      uint4 w[4];
+      int v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = t0 + j * 32, h = t / mine, r = t - h * mine;
+        v[j] = t < items ? (b0 + warp + r / U * WARPS) * 32 * U + r % U * 32 + hot[warp][h] : nv;
+        w[j] = vector(v[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[N];
+        Vec<T>::unpack(w[j], f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const u64 k = key_of(f[i], v[j] * N - skew + i);
+          if ((uint32_t)(k >> 32) >= bound && id_of(k) >= 0 && id_of(k) < a.V && t0 + j * 32 < items) {
+            const int at = atomicAdd(&count, 1);                   // (in any order: they are sorted)
+            if (at < ROOM) found[at] = k;
           }
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < U; ++i) u[i] = next[i];
+    __syncthreads();
+    const int n = count;
+    if (n <= ROOM) {                                               // some more than top, 32 by 32 by warp 0
+      list = 0;
+      if (warp == 0)
+        for (int i = 0; i < n; i += 32) list = merge_down(list, sort_up(i + lane < n ? found[i + lane] : 0, lane), lane);
+    } else {                                                       // many equal ones: every warp looks at all of its logits again, with the least of its list for a bound
+      list = 0;
+      u64 least = 0;
+      for (int b = b0 + warp; b < b1; b += WARPS)
+        for (int i = 0; i < U; ++i) {
+          float f[N];
+          const int v = b * 32 * U + i * 32 + lane;
+          Vec<T>::unpack(vector(v), f);
+          for (int j = 0; j < N; ++j) {
+            const int id = v * N - skew + j;
+            const u64 k = id >= 0 && id < a.V ? key_of(f[j], id) : 0;
+            if (__any_sync(0xffffffffu, k > least)) {
+              list = merge_down(list, sort_up(k, lane), lane);
+              least = __shfl_sync(0xffffffffu, list, 31);
+            }
+          }
+        }
+      list = join_lists<WARPS>(list, lists, warp, lane);
+    }
   }
-  if (a.top > 0 && held > 0) take(held);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) join(s, from_lane(s, o));
-  __syncwarp();
-  if (a.top > 0) mine[31 - lane] = list;                           // rising
   if (lane == 0) warp_sums[warp] = s;
   __syncthreads();
   if (warp != 0) return;
   s = warp_sums[0];
-  for (int w = 1; w < WARPS; ++w) {
-    join(s, warp_sums[w]);
-    if (a.top > 0) list = merge_down(list, gathered[w][lane], lane);
-  }
+  for (int w = 1; w < WARPS; ++w) join(s, warp_sums[w]);
   if (a.splits == 1) {
     finish<T>(a, row, s, list, lane);
   } else {
     if (lane == 0) a.part_sums[blockIdx.x] = s;
-    if (a.top > 0) a.part_lists[(long long)blockIdx.x * 32 + lane] = list;
+    if (a.top > 0) a.part_lists[(long long)blockIdx.x * 32 + 31 - lane] = list;         // rising
   }
 }
 
+// The parts of a row, a few by each of four warps, always in the same order
 template <typename T>
-__global__ void __launch_bounds__(32) token_logprobs_join_kernel(const Args a) {
+__global__ void __launch_bounds__(128) token_logprobs_join_kernel(const Args a) {
+  __shared__ u64 lists[4][32];
+  __shared__ Sums sums[4];
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x, lane = threadIdx.x;
+  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long at = (long long)row * a.splits;
-  Sums s = a.part_sums[at];
-  u64 list = a.top > 0 ? a.part_lists[at * 32 + lane] : 0;
-  for (int i = 1; i < a.splits; ++i) {
-    join(s, a.part_sums[at + i]);
-    if (a.top > 0) list = merge_down(list, a.part_lists[(at + i) * 32 + 31 - lane], lane);
+  Sums s{-INFINITY, 0.f, 0.f};
+  u64 list = 0;
+  for (int i = warp; i < a.splits; i += 16) {
+    u64 part[4];
+    Sums q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool there = i + j * 4 < a.splits;
+      part[j] = there && a.top > 0 ? a.part_lists[(at + i + j * 4) * 32 + lane] : 0;
+      q[j] = there ? a.part_sums[at + i + j * 4] : Sums{-INFINITY, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      join(s, q[j]);
+      if (a.top > 0 && i + j * 4 < a.splits) list = merge_down(list, part[j], lane);
+    }
   }
+  if (lane == 0) sums[warp] = s;
+  list = join_lists<4>(list, lists, warp, lane);
+  if (warp != 0) return;
+  for (int w = 1; w < 4; ++w) join(s, sums[w]);
   finish<T>(a, row, s, list, lane);
 }
 
 // Blocks of threads of a row: as many as fill the GPU four blocks an SM, none with less than one block of logits a warp
 int splits_of(int M, int V, int act_f32) {
-  const int per = WARPS * 512, most = (V + per - 1) / per, want = (4 * lia_sm_count() + M - 1) / M;
+  const int per = WARPS * 512, most = (V + per - 1) / per, want = 4 * lia_sm_count() / M;
   (void)act_f32;
   return want < 1 ? 1 : want < most ? want : most;
 }
@@ -290,8 +361,8 @@ extern "C" int lia_token_logprobs(const void* logits, int act_f32, long long ld,
   if (act_f32) LIA_CUDA(lia_launch(token_logprobs_kernel<float>, dim3(M * splits), dim3(THREADS), 0, stream, a));
   else LIA_CUDA(lia_launch(token_logprobs_kernel<bf16>, dim3(M * splits), dim3(THREADS), 0, stream, a));
   if (splits > 1) {
-    if (act_f32) LIA_CUDA(lia_launch(token_logprobs_join_kernel<float>, dim3(M), dim3(32), 0, stream, a));
-    else LIA_CUDA(lia_launch(token_logprobs_join_kernel<bf16>, dim3(M), dim3(32), 0, stream, a));
+    if (act_f32) LIA_CUDA(lia_launch(token_logprobs_join_kernel<float>, dim3(M), dim3(128), 0, stream, a));
+    else LIA_CUDA(lia_launch(token_logprobs_join_kernel<bf16>, dim3(M), dim3(128), 0, stream, a));
   }
   return LIA_OK;
 }
