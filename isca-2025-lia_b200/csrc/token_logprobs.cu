@@ -9,38 +9,13 @@
 // Few rows share out a row's blocks over several blocks of threads, and a second kernel joins the parts (in the same order each time).
 //
 // Memory bounds it for many rows (a logit is read once, eight instructions each), the latency of one block of logits and two launches for few.
-#include "common.cuh"
+#include "pairs.cuh"
 
 namespace {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32, MAX_TOP = 32;
 constexpr float LOG2E = 1.4426950408889634f;
 typedef unsigned long long u64;
-
-// pairs of numbers, in one instruction each
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float x, float y) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ f32x2 both(float x) { return pack2(x, x); }
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -10,10 +10,10 @@
 // 8-bit codes are exact in fp16 and so are multiplied there: q goes to fp16 by a power of two of its own for each row (its 8 bits fit; what is 2^-29 of the row's largest is
 // less exact), a key's scale is multiplied into its scores, and a value's into its weight -- in the exponent, s + log2 vs, so that the running maximum bounds the product and no scale is
 // too large or small: weights are 2^(s + log2 vs - max + 14) in fp16, 11 bits, and their sum takes p = weight / vs in fp32.  With bf16 caches weights are two bf16 parts: 16 bits.
-#include <cuda_fp16.h>
-
 #include "mma.cuh"
 #include "tree_attn.cuh"
+
+int lia_tree_attn_tc(const void* args, int type, int nseg, lia_stream_t stream);      // tree_attn_sm100.cu
 
 namespace {
 
@@ -24,26 +24,6 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-// two codes as fp16: e4m3 in the low 16 bits
-__device__ __forceinline__ uint32_t e4m3x2(uint32_t u) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)u, __NV_E4M3);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t int8x2(uint32_t u) {           // bytes 0x64, code + 128 of two numbers: 1024 + 128 + code
-  const uint32_t off = 0x64806480u;                                // 1152
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
 template <int DIM, int VDIM, int KIND, int RT>
 struct Shape {
   static constexpr bool BITS8 = KIND != LIA_CACHE_BF16;
@@ -89,13 +69,12 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
     if constexpr (BITS8) {
       uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
       top = __reduce_max_sync(0xffffffffu, top);
-      const int e = min(max((int)(top >> 7), 27), 253);            // the largest's exponent; its row becomes 2^14 and less
-      const float down = __uint_as_float((uint32_t)(254 + 14 - max(e, 15)) << 23);
+      const Down down = down_of(top);
       float x[4];
       unpack_bf16x2(u.x, x[0], x[1]);
       unpack_bf16x2(u.y, x[2], x[3]);
-      w = make_uint2(pack_f16x2(x[0] * down, x[1] * down), pack_f16x2(x[2] * down, x[3] * down));
-      f /= down;
+      w = make_uint2(pack_f16x2(x[0] * down.by, x[1] * down.by), pack_f16x2(x[2] * down.by, x[3] * down.by));
+      f *= down.back;
     }
     if (lane < DIM / 4) {
       const int c = lane * 4, t = BITS8 ? (c >> 4) & 3 : (c >> 3) & 3, step = BITS8 ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
@@ -395,16 +374,20 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
 
 // How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history
 struct Plan {
-  int rt, tiles, splits;
+  int rt, tiles, splits;                                           // rt: 16 rows each; 8 on tcgen05
 };
+#ifndef TC_ROWS
+#define TC_ROWS 32
+#endif
 Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window) {
   const long long R = (long long)rows * (H / G);
   Plan p;
-  p.rt = R <= 16 ? 1 : 2;
+  p.rt = R > TC_ROWS ? 8 : R <= 16 ? 1 : 2;
   p.tiles = (int)((R + 16 * p.rt - 1) / (16 * p.rt));
-  const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.rt == 1 ? 3 : 2);
+  const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.rt == 1 ? 3 : p.rt == 2 ? 2 : 1);
   const long long span = window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx;
-  long long s = room / blocks, most = (span + 255) / 256;          // (16 blocks of keys a block of threads at least)
+  const long long least = p.rt == 8 ? 512 : 256;                   // keys of a block of threads: eight blocks of 64, or four of 16 a warp
+  long long s = room / blocks, most = (span + least - 1) / least;
   if (s > most) s = most;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   p.splits = s < 1 ? 1 : (int)s;
@@ -422,11 +405,12 @@ template <int DIM, int VDIM, int KIND, int RT> int launch(const TreeArgs& a, int
     if (dev < 64) configured[dev] = true;
   }
   LIA_CUDA(lia_launch(tree_attn_kernel<DIM, VDIM, KIND, RT>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), S::SMEM, stream, a));
-  if (a.splits > 1) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
   return LIA_OK;
 }
 template <int DIM, int VDIM, int KIND> int launch_rt(const TreeArgs& a, int rt, int nseg, cudaStream_t stream) {
-  return rt == 1 ? launch<DIM, VDIM, KIND, 1>(a, nseg, stream) : launch<DIM, VDIM, KIND, 2>(a, nseg, stream);
+  const int rc = rt == 8 ? lia_tree_attn_tc(&a, KIND, nseg, stream) : rt == 1 ? launch<DIM, VDIM, KIND, 1>(a, nseg, stream) : launch<DIM, VDIM, KIND, 2>(a, nseg, stream);
+  if (rc == LIA_OK && a.splits > 1) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
+  return rc;
 }
 template <int KIND> int launch_dims(const TreeArgs& a, int rt, int nseg, cudaStream_t stream) {
   if (a.k.dim == 128) return a.v.dim == 128 ? launch_rt<128, 128, KIND>(a, rt, nseg, stream) : launch_rt<128, 64, KIND>(a, rt, nseg, stream);

@@ -1,5 +1,6 @@
 // What the kernels of attention of drafted tokens share (tree_attn.cu, tree_attn_sm100.cu): a portion, which keys its rows see, and rows that are formed key by key.
 #pragma once
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include "cache8.cuh"
@@ -65,6 +66,34 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// two codes as fp16: e4m3 in the low 16 bits; int8 as the bytes code + 128, 0x64 each (1024 + 128 + code)
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t u) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)u, __NV_E4M3);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t int8x2(uint32_t u) {
+  const uint32_t off = 0x64806480u;                                // 1152
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// The power of two that a row of queries is multiplied by on its way to fp16, and its inverse, by the bits (without sign) of its largest number: that becomes 2^14 to 2^15
+struct Down {
+  float by, back;
+};
+__device__ __forceinline__ Down down_of(uint32_t top) {
+  const uint32_t e = min(max(top >> 7, 27u), 253u);
+  return {__uint_as_float((268 - e) << 23), __uint_as_float((e - 14) << 23)};
+}
+
 // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))): off by a rounding of cap
 __device__ __forceinline__ float capped(float x, float cap, float two_log2e_by_cap) { return cap - __fdividef(2.f * cap, 1.f + ex2(x * two_log2e_by_cap)); }
 
