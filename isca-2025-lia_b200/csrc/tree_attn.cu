@@ -24,26 +24,40 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int DIM, int VDIM, int KIND, int RT>
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {       // of 8 x 8 numbers of 16 bits, a row's two neighbours a lane
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// blocks of an SM, by the registers that the rows' sums and the keys and values on their way take
+constexpr int blocks_an_sm(int kind, int nr) { return nr == 1 ? (kind == LIA_CACHE_BF16 ? 3 : 4) : nr == 2 ? (kind == LIA_CACHE_BF16 ? 2 : 3) : 2; }
+
+template <int DIM, int VDIM, int KIND, int NR>
 struct Shape {
   static constexpr bool BITS8 = KIND != LIA_CACHE_BF16;
-  static constexpr int STEPS = DIM / 16;                           // products of a block of 16 keys with q
-  static constexpr int NT = VDIM / 8;                              // products' columns of 8 channels
+  static constexpr int STEPS = DIM / 16;                           // products of a block of 16 keys with 8 rows' queries
+  static constexpr int MT = VDIM / 16;                             // products of 16 channels of a block's values with 8 rows' weights
   static constexpr int KV = DIM * (BITS8 ? 1 : 2) / 64;            // 16-byte vectors of a key in a lane
   static constexpr int VB = VDIM * (BITS8 ? 1 : 2) / 8;            // bytes of a value in a lane
-  static constexpr int ROWS = 16 * RT;
-  static constexpr int Q_BYTES = RT * STEPS * 32 * 16, O_BYTES = WARPS * ROWS * VDIM * 4, SMEM = (Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES) + 3 * WARPS * ROWS * 4;
-  // the channel of column `col` of the nt-th product with the values
-  static __device__ __forceinline__ int channel(int nt, int col) { return BITS8 ? col * (VDIM / 8) + nt : (nt >> 3) * 64 + col * 8 + (nt & 7); }
+  static constexpr int ROWS = 8 * NR;
+  static constexpr int Q_BYTES = NR * STEPS * 32 * 8, O_BYTES = WARPS * ROWS * VDIM * 4, BIG = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
+  static constexpr int SMEM = BIG + ROWS * 4 + WARPS * ROWS * 8;
+  static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // weights are 2^(x - maximum + LIFT): below 2^15 in fp16
+  // the channel of the first of a lane's pair in the i-th product with the values
+  static __device__ __forceinline__ int channel(int i, int gq) { return BITS8 ? gq * (VDIM / 8) + 2 * i : (i >> 2) * 64 + gq * 8 + (i & 3) * 2; }
 };
+constexpr float NONE = -1e30f, SLACK = 8.f;                        // a maximum of no keys; how far, in powers of two, weights may exceed 1
 
-template <int DIM, int VDIM, int KIND, int RT>
-__global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(const TreeArgs a) {
-  using S = Shape<DIM, VDIM, KIND, RT>;
+template <int DIM, int VDIM, int KIND, int NR>
+__global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_kernel(const TreeArgs a) {
+  using S = Shape<DIM, VDIM, KIND, NR>;
   constexpr bool BITS8 = S::BITS8;
+  constexpr int RQ = BITS8 ? 1 : 2;
   extern __shared__ uint4 smem[];
-  float* row_f = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + (S::Q_BYTES > S::O_BYTES ? S::Q_BYTES : S::O_BYTES));   // [ROWS] what a row's products with keys are multiplied by
+  float* row_f = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + S::BIG);        // [ROWS] what a row's products with keys are multiplied by
   float2* part = reinterpret_cast<float2*>(row_f + S::ROWS);       // [WARPS][ROWS] maximum, sum
+  uint2* qs = reinterpret_cast<uint2*>(smem);                      // [NR][STEPS][32]
   pdl_launch_dependents();
   pdl_wait();
   const Portion p = portion_of(a, blockIdx.z);
@@ -60,35 +74,31 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
     const bool there = r0 + r < R;
     const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
     uint2 u = make_uint2(0u, 0u);
-    if (there && lane < DIM / 4) {
-      const bf16* src = a.q + (p.row + i) * a.ldq + h * DIM + lane * 4;
-      u = *reinterpret_cast<const uint2*>(src);
-    }
+    if (there && lane < DIM / 4) u = *reinterpret_cast<const uint2*>(a.q + (p.row + i) * a.ldq + h * DIM + lane * 4);
     float f = a.scale * (a.temp != nullptr && there ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
     uint2 w = u;
     if constexpr (BITS8) {
       uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
-      top = __reduce_max_sync(0xffffffffu, top);
-      const Down down = down_of(top);
+      const Down down = down_of(__reduce_max_sync(0xffffffffu, top));
       float x[4];
       unpack_bf16x2(u.x, x[0], x[1]);
       unpack_bf16x2(u.y, x[2], x[3]);
       w = make_uint2(pack_f16x2(x[0] * down.by, x[1] * down.by), pack_f16x2(x[2] * down.by, x[3] * down.by));
       f *= down.back;
     }
-    if (lane < DIM / 4) {
+    if (lane < DIM / 4) {                                          // four neighbouring channels are a lane's operand of one step
       const int c = lane * 4, t = BITS8 ? (c >> 4) & 3 : (c >> 3) & 3, step = BITS8 ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
-      uint32_t* dst = reinterpret_cast<uint32_t*>(smem + ((r >> 4) * S::STEPS + step) * 32 + (r & 7) * 4 + t) + ((r >> 3) & 1);
-      dst[0] = w.x;
-      dst[2] = w.y;
+      qs[((r >> 3) * S::STEPS + step) * 32 + (r & 7) * 4 + t] = w;
     }
     if (lane == 0) row_f[r] = f;
   }
   __syncthreads();
-  uint32_t qa[RT == 1 ? S::STEPS : 1][4];                          // 16 rows' queries stay in registers, those of 32 in shared memory
-  if constexpr (RT == 1) {
+  uint2 qa[NR <= RQ ? NR : 1][NR <= RQ ? S::STEPS : 1];            // few rows' queries stay in registers, the others' in shared memory
+  if constexpr (NR <= RQ) {
 #pragma unroll
-    for (int s = 0; s < S::STEPS; ++s) *reinterpret_cast<uint4*>(qa[s]) = smem[s * 32 + lane];
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int s = 0; s < S::STEPS; ++s) qa[r][s] = qs[(r * S::STEPS + s) * 32 + lane];
   }
 
   // ---- which keys
@@ -105,55 +115,48 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
     near = __reduce_min_sync(0xffffffffu, near);
     far = __reduce_max_sync(0xffffffffu, far);
   }
-  const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = a.mask != nullptr ? p.p0 : p.p0 + i0 + 1;
+  const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = min(hi, a.mask != nullptr ? p.p0 : p.p0 + i0 + 1);
   const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
 
-  int ri[RT][2], rd[RT][2];                                        // of the lane's rows gq and gq + 8: token and depth
-  float rf[RT][2], m[RT][2], l[RT][2];
+  float rf[NR][2], m[NR][2], l[NR][2];                             // of the lane's rows 2 t4 and 2 t4 + 1 of every eight
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
+  for (int r = 0; r < NR; ++r)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = rt * 16 + e * 8 + gq;
-      ri[rt][e] = min((r0 + r) / a.rep, p.n - 1);
-      rd[rt][e] = depth_of(a, p, ri[rt][e]);
-      rf[rt][e] = row_f[r];
-      m[rt][e] = -INFINITY;
-      l[rt][e] = 0.f;
+      rf[r][e] = row_f[r * 8 + t4 * 2 + e];
+      m[r][e] = NONE;
+      l[r][e] = 0.f;
     }
-  float o[RT][S::NT][4];
+  float o[NR][S::MT][4];                                           // [..][0]: a lane's first channel of a pair and row 2 t4, [1]: row 2 t4 + 1, [2], [3]: its second channel
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
+  for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int n = 0; n < S::NT; ++n)
+    for (int n = 0; n < S::MT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[rt][n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) o[r][n][e] = 0.f;
 
   const uint8_t *kbase = a.k.at(p.slot, 0, g) + t4 * 16, *vbase = a.v.at(p.slot, 0, g) + gq * (BITS8 ? S::VB : 16);
   const float *ksc = BITS8 ? a.k.scale_at(p.slot, g) : nullptr, *vsc = BITS8 ? a.v.scale_at(p.slot, g) : nullptr;
-  uint4 kr[2][S::KV];
-  uint32_t vr[4][S::VB / 4];
-  float ks[4], vs[4];
-  auto key_of = [&](int b, int c) { return min(lo + b * 16 + ((c >> 1) * 8 + t4 * 2 + (c & 1)), hi - 1); };   // of the lane's columns of scores
+  uint4 kr[2][S::KV];                                              // keys gq and gq + 8
+  uint32_t vr[4][S::VB / 4];                                       // values 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4
+  float ks[2], vs[2];                                              // of keys gq and gq + 8
   auto load_k = [&](int b) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint8_t* src = kbase + (long long)min(lo + b * 16 + j * 8 + gq, hi - 1) * a.k.pos;
+      const int key = min(lo + b * 16 + j * 8 + gq, hi - 1);
+      const uint8_t* src = kbase + (long long)key * a.k.pos;
 #pragma unroll
       for (int c = 0; c < S::KV; ++c) kr[j][c] = ldg_act(src + c * 64);
-    }
-    if constexpr (BITS8) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        ks[c] = __ldcg(ksc + key_of(b, c));
-        vs[c] = __ldcg(vsc + key_of(b, c));
+      if constexpr (BITS8) {
+        ks[j] = __ldcg(ksc + key);
+        vs[j] = __ldcg(vsc + key);
       }
     }
   };
   auto load_v = [&](int b) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint8_t* src = vbase + (long long)key_of(b, c) * a.v.pos;
+      const uint8_t* src = vbase + (long long)min(lo + b * 16 + (c >> 1) * 8 + t4 * 2 + (c & 1), hi - 1) * a.v.pos;
       if constexpr (S::VB == 8) {
         const uint2 u = __ldcg(reinterpret_cast<const uint2*>(src));
         vr[c][0] = u.x;
@@ -170,18 +173,17 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
     load_v(b0 + warp);
   }
   const float two_by_cap = a.softcap > 0.f ? 2.f * LOG2E / a.softcap : 0.f;
+#pragma unroll 1
   for (int b = b0 + warp; b < b1; b += WARPS) {
-    // ---- scores of 16 keys
-    float s[RT][2][4];
+    // ---- products of 16 keys and all rows: s[r][0], [1]: key gq and rows 2 t4, 2 t4 + 1; [2], [3]: key gq + 8
+    float s[NR][4];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[rt][j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
 #pragma unroll
     for (int st = 0; st < S::STEPS; ++st) {
-      uint32_t kb[2][2];
+      uint32_t ka[4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if constexpr (BITS8) {
@@ -189,96 +191,109 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
           uint32_t w = (st & 3) == 0 ? u.x : (st & 3) == 1 ? u.y : (st & 3) == 2 ? u.z : u.w;
           if constexpr (KIND == LIA_CACHE_INT8) {
             w ^= 0x80808080u;
-            kb[j][0] = int8x2(__byte_perm(w, 0x64646464u, 0x4140));
-            kb[j][1] = int8x2(__byte_perm(w, 0x64646464u, 0x4342));
+            ka[j] = int8x2(__byte_perm(w, 0x64646464u, 0x4140));
+            ka[2 + j] = int8x2(__byte_perm(w, 0x64646464u, 0x4342));
           } else {
-            kb[j][0] = e4m3x2(w & 0xffffu);
-            kb[j][1] = e4m3x2(w >> 16);
+            ka[j] = e4m3x2(w & 0xffffu);
+            ka[2 + j] = e4m3x2(w >> 16);
           }
         } else {
           const uint4& u = kr[j][st >> 1];
-          kb[j][0] = st & 1 ? u.z : u.x;
-          kb[j][1] = st & 1 ? u.w : u.y;
+          ka[j] = st & 1 ? u.z : u.x;
+          ka[2 + j] = st & 1 ? u.w : u.y;
         }
       }
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        uint32_t qf[4];
-        if constexpr (RT == 1) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qf[e] = qa[st][e];
-        } else {
-          *reinterpret_cast<uint4*>(qf) = smem[(rt * S::STEPS + st) * 32 + lane];
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if constexpr (BITS8) mma_f16(s[rt][j], qf, kb[j][0], kb[j][1]);
-          else mma_bf16(s[rt][j], qf, kb[j][0], kb[j][1]);
-        }
+      for (int r = 0; r < NR; ++r) {
+        uint2 q;
+        if constexpr (NR <= RQ) q = qa[r][st];
+        else q = qs[(r * S::STEPS + st) * 32 + lane];
+        if constexpr (BITS8) mma_f16(s[r], ka, q.x, q.y);
+        else mma_bf16(s[r], ka, q.x, q.y);
       }
     }
-    float kf[4], lv[4], rv[4];
+    float kf[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f}, rv[2] = {1.f, 1.f};
+    if constexpr (BITS8) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      kf[c] = BITS8 ? ks[c] : 1.f;
-      if constexpr (BITS8) vs[c] = max_nan(vs[c], 0x1p-120f);      // (a scale of 0 weighs nothing, and its score still counts)
-      lv[c] = BITS8 ? lg2(vs[c]) : 0.f;
-      rv[c] = BITS8 ? __fdividef(1.f, vs[c]) : 1.f;
+      for (int j = 0; j < 2; ++j) {
+        kf[j] = ks[j];
+        const float y = max_nan(vs[j], LEAST_SCALE);
+        lv[j] = lg2(y);
+        rv[j] = __fdividef(1.f, y);
+      }
     }
     if (b + WARPS < b1) load_k(b + WARPS);
-    // ---- weights
+    // ---- scores, as powers of two and with the values' scales
     const int key0 = lo + b * 16;
-    const bool every = key0 >= all_lo && key0 + 16 <= min(all_hi, hi);
-    uint32_t pa[RT][BITS8 ? 1 : 2][4];
+    if (a.softcap > 0.f) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float top = -INFINITY;
+        for (int e = 0; e < 4; ++e) s[r][e] = fmaf(capped(s[r][e] * kf[e >> 1] * rf[r][e & 1], a.softcap, two_by_cap), LOG2E, lv[e >> 1]);
+    } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float& x = s[rt][c >> 1][e * 2 + (c & 1)];
-          x *= rf[rt][e];
-          if constexpr (BITS8) x *= kf[c];
-          if (a.softcap > 0.f) x = capped(x, a.softcap, two_by_cap) * LOG2E;
-          if constexpr (BITS8) x += lv[c];
-          if (!every) {
-            const int t = key0 + (c >> 1) * 8 + t4 * 2 + (c & 1);
-            if (t >= hi || !sees(a, p, ri[rt][e], rd[rt][e], t)) x = -INFINITY;
-          }
-          top = fmaxf(top, x);
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(m[rt][e], top), base = mn == -INFINITY ? 0.f : mn, keep = ex2(m[rt][e] - base);
-        m[rt][e] = mn;
-        l[rt][e] *= keep;
-        if (__any_sync(0xffffffffu, keep != 1.f)) {
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int n = 0; n < S::NT; ++n) {
-            o[rt][n][e * 2] *= keep;
-            o[rt][n][e * 2 + 1] *= keep;
+        for (int e = 0; e < 4; ++e) s[r][e] = BITS8 ? fmaf(s[r][e] * kf[e >> 1], rf[r][e & 1], lv[e >> 1]) : s[r][e] * rf[r][e & 1];
+    }
+    if (key0 < all_lo || key0 + 16 > all_hi) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = min((r0 + r * 8 + t4 * 2 + e) / a.rep, p.n - 1), d = depth_of(a, p, i);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int t = key0 + j * 8 + gq;
+            if (t >= hi || !sees(a, p, i, d, t)) s[r][j * 2 + e] = -INFINITY;
           }
         }
-        float w[4];
+    }
+    // ---- the maximum moves only for rows that have outgrown it
+    bool grown = false;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float x = s[rt][c >> 1][e * 2 + (c & 1)];
-          w[c] = ex2(x - base + (BITS8 ? 14.f : 0.f));
-          l[rt][e] = BITS8 ? (x == -INFINITY ? l[rt][e] : fmaf(w[c], rv[c], l[rt][e])) : l[rt][e] + w[c];
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) grown |= s[r][e] > m[r][e & 1] + SLACK;
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(s[r][e], s[r][2 + e]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const bool up = top > m[r][e] + SLACK;
+          const float keep = up ? ex2(m[r][e] - top) : 1.f;
+          if (up) m[r][e] = top;
+          l[r][e] *= keep;
+#pragma unroll
+          for (int n = 0; n < S::MT; ++n) {
+            o[r][n][e] *= keep;
+            o[r][n][2 + e] *= keep;
+          }
         }
+    }
+    // ---- weights, turned into the products' other operand
+    uint32_t pb[BITS8 ? 1 : 2][NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = ex2(s[r][e] - m[r][e & 1] + S::LIFT);
+        l[r][e & 1] = BITS8 ? fmaf(w[e], rv[e >> 1], l[r][e & 1]) : l[r][e & 1] + w[e];
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
         if constexpr (BITS8) {
-          pa[rt][0][e] = pack_f16x2(w[0], w[1]);
-          pa[rt][0][2 + e] = pack_f16x2(w[2], w[3]);
+          pb[0][r][j] = transposed(pack_f16x2(w[2 * j], w[2 * j + 1]));
         } else {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t top2 = pack_bf16x2(w[2 * c], w[2 * c + 1]);
-            float x, y;
-            unpack_bf16x2(top2, x, y);
-            pa[rt][0][c * 2 + e] = top2;
-            pa[rt][BITS8 ? 0 : 1][c * 2 + e] = pack_bf16x2(w[2 * c] - x, w[2 * c + 1] - y);
-          }
+          const uint32_t hi2 = pack_bf16x2(w[2 * j], w[2 * j + 1]);
+          float x, y;
+          unpack_bf16x2(hi2, x, y);
+          pb[0][r][j] = transposed(hi2);
+          pb[BITS8 ? 0 : 1][r][j] = transposed(pack_bf16x2(w[2 * j] - x, w[2 * j + 1] - y));
         }
       }
     }
@@ -286,7 +301,7 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
 #pragma unroll
     for (int w = 0; w < S::VB / 4; ++w) {
       constexpr int PER = BITS8 ? 4 : 2;                           // channels of a word
-      uint32_t vb[PER][2];
+      uint32_t va[PER][2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const uint32_t u0 = vr[2 * c][w], u1 = vr[2 * c + 1][w];
@@ -295,32 +310,35 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
           if constexpr (KIND == LIA_CACHE_INT8) {
             x ^= 0x80808080u;
             y ^= 0x80808080u;
-            vb[0][c] = int8x2(__byte_perm(x, 0x64646464u, 0x4140));
-            vb[1][c] = int8x2(__byte_perm(x, 0x64646464u, 0x4342));
-            vb[2][c] = int8x2(__byte_perm(y, 0x64646464u, 0x4140));
-            vb[3][c] = int8x2(__byte_perm(y, 0x64646464u, 0x4342));
+            va[0][c] = int8x2(__byte_perm(x, 0x64646464u, 0x4140));
+            va[1][c] = int8x2(__byte_perm(x, 0x64646464u, 0x4342));
+            va[2][c] = int8x2(__byte_perm(y, 0x64646464u, 0x4140));
+            va[3][c] = int8x2(__byte_perm(y, 0x64646464u, 0x4342));
           } else {
-            vb[0][c] = e4m3x2(x & 0xffffu);
-            vb[1][c] = e4m3x2(x >> 16);
-            vb[2][c] = e4m3x2(y & 0xffffu);
-            vb[3][c] = e4m3x2(y >> 16);
+            va[0][c] = e4m3x2(x & 0xffffu);
+            va[1][c] = e4m3x2(x >> 16);
+            va[2][c] = e4m3x2(y & 0xffffu);
+            va[3][c] = e4m3x2(y >> 16);
           }
         } else {
-          vb[0][c] = __byte_perm(u0, u1, 0x5410);
-          vb[1][c] = __byte_perm(u0, u1, 0x7632);
+          va[0][c] = __byte_perm(u0, u1, 0x5410);
+          va[1][c] = __byte_perm(u0, u1, 0x7632);
         }
       }
 #pragma unroll
-      for (int c = 0; c < PER; ++c)
+      for (int c = 0; c < PER; c += 2) {
+        const uint32_t v4[4] = {va[c][0], va[c + 1][0], va[c][1], va[c + 1][1]};
+        const int n = (w * PER + c) >> 1;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int r = 0; r < NR; ++r) {
           if constexpr (BITS8) {
-            mma_f16(o[rt][w * 4 + c], pa[rt][0], vb[c][0], vb[c][1]);
+            mma_f16(o[r][n], v4, pb[0][r][0], pb[0][r][1]);
           } else {
-            mma_bf16(o[rt][w * 2 + c], pa[rt][0], vb[c][0], vb[c][1]);
-            mma_bf16(o[rt][w * 2 + c], pa[rt][BITS8 ? 0 : 1], vb[c][0], vb[c][1]);
+            mma_bf16(o[r][n], v4, pb[0][r][0], pb[0][r][1]);
+            mma_bf16(o[r][n], v4, pb[BITS8 ? 0 : 1][r][0], pb[BITS8 ? 0 : 1][r][1]);
           }
         }
+      }
     }
     if (b + WARPS < b1) load_v(b + WARPS);
   }
@@ -329,34 +347,29 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
   __syncthreads();                                                 // (queries have been read)
   float* os = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
+  for (int r = 0; r < NR; ++r)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float x = l[rt][e];
-      x += __shfl_xor_sync(0xffffffffu, x, 1);
-      x += __shfl_xor_sync(0xffffffffu, x, 2);
-      const int r = warp * S::ROWS + rt * 16 + e * 8 + gq;
-      if (t4 == 0) part[r] = make_float2(m[rt][e], x);
+      float x = l[r][e];
 #pragma unroll
-      for (int n = 0; n < S::NT; n += 4)
+      for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      const int at = warp * S::ROWS + r * 8 + t4 * 2 + e;
+      if (gq == 0) part[at] = make_float2(m[r][e], x);
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          *reinterpret_cast<float4*>(os + r * VDIM + S::channel(n, t4 * 2 + c)) =
-              make_float4(o[rt][n][e * 2 + c], o[rt][n + 1][e * 2 + c], o[rt][n + 2][e * 2 + c], o[rt][n + 3][e * 2 + c]);
+      for (int n = 0; n < S::MT; ++n) *reinterpret_cast<float2*>(os + at * VDIM + S::channel(n, gq)) = make_float2(o[r][n][e], o[r][n][2 + e]);
     }
   __syncthreads();
   constexpr int N = VDIM / 32;
   const long long rows = (long long)a.M * a.H;
   for (int r = warp; r < S::ROWS && r0 + r < R; r += WARPS) {
     const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
-    float top = -INFINITY, sum = 0.f, y[N] = {};
+    float top = NONE, sum = 0.f, y[N] = {};
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w * S::ROWS + r].x);
-    const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float2 x = part[w * S::ROWS + r];
-      const float f = ex2(x.x - base);
+      const float f = ex2(x.x - top);
       sum = fmaf(x.y, f, sum);
 #pragma unroll
       for (int c = 0; c < N; ++c) y[c] = fmaf(os[(w * S::ROWS + r) * VDIM + lane * N + c], f, y[c]);
@@ -374,19 +387,19 @@ __global__ void __launch_bounds__(THREADS, RT == 1 ? 3 : 2) tree_attn_kernel(con
 
 // How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history
 struct Plan {
-  int rt, tiles, splits;                                           // rt: 16 rows each; 8 on tcgen05
+  int nr, tiles, splits;                                           // nr: eights of rows; 16 of them on tcgen05
 };
 #ifndef TC_ROWS
 #define TC_ROWS 32
 #endif
-Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window) {
+Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
   const long long R = (long long)rows * (H / G);
   Plan p;
-  p.rt = R > TC_ROWS ? 8 : R <= 16 ? 1 : 2;
-  p.tiles = (int)((R + 16 * p.rt - 1) / (16 * p.rt));
-  const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.rt == 1 ? 3 : p.rt == 2 ? 2 : 1);
+  p.nr = R > TC_ROWS ? 16 : R > 16 ? 4 : R > 8 ? 2 : 1;
+  p.tiles = (int)((R + 8 * p.nr - 1) / (8 * p.nr));
+  const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.nr == 16 ? 1 : blocks_an_sm(type, p.nr));
   const long long span = window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx;
-  const long long least = p.rt == 8 ? 512 : 256;                   // keys of a block of threads: eight blocks of 64, or four of 16 a warp
+  const long long least = p.nr == 16 ? 512 : 256;                   // keys of a block of threads: eight blocks of 64, or four of 16 a warp
   long long s = room / blocks, most = (span + least - 1) / least;
   if (s > most) s = most;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
@@ -395,34 +408,36 @@ Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window) {
 }
 size_t floats_of(const Plan& p, int M, int H, int vdim) { return p.splits > 1 ? (size_t)p.splits * M * H * (vdim + 2) : 0; }
 
-template <int DIM, int VDIM, int KIND, int RT> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
-  using S = Shape<DIM, VDIM, KIND, RT>;
+template <int DIM, int VDIM, int KIND, int NR> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
+  using S = Shape<DIM, VDIM, KIND, NR>;
   static bool configured[64] = {};                                 // per device
   int dev = 0;
   LIA_CUDA(cudaGetDevice(&dev));
   if (S::SMEM > 48 * 1024 && (dev >= 64 || !configured[dev])) {
-    LIA_CUDA(cudaFuncSetAttribute(tree_attn_kernel<DIM, VDIM, KIND, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    LIA_CUDA(cudaFuncSetAttribute(tree_attn_kernel<DIM, VDIM, KIND, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     if (dev < 64) configured[dev] = true;
   }
-  LIA_CUDA(lia_launch(tree_attn_kernel<DIM, VDIM, KIND, RT>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), S::SMEM, stream, a));
+  LIA_CUDA(lia_launch(tree_attn_kernel<DIM, VDIM, KIND, NR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), S::SMEM, stream, a));
   return LIA_OK;
 }
-template <int DIM, int VDIM, int KIND> int launch_rt(const TreeArgs& a, int rt, int nseg, cudaStream_t stream) {
-  const int rc = rt == 8 ? lia_tree_attn_tc(&a, KIND, nseg, stream) : rt == 1 ? launch<DIM, VDIM, KIND, 1>(a, nseg, stream) : launch<DIM, VDIM, KIND, 2>(a, nseg, stream);
+template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
+  const int rc = nr == 16 ? lia_tree_attn_tc(&a, KIND, nseg, stream)
+                 : nr == 4 ? launch<DIM, VDIM, KIND, 4>(a, nseg, stream)
+                 : nr == 2 ? launch<DIM, VDIM, KIND, 2>(a, nseg, stream) : launch<DIM, VDIM, KIND, 1>(a, nseg, stream);
   if (rc == LIA_OK && a.splits > 1) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
   return rc;
 }
-template <int KIND> int launch_dims(const TreeArgs& a, int rt, int nseg, cudaStream_t stream) {
-  if (a.k.dim == 128) return a.v.dim == 128 ? launch_rt<128, 128, KIND>(a, rt, nseg, stream) : launch_rt<128, 64, KIND>(a, rt, nseg, stream);
-  return a.v.dim == 128 ? launch_rt<64, 128, KIND>(a, rt, nseg, stream) : launch_rt<64, 64, KIND>(a, rt, nseg, stream);
+template <int KIND> int launch_dims(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
+  if (a.k.dim == 128) return a.v.dim == 128 ? launch_rows<128, 128, KIND>(a, nr, nseg, stream) : launch_rows<128, 64, KIND>(a, nr, nseg, stream);
+  return a.v.dim == 128 ? launch_rows<64, 128, KIND>(a, nr, nseg, stream) : launch_rows<64, 64, KIND>(a, nr, nseg, stream);
 }
 
 }  // namespace
 
 extern "C" size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx, int M, int H, int G, int dim, int vdim, int window, int type) {
-  (void)dim; (void)type;
+  (void)dim;
   if (nseg <= 0 || rows <= 0 || M <= 0 || G <= 0 || H <= 0 || H % G || vdim <= 0) return 0;
-  return floats_of(plan_of(nseg, rows, max_ctx, H, G, window), M, H, vdim);
+  return floats_of(plan_of(nseg, rows, max_ctx, H, G, window, type), M, H, vdim);
 }
 
 extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
@@ -437,15 +452,15 @@ extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* k
   LIA_CHECK_ARG(q && segs && out && (mask == nullptr || words > 0), "lia_tree_attn: null pointer");
   LIA_CHECK_ARG(ldq >= (long long)H * kc->dim && ldq % 4 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0, "lia_tree_attn: queries and outputs have to be whole 8-byte vectors");
   LIA_CHECK_ARG(mask == nullptr || rows <= 64 * words, "lia_tree_attn: %d words of mask do not hold %d tokens", words, rows);
-  const Plan plan = plan_of(nseg, rows, max_ctx, H, G, window);
+  const Plan plan = plan_of(nseg, rows, max_ctx, H, G, window, kc->type);
   LIA_CHECK_ARG(nseg <= 65535 && (long long)plan.tiles * G <= 65535, "lia_tree_attn: too many portions, or rows of one");
   LIA_CHECK_ARG(plan.splits == 1 || (ws && ws_floats >= floats_of(plan, M, H, vc->dim) && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_tree_attn: needs a workspace of %zu floats",
                 floats_of(plan, M, H, vc->dim));
   const TreeArgs a{reinterpret_cast<const bf16*>(q), ldq, cache8(kc), cache8(vc), segs, reinterpret_cast<const unsigned long long*>(mask), words, depth, temp,
                    reinterpret_cast<bf16*>(out), ws, M, H, G, H / G, rows, window > 0 ? window : 1 << 30, plan.splits, plan.tiles, scale, softcap};
   switch (kc->type) {
-    case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, plan.rt, nseg, stream);
-    case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, plan.rt, nseg, stream);
-    default: return launch_dims<LIA_CACHE_E4M3>(a, plan.rt, nseg, stream);
+    case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, plan.nr, nseg, stream);
+    case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, plan.nr, nseg, stream);
+    default: return launch_dims<LIA_CACHE_E4M3>(a, plan.nr, nseg, stream);
   }
 }

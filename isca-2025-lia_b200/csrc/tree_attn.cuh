@@ -8,6 +8,9 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+// Values whose scale is below this count as if it were this, which puts them off by 2^-71 at most.  Their scores count all the same: a weight is p times the scale, relative to the largest such
+// product, and with scales up to 2^29 a p of 2^-24 stays above the smallest normal number, from where it goes into the sum of the p.
+constexpr float LEAST_SCALE = 0x1p-80f;
 
 struct TreeArgs {
   const bf16* q;
@@ -58,12 +61,12 @@ __device__ __forceinline__ int end_key(const TreeArgs& a, const Portion& p, int 
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));            // (below 2^-126: 0; keeping those took three instructions more)
   return y;
 }
 __device__ __forceinline__ float lg2(float x) {
   float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {

@@ -222,38 +222,40 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
         tmem_ld_wait();
         const int t = start + j * KEYS;
         // ---- scores in powers of two (with the values' scales)
-        if constexpr (BITS8) {
+        auto scaled = [&](auto with) {                             // with(pair of products times the row's factor, log2 of the values' scales)
 #pragma unroll
           for (int c = 0; c < KEYS; c += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(&sm.ks[st][c]), l4 = *reinterpret_cast<const float4*>(&sm.lv[st][c]);
-            const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, ll[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              f32x2 x = mul2(pack2(__uint_as_float(v[c + e]), __uint_as_float(v[c + e + 1])), pack2(kk[e], kk[e + 1]));
-              float x0, x1;
-              if (a.softcap > 0.f) {
-                unpack2(mul2(x, both(rf)), x0, x1);
-                x = fma2(pack2(capped(x0, a.softcap, two_by_cap), capped(x1, a.softcap, two_by_cap)), both(LOG2E), pack2(ll[e], ll[e + 1]));
-              } else {
-                x = fma2(x, both(rf), pack2(ll[e], ll[e + 1]));
-              }
-              unpack2(x, x0, x1);
-              v[c + e] = __float_as_uint(x0);
-              v[c + e + 1] = __float_as_uint(x1);
+            float4 k4 = make_float4(1.f, 1.f, 1.f, 1.f), l4 = make_float4(0.f, 0.f, 0.f, 0.f);
+            if constexpr (BITS8) {
+              k4 = *reinterpret_cast<const float4*>(&sm.ks[st][c]);
+              l4 = *reinterpret_cast<const float4*>(&sm.lv[st][c]);
             }
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < KEYS; c += 2) {
+            f32x2 x = pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), y = pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+            if constexpr (BITS8) {
+              x = mul2(x, pack2(k4.x, k4.y));
+              y = mul2(y, pack2(k4.z, k4.w));
+            }
+            x = with(x, pack2(l4.x, l4.y));
+            y = with(y, pack2(l4.z, l4.w));
             float x0, x1;
-            unpack2(mul2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), both(rf)), x0, x1);
-            if (a.softcap > 0.f) {
-              x0 = capped(x0, a.softcap, two_by_cap) * LOG2E;
-              x1 = capped(x1, a.softcap, two_by_cap) * LOG2E;
-            }
+            unpack2(x, x0, x1);
             v[c] = __float_as_uint(x0);
             v[c + 1] = __float_as_uint(x1);
+            unpack2(y, x0, x1);
+            v[c + 2] = __float_as_uint(x0);
+            v[c + 3] = __float_as_uint(x1);
           }
+        };
+        if (a.softcap > 0.f) {
+          scaled([&](f32x2 x, f32x2 lv) {
+            float x0, x1;
+            unpack2(mul2(x, both(rf)), x0, x1);
+            return fma2(pack2(capped(x0, a.softcap, two_by_cap), capped(x1, a.softcap, two_by_cap)), both(LOG2E), lv);
+          });
+        } else if constexpr (BITS8) {
+          scaled([&](f32x2 x, f32x2 lv) { return fma2(x, both(rf), lv); });
+        } else {
+          scaled([&](f32x2 x, f32x2) { return mul2(x, both(rf)); });
         }
         if (t < all_lo || t + KEYS > min(all_hi, hi)) {
 #pragma unroll
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
           if (th < KEYS) {
             sm.ks[st][th] = sc[x];
           } else if (th < 2 * KEYS) {
-            const float y = max_nan(sc[x], 0x1p-120f);             // (a scale of 0 weighs nothing, and its score still counts)
+            const float y = max_nan(sc[x], LEAST_SCALE);
             sm.lv[st][th - KEYS] = lg2(y);
             sm.rv[st][th - KEYS] = __fdividef(1.f, y);
           }
