@@ -683,11 +683,9 @@ int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const Li
                   const float* temp, void* out, float* ws, size_t ws_floats, int M, int H, int G, int rows, int max_ctx, int window, float scale, float softcap, lia_stream_t stream);
 
 /* Of every row of logits [M, V] (bf16 or fp32, ld apart): logp[n] of the n given tokens (an id outside [0, V) has NaN), the entropy of the distribution in nats, and the `top` <= 32
- * largest logits' ids (int64; of equal ones the lowest first, NaN counts as -inf) and log probabilities.  Rows that hold NaN or +inf, or -inf alone, have NaN for all but the ids.
- * ws: lia_token_logprobs_workspace_floats() floats (0: NULL will do). */
-size_t lia_token_logprobs_workspace_floats(int M, int V, int act_f32);
+ * largest logits' ids (int64; of equal ones the lowest first, NaN counts as -inf) and log probabilities.  Rows that hold NaN or +inf, or -inf alone, have NaN for all but the ids. */
 int lia_token_logprobs(const void* logits, int act_f32, long long ld, int M, int V, const int64_t* tokens, int n, float* logp, float* entropy, int top, float* top_logp, int64_t* top_ids,
-                       float* ws, size_t ws_floats, lia_stream_t stream);
+                       lia_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -241,8 +241,7 @@ _PROTOTYPES = {
     "lia_tree_attn_workspace_floats": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "lia_tree_attn": (c_int, [c_void_p, c_longlong, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                               c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p]),
-    "lia_token_logprobs_workspace_floats": (c_size_t, [c_int, c_int, c_int]),
-    "lia_token_logprobs": (c_int, [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "lia_token_logprobs": (c_int, [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
 }
 
 EXPORTS = tuple(_PROTOTYPES)

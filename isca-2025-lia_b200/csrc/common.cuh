@@ -65,6 +65,25 @@ inline cudaError_t lia_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
                               Args&&... args) {
   return lia_launch_as(true, kernel, grid, block, smem, stream, std::forward<Args>(args)...);
 }
+// With clusters of `cluster` blocks along x (up to 8), which see one another's shared memory
+template <typename... KArgs, typename... Args>
+inline cudaError_t lia_launch_cluster(int cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                      Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = lia_pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
 // Without that: for kernels of long-running blocks that fill the GPU once.  Placed while the previous kernel drains, their blocks crowd the SMs
 // that empty first (state-space scan of 2048 tokens: the mixer 495 us instead of 414).
 template <typename... KArgs, typename... Args>
@@ -139,5 +158,31 @@ __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepc
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// clusters: a barrier of all their blocks, and the place in block `rank` that is a block's own at `addr`
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_place(const void* addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(addr)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint64_t cluster_ld64(uint32_t at) {
+  uint64_t v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_ld_f4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_ld_f2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
 
 #endif  // __CUDACC__

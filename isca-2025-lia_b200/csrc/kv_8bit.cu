@@ -5,8 +5,9 @@
 //          loses nothing against a / 448 down to a / 28672, and makes scaling and reading back exact.
 // One scale for each head of each token: a token that comes later changes nothing that is there, and attention multiplies scores and weights by scales instead of channels by them.
 //
-// Both kernels move each number once and compute about ten operations on it, so memory bounds them.  A group of 8 to 32 neighbouring lanes has a head of a token, eight channels a
-// lane: its largest magnitude takes three to five shuffles, and no shared memory.
+// Both kernels move each number once; storing computes ten operations on it, so that instructions would bound it before memory does if each lane had few numbers: a lane has 32
+// neighbouring channels of a head (four lanes a head of 128), which divides the addresses, the scale and the steps of finding the largest magnitude among them.  Magnitudes of bf16 numbers
+// are compared as pairs of whole numbers, and a normed head's largest is the largest before, times the norm's factor, because rounding keeps order.
 #include <cuda_fp8.h>
 
 #include "cache8.cuh"
@@ -16,20 +17,44 @@ namespace {
 constexpr int THREADS = 256;
 constexpr float LEAST = 7.888609052210118e-31f;                    // 2^-100: keeps scales and their inverses normal numbers
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, bool vec, float* f) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec) {
-      unpack8(ldg_act(p), f);
-      return;
-    }
-  } else if (vec) {
-    const uint4 u = ldg_act(p), w = ldg_act(p + 4);
-    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-    f[4] = __uint_as_float(w.x); f[5] = __uint_as_float(w.y); f[6] = __uint_as_float(w.z); f[7] = __uint_as_float(w.w);
-    return;
-  }
+// Eight numbers as they come: one or two 16-byte vectors
+template <typename T> struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+};
+template <typename T> __device__ __forceinline__ Raw8<T> load8(const T* p, bool vec) {
+  Raw8<T> r;
+  if (vec) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = (float)p[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = ldg_act(p + 8 / (sizeof(T) / 2) * i);
+  } else {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(t)[i];
+  }
+  return r;
+}
+template <typename T> __device__ __forceinline__ void numbers_of(const Raw8<T>& r, float* f) {
+  if constexpr (sizeof(T) == 2) {
+    unpack8(r.u[0], f);
+  } else {
+    f[0] = __uint_as_float(r.u[0].x); f[1] = __uint_as_float(r.u[0].y); f[2] = __uint_as_float(r.u[0].z); f[3] = __uint_as_float(r.u[0].w);
+    f[4] = __uint_as_float(r.u[1].x); f[5] = __uint_as_float(r.u[1].y); f[6] = __uint_as_float(r.u[1].z); f[7] = __uint_as_float(r.u[1].w);
+  }
+}
+// The largest magnitude's bits: of fp32 numbers, or of bf16 ones in both halves (as whole numbers NaN is above infinity and that above the rest)
+template <typename T> __device__ __forceinline__ uint32_t most_of(const Raw8<T>& r, uint32_t m) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    const uint32_t w[4] = {r.u[i].x, r.u[i].y, r.u[i].z, r.u[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 2) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+      else m = max(m, w[j] & 0x7fffffffu);
+    }
+  }
+  return m;
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, bool vec, const float* f) {
   if constexpr (sizeof(T) == 2) {
@@ -46,113 +71,144 @@ template <typename T> __device__ __forceinline__ void store8(T* p, bool vec, con
   for (int i = 0; i < 8; ++i) p[i] = (T)f[i];
 }
 
-// max over the 1 << bits lanes of a group
-__device__ __forceinline__ uint32_t group_max(uint32_t v, int bits) {
-  for (int o = (1 << bits) >> 1; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float group_sum(float v, int bits) {
-  for (int o = (1 << bits) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// A lane's eight codes, given the head's largest magnitude as bits, and the scale
-template <bool INT8> __device__ __forceinline__ uint2 codes8(const float* x, uint32_t top, float& scale) {
-  if (top >= 0x7f800000u) {                                        // an infinity or NaN is among them
-    scale = __uint_as_float(0x7fc00000u);
-    return make_uint2(0u, 0u);
+// How a head's numbers become codes, by its largest magnitude
+template <bool INT8> struct Coder {
+  float scale, f, y, as;                                           // scale NaN: codes are 0
+  bool last;
+  __device__ __forceinline__ explicit Coder(float largest) {
+    if (!(largest <= 3.402823466e38f)) {                           // an infinity or NaN is among them
+      scale = __uint_as_float(0x7fc00000u);
+      f = y = as = 0.f;
+      last = false;
+      return;
+    }
+    const float a = fmaxf(largest, LEAST);
+    const int e = (int)(__float_as_uint(a) >> 23) - 127;           // a = 1.m 2^e, -100 <= e <= 127
+    if constexpr (INT8) {
+      // 127 x / a, correctly rounded (a quotient's estimate and one correction by its exact remainder), so that a tie is a tie: x = a / 2 is 63.5 whatever 1 / a rounds to.
+      // Both sides are divided by 128 and by a power of two near a, which is exact and keeps 127 x and 1 / a among the normal numbers.
+      const float down = __uint_as_float((uint32_t)(127 - min(e, 126)) << 23);
+      scale = a / 127.f;
+      as = a * down;
+      y = __frcp_rn(as);
+      f = down * (127.f / 128.f);
+      last = false;
+    } else {
+      const int s = e - 8 + ((__float_as_uint(a) & 0x7fffffu) > 0x600000u);            // 448 = 1.75 * 2^8
+      scale = __uint_as_float((uint32_t)(127 + s) << 23);
+      f = __uint_as_float((uint32_t)(127 - s) << 23);
+      last = s == 120;
+    }
   }
-  const float a = fmaxf(__uint_as_float(top), LEAST);
-  const int e = (int)(__float_as_uint(a) >> 23) - 127;             // a = 1.m 2^e, -100 <= e <= 127
-  uint2 r;
-  if constexpr (INT8) {
-    scale = a / 127.f;
-    // 127 x / a, correctly rounded (a quotient's estimate and one correction by its exact remainder), so that a tie is a tie: x = a / 2 is 63.5 whatever 1 / a rounds to.
-    // Both sides are divided by 128 and by a power of two near a, which is exact and keeps 127 x and 1 / a among the normal numbers.
-    const float down = __uint_as_float((uint32_t)(127 - min(e, 126)) << 23), as = a * down, y = __frcp_rn(as), f = down * (127.f / 128.f);
+  __device__ __forceinline__ uint2 operator()(const float* x) const {
     uint32_t c[8];
+    if constexpr (INT8) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float n = x[i] * f, q = n * y;
-      c[i] = (uint32_t)__float2int_rn(fmaf(fmaf(-as, q, n), y, q) * 128.f);
-    }
-    r.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-    r.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-  } else {
-    const int s = e - 8 + ((__float_as_uint(a) & 0x7fffffu) > 0x600000u);   // 448 = 1.75 * 2^8
-    scale = __uint_as_float((uint32_t)(127 + s) << 23);
-    const float inv = __uint_as_float((uint32_t)(127 - s) << 23);
-    uint32_t c[4];
+      for (int i = 0; i < 8; ++i) {                                // (the sum's lowest bits are the rounded number: as = 0 gives 0)
+        const float n = x[i] * f, q = n * y;
+        c[i] = __float_as_uint(fmaf(fmaf(fmaf(-as, q, n), y, q), 128.f, 12582912.f));
+      }
+      if (as == 0.f) return make_uint2(0u, 0u);
+      return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                        __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 y = make_float2(x[2 * i] * inv, x[2 * i + 1] * inv);
-      if (s == 120) y = make_float2(fminf(fmaxf(y.x, -240.f), 240.f), fminf(fmaxf(y.y, -240.f), 240.f));   // (256 would read back as 2^128)
-      c[i] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+      for (int i = 0; i < 4; ++i) {
+        float2 t = make_float2(x[2 * i] * f, x[2 * i + 1] * f);
+        if (last) t = make_float2(fminf(fmaxf(t.x, -240.f), 240.f), fminf(fmaxf(t.y, -240.f), 240.f));   // (256 would read back as 2^128)
+        c[i] = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
+      }
+      if (f == 0.f) return make_uint2(0u, 0u);
+      return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
     }
-    r.x = c[0] | c[1] << 16;
-    r.y = c[2] | c[3] << 16;
   }
-  return r;
-}
+};
+
+constexpr int NV = 4;                                              // vectors of eight neighbouring channels of a lane
 
 struct Side {
   const void* x;                                                   // rows of activations (store) or where they go (load)
   long long ld;
   Cache8 c;
-  int bits, vec, norm;                                             // lanes of a head as a power of two; rows are whole 16-byte vectors apart
+  int bits, vec, wide, norm;                                       // lanes of a head as a power of two; rows, and codes, are whole 16-byte vectors apart
 };
+struct Head {
+  bool there;
+  int row, g, lane, slot, pos;                                     // lane: of the head's
+};
+__device__ __forceinline__ Head head_of(const Side& s, int block, const int* meta, int M, int G) {
+  Head h;
+  const unsigned i = block * (THREADS >> s.bits) + (threadIdx.x >> s.bits);
+  h.there = i < (unsigned)M * G;
+  h.row = h.there ? i / (unsigned)G : 0;
+  h.g = h.there ? i - h.row * (unsigned)G : 0;
+  h.lane = threadIdx.x & ((1 << s.bits) - 1);
+  h.slot = h.there ? meta[2ll * h.row] : -1;
+  h.pos = h.there ? meta[2ll * h.row + 1] : -1;
+  return h;
+}
 
 // Grid: blocks of heads of k and, behind them, of v
-template <typename T, bool INT8, int NV>
+template <typename T, bool INT8>
 __global__ void __launch_bounds__(THREADS) kv_store_8bit_kernel(Side k, Side v, const int* __restrict__ meta, int M, int G, int k_blocks, float eps) {
   pdl_launch_dependents();
   pdl_wait();
   const bool is_v = (int)blockIdx.x >= k_blocks;
   const Side& s = is_v ? v : k;
-  const int lane = threadIdx.x & ((1 << s.bits) - 1);
-  const unsigned i = (is_v ? blockIdx.x - k_blocks : blockIdx.x) * (THREADS >> s.bits) + (threadIdx.x >> s.bits);
-  const bool there = i < (unsigned)M * G;
-  const int row = there ? i / (unsigned)G : 0, g = there ? i - row * G : 0;
-  const int2 at = make_int2(meta[2ll * row], meta[2ll * row + 1]);
-  const int vecs = s.c.dim >> 3;
-  const T* src = reinterpret_cast<const T*>(s.x) + row * s.ld + g * s.c.dim;
-  float x[NV][8];
-  uint32_t top = 0u;
-  float ss = 0.f;
+  const Head h = head_of(s, is_v ? blockIdx.x - k_blocks : blockIdx.x, meta, M, G);
+  const int vecs = s.c.dim >> 3, c0 = h.lane * NV;
+  const T* src = reinterpret_cast<const T*>(s.x) + h.row * s.ld + h.g * s.c.dim + c0 * 8;
+  Raw8<T> raw[NV];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    const int c = lane + (n << s.bits);
-    if (there && c < vecs) {
-      load8(src + c * 8, s.vec, x[n]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[n][j] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(x[n][j], x[n][j], ss);
+    if (h.there && c0 + n < vecs) raw[n] = load8(src + n * 8, s.vec);
+    else raw[n] = Raw8<T>{};
   }
+  uint32_t most = 0u;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) most = most_of(raw[n], most);
+  for (int o = (1 << s.bits) >> 1; o > 0; o >>= 1) {
+    const uint32_t m = __shfl_xor_sync(0xffffffffu, most, o);
+    most = sizeof(T) == 2 ? __vmaxu2(most, m) : max(most, m);
+  }
+  float largest = __uint_as_float(sizeof(T) == 2 ? max(most & 0xffffu, most >> 16) << 16 : most), inv = 1.f;
   if (s.norm) {
-    const float inv = 1.f / sqrtf(group_sum(ss, s.bits) / (float)s.c.dim + eps);
+    float ss = 0.f;
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+    for (int n = 0; n < NV; ++n) {
+      float x[8];
+      numbers_of(raw[n], x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[n][j] *= inv;
+      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+    }
+    for (int o = (1 << s.bits) >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    inv = 1.f / sqrtf(ss / (float)s.c.dim + eps);
+    largest *= inv;
   }
+  if (!s.c.holds(h.slot, h.pos)) return;
+  const Coder<INT8> code(largest);
+  uint8_t* dst = s.c.at(h.slot, h.pos, h.g) + c0 * 8;
 #pragma unroll
-  for (int n = 0; n < NV; ++n)
+  for (int n = 0; n < NV; n += 2) {
+    float x[8], y[8];
+    numbers_of(raw[n], x);
+    numbers_of(raw[n + 1], y);
+    if (s.norm) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[n][j]) & 0x7fffffffu);     // (as whole numbers: NaN above infinity above the rest)
-  top = group_max(top, s.bits);
-  if (!there || !s.c.holds(at.x, at.y)) return;
-  uint8_t* dst = s.c.at(at.x, at.y, g);
-  float scale;
-#pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int c = lane + (n << s.bits);
-    const uint2 r = codes8<INT8>(x[n], top, scale);
-    if (c < vecs) *reinterpret_cast<uint2*>(dst + c * 8) = r;
+      for (int j = 0; j < 8; ++j) {
+        x[j] *= inv;
+        y[j] *= inv;
+      }
+    }
+    const uint2 r = code(x), q = code(y);
+    if (s.wide && c0 + n + 1 < vecs) {
+      *reinterpret_cast<uint4*>(dst + n * 8) = make_uint4(r.x, r.y, q.x, q.y);
+    } else {
+      if (c0 + n < vecs) *reinterpret_cast<uint2*>(dst + n * 8) = r;
+      if (c0 + n + 1 < vecs) *reinterpret_cast<uint2*>(dst + n * 8 + 8) = q;
+    }
   }
-  if (lane == 0) s.c.scale_at(at.x, g)[at.y] = scale;
+  if (h.lane == 0) s.c.scale_at(h.slot, h.g)[h.pos] = code.scale;
 }
 
 template <bool INT8> __device__ __forceinline__ void numbers8(const uint2& u, float scale, float* f) {
@@ -179,30 +235,42 @@ __global__ void __launch_bounds__(THREADS) kv_load_8bit_kernel(Side k, Side v, c
   pdl_wait();
   const bool is_v = (int)blockIdx.x >= k_blocks;
   const Side& s = is_v ? v : k;
-  const int lane = threadIdx.x & ((1 << s.bits) - 1);
-  const unsigned i = (is_v ? blockIdx.x - k_blocks : blockIdx.x) * (THREADS >> s.bits) + (threadIdx.x >> s.bits);
-  if (i >= (unsigned)M * G) return;
-  const int row = i / (unsigned)G, g = i - row * G;
-  const int2 at = make_int2(meta[2ll * row], meta[2ll * row + 1]);
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(s.x)) + row * s.ld + g * s.c.dim;
-  const bool held = s.c.holds(at.x, at.y);
-  const uint8_t* src = held ? s.c.at(at.x, at.y, g) : nullptr;
-  const float scale = held ? s.c.scale_at(at.x, g)[at.y] : __uint_as_float(0x7fc00000u);
-  for (int c = lane; c < s.c.dim >> 3; c += 1 << s.bits) {
+  const Head h = head_of(s, is_v ? blockIdx.x - k_blocks : blockIdx.x, meta, M, G);
+  if (!h.there) return;
+  const int vecs = s.c.dim >> 3, c0 = h.lane * NV;
+  const bool held = s.c.holds(h.slot, h.pos);
+  const uint8_t* src = held ? s.c.at(h.slot, h.pos, h.g) + c0 * 8 : nullptr;
+  const float scale = held ? __ldcg(s.c.scale_at(h.slot, h.g) + h.pos) : __uint_as_float(0x7fc00000u);
+  uint2 codes[NV];
+#pragma unroll
+  for (int n = 0; n < NV; n += 2) {
+    codes[n] = codes[n + 1] = make_uint2(0u, 0u);
+    if (held && s.wide && c0 + n + 1 < vecs) {
+      const uint4 u = ldg_act(src + n * 8);
+      codes[n] = make_uint2(u.x, u.y);
+      codes[n + 1] = make_uint2(u.z, u.w);
+    } else if (held) {
+      if (c0 + n < vecs) codes[n] = __ldcg(reinterpret_cast<const uint2*>(src + n * 8));
+      if (c0 + n + 1 < vecs) codes[n + 1] = __ldcg(reinterpret_cast<const uint2*>(src + n * 8 + 8));
+    }
+  }
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(s.x)) + h.row * s.ld + h.g * s.c.dim + c0 * 8;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
     float f[8];
-    numbers8<INT8>(held ? *reinterpret_cast<const uint2*>(src + c * 8) : make_uint2(0u, 0u), scale, f);
-    store8(dst + c * 8, s.vec, f);
+    numbers8<INT8>(codes[n], scale, f);
+    if (c0 + n < vecs) store8(dst + n * 8, s.vec, f);
   }
 }
 
 Side make_side(const void* x, long long ld, int act_f32, const LiaCacheView* view, int norm) {
-  Side s{x, ld, cache8(view), 0, 0, norm};
-  const int vecs = view->dim / 8;
-  while ((1 << s.bits) < vecs && s.bits < 5) ++s.bits;
-  const int per = act_f32 ? 4 : 8;
-  s.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld % per == 0;
+  Side s{x, ld, cache8(view), 0, 0, 0, norm};
+  while ((NV << s.bits) < view->dim / 8) ++s.bits;                 // (5 at most: 1024 channels)
+  s.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld % (act_f32 ? 4 : 8) == 0;
+  s.wide = cache8_wrong(view, 16) == nullptr;
   return s;
 }
+int head_blocks(const Side& s, int M, int G) { return (int)((((long long)M * G << s.bits) + THREADS - 1) / THREADS); }
 
 const char* sides_wrong(const void* k, const void* v, const void* meta, const LiaCacheView* kc, const LiaCacheView* vc, long long ldk, long long ldv, int M, int G) {
   const char* w = nullptr;
@@ -216,8 +284,6 @@ const char* sides_wrong(const void* k, const void* v, const void* meta, const Li
   return w;
 }
 
-long long head_blocks(const Side& s, int M, int G) { return (((long long)M * G << s.bits) + THREADS - 1) / THREADS; }   // (at most 2^28)
-
 }  // namespace
 
 extern "C" int lia_kv_store_8bit(const void* k, long long ldk, const void* v, long long ldv, int act_f32, const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, int M, int G,
@@ -226,19 +292,11 @@ extern "C" int lia_kv_store_8bit(const void* k, long long ldk, const void* v, lo
   LIA_CHECK_ARG(!wrong, "lia_kv_store_8bit: %s", wrong);
   if (M == 0) return LIA_OK;
   const Side a = make_side(k, ldk, act_f32, kc, 0), b = make_side(v, ldv, act_f32, vc, norm_values != 0);
-  const long long ka = head_blocks(a, M, G), blocks = ka + head_blocks(b, M, G);
-  const int widest = kc->dim > vc->dim ? kc->dim : vc->dim;
-  auto go = [&](auto kernel) {
-    return lia_launch(kernel, dim3((unsigned)blocks), dim3(THREADS), 0, reinterpret_cast<cudaStream_t>(stream), a, b, meta, M, G, (int)ka, eps);
-  };
+  const int ka = head_blocks(a, M, G), blocks = ka + head_blocks(b, M, G);
+  auto go = [&](auto kernel) { return lia_launch(kernel, dim3(blocks), dim3(THREADS), 0, reinterpret_cast<cudaStream_t>(stream), a, b, meta, M, G, ka, eps); };
   const bool i8 = kc->type == LIA_CACHE_INT8;
-  if (widest <= 256) {                                             // one vector a lane
-    if (act_f32) LIA_CUDA(i8 ? go(kv_store_8bit_kernel<float, true, 1>) : go(kv_store_8bit_kernel<float, false, 1>));
-    else LIA_CUDA(i8 ? go(kv_store_8bit_kernel<bf16, true, 1>) : go(kv_store_8bit_kernel<bf16, false, 1>));
-  } else {
-    if (act_f32) LIA_CUDA(i8 ? go(kv_store_8bit_kernel<float, true, 4>) : go(kv_store_8bit_kernel<float, false, 4>));
-    else LIA_CUDA(i8 ? go(kv_store_8bit_kernel<bf16, true, 4>) : go(kv_store_8bit_kernel<bf16, false, 4>));
-  }
+  if (act_f32) LIA_CUDA(i8 ? go(kv_store_8bit_kernel<float, true>) : go(kv_store_8bit_kernel<float, false>));
+  else LIA_CUDA(i8 ? go(kv_store_8bit_kernel<bf16, true>) : go(kv_store_8bit_kernel<bf16, false>));
   return LIA_OK;
 }
 
@@ -248,10 +306,8 @@ extern "C" int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const L
   LIA_CHECK_ARG(!wrong, "lia_kv_load_8bit: %s", wrong);
   if (M == 0) return LIA_OK;
   const Side a = make_side(k, ldk, out_f32, kc, 0), b = make_side(v, ldv, out_f32, vc, 0);
-  const long long ka = head_blocks(a, M, G), blocks = ka + head_blocks(b, M, G);
-  auto go = [&](auto kernel) {
-    return lia_launch(kernel, dim3((unsigned)blocks), dim3(THREADS), 0, reinterpret_cast<cudaStream_t>(stream), a, b, meta, M, G, (int)ka);
-  };
+  const int ka = head_blocks(a, M, G), blocks = ka + head_blocks(b, M, G);
+  auto go = [&](auto kernel) { return lia_launch(kernel, dim3(blocks), dim3(THREADS), 0, reinterpret_cast<cudaStream_t>(stream), a, b, meta, M, G, ka); };
   const bool i8 = kc->type == LIA_CACHE_INT8;
   if (out_f32) LIA_CUDA(i8 ? go(kv_load_8bit_kernel<float, true>) : go(kv_load_8bit_kernel<float, false>));
   else LIA_CUDA(i8 ? go(kv_load_8bit_kernel<bf16, true>) : go(kv_load_8bit_kernel<bf16, false>));

@@ -6,9 +6,9 @@
 // found from what that leaves: the top-th largest of the 256 threads' maxima is reached by at least `top` logits and, as the largest ones seldom share a thread, by few more; the threads
 // that have one are known by their maxima, so that only their logits are read again (a tenth of the row, from L2), by all lanes of their warps.  What reaches the bound is sorted across a warp's lanes,
 // as whole numbers that order by value and then by lower id.  (A list of the largest ones kept by every warp through the pass took 34 instructions a logit instead of 7.)
-// Few rows share out a row's blocks over several blocks of threads, and a second kernel joins the parts (in the same order each time).
+// Few rows share out a row over a cluster of up to eight blocks of threads, whose first one joins the parts (in the same order each time).
 //
-// Memory bounds it for many rows (a logit is read once, eight instructions each), the latency of one block of logits and two launches for few.
+// Memory bounds it for many rows (a logit is read once, eight instructions each), the latency of one block of logits and of sorting for few.
 #include "pairs.cuh"
 
 namespace {
@@ -97,8 +97,6 @@ struct Args {
   const long long* tokens;
   float *logp, *entropy, *top_logp;
   long long* top_ids;
-  Sums* part_sums;                                                 // [M][splits], then
-  u64* part_lists;                                                 // [M][splits][32]
 };
 
 __device__ __forceinline__ float logit(const float* p) { return *p; }
@@ -265,79 +263,60 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   for (int o = 16; o > 0; o >>= 1) join(s, from_lane(s, o));
   if (lane == 0) warp_sums[warp] = s;
   __syncthreads();
-  if (warp != 0) return;
-  s = warp_sums[0];
-  for (int w = 1; w < WARPS; ++w) join(s, warp_sums[w]);
-  if (a.splits == 1) {
-    finish<T>(a, row, s, list, lane);
-  } else {
-    if (lane == 0) a.part_sums[blockIdx.x] = s;
-    if (a.top > 0) a.part_lists[(long long)blockIdx.x * 32 + 31 - lane] = list;         // rising
+  if (warp == 0) {
+    s = warp_sums[0];
+    for (int w = 1; w < WARPS; ++w) join(s, warp_sums[w]);
   }
-}
-
-// The parts of a row, a few by each of four warps, always in the same order
-template <typename T>
-__global__ void __launch_bounds__(128) token_logprobs_join_kernel(const Args a) {
-  __shared__ u64 lists[4][32];
-  __shared__ Sums sums[4];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long at = (long long)row * a.splits;
-  Sums s{-INFINITY, 0.f, 0.f};
-  u64 list = 0;
-  for (int i = warp; i < a.splits; i += 16) {
-    u64 part[4];
-    Sums q[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool there = i + j * 4 < a.splits;
-      part[j] = there && a.top > 0 ? a.part_lists[(at + i + j * 4) * 32 + lane] : 0;
-      q[j] = there ? a.part_sums[at + i + j * 4] : Sums{-INFINITY, 0.f, 0.f};
+  if (a.splits > 1) {                                              // the row's other blocks are the cluster's: the first one fetches their parts, a warp each
+    __syncthreads();                                               // (the sums and lists of the warps have been read)
+    if (warp == 0) {
+      if (lane == 0) warp_sums[0] = s;
+      lists[0][lane] = list;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      join(s, q[j]);
-      if (a.top > 0 && i + j * 4 < a.splits) list = merge_down(list, part[j], lane);
+    cluster_barrier();
+    if (split == 0) {
+      list = 0;
+      s = {-INFINITY, 0.f, 0.f};
+      if (warp < a.splits) {
+        const float4 q = cluster_ld_f4(cluster_place(&warp_sums[0], warp));
+        s = {q.x, q.y, q.z};
+        if (a.top > 0) list = cluster_ld64(cluster_place(&lists[0][lane], warp));
+      }
+      __syncthreads();                                             // (its own part among them)
+      if (lane == 0) warp_sums[warp] = s;
+      if (a.top > 0) list = join_lists<WARPS>(list, lists, warp, lane);
+      __syncthreads();
+      if (warp == 0) {
+        s = warp_sums[0];
+        for (int w = 1; w < a.splits; ++w) join(s, warp_sums[w]);
+      }
     }
   }
-  if (lane == 0) sums[warp] = s;
-  list = join_lists<4>(list, lists, warp, lane);
-  if (warp != 0) return;
-  for (int w = 1; w < 4; ++w) join(s, sums[w]);
-  finish<T>(a, row, s, list, lane);
+  if (warp == 0 && split == 0) finish<T>(a, row, s, list, lane);
+  if (a.splits > 1) cluster_barrier();                             // (no block leaves while it is read)
 }
 
-// Blocks of threads of a row: as many as fill the GPU four blocks an SM, none with less than one block of logits a warp
-int splits_of(int M, int V, int act_f32) {
-  const int per = WARPS * 512, most = (V + per - 1) / per, want = 4 * lia_sm_count() / M;
-  (void)act_f32;
-  return want < 1 ? 1 : want < most ? want : most;
+// Blocks of threads of a row, one cluster of them: 1, 2, 4 or 8, as many as fill the GPU four blocks an SM, none with less than a block of logits a warp
+int splits_of(int M, int V) {
+  int s = WARPS;
+  while (s > 1 && ((long long)s * M > 4 * lia_sm_count() || s * WARPS * 512 > V + WARPS * 512)) s /= 2;
+  return s;
 }
-size_t floats_of(int M, int splits) { return splits > 1 ? (size_t)M * splits * (4 + 64) : 0; }
 
 }  // namespace
 
-extern "C" size_t lia_token_logprobs_workspace_floats(int M, int V, int act_f32) { return M > 0 && V > 0 ? floats_of(M, splits_of(M, V, act_f32)) : 0; }
-
 extern "C" int lia_token_logprobs(const void* logits, int act_f32, long long ld, int M, int V, const int64_t* tokens, int n, float* logp, float* entropy, int top, float* top_logp,
-                                  int64_t* top_ids, float* ws, size_t ws_floats, lia_stream_t stream_) {
+                                  int64_t* top_ids, lia_stream_t stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   LIA_CHECK_ARG(M >= 0 && V > 0 && V < (1 << 30) && ld >= V && top >= 0 && top <= MAX_TOP && top <= V && n >= 0, "lia_token_logprobs: bad sizes (top is at most %d and V)", MAX_TOP);
   if (M == 0) return LIA_OK;
   LIA_CHECK_ARG(logits && entropy && (n == 0 || (tokens && logp)) && (top == 0 || (top_logp && top_ids)), "lia_token_logprobs: null pointer");
   LIA_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % (act_f32 ? 4 : 2) == 0, "lia_token_logprobs: misaligned logits");
-  const int splits = splits_of(M, V, act_f32);
-  LIA_CHECK_ARG(splits == 1 || (ws && ws_floats >= floats_of(M, splits) && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_token_logprobs: needs a workspace of %zu floats", floats_of(M, splits));
-  LIA_CHECK_ARG((long long)M * splits < (1ll << 31), "lia_token_logprobs: too many rows");
-  Args a{logits, ld, M, V, splits, top, n, reinterpret_cast<const long long*>(tokens), logp, entropy, top_logp, reinterpret_cast<long long*>(top_ids), reinterpret_cast<Sums*>(ws),
-         reinterpret_cast<u64*>(ws + (size_t)M * splits * 4)};
-  if (act_f32) LIA_CUDA(lia_launch(token_logprobs_kernel<float>, dim3(M * splits), dim3(THREADS), 0, stream, a));
-  else LIA_CUDA(lia_launch(token_logprobs_kernel<bf16>, dim3(M * splits), dim3(THREADS), 0, stream, a));
-  if (splits > 1) {
-    if (act_f32) LIA_CUDA(lia_launch(token_logprobs_join_kernel<float>, dim3(M), dim3(128), 0, stream, a));
-    else LIA_CUDA(lia_launch(token_logprobs_join_kernel<bf16>, dim3(M), dim3(128), 0, stream, a));
-  }
+  const int splits = splits_of(M, V);
+  const Args a{logits, ld, M, V, splits, top, n, reinterpret_cast<const long long*>(tokens), logp, entropy, top_logp, reinterpret_cast<long long*>(top_ids)};
+  auto go = [&](auto kernel) {
+    return splits == 1 ? lia_launch(kernel, dim3(M), dim3(THREADS), 0, stream, a) : lia_launch_cluster(splits, kernel, dim3(M * splits), dim3(THREADS), 0, stream, a);
+  };
+  LIA_CUDA(act_f32 ? go(token_logprobs_kernel<float>) : go(token_logprobs_kernel<bf16>));
   return LIA_OK;
 }

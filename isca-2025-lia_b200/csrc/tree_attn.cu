@@ -43,7 +43,7 @@ struct Shape {
   static constexpr int ROWS = 8 * NR;
   static constexpr int Q_BYTES = NR * STEPS * 32 * 8, O_BYTES = WARPS * ROWS * VDIM * 4, BIG = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
   static constexpr int SMEM = BIG + ROWS * 4 + WARPS * ROWS * 8;
-  static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // weights are 2^(x - maximum + LIFT): below 2^15 in fp16
+  static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // a weight of the maximum is 2^LIFT, one that is just not outgrown 2^15 in fp16
   // the channel of the first of a lane's pair in the i-th product with the values
   static __device__ __forceinline__ int channel(int i, int gq) { return BITS8 ? gq * (VDIM / 8) + 2 * i : (i >> 2) * 64 + gq * 8 + (i & 3) * 2; }
 };
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     if (a.splits == 1 && blockIdx.y == 0) nan_rows<VDIM>(a, p);
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t4 = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, gq = lane >> 2, t4 = lane & 3;   // (known to be the same in all lanes)
   const int tile = blockIdx.y / a.G, g = blockIdx.y - tile * a.G, r0 = tile * S::ROWS, R = p.n * a.rep;
   if (r0 >= R) return;
 
@@ -249,12 +249,12 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
           }
         }
     }
-    // ---- the maximum moves only for rows that have outgrown it
+    // ---- the maximum (m: less LIFT) moves only for rows that have outgrown it
     bool grown = false;
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) grown |= s[r][e] > m[r][e & 1] + SLACK;
+      for (int e = 0; e < 4; ++e) grown |= s[r][e] - m[r][e & 1] > SLACK + S::LIFT;
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
       for (int r = 0; r < NR; ++r)
@@ -263,9 +263,9 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
           float top = fmaxf(s[r][e], s[r][2 + e]);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          const bool up = top > m[r][e] + SLACK;
-          const float keep = up ? ex2(m[r][e] - top) : 1.f;
-          if (up) m[r][e] = top;
+          const bool up = top - m[r][e] > SLACK + S::LIFT;
+          const float keep = up ? ex2(m[r][e] - (top - S::LIFT)) : 1.f;
+          if (up) m[r][e] = top - S::LIFT;
           l[r][e] *= keep;
 #pragma unroll
           for (int n = 0; n < S::MT; ++n) {
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
       float w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        w[e] = ex2(s[r][e] - m[r][e & 1] + S::LIFT);
+        w[e] = ex2(s[r][e] - m[r][e & 1]);
         l[r][e & 1] = BITS8 ? fmaf(w[e], rv[e >> 1], l[r][e & 1]) : l[r][e & 1] + w[e];
       }
 #pragma unroll

@@ -1397,49 +1397,60 @@ def rglru_scan(u, z, z_bias, c, y, y_bias, state, segs, blocks, out):
 _CACHE_TYPES = {BF16: _lib.CACHE_BF16, torch.int8: _lib.CACHE_INT8, torch.float8_e4m3fn: _lib.CACHE_E4M3}
 
 
-def _here(t, name, dtype):
-    """A tensor of ``dtype`` on the current device, where the kernel will run."""
-    if t.dtype != dtype or not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
-        raise _lib.LiaError(f"{name}: need a {dtype} tensor on the current CUDA device, got {t.dtype} on {t.device}")
-    return t
+def _device(t, what):
+    """The number of a tensor's device, which has to be the current one: the kernel will run there."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise _lib.LiaError(f"{what}: need tensors on the current CUDA device, got one on {t.device}")
+    return dev
 
 
-def _cache_view(what, name, cache, scale, heads, dim):
+def _need(t, dtype, shape, dev, what):
+    """The address of a contiguous tensor of that shape."""
+    if t.dtype is not dtype or t.get_device() != dev or tuple(t.shape) != shape or not t.is_contiguous():
+        raise _lib.LiaError(f"{what}: need a contiguous {dtype} {list(shape)} tensor on the current CUDA device, got {t.dtype} {list(t.shape)} on {t.device}, strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _rows_of(t, dtype, shape, dev, what):
+    """The same for rows that may lie apart: (address, numbers from row to row)."""
+    strides = t.stride()
+    if t.dtype is not dtype or t.get_device() != dev or tuple(t.shape) != shape or (strides[1] != 1 and shape[1] != 1):
+        raise _lib.LiaError(f"{what}: need a {dtype} {list(shape)} tensor with neighbouring columns on the current CUDA device, got {t.dtype} {list(t.shape)} on {t.device}, strides {strides}")
+    return t.data_ptr(), strides[0] if shape[0] > 1 else shape[1]
+
+
+def _cache_view(what, cache, scale, heads, dim, dev):
     """A cache [slots, capacity, heads * dim] or [slots, capacity, heads, dim] with neighbouring channels (any strides else) and its scales [slots, heads, capacity]."""
-    kind = _CACHE_TYPES.get(cache.dtype)
-    if kind is None:
-        raise _lib.LiaError(f"{what}: {name} has to be bf16, int8 or float8_e4m3fn, not {cache.dtype}")
-    _here(cache, f"{what}: {name}", cache.dtype)
     shape, strides = cache.shape, cache.stride()
+    kind = _CACHE_TYPES.get(cache.dtype)
+    if kind is None or cache.get_device() != dev:
+        raise _lib.LiaError(f"{what} has to be bf16, int8 or float8_e4m3fn on the current CUDA device, not {cache.dtype} on {cache.device}")
     if len(shape) == 3 and shape[2] == heads * dim:
         head = dim
     elif len(shape) == 4 and shape[2] == heads and shape[3] == dim:
         head = strides[2]
     else:
-        raise _lib.LiaError(f"{what}: {name} has to be [slots, capacity, {heads} * {dim}] or [slots, capacity, {heads}, {dim}], not {tuple(shape)}")
+        raise _lib.LiaError(f"{what} has to be [slots, capacity, {heads} * {dim}] or [slots, capacity, {heads}, {dim}], not {tuple(shape)}")
+    slots, capacity = shape[0], shape[1]
     if strides[-1] != 1:
-        raise _lib.LiaError(f"{what}: {name}'s channels have to be neighbours, strides are {strides}")
+        raise _lib.LiaError(f"{what}: its channels have to be neighbours, strides are {strides}")
     if kind == _lib.CACHE_BF16:
         if scale is not None:
-            raise _lib.LiaError(f"{what}: a bf16 cache has no scales")
-        return _lib.LiaCacheView(cache.data_ptr(), None, strides[0], strides[1], head, 0, 0, shape[0], shape[1], kind, dim)
-    if scale is None or tuple(scale.shape) != (shape[0], heads, shape[1]) or (shape[1] > 1 and scale.stride(2) != 1):
-        raise _lib.LiaError(f"{what}: {name} of 8 bits needs scales [slots, {heads}, capacity] with neighbouring positions")
-    _here(scale, f"{what}: scales of {name}", F32)
-    return _lib.LiaCacheView(cache.data_ptr(), scale.data_ptr(), strides[0], strides[1], head, scale.stride(0), scale.stride(1), shape[0], shape[1], kind, dim)
+            raise _lib.LiaError(f"{what} is bf16, which has no scales")
+        return _lib.LiaCacheView(cache.data_ptr(), None, strides[0], strides[1], head, 0, 0, slots, capacity, kind, dim)
+    if scale is None or scale.dtype is not F32 or scale.get_device() != dev or tuple(scale.shape) != (slots, heads, capacity):
+        raise _lib.LiaError(f"{what} is of 8 bits and needs fp32 scales [slots, {heads}, capacity] on the current CUDA device")
+    apart = scale.stride()
+    if capacity > 1 and apart[2] != 1:
+        raise _lib.LiaError(f"{what}: the positions of its scales have to be neighbours, strides are {apart}")
+    return _lib.LiaCacheView(cache.data_ptr(), scale.data_ptr(), strides[0], strides[1], head, apart[0], apart[1], slots, capacity, kind, dim)
 
 
 def _cache_rows(what, k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim):
-    ldk, ldv = _rowmajor(k, f"{what}: k"), _rowmajor(v, f"{what}: v")
-    f32 = _f32(k)
-    _here(k, f"{what}: k", k.dtype)
-    _here(v, f"{what}: v", k.dtype)
-    M = k.shape[0]
-    if k.shape[1] != G * dim or tuple(v.shape) != (M, G * vdim):
-        raise _lib.LiaError(f"{what}: k and v have to be [rows, {G} * {dim}] and [rows, {G} * {vdim}], not {tuple(k.shape)} and {tuple(v.shape)}")
-    if tuple(_here(meta, f"{what}: meta", I32).shape) != (M, 2) or not meta.is_contiguous():
-        raise _lib.LiaError(f"{what}: meta has to be a contiguous int32 [rows, 2] tensor")
-    return ldk, ldv, f32, M, _cache_view(what, "kcache", kcache, k_scale, G, dim), _cache_view(what, "vcache", vcache, v_scale, G, vdim)
+    dev, M, f32 = _device(k, what), k.shape[0], _f32(k)
+    return (*_rows_of(k, k.dtype, (M, G * dim), dev, what), *_rows_of(v, k.dtype, (M, G * vdim), dev, what), f32, _need(meta, I32, (M, 2), dev, what),
+            _cache_view(f"{what}: kcache", kcache, k_scale, G, dim, dev), _cache_view(f"{what}: vcache", vcache, v_scale, G, vdim, dev), M)
 
 
 def kv_store_8bit(k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim, eps=0.0, norm_values=False):
@@ -1447,16 +1458,16 @@ def kv_store_8bit(k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim, ep
     in ``meta``, with one scale for each head of each row in ``k_scale`` / ``v_scale`` [slots, G, capacity]: code * scale is the number.  int8: the largest magnitude a of the head is
     127, code = round(127 x / a); e4m3: scale is the least power of two with a / scale <= 448.  A head that holds an infinity or NaN reads back as NaN.  ``norm_values``: values are
     divided by their head's root mean square first (sqrt(mean + eps)).  Rows whose slot or position the caches lack are left out; no two rows may name one place."""
-    ldk, ldv, f32, M, kc, vc = _cache_rows("kv_store_8bit", k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim)
-    check(_lib.load().lia_kv_store_8bit(k.data_ptr(), ldk, v.data_ptr(), ldv, f32, meta.data_ptr(), kc, vc, M, G, eps, norm_values, _stream()), "lia_kv_store_8bit")
+    kp, ldk, vp, ldv, f32, at, kc, vc, M = _cache_rows("kv_store_8bit", k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim)
+    check(_lib.load().lia_kv_store_8bit(kp, ldk, vp, ldv, f32, at, kc, vc, M, G, eps, norm_values, _stream()), "lia_kv_store_8bit")
     count_launches()
 
 
 def kv_load_8bit(meta, kcache, vcache, k_scale, v_scale, k, v, G, dim, vdim):
     """The rows at ``meta`` of 8-bit caches as numbers, code * scale rounded once, into ``k`` [M, G * dim] and ``v`` [M, G * vdim] (bf16 or fp32; column slices are fine).  NaN for a
     row whose slot or position the caches lack."""
-    ldk, ldv, f32, M, kc, vc = _cache_rows("kv_load_8bit", k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim)
-    check(_lib.load().lia_kv_load_8bit(meta.data_ptr(), kc, vc, k.data_ptr(), ldk, v.data_ptr(), ldv, f32, M, G, _stream()), "lia_kv_load_8bit")
+    kp, ldk, vp, ldv, f32, at, kc, vc, M = _cache_rows("kv_load_8bit", k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim)
+    check(_lib.load().lia_kv_load_8bit(at, kc, vc, kp, ldk, vp, ldv, f32, M, G, _stream()), "lia_kv_load_8bit")
     count_launches()
 
 
@@ -1471,29 +1482,22 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
     neighbouring channels; heads of 64 or 128 channels.  ``q`` [M, H * dim] and ``out`` [M, H * vdim] are bf16.  ``rows``: the most tokens of a portion; ``max_ctx``: the longest p0 + n,
     about (it decides how many blocks share a history, not what is read).  A row that sees nothing is 0; rows of no portion are left as they are; a portion that does not fit its slot, the
     rows, ``rows`` or the mask's words gives NaN rows."""
-    ldq = _rowmajor(q, "tree_attn: q")
-    _here(q, "tree_attn: q", BF16)
-    _here(out, "tree_attn: out", BF16)
-    M = q.shape[0]
-    if q.shape[1] != H * dim or tuple(out.shape) != (M, H * vdim) or not out.is_contiguous():
-        raise _lib.LiaError(f"tree_attn: q has to be [M, {H} * {dim}] and out a contiguous [M, {H} * {vdim}] tensor, not {tuple(q.shape)} and {tuple(out.shape)}")
-    if segs.dim() != 2 or segs.shape[1] != 4 or not _here(segs, "tree_attn: segs", I32).is_contiguous():
-        raise _lib.LiaError("tree_attn: segs has to be a contiguous int32 [nseg, 4] tensor")
-    words = 0
+    dev, M, nseg = _device(q, "tree_attn"), q.shape[0], segs.shape[0]
+    qp, ldq = _rows_of(q, BF16, (M, H * dim), dev, "tree_attn: q")
+    op, sp = _need(out, BF16, (M, H * vdim), dev, "tree_attn: out"), _need(segs, I32, (nseg, 4), dev, "tree_attn: segs")
+    words, mp, dp, tp = 0, None, None, None
     if mask is not None:
-        if mask.dim() != 2 or mask.shape[0] != M or mask.shape[1] < 1 or not _here(mask, "tree_attn: mask", torch.int64).is_contiguous():
-            raise _lib.LiaError("tree_attn: mask has to be a contiguous int64 [M, words] tensor")
-        words = mask.shape[1]
-    if depth is not None and (tuple(_here(depth, "tree_attn: depth", I32).shape) != (M,) or not depth.is_contiguous()):
-        raise _lib.LiaError("tree_attn: depth has to be a contiguous int32 [M] tensor")
-    if temp is not None and (tuple(_here(temp, "tree_attn: temp", F32).shape) != (H,) or not temp.is_contiguous()):
-        raise _lib.LiaError("tree_attn: temp has to be a contiguous fp32 [H] tensor")
-    kc, vc = _cache_view("tree_attn", "kcache", kcache, k_scale, G, dim), _cache_view("tree_attn", "vcache", vcache, v_scale, G, vdim)
-    lib, nseg = _lib.load(), segs.shape[0]
+        words = mask.shape[-1]
+        mp = _need(mask, torch.int64, (M, words), dev, "tree_attn: mask")
+    if depth is not None:
+        dp = _need(depth, I32, (M,), dev, "tree_attn: depth")
+    if temp is not None:
+        tp = _need(temp, F32, (H,), dev, "tree_attn: temp")
+    kc, vc = _cache_view("tree_attn: kcache", kcache, k_scale, G, dim, dev), _cache_view("tree_attn: vcache", vcache, v_scale, G, vdim, dev)
+    lib = _lib.load()
     floats = lib.lia_tree_attn_workspace_floats(nseg, rows, max_ctx, M, H, G, dim, vdim, window, kc.type)
     ws = torch.empty(floats, dtype=F32, device=q.device) if floats else None
-    check(lib.lia_tree_attn(q.data_ptr(), ldq, kc, vc, segs.data_ptr(), nseg, _p(mask), words, _p(depth), _p(temp), out.data_ptr(), _p(ws), floats, M, H, G, rows, max_ctx, window, scale,
-                            softcap, _stream()), "lia_tree_attn")
+    check(lib.lia_tree_attn(qp, ldq, kc, vc, sp, nseg, mp, words, dp, tp, op, _p(ws), floats, M, H, G, rows, max_ctx, window, scale, softcap, _stream()), "lia_tree_attn")
     count_launches(2 if floats else 1)
     return out
 
@@ -1502,24 +1506,19 @@ def token_logprobs(logits, tokens=None, top=0):
     """Of every row of ``logits`` [M, V] (bf16 or fp32; rows may lie apart): the log probability of its ``tokens`` (int64 [M] or [M, n]; NaN for an id outside the vocabulary), the
     entropy of its distribution in nats, and its ``top`` <= 32 most likely tokens (csrc/token_logprobs.cu).  Returns (logp, entropy [M], top_logp [M, top], top_ids int64 [M, top]), fp32, logp
     in the shape of ``tokens`` (None without).  Of equal logits the lower id comes first; -inf are tokens of probability 0; a row with NaN or +inf, or of nothing but -inf, gives NaN."""
-    ld = _rowmajor(logits, "token_logprobs: logits")
-    f32 = _f32(logits)
-    _here(logits, "token_logprobs: logits", logits.dtype)
     M, V = logits.shape
-    dev, n, logp = logits.device, 0, None
+    dev, f32, n, logp, tp, lp = _device(logits, "token_logprobs"), _f32(logits), 0, None, None, None
+    xp, ld = _rows_of(logits, logits.dtype, (M, V), dev, "token_logprobs: logits")
     if not 0 <= top <= min(32, V):
         raise _lib.LiaError(f"token_logprobs: {top} alternatives of {V} tokens: at most 32, and no more than there are")
+    on = logits.device
     if tokens is not None:
-        if tokens.dim() not in (1, 2) or tokens.shape[0] != M or not _here(tokens, "token_logprobs: tokens", torch.int64).is_contiguous():
-            raise _lib.LiaError(f"token_logprobs: tokens have to be a contiguous int64 [{M}] or [{M}, n] tensor, not {tuple(tokens.shape)}")
-        n = 1 if tokens.dim() == 1 else tokens.shape[1]
-        logp = torch.empty(tokens.shape, dtype=F32, device=dev)
-    entropy, top_logp = torch.empty(M, dtype=F32, device=dev), torch.empty(M, top, dtype=F32, device=dev)
-    top_ids = torch.empty(M, top, dtype=torch.int64, device=dev)
-    lib = _lib.load()
-    floats = lib.lia_token_logprobs_workspace_floats(M, V, f32)
-    ws = torch.empty(floats, dtype=F32, device=dev) if floats else None
-    check(lib.lia_token_logprobs(logits.data_ptr(), f32, ld if M > 1 else V, M, V, _p(tokens), n, _p(logp), entropy.data_ptr(), top, top_logp.data_ptr(), top_ids.data_ptr(), _p(ws), floats,
-                                 _stream()), "lia_token_logprobs")
-    count_launches(2 if floats else 1)
+        shape = tuple(tokens.shape)
+        n = shape[1] if len(shape) == 2 else 1
+        tp = _need(tokens, torch.int64, (M, n) if len(shape) == 2 else (M,), dev, "token_logprobs: tokens")
+        logp = torch.empty(shape, dtype=F32, device=on)
+        lp = logp.data_ptr()
+    entropy, top_logp, top_ids = torch.empty(M, dtype=F32, device=on), torch.empty(M, top, dtype=F32, device=on), torch.empty(M, top, dtype=torch.int64, device=on)
+    check(_lib.load().lia_token_logprobs(xp, f32, ld, M, V, tp, n, lp, entropy.data_ptr(), top, top_logp.data_ptr(), top_ids.data_ptr(), _stream()), "lia_token_logprobs")
+    count_launches()
     return logp, entropy, top_logp, top_ids

@@ -78,10 +78,10 @@ def test_attention_of_nothing(lib):
 
 @pytest.mark.parametrize("args,message", [
     (dict(V=0), "sizes"), (dict(top=33), "sizes"), (dict(V=4, top=5), "sizes"), (dict(ld=99), "sizes"), (dict(n=-1), "sizes"), (dict(logits=None), "null"), (dict(logits=2), "misaligned"),
-    (dict(top=3, ids=None), "null"), (dict(n=1, tokens=None), "null"), (dict(V=50000, ld=50000), "workspace")])
+    (dict(top=3, ids=None), "null"), (dict(n=1, tokens=None), "null")])
 def test_logprobs_refuse(lib, args, message):
-    a = dict(logits=16, f32=1, ld=100, M=2, V=100, tokens=16, n=1, logp=16, entropy=16, top=0, best=16, ids=16, ws=None, floats=0) | args
-    rc = lib.load().lia_token_logprobs(a["logits"], a["f32"], a["ld"], a["M"], a["V"], a["tokens"], a["n"], a["logp"], a["entropy"], a["top"], a["best"], a["ids"], a["ws"], a["floats"], None)
+    a = dict(logits=16, f32=1, ld=100, M=2, V=100, tokens=16, n=1, logp=16, entropy=16, top=0, best=16, ids=16) | args
+    rc = lib.load().lia_token_logprobs(a["logits"], a["f32"], a["ld"], a["M"], a["V"], a["tokens"], a["n"], a["logp"], a["entropy"], a["top"], a["best"], a["ids"], None)
     assert rc == -1 and message in lib.last_error()
 
 
@@ -97,7 +97,7 @@ def test_wrappers_refuse(lib):
     with pytest.raises(E):
         ops.token_logprobs(z(2, 10))
     with pytest.raises(E, match="float8_e4m3fn"):
-        ops._cache_view("x", "kcache", z(1, 4, 128), None, 1, 128)
+        ops._cache_view("x", z(1, 4, 128), None, 1, 128, -1)
 
 
 def test_slots_of_8_bit_rows():
