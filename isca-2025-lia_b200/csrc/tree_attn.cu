@@ -13,7 +13,7 @@
 #include "mma.cuh"
 #include "tree_attn.cuh"
 
-int lia_tree_attn_tc(const void* args, int type, int nseg, lia_stream_t stream);      // tree_attn_sm100.cu
+int lia_tree_attn_tc(const void* args, int type, int rows, int nseg, lia_stream_t stream);      // tree_attn_sm100.cu
 
 namespace {
 
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 
 // How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history
 struct Plan {
-  int nr, tiles, splits;                                           // nr: eights of rows; 16 of them on tcgen05
+  int nr, tiles, splits;                                           // nr: eights of rows; 16 and 32 of them on tcgen05
 };
 #ifndef TC_ROWS
 #define TC_ROWS 32
@@ -395,11 +395,11 @@ struct Plan {
 Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
   const long long R = (long long)rows * (H / G);
   Plan p;
-  p.nr = R > TC_ROWS ? 16 : R > 16 ? 4 : R > 8 ? 2 : 1;
+  p.nr = R > TC_ROWS ? (R > 128 ? 32 : 16) : R > 16 ? 4 : R > 8 ? 2 : 1;
   p.tiles = (int)((R + 8 * p.nr - 1) / (8 * p.nr));
-  const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.nr == 16 ? 1 : blocks_an_sm(type, p.nr));
+  const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.nr >= 16 ? 1 : blocks_an_sm(type, p.nr));
   const long long span = window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx;
-  const long long least = p.nr == 16 ? 512 : 256;                   // keys of a block of threads: eight blocks of 64, or four of 16 a warp
+  const long long least = p.nr >= 16 ? 512 : 256;                   // keys of a block of threads: eight blocks of 64, or four of 16 a warp
   long long s = room / blocks, most = (span + least - 1) / least;
   if (s > most) s = most;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
@@ -421,7 +421,7 @@ template <int DIM, int VDIM, int KIND, int NR> int launch(const TreeArgs& a, int
   return LIA_OK;
 }
 template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
-  const int rc = nr == 16 ? lia_tree_attn_tc(&a, KIND, nseg, stream)
+  const int rc = nr >= 16 ? lia_tree_attn_tc(&a, KIND, nr * 8, nseg, stream)
                  : nr == 4 ? launch<DIM, VDIM, KIND, 4>(a, nseg, stream)
                  : nr == 2 ? launch<DIM, VDIM, KIND, 2>(a, nseg, stream) : launch<DIM, VDIM, KIND, 1>(a, nseg, stream);
   if (rc == LIA_OK && a.splits > 1) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));

@@ -1,17 +1,22 @@
-// Attention of drafted tokens (tree_attn.cu has the formulas) for many rows of a key head: 128 rows of (token, head) to a block, on tcgen05.
+// Attention of drafted tokens (tree_attn.cu has the formulas) for many rows of a key head, on tcgen05: 128 rows of (token, head) to a block, or 256 where there are more.
 //
-//   warps 0-3, 4-7   two groups that take the history's blocks of 64 keys in turn, each with a maximum, a sum and weighted values of its own; a thread has one row, which is one
-//                    lane of TMEM.  They meet at the end.
+//   warps 0-3, 4-7   two groups, each with a maximum, a sum and weighted values of its own; a thread has one row, which is one lane of TMEM.  Of 256 rows each group has 128; of up
+//                    to 128 both have the same rows and take the history's blocks of 64 keys in turn, and they meet at the end.
 //   warps 8-15       bring keys and values: 16 bytes a lane from memory, 8-bit codes as fp16, into shared memory as the products want them (128-byte swizzle).  Positions behind the last key
 //                    become zeros, so that nothing unwritten is multiplied.
 //   warp 16          the products (three more are there for their registers)
-// TMEM, 512 columns: group s has its scores at 64 s, in their place its weights (fp16, or two bf16 parts), and its weighted values at 128 + 128 s; the queries, from where
-// they are the products' first operand, lie at QUERIES: shared memory, which takes 128 bytes a clock, is left to keys and values.
+// TMEM, 512 columns: group s has the scores of two blocks, one being worked on and the next one, at 128 s and 128 s + 64, in their place its weights (fp16, or two bf16 parts), and its
+// weighted values at 256 + 128 s.  (With one block's scores and the queries in TMEM too, a group waited 40 % of its time for scores that are issued behind its weights' products: an instruction
+// takes 65 clocks to issue, and a block 12.  The queries in shared memory cost nothing: 6 KB a product of 65 clocks are less than it takes in that time.)
 // The weighted values stay in TMEM from block to block.  Weights are relative to a maximum that moves only when a row has exceeded it by 2^8 (they fit fp16 up to there); only then
 // its group multiplies what it has, behind the products of its last block.
 //
-// What bounds it at 128 rows: the powers (one a score, 16 a clock and SM: 1024 clocks for 128 keys of 128 rows) as well as the tensor cores (1024 with 8-bit codes, 1536 with bf16 and its two
-// parts of weights); with fewer rows memory (1400 clocks for 128 keys of 8 bits, 2800 of bf16).
+// 8-bit scales: a key's is multiplied into its scores in fp32.  A value's is multiplied into its channels on their way to fp16, relative to the power of two REF of the first keys' largest
+// (rounded to 11 bits twice: 2^-11 each, as the weights are), which leaves the softmax one instruction less in three.  A value whose scale is not within 2^-8 to 2^6 of REF, one of nothing or NaN
+// among them, stays as it is and its scale joins the exponent (tree_attn.cu); a block with one takes a slower way.
+//
+// What bounds it at 128 rows and more: the powers (one a score, 16 a clock and SM: 512 clocks for 64 keys of 128 rows) as well as the tensor cores (512 with 8-bit codes, 768 with bf16 and its two
+// parts of weights) and, with 8 bits, the instructions that widen the codes; with fewer rows memory (700 clocks for 64 keys of 8 bits, 1400 of bf16).
 #include "pairs.cuh"
 #include "tree_attn.cuh"
 #include "umma.cuh"
@@ -21,25 +26,27 @@ int* lia_timeout_word();                                           // moe_sm100.
 namespace {
 
 constexpr int ROWS = 128, KEYS = 64, THREADS = 640, LOADERS = 256, ISSUER = 16;
-constexpr int SOFTMAX_REGS = 128, LOADER_REGS = 96, OTHER_REGS = 24; // of a thread, by what its four warps do (setmaxnreg: multiples of 8); the launch gives 96
-constexpr uint32_t VALUES = 128, QUERIES = 384;
+constexpr int SOFTMAX_REGS = 128, LOADER_REGS = 96, OTHER_REGS = 32; // of a thread, by what its four warps do (setmaxnreg: multiples of 8); the launch gives 96
+constexpr uint32_t VALUES = 256;
 constexpr float SLACK = 8.f;                                       // how far, in powers of two, weights may exceed 1
 
-template <int DIM, int VDIM, int KIND>
+template <int DIM, int VDIM, int KIND, bool PAIR>
 struct Tc {
   static constexpr bool BITS8 = KIND != LIA_CACHE_BF16;
   static constexpr int SLAB = KEYS * 128;                          // 64 channels of 16 bits of a block's keys
   static constexpr int K_BYTES = DIM / 64 * SLAB, V_BYTES = VDIM / 64 * SLAB, STAGE = K_BYTES + V_BYTES;
-  static constexpr int STAGES = 196608 / STAGE > 8 ? 8 : 196608 / STAGE;
+  static constexpr int Q_SLAB = ROWS * 128, Q_BYTES = DIM / 64 * Q_SLAB;                        // a group's queries
+  static constexpr int ALL_Q = (PAIR ? 2 : 1) * Q_BYTES, ROOM = (221184 - ALL_Q) / STAGE, STAGES = ROOM > 8 ? 8 : ROOM;
   static constexpr int KT = DIM * (BITS8 ? 1 : 2) / 16, VT = VDIM * (BITS8 ? 1 : 2) / 16;      // lanes of a key, of a value
   static constexpr int KN = KEYS * KT / LOADERS, VN = KEYS * VT / LOADERS;                       // vectors of a lane
-  static constexpr int AHEAD = BITS8 ? 4 : 2;                      // blocks on their way from memory
+  static constexpr int AHEAD = BITS8 ? 3 : 2;                      // blocks on their way from memory
   static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // weights are 2^(x - maximum + LIFT): below 2^15 in fp16
 };
 struct Tail {
-  float ks[8][KEYS], lv[8][KEYS], rv[8][KEYS];                     // of a stage's keys: scale; of its values: log2 of the scale, its inverse
+  float ks[8][KEYS], lv[8][KEYS], rv[8][KEYS];                     // of a stage's keys: scale; of its values: log2 of what is left of the scale, and the inverse of that
+  uint64_t odd[8];                                                 // of a stage: a byte for every warp that has brought a value with a scale far from REF
   float2 ml[ROWS];
-  uint64_t full[8], empty[8], s_full[2], p_full[2], o_done[2], q_full, drain;
+  uint64_t full[8], empty[8], s_full[2][2], p_full[2][2], o_done[2], q_full, drain;
   uint32_t tmem;
   int dead;
 };
@@ -64,6 +71,11 @@ template <int KIND> __device__ __forceinline__ void widen(const uint4& u, uint4&
   }
   lo = make_uint4(r[0], r[1], r[2], r[3]);
   hi = make_uint4(r[4], r[5], r[6], r[7]);
+}
+__device__ __forceinline__ void scale4(uint4& u, __half2 f) {
+  __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __hmul2(h[i], f);
 }
 __device__ __forceinline__ void put16(uint32_t addr, const uint4& u) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
@@ -90,38 +102,64 @@ __device__ __forceinline__ uint32_t seen32(const TreeArgs& a, const Portion& p, 
   return bits;
 }
 
-template <int DIM, int VDIM, int KIND>
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// REF, as an exponent: of the largest finite scale of `n` <= 64 positions
+__device__ __forceinline__ int ref_of(const float* scale, int n) {
+  const int lane = threadIdx.x & 31;
+  uint32_t top = 0;
+#pragma unroll
+  for (int x = 0; x < 64; x += 32) {
+    const uint32_t u = x + lane < n ? __float_as_uint(__ldcg(scale + x + lane)) : 0u;
+    if (u < 0x7f800000u) top = max(top, u);                        // (not a negative one either)
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  return top >= 0x00800000u ? min((int)(top >> 23) - 127, 100) : 0;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
+
+template <int DIM, int VDIM, int KIND, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs a, int* __restrict__ timeouts) {
-  using C = Tc<DIM, VDIM, KIND>;
+  using C = Tc<DIM, VDIM, KIND, PAIR>;
   constexpr bool BITS8 = C::BITS8;
+  constexpr int TILE = PAIR ? 2 * ROWS : ROWS, STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem - smem_u32(smem_raw));
-  Tail& sm = *reinterpret_cast<Tail*>(smem_gen + C::STAGES * C::STAGE);
+  const uint32_t queries = smem + STAGES * C::STAGE;               // [groups' own rows][DIM]
+  Tail& sm = *reinterpret_cast<Tail*>(smem_gen + STAGES * C::STAGE + C::ALL_Q);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
   pdl_wait();
-  const Portion p = portion_of(a, blockIdx.z);
+  Portion p = portion_of(a, blockIdx.z);
   if (!p.held) {
     if (a.splits == 1 && blockIdx.y == 0) nan_rows<VDIM>(a, p);
     return;
   }
-  const int g = blockIdx.y % a.G, R = p.n * a.rep, tiles = (R + ROWS - 1) / ROWS, tile = tiles - 1 - (int)blockIdx.y / a.G, r0 = tile * ROWS;   // (the last ones see most)
+  // (known to be the same in all lanes, so that what the products' instructions take needs no moves to uniform registers)
+  p.slot = __shfl_sync(0xffffffffu, p.slot, 0), p.p0 = __shfl_sync(0xffffffffu, p.p0, 0), p.row = __shfl_sync(0xffffffffu, p.row, 0), p.n = __shfl_sync(0xffffffffu, p.n, 0);
+  const int g = blockIdx.y % a.G, R = p.n * a.rep, tiles = (R + TILE - 1) / TILE, tile = tiles - 1 - (int)blockIdx.y / a.G, r0 = tile * TILE;   // (the last ones see most)
   if (tile < 0) return;
+  const int groups = !PAIR || r0 + ROWS < R ? 2 : 1;               // (with one the second has no rows and no blocks)
 
   if (threadIdx.x == 0) {
     sm.dead = 0;
-    for (int i = 0; i < C::STAGES; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(smem_u32(&sm.full[i]), LOADERS / 32);
       mbar_init(smem_u32(&sm.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sm.s_full[i]), 1);
-      mbar_init(smem_u32(&sm.p_full[i]), 4);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(smem_u32(&sm.s_full[i][x]), 1);
+        mbar_init(smem_u32(&sm.p_full[i][x]), 4);
+      }
       mbar_init(smem_u32(&sm.o_done[i]), 1);
     }
-    mbar_init(smem_u32(&sm.q_full), 4);
+    mbar_init(smem_u32(&sm.q_full), PAIR ? 8 : 4);
     mbar_init(smem_u32(&sm.drain), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -136,7 +174,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
   volatile int* dead = &sm.dead;
 
   // ---- which keys
-  const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + ROWS - 1) / a.rep);
+  const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + TILE - 1) / a.rep);
   int near = i0, far = i1;
   if (a.depth != nullptr) {
     near = 1 << 29;
@@ -157,12 +195,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     // ================================================================ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     const int s = warp >> 2, w = warp & 3, r = w * 32 + lane;
-    const bool there = r0 + r < R, warp_there = r0 + w * 32 < R;
-    const int i = there ? (r0 + r) / a.rep : p.n - 1, h = there ? g * a.rep + (r0 + r) - i * a.rep : g * a.rep;
+    const int row = r0 + (PAIR ? s * ROWS : 0) + r;
+    const bool there = row < R, warp_there = row - lane < R;
+    const int i = there ? row / a.rep : p.n - 1, h = there ? g * a.rep + row - i * a.rep : g * a.rep;
     const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
     float rf = a.scale * (a.temp != nullptr ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
     const bool flip = rf < 0.f;                                    // (so that the largest product is the largest score)
-    {                                                              // queries: group 0's go to TMEM, both know their factor
+    {                                                              // queries go to shared memory (those of both groups' rows from the first), and their factor is known
       const bf16* src = a.q + (long long)(p.row + i) * a.ldq + h * DIM;
       uint32_t top = 0;
       uint2 u[DIM / 4];
@@ -175,87 +214,103 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
       const float by = flip ? -down.by : down.by;
       if constexpr (BITS8) rf *= down.back;
       rf = fabsf(rf);
-      if (s == 0) {
+      if (PAIR || s == 0) {
+        const uint32_t to = queries + (PAIR ? s * C::Q_BYTES : 0) + r * 128;
 #pragma unroll
-        for (int c0 = 0; c0 < DIM / 2; c0 += 16) {                 // 32 numbers of a row
-          uint32_t q[16];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {                            // four of them
-            if constexpr (BITS8) {
-              const int at = c0 * 2 + e * 4, c = DIM == 128 ? (at & 63) / 8 * 16 + (at >> 6) * 8 + (at & 7) : at;
-              float x[4];
-              unpack_bf16x2(u[c / 4].x, x[0], x[1]);
-              unpack_bf16x2(u[c / 4].y, x[2], x[3]);
-              q[2 * e] = pack_f16x2(x[0] * by, x[1] * by);
-              q[2 * e + 1] = pack_f16x2(x[2] * by, x[3] * by);
-            } else {
-              const uint32_t sign = flip ? 0x80008000u : 0u;
-              q[2 * e] = u[c0 / 2 + e].x ^ sign;
-              q[2 * e + 1] = u[c0 / 2 + e].y ^ sign;
-            }
+        for (int e = 0; e < DIM / 8; ++e) {                        // eight of the products' columns
+          uint4 q;
+          if constexpr (BITS8) {
+            const int at = e * 8, c = DIM == 128 ? (at & 63) / 8 * 16 + (at >> 6) * 8 : at;
+            float x[8];
+            unpack_bf16x2(u[c / 4].x, x[0], x[1]);
+            unpack_bf16x2(u[c / 4].y, x[2], x[3]);
+            unpack_bf16x2(u[c / 4 + 1].x, x[4], x[5]);
+            unpack_bf16x2(u[c / 4 + 1].y, x[6], x[7]);
+            q = make_uint4(pack_f16x2(x[0] * by, x[1] * by), pack_f16x2(x[2] * by, x[3] * by), pack_f16x2(x[4] * by, x[5] * by), pack_f16x2(x[6] * by, x[7] * by));
+          } else {
+            const uint32_t sign = flip ? 0x80008000u : 0u;
+            q = make_uint4(u[2 * e].x ^ sign, u[2 * e].y ^ sign, u[2 * e + 1].x ^ sign, u[2 * e + 1].y ^ sign);
           }
-          tmem_st16(lanes + QUERIES + c0, q);
+          put16(to + (e >> 3) * C::Q_SLAB + (((e & 7) ^ (r & 7)) << 4), q);
         }
-        tmem_st_wait();
-        tcgen05_fence_before();
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.q_full));
       }
     }
     const int first = first_key(a, p, depth_of(a, p, i));
     const float two_by_cap = a.softcap > 0.f ? 2.f * LOG2E / a.softcap : 0.f;
-    const uint32_t scores = lanes + s * KEYS, values = lanes + VALUES + s * 128;
-    float m = -INFINITY, l = 0.f;
+    const uint32_t values = lanes + VALUES + s * 128;
+    float m = -1e30f, l = 0.f;
     bool alive = true;
     int done = 0;                                                  // of the group's blocks
+    const int ref = BITS8 && n > 0 ? ref_of(a.v.scale_at(p.slot, g) + start, min(hi - start, KEYS)) : 0;
+    const float ref_l = (float)ref, ref_inv = pow2(-ref);
+    // (a row's first block sees to a maximum; -1e30 stands for none, so that nothing is less than it but -inf)
 #pragma unroll 1
-    for (int j = s; j < n; j += 2, ++done) {
-      const int st = j % C::STAGES;
-      if constexpr (BITS8)
-        if (!(alive = warp_wait(smem_u32(&sm.full[st]), (j / C::STAGES) & 1, dead))) break;
-      if (!(alive = warp_wait(smem_u32(&sm.s_full[s]), done & 1, dead))) break;
+    for (int j = PAIR ? 0 : s; j < n && s < groups; j += PAIR ? 1 : 2, ++done) {
+      const int st = j % STAGES, buf = done & 1;
+      const uint32_t scores = lanes + s * 128 + buf * KEYS;
+      float4 k4[BITS8 ? 8 : 1];                                    // half of the keys' scales, asked for together
+      auto ask_scales = [&](int half) {
+#pragma unroll
+        for (int c = 0; c < (BITS8 ? 8 : 0); ++c) k4[c] = *reinterpret_cast<const float4*>(&sm.ks[st][half * 32 + c * 4]);
+      };
+      if constexpr (BITS8) {
+        if (!(alive = warp_wait(smem_u32(&sm.full[st]), (j / STAGES) & 1, dead))) break;
+        ask_scales(0);
+      }
+      if (!(alive = warp_wait(smem_u32(&sm.s_full[s][buf]), (done >> 1) & 1, dead))) break;
       tcgen05_fence_after();
       if (warp_there) {
         uint32_t v[KEYS];
         tmem_ld32(scores, v);
         tmem_ld32(scores + 32, v + 32);
         tmem_ld_wait();
-        const int t = start + j * KEYS;
-        // ---- scores in powers of two (with the values' scales)
-        auto scaled = [&](auto with) {                             // with(pair of products times the row's factor, log2 of the values' scales)
+        if constexpr (BITS8) {
 #pragma unroll
-          for (int c = 0; c < KEYS; c += 4) {
-            float4 k4 = make_float4(1.f, 1.f, 1.f, 1.f), l4 = make_float4(0.f, 0.f, 0.f, 0.f);
-            if constexpr (BITS8) {
-              k4 = *reinterpret_cast<const float4*>(&sm.ks[st][c]);
-              l4 = *reinterpret_cast<const float4*>(&sm.lv[st][c]);
+          for (int half = 0; half < 2; ++half) {
+            float4 f4[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) f4[c] = k4[c];
+            if (half == 0) ask_scales(1);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const int x = half * 32 + c * 4;
+              float a0, a1;
+              unpack2(mul2(pack2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), pack2(f4[c].x, f4[c].y)), a0, a1);
+              v[x] = __float_as_uint(a0);
+              v[x + 1] = __float_as_uint(a1);
+              unpack2(mul2(pack2(__uint_as_float(v[x + 2]), __uint_as_float(v[x + 3])), pack2(f4[c].z, f4[c].w)), a0, a1);
+              v[x + 2] = __float_as_uint(a0);
+              v[x + 3] = __float_as_uint(a1);
             }
-            f32x2 x = pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), y = pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
-            if constexpr (BITS8) {
-              x = mul2(x, pack2(k4.x, k4.y));
-              y = mul2(y, pack2(k4.z, k4.w));
-            }
-            x = with(x, pack2(l4.x, l4.y));
-            y = with(y, pack2(l4.z, l4.w));
+          }
+        }
+        const int t = start + j * KEYS;
+        const bool odd = BITS8 && sm.odd[st] != 0;
+        float factor = rf, add = ref_l;                            // x = v * factor + add, in powers of two (with the values' scales)
+        if (odd || a.softcap > 0.f) {
+          factor = 1.f;
+          add = 0.f;
+        }
+        auto each = [&](auto with) {                               // with(pair of products with their keys' scales, column of the first)
+#pragma unroll
+          for (int c = 0; c < KEYS; c += 2) {
             float x0, x1;
-            unpack2(x, x0, x1);
+            unpack2(with(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), c), x0, x1);
             v[c] = __float_as_uint(x0);
             v[c + 1] = __float_as_uint(x1);
-            unpack2(y, x0, x1);
-            v[c + 2] = __float_as_uint(x0);
-            v[c + 3] = __float_as_uint(x1);
           }
         };
         if (a.softcap > 0.f) {
-          scaled([&](f32x2 x, f32x2 lv) {
+          each([&](f32x2 x, int c) {
             float x0, x1;
             unpack2(mul2(x, both(rf)), x0, x1);
-            return fma2(pack2(capped(x0, a.softcap, two_by_cap), capped(x1, a.softcap, two_by_cap)), both(LOG2E), lv);
+            return fma2(pack2(capped(x0, a.softcap, two_by_cap), capped(x1, a.softcap, two_by_cap)), both(LOG2E), BITS8 ? pack2(sm.lv[st][c], sm.lv[st][c + 1]) : both(0.f));
           });
-        } else if constexpr (BITS8) {
-          scaled([&](f32x2 x, f32x2 lv) { return fma2(x, both(rf), lv); });
-        } else {
-          scaled([&](f32x2 x, f32x2) { return mul2(x, both(rf)); });
+        } else if (odd) {
+          each([&](f32x2 x, int c) { return fma2(x, both(rf), pack2(sm.lv[st][c], sm.lv[st][c + 1])); });
         }
         if (t < all_lo || t + KEYS > min(all_hi, hi)) {
 #pragma unroll
@@ -268,10 +323,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
         }
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c) tops[c & 3] = fmaxf(tops[c & 3], __uint_as_float(v[c]));
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        for (int c = 0; c < KEYS; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], __uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
+        const float top = fmaf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), factor, add);
         // ---- the maximum moves for rows that have outgrown it
-        const bool grown = top > m + SLACK || (m == -INFINITY && top != -INFINITY);
+        const bool grown = top - m > SLACK;
         if (__any_sync(0xffffffffu, grown)) {
           const float to = grown ? top : m, keep = grown ? ex2(m - to) : 1.f;
           m = to;
@@ -290,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
             }
           }
         }
-        const float off = C::LIFT - (m == -INFINITY ? 0.f : m);
+        const f32x2 by = both(factor), off = both(add + C::LIFT - m);
         // ---- weights
         f32x2 sum = 0ull;
 #pragma unroll
@@ -299,20 +356,21 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             float w0, w1, w2, w3;
-            unpack2(add2(pack2(__uint_as_float(v[c + e]), __uint_as_float(v[c + e + 1])), both(off)), w0, w1);
-            unpack2(add2(pack2(__uint_as_float(v[c + e + 2]), __uint_as_float(v[c + e + 3])), both(off)), w2, w3);
+            unpack2(fma2(pack2(__uint_as_float(v[c + e]), __uint_as_float(v[c + e + 1])), by, off), w0, w1);
+            unpack2(fma2(pack2(__uint_as_float(v[c + e + 2]), __uint_as_float(v[c + e + 3])), by, off), w2, w3);
             w0 = ex2(w0);
             w1 = ex2(w1);
             w2 = ex2(w2);
             w3 = ex2(w3);
+            sum = add2(sum, add2(pack2(w0, w1), pack2(w2, w3)));
             if constexpr (BITS8) {
-              const float4 r4 = *reinterpret_cast<const float4*>(&sm.rv[st][c + e]);
-              sum = fma2(pack2(w0, w1), pack2(r4.x, r4.y), sum);
-              sum = fma2(pack2(w2, w3), pack2(r4.z, r4.w), sum);
               hi16[e / 2] = pack_f16x2(w0, w1);
               hi16[e / 2 + 1] = pack_f16x2(w2, w3);
+              v[c + e] = __float_as_uint(w0);
+              v[c + e + 1] = __float_as_uint(w1);
+              v[c + e + 2] = __float_as_uint(w2);
+              v[c + e + 3] = __float_as_uint(w3);
             } else {
-              sum = add2(sum, add2(pack2(w0, w1), pack2(w2, w3)));
               float x0, x1;
               hi16[e / 2] = pack_bf16x2(w0, w1);
               unpack_bf16x2(hi16[e / 2], x0, x1);
@@ -326,39 +384,57 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
           if constexpr (!BITS8) tmem_st8(scores + 32 + c / 2, lo16);
         }
         float s0, s1;
+        if (odd) {                                                 // p = weight / what is left of the scale
+          sum = 0ull;
+#pragma unroll
+          for (int c = 0; c < KEYS; c += 4) {
+            const float4 r4 = *reinterpret_cast<const float4*>(&sm.rv[st][c]);
+            sum = fma2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), pack2(r4.x, r4.y), sum);
+            sum = fma2(pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), pack2(r4.z, r4.w), sum);
+          }
+        }
         unpack2(sum, s0, s1);
-        l += s0 + s1;
+        l = fmaf(s0 + s1, odd ? 1.f : ref_inv, l);
         tmem_st_wait();
         tcgen05_fence_before();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[s]));
+      if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[s][buf]));
     }
+    // (the last scores come before the last but one weights' products: those are waited for first, lest their phase be taken for the last one's)
+    if (alive && done > 1) alive = warp_wait(smem_u32(&sm.o_done[s]), done & 1, dead);
     if (alive && done > 0) alive = warp_wait(smem_u32(&sm.o_done[s]), (done - 1) & 1, dead);
     if (!alive) l = __uint_as_float(0x7fc00000u);
     tcgen05_fence_after();
-    // ---- the groups' rows meet: the second's by way of shared memory, where the keys were (both groups' last products are done, and with them the loads)
-    auto groups_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    // ---- groups of the same rows meet: the second's by way of shared memory, where the keys were (both groups' last products are done, and with them the loads)
     float* other = reinterpret_cast<float*>(smem_gen);             // [VDIM][ROWS], a row's channels a thread's own
-    groups_sync();
-    if (s == 1) {
-      sm.ml[r] = make_float2(m, l);
-      if (n > 1) {
+    float top = m, sum = l, f0 = n > 0 ? 1.f : 0.f, f1 = 0.f;
+    const bool two = !PAIR && n > 1;
+    if constexpr (!PAIR) {
+      auto groups_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+      groups_sync();
+      if (s == 1) {
+        sm.ml[r] = make_float2(m, l);
+        if (two) {
 #pragma unroll 1
-        for (int c = 0; c < VDIM; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(values + c, o);
-          tmem_ld_wait();
+          for (int c = 0; c < VDIM; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(values + c, o);
+            tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) other[(c + e) * ROWS + r] = __uint_as_float(o[e]);
+            for (int e = 0; e < 32; ++e) other[(c + e) * ROWS + r] = __uint_as_float(o[e]);
+          }
         }
       }
-    }
-    groups_sync();
-    if (s == 0 && warp_there) {
+      groups_sync();
       const float2 ml = sm.ml[r];
-      const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top, f0 = n > 0 ? ex2(m - base) : 0.f, f1 = n > 1 ? ex2(ml.x - base) : 0.f;
-      const float sum = l * f0 + ml.y * f1;                        // (NaN if a wait ran out)
+      top = fmaxf(m, ml.x);
+      f0 = n > 0 ? ex2(m - top) : 0.f;
+      f1 = two ? ex2(ml.x - top) : 0.f;
+      sum = l * f0 + ml.y * f1;                                    // (NaN if a wait ran out)
+      if (isnan(l) || isnan(ml.y)) sum = l + ml.y;
+    }
+    if ((PAIR || s == 0) && warp_there) {
       const long long rows = (long long)a.M * a.H, at = (long long)(p.row + i) * a.H + h;
       const bool whole = a.splits == 1;
       const float inv = whole ? 1.f / sum : 1.f;
@@ -376,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             y[x] = n > 0 ? __uint_as_float(o[e + x]) * f0 : 0.f;
-            if (n > 1) y[x] = fmaf(other[(c + e + x) * ROWS + r], f1, y[x]);
+            if (two) y[x] = fmaf(other[(c + e + x) * ROWS + r], f1, y[x]);
             y[x] *= inv;
             probe = fmaf(y[x], 0.f, probe);
           }
@@ -410,36 +486,55 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
   } else if (warp < ISSUER) {
     // ================================================================ keys and values
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LOADER_REGS));
-    const int th = threadIdx.x - 256, kt = th % C::KT, vt = th % C::VT;
-    const uint8_t *kbase = a.k.at(p.slot, 0, g) + kt * 16, *vbase = a.v.at(p.slot, 0, g) + vt * 16;
-    const float* scales = BITS8 && th < 2 * KEYS ? (th < KEYS ? a.k.scale_at(p.slot, g) : a.v.scale_at(p.slot, g)) : nullptr;
+    const int th = threadIdx.x - 256, kt = th % C::KT, vt = th % C::VT, k0 = th / C::KT, v0 = th / C::VT;
+    constexpr int KSTEP = LOADERS / C::KT, VSTEP = LOADERS / C::VT;                            // a lane's keys are so far apart
+    // the lane's places in the next block to ask for
+    const uint8_t *kp = a.k.at(p.slot, start + k0, g) + kt * 16, *vp = a.v.at(p.slot, start + v0, g) + vt * 16;
+    const float *ksp = BITS8 ? a.k.scale_at(p.slot, g) + start : nullptr, *vsp = BITS8 ? a.v.scale_at(p.slot, g) + start : nullptr;
+    const int ref = BITS8 && n > 0 ? ref_of(vsp, min(hi - start, KEYS)) : 0;
+    const float ref_inv = pow2(-ref);
     uint4 kr[C::AHEAD][C::KN], vr[C::AHEAD][C::VN];
-    float sc[C::AHEAD];
+    float ks[C::AHEAD], vs[C::AHEAD][C::VN];                       // of key th < 64, and of the lane's values
     auto ask = [&](int j, int x) {
-      const int t = start + j * KEYS;
+      if (j >= n) return;
+      const int left = hi - start - j * KEYS;                      // keys from the block's first on
+      if (left >= KEYS) {
 #pragma unroll
-      for (int c = 0; c < C::KN; ++c) {
-        const int key = t + th / C::KT + c * (LOADERS / C::KT);
-        kr[x][c] = j < n && key < hi ? ldg_act(kbase + (long long)key * a.k.pos) : make_uint4(0u, 0u, 0u, 0u);
-      }
+        for (int c = 0; c < C::KN; ++c) kr[x][c] = ldg_act(kp + c * KSTEP * a.k.pos);
 #pragma unroll
-      for (int c = 0; c < C::VN; ++c) {
-        const int key = t + th / C::VT + c * (LOADERS / C::VT);
-        vr[x][c] = j < n && key < hi ? ldg_act(vbase + (long long)key * a.v.pos) : make_uint4(0u, 0u, 0u, 0u);
-      }
-      if constexpr (BITS8)
-        if (th < 2 * KEYS) sc[x] = j < n && t + (th & (KEYS - 1)) < hi ? __ldcg(scales + t + (th & (KEYS - 1))) : 1.f;
-    };
-    auto put = [&](uint32_t tile_at, int key, int tid, int wide, const uint4& u) {
-      if constexpr (BITS8) {
-        uint4 x, y;
-        widen<KIND>(u, x, y);
-        const int p0 = wide == 128 ? place_of<128>(tid, 0) : place_of<64>(tid, 0), p1 = wide == 128 ? place_of<128>(tid, 1) : place_of<64>(tid, 1);
-        put16(tile_at + (p0 >> 6) * C::SLAB + key * 128 + ((((p0 & 63) >> 3) ^ (key & 7)) << 4), x);
-        put16(tile_at + (p1 >> 6) * C::SLAB + key * 128 + ((((p1 & 63) >> 3) ^ (key & 7)) << 4), y);
+        for (int c = 0; c < C::VN; ++c) vr[x][c] = ldg_act(vp + c * VSTEP * a.v.pos);
+        if constexpr (BITS8) {
+          if (th < KEYS) ks[x] = __ldcg(ksp + th);
+#pragma unroll
+          for (int c = 0; c < C::VN; ++c) vs[x][c] = __ldcg(vsp + v0 + c * VSTEP);
+        }
       } else {
-        put16(tile_at + (tid >> 3) * C::SLAB + key * 128 + (((tid & 7) ^ (key & 7)) << 4), u);
+#pragma unroll
+        for (int c = 0; c < C::KN; ++c) kr[x][c] = k0 + c * KSTEP < left ? ldg_act(kp + c * KSTEP * a.k.pos) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int c = 0; c < C::VN; ++c) vr[x][c] = v0 + c * VSTEP < left ? ldg_act(vp + c * VSTEP * a.v.pos) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (BITS8) {
+          if (th < KEYS) ks[x] = th < left ? __ldcg(ksp + th) : 0.f;
+#pragma unroll
+          for (int c = 0; c < C::VN; ++c) vs[x][c] = v0 + c * VSTEP < left ? __ldcg(vsp + v0 + c * VSTEP) : pow2(ref);
+        }
       }
+      kp += KEYS * a.k.pos;
+      vp += KEYS * a.v.pos;
+      if constexpr (BITS8) {
+        ksp += KEYS;
+        vsp += KEYS;
+      }
+    };
+    // where the lane's vectors go: the second half of 16 codes beside the first or in the next slab, the vectors of other keys some rows of 128 bytes on
+    auto place = [&](int key, int tid, int wide) {
+      const int p0 = BITS8 ? (wide == 128 ? place_of<128>(tid, 0) : place_of<64>(tid, 0)) : tid * 8;
+      return (uint32_t)((p0 >> 6) * C::SLAB + key * 128 + ((((p0 & 63) >> 3) ^ (key & 7)) << 4));
+    };
+    const uint32_t k_at = place(k0, kt, DIM), v_at = C::K_BYTES + place(v0, vt, VDIM);
+    auto put = [&](uint32_t at, bool wide, const uint4& x, const uint4& y) {
+      put16(at, x);
+      put16(wide ? at + C::SLAB : at ^ 16u, y);                    // (of 64 channels they are neighbours, which the swizzle keeps in one pair)
     };
 #pragma unroll
     for (int x = 0; x < C::AHEAD; ++x) ask(x, x);
@@ -448,22 +543,43 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     for (int j0 = 0; j0 < n && alive; j0 += C::AHEAD) {
 #pragma unroll
       for (int x = 0; x < C::AHEAD; ++x) {
-        const int j = j0 + x, st = j % C::STAGES;
+        const int j = j0 + x, st = j % STAGES;
         if (j >= n) break;
-        if (!(alive = warp_wait(smem_u32(&sm.empty[st]), ((j / C::STAGES) & 1) ^ 1u, dead))) break;
+        if (!(alive = warp_wait(smem_u32(&sm.empty[st]), ((j / STAGES) & 1) ^ 1u, dead))) break;
         const uint32_t at = smem + st * C::STAGE;
-#pragma unroll
-        for (int c = 0; c < C::KN; ++c) put(at, th / C::KT + c * (LOADERS / C::KT), kt, DIM, kr[x][c]);
-#pragma unroll
-        for (int c = 0; c < C::VN; ++c) put(at + C::K_BYTES, th / C::VT + c * (LOADERS / C::VT), vt, VDIM, vr[x][c]);
         if constexpr (BITS8) {
-          if (th < KEYS) {
-            sm.ks[st][th] = sc[x];
-          } else if (th < 2 * KEYS) {
-            const float y = max_nan(sc[x], LEAST_SCALE);
-            sm.lv[st][th - KEYS] = lg2(y);
-            sm.rv[st][th - KEYS] = __fdividef(1.f, y);
+#pragma unroll
+          for (int c = 0; c < C::KN; ++c) {
+            uint4 lo16, hi16;
+            widen<KIND>(kr[x][c], lo16, hi16);
+            put(at + k_at + c * KSTEP * 128, DIM == 128, lo16, hi16);
           }
+          if (th < KEYS) sm.ks[st][th] = ks[x];
+          bool odd = false;
+#pragma unroll
+          for (int c = 0; c < C::VN; ++c) {
+            uint4 lo16, hi16;
+            widen<KIND>(vr[x][c], lo16, hi16);
+            const float f = vs[x][c] * ref_inv;
+            const bool near = f >= 0x1p-8f && f < 64.f;
+            odd |= !near;
+            const __half2 f2 = __float2half2_rn(near ? f : 1.f);
+            scale4(lo16, f2);
+            scale4(hi16, f2);
+            put(at + v_at + c * VSTEP * 128, VDIM == 128, lo16, hi16);
+            if (vt == 0) {
+              const float y = near ? pow2(ref) : max_nan(vs[x][c], LEAST_SCALE);
+              sm.lv[st][v0 + c * VSTEP] = lg2(y);
+              sm.rv[st][v0 + c * VSTEP] = __fdividef(1.f, y);
+            }
+          }
+          odd = __any_sync(0xffffffffu, odd);
+          if (lane == 0) reinterpret_cast<uint8_t*>(&sm.odd[st])[warp - 8] = odd;
+        } else {
+#pragma unroll
+          for (int c = 0; c < C::KN; ++c) put16(at + k_at + c * KSTEP * 128, kr[x][c]);
+#pragma unroll
+          for (int c = 0; c < C::VN; ++c) put16(at + v_at + c * VSTEP * 128, vr[x][c]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -480,32 +596,51 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
       constexpr uint32_t idesc_qk = (1u << 4) | types | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       constexpr uint32_t idesc_pv = (1u << 4) | types | (1u << 16) | ((uint32_t)(VDIM >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);      // (the values lie with the keys as rows)
       bool alive = n > 0 && warp_wait(smem_u32(&sm.q_full), 0, dead);
-      auto scores = [&](int j) {
-        const int st = j % C::STAGES;
-        if (!warp_wait(smem_u32(&sm.full[st]), (j / C::STAGES) & 1, dead)) return false;
+      auto scores = [&](int j, int s, int done) {                  // of group s's block number `done`
+        const int st = j % STAGES, buf = done & 1;
+        if (!warp_wait(smem_u32(&sm.full[st]), (j / STAGES) & 1, dead)) return false;
         tcgen05_fence_after();
-        const uint32_t at = smem + st * C::STAGE;
+        const uint32_t at = smem + st * C::STAGE, q = queries + (PAIR ? s * C::Q_BYTES : 0);
 #pragma unroll
-        for (int k = 0; k < DIM / 16; ++k) mma_tmem_a_if(one, tmem + (j & 1) * KEYS, tmem + QUERIES + k * 8, make_smem_desc(at + (k >> 2) * C::SLAB + (k & 3) * 32), idesc_qk, k > 0);
-        commit_if(one, smem_u32(&sm.s_full[j & 1]));
+        for (int k = 0; k < DIM / 16; ++k)
+          mma_if(one, tmem + s * 128 + buf * KEYS, make_smem_desc(q + (k >> 2) * C::Q_SLAB + (k & 3) * 32), make_smem_desc(at + (k >> 2) * C::SLAB + (k & 3) * 32), idesc_qk, k > 0);
+        commit_if(one, smem_u32(&sm.s_full[s][buf]));
         return true;
       };
-      if (alive) alive = scores(0);
-      if (alive && n > 1) alive = scores(1);
-#pragma unroll 1
-      for (int j = 0; j < n && alive; ++j) {
-        const int st = j % C::STAGES, s = j & 1;
-        if (!(alive = warp_wait(smem_u32(&sm.p_full[s]), (j >> 1) & 1, dead))) break;
+      auto weighted = [&](int j, int s, int done) {
+        const int st = j % STAGES, buf = done & 1;
+        if (!warp_wait(smem_u32(&sm.p_full[s][buf]), (done >> 1) & 1, dead)) return false;
         tcgen05_fence_after();
         const uint32_t at = smem + st * C::STAGE + C::K_BYTES;
 #pragma unroll
         for (int part = 0; part < (BITS8 ? 1 : 2); ++part)
 #pragma unroll
           for (int k = 0; k < KEYS / 16; ++k)
-            mma_tmem_a_if(one, tmem + VALUES + s * 128, tmem + s * KEYS + part * 32 + k * 8, make_smem_desc_mn(at + k * 16 * 128, C::SLAB), idesc_pv, j > 1 || part > 0 || k > 0);
-        commit_if(one, smem_u32(&sm.empty[st]));
-        commit_if(one, smem_u32(&sm.o_done[s]));
-        if (j + 2 < n) alive = scores(j + 2);
+            mma_tmem_a_if(one, tmem + VALUES + s * 128, tmem + s * 128 + buf * KEYS + part * 32 + k * 8, make_smem_desc_mn(at + k * 16 * 128, C::SLAB), idesc_pv,
+                          done > 0 || part > 0 || k > 0);
+        return true;
+      };
+      // A group's scores come behind the products with the weights whose place they take, a block ahead of its softmax
+      if constexpr (PAIR) {
+        for (int s = 0; s < groups && alive; ++s) alive = scores(0, s, 0);
+#pragma unroll 1
+        for (int j = 0; j < n && alive; ++j) {
+          for (int s = 0; s < groups && alive && j + 1 < n; ++s) alive = scores(j + 1, s, j + 1);
+          for (int s = 0; s < groups && alive; ++s) {
+            if (!(alive = weighted(j, s, j))) break;
+            commit_if(one, smem_u32(&sm.o_done[s]));
+            if (s == groups - 1) commit_if(one, smem_u32(&sm.empty[j % STAGES]));
+          }
+        }
+      } else {
+        for (int j = 0; j < 3 && j < n && alive; ++j) alive = scores(j, j & 1, j >> 1);
+#pragma unroll 1
+        for (int j = 0; j < n && alive; ++j) {
+          if (j + 3 < n && !(alive = scores(j + 3, (j + 3) & 1, (j + 3) >> 1))) break;
+          if (!(alive = weighted(j, j & 1, j >> 1))) break;
+          commit_if(one, smem_u32(&sm.empty[j % STAGES]));
+          commit_if(one, smem_u32(&sm.o_done[j & 1]));
+        }
       }
     }
   }
@@ -526,41 +661,44 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
   }
 }
 
-template <int DIM, int VDIM, int KIND> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
-  using C = Tc<DIM, VDIM, KIND>;
-  constexpr int SMEM = C::STAGES * C::STAGE + (int)sizeof(Tail) + 1024;
-  static_assert(SMEM <= 232448 && C::STAGES * C::STAGE >= ROWS * VDIM * 4, "shared memory");
+template <int DIM, int VDIM, int KIND, bool PAIR> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
+  using C = Tc<DIM, VDIM, KIND, PAIR>;
+  constexpr int SMEM = C::STAGES * C::STAGE + C::ALL_Q + (int)sizeof(Tail) + 1024;
+  static_assert(SMEM <= 232448 && C::STAGES * C::STAGE >= ROWS * VDIM * 4 && C::STAGES >= 4, "shared memory");
   static bool configured[64] = {};                                 // per device
   int dev = 0;
   LIA_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !configured[dev]) {
-    LIA_CUDA(cudaFuncSetAttribute(tree_attn_tc_kernel<DIM, VDIM, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    LIA_CUDA(cudaFuncSetAttribute(tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 64) configured[dev] = true;
   }
   static const bool split_fits = [] {                              // the registers that the warps trade must be those that the block gets
     cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, tree_attn_tc_kernel<DIM, VDIM, KIND>) == cudaSuccess && at.numRegs * THREADS >= 128 * (2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS);
+    return cudaFuncGetAttributes(&at, tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>) == cudaSuccess && at.numRegs * THREADS >= 128 * (2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS);
   }();
   LIA_CHECK_ARG(split_fits, "lia_tree_attn: the kernel was built with too few registers");
   int* timeouts = lia_timeout_word();
   LIA_CHECK_ARG(timeouts, "lia_tree_attn: no memory for the count of waits that ran out");
-  LIA_CUDA(lia_launch_after(tree_attn_tc_kernel<DIM, VDIM, KIND>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), SMEM, stream, a, timeouts));
+  LIA_CUDA(lia_launch_after(tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), SMEM, stream, a, timeouts));
   return LIA_OK;
 }
-template <int KIND> int launch_dims(const TreeArgs& a, int nseg, cudaStream_t stream) {
-  if (a.k.dim == 128) return a.v.dim == 128 ? launch<128, 128, KIND>(a, nseg, stream) : launch<128, 64, KIND>(a, nseg, stream);
-  return a.v.dim == 128 ? launch<64, 128, KIND>(a, nseg, stream) : launch<64, 64, KIND>(a, nseg, stream);
+template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int rows, int nseg, cudaStream_t stream) {
+  return rows > ROWS ? launch<DIM, VDIM, KIND, true>(a, nseg, stream) : launch<DIM, VDIM, KIND, false>(a, nseg, stream);
+}
+template <int KIND> int launch_dims(const TreeArgs& a, int rows, int nseg, cudaStream_t stream) {
+  if (a.k.dim == 128) return a.v.dim == 128 ? launch_rows<128, 128, KIND>(a, rows, nseg, stream) : launch_rows<128, 64, KIND>(a, rows, nseg, stream);
+  return a.v.dim == 128 ? launch_rows<64, 128, KIND>(a, rows, nseg, stream) : launch_rows<64, 64, KIND>(a, rows, nseg, stream);
 }
 
 }  // namespace
 
-// blocks of 128 rows (a.tiles of them a portion); parts of split histories are left in a.ws
-int lia_tree_attn_tc(const void* args, int type, int nseg, lia_stream_t stream_) {
+// blocks of `rows` rows, 128 or 256 (a.tiles of them a portion); parts of split histories are left in a.ws
+int lia_tree_attn_tc(const void* args, int type, int rows, int nseg, lia_stream_t stream_) {
   const TreeArgs& a = *reinterpret_cast<const TreeArgs*>(args);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   switch (type) {
-    case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, nseg, stream);
-    case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, nseg, stream);
-    default: return launch_dims<LIA_CACHE_E4M3>(a, nseg, stream);
+    case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, rows, nseg, stream);
+    case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, rows, nseg, stream);
+    default: return launch_dims<LIA_CACHE_E4M3>(a, rows, nseg, stream);
   }
 }
