@@ -27,6 +27,8 @@ namespace {
 
 constexpr int ROWS = 128, KEYS = 64, THREADS = 640, LOADERS = 256, ISSUER = 16;
 constexpr int SOFTMAX_REGS = 128, LOADER_REGS = 96, OTHER_REGS = 32; // of a thread, by what its four warps do (setmaxnreg: multiples of 8); the launch gives 96
+constexpr int LAUNCH_REGS = 96;
+static_assert(SOFTMAX_REGS >= LAUNCH_REGS && LOADER_REGS <= LAUNCH_REGS && OTHER_REGS <= LAUNCH_REGS && 2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS <= THREADS / 128 * LAUNCH_REGS, "shares");
 constexpr uint32_t VALUES = 256;
 constexpr float SLACK = 8.f;                                       // how far, in powers of two, weights may exceed 1
 
@@ -262,6 +264,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
       }
       if (!(alive = warp_wait(smem_u32(&sm.s_full[s][buf]), (done >> 1) & 1, dead))) break;
       tcgen05_fence_after();
+      float keep = 1.f;
+      bool moved = false;
       if (warp_there) {
         uint32_t v[KEYS];
         tmem_ld32(scores, v);
@@ -329,23 +333,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
         const float top = fmaf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), factor, add);
         // ---- the maximum moves for rows that have outgrown it
         const bool grown = top - m > SLACK;
-        if (__any_sync(0xffffffffu, grown)) {
-          const float to = grown ? top : m, keep = grown ? ex2(m - to) : 1.f;
+        moved = __any_sync(0xffffffffu, grown);
+        if (moved) {
+          const float to = grown ? top : m;
+          keep = grown ? ex2(m - to) : 1.f;
           m = to;
           l *= keep;
-          if (done > 0) {
-            if (!(alive = warp_wait(smem_u32(&sm.o_done[s]), (done - 1) & 1, dead))) break;
-            tcgen05_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < VDIM; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(values + c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-              tmem_st16(values + c, o);
-            }
-          }
         }
         const f32x2 by = both(factor), off = both(add + C::LIFT - m);
         // ---- weights
@@ -395,14 +388,28 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
         }
         unpack2(sum, s0, s1);
         l = fmaf(s0 + s1, odd ? 1.f : ref_inv, l);
-        tmem_st_wait();
-        tcgen05_fence_before();
       }
+      // The products of the group's last block are waited for every time, so that no phase of theirs is missed (two later, it would look like one that has yet to come)
+      if (done > 0) {
+        if (!(alive = warp_wait(smem_u32(&sm.o_done[s]), (done - 1) & 1, dead))) break;
+        if (moved) {
+          tcgen05_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < VDIM; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(values + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st16(values + c, o);
+          }
+        }
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[s][buf]));
     }
-    // (the last scores come before the last but one weights' products: those are waited for first, lest their phase be taken for the last one's)
-    if (alive && done > 1) alive = warp_wait(smem_u32(&sm.o_done[s]), done & 1, dead);
     if (alive && done > 0) alive = warp_wait(smem_u32(&sm.o_done[s]), (done - 1) & 1, dead);
     if (!alive) l = __uint_as_float(0x7fc00000u);
     tcgen05_fence_after();
@@ -674,7 +681,7 @@ template <int DIM, int VDIM, int KIND, bool PAIR> int launch(const TreeArgs& a, 
   }
   static const bool split_fits = [] {                              // the registers that the warps trade must be those that the block gets
     cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>) == cudaSuccess && at.numRegs * THREADS >= 128 * (2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS);
+    return cudaFuncGetAttributes(&at, tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>) == cudaSuccess && at.numRegs == LAUNCH_REGS;
   }();
   LIA_CHECK_ARG(split_fits, "lia_tree_attn: the kernel was built with too few registers");
   int* timeouts = lia_timeout_word();

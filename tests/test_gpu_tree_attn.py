@@ -429,3 +429,23 @@ def test_a_drafted_tree_from_store_to_acceptance(ops):
         two = ops.tree_attn(q, pk, pv, torch.tensor([(1, p0 + 3, 0, 1)], dtype=torch.int32, device="cuda"), torch.empty(1, H * dim, dtype=BF16, device="cuda"), H, G, dim, dim, dim ** -0.5,
                             rows=1, max_ctx=p0 + 4, k_scale=pks, v_scale=pvs)
         assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("n,G,past", [(33, 56, 280), (130, 16, 200)])
+def test_many_blocks_and_no_wait_runs_out(ops, kind, n, G, past):
+    """Thousands of blocks of few steps each, over and over: every hand-over between a block's warps happens, the same bits come out, and no bounded wait has run out (a row whose block gave
+    one up is formed key by key, so that the result alone would not tell)."""
+    seqs = 64
+    kc, vc = (rnd(seqs, past + n, G, 128, seed=s) for s in (1, 2))
+    ks = vs = None
+    if kind != "bf16":
+        kc, vc = ((x.float() * 20).to(torch.int8) if kind == "int8" else x.to(E4M3) for x in (kc, vc))
+        ks, vs = (torch.rand(seqs, G, past + n, generator=torch.Generator("cuda").manual_seed(s), device="cuda") * 0.1 + 0.01 for s in (3, 4))
+    q = rnd(seqs * n, G * 128, seed=5)
+    segs = torch.tensor([(i, past - i, i * n, n) for i in range(seqs)], dtype=torch.int32, device="cuda")
+    from lia_b200 import _lib
+    before = _lib.load().lia_moe_timeouts()
+    outs = [ops.tree_attn(q, kc, vc, segs, torch.empty_like(q), G, G, 128, 128, 128 ** -0.5, rows=n, max_ctx=past + n, k_scale=ks, v_scale=vs) for _ in range(12)]
+    assert _lib.load().lia_moe_timeouts() == before
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
