@@ -5,8 +5,8 @@ requests per step.
 a portion of one, or a single decoded token) and the places among them whose logits are wanted; the engine gives a new
 request a slot of the model's per-sequence state (seq_state.SlotState), lays the entries' tokens out as the rows of one
 batch, cuts what exceeds the row budget into further passes, runs the model's ``forward_rows`` and frees the slots of the
-requests named in ``end``.  ``Engine.generate`` is greedy decoding on top of it (argmax on the device); the trace runner
-(bin/trace_run) drives the same ``step``.
+requests named in ``end``.  ``Engine.generate`` is greedy decoding on top of it (argmax on the device), ``Engine.score`` says how
+likely given texts are (log probabilities, entropies and alternatives on the device); the trace runner (bin/trace_run) drives the same ``step``.
 
 A pass in which every request brings ONE token (a decode step) is launch-bound when run eagerly -- some sixty kernels of
 a few microseconds each -- so it is captured as a CUDA graph the second time its shape comes up and replayed from then
@@ -217,4 +217,37 @@ class Engine:
                 out[i].append(tok)
         for i in ids:
             self.slots.free(i)
+        return out
+
+    def score(self, prompts, top=0, chunk=None):
+        """How likely each token of ``prompts`` (lists of ids, any lengths) was after those before it, as one batch: prompts in portions of ``chunk`` tokens (None: as many as fill a pass).
+        Returns a dict per prompt with lists over its tokens but the first: ``logp``, the ``entropy`` of the distribution that the token came from (nats), and the ``top`` <= 32 most likely
+        tokens there, as (id, log probability) pairs in ``alternatives``."""
+        prompts = [[int(t) for t in p] for p in prompts]
+        keys = [("score", i) for i in range(len(prompts))]
+        out = [{"logp": [], "entropy": [], "alternatives": []} for _ in prompts]
+        portion = chunk or max(1, self.max_rows // max(1, len(prompts)))
+        try:
+            for at in range(0, max((len(p) for p in prompts), default=0), portion):
+                entries, given, whose = [], [], []
+                for i, p in enumerate(prompts):
+                    t, nxt = p[at:at + portion], p[at + 1:at + 1 + portion]
+                    if t:
+                        entries.append({"id": keys[i], "tokens": t, "want": list(range(len(nxt)))})
+                        given += nxt
+                        whose += [i] * len(nxt)
+                logits = self.step(entries)
+                if logits is None:
+                    continue
+                logp, entropy, best, ids = ops.token_logprobs(logits, torch.tensor(given, dtype=torch.int64, device=self.device), top=top)
+                logp, entropy, best, ids = (t.tolist() for t in (logp, entropy, best, ids))
+                self.check()
+                for r, i in enumerate(whose):
+                    out[i]["logp"].append(logp[r])
+                    out[i]["entropy"].append(entropy[r])
+                    out[i]["alternatives"].append(list(zip(ids[r], best[r])))
+        finally:
+            for k in keys:
+                if self.slots.slot_of(k) is not None:
+                    self.slots.free(k)
         return out

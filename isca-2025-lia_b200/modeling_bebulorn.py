@@ -138,11 +138,12 @@ class _Layer:
 class BebulornForCausalLM:
     step_serving = True          # served through engine.Engine (requests, slots, portions)
 
-    def __init__(self, config, device="cuda", dtype=BF16):
+    def __init__(self, config, device="cuda", dtype=BF16, cache_dtype=None):
+        """``cache_dtype``: int8 or float8_e4m3fn for the attention layers' keys and values (None: ``dtype``)."""
         _lib.load()
         if dtype not in (BF16, F32):
             raise ValueError("dtype must be torch.bfloat16 or torch.float32")
-        self.config, self.device, self.dtype = config, torch.device(device), dtype
+        self.config, self.device, self.dtype, self.cache_dtype = config, torch.device(device), dtype, cache_dtype
         self.layers = []
         self.runs = config.layer_runs()
         self.embed = self.head = self.final_norm = None
@@ -174,7 +175,7 @@ class BebulornForCausalLM:
                 mixer = DecayLinearAttentionMixer(w, m["heads"], m["dim"], m["vdim"], m["decay"], cfg.norm_eps, dt, dev)
             elif l["type"] == "attention":
                 mixer = WindowAttentionMixer(w, m["heads"], m["kv_heads"], m["dim"], m["vdim"], m["mask"]["size"], m["scale"], m.get("softcap", 0.0),
-                                             cfg.norm_eps, dt, dev)
+                                             cfg.norm_eps, dt, dev, cache_dtype=self.cache_dtype)
             else:
                 mixer = DeltaRuleMixer(w, m["heads"], m["kv_heads"], m["dim"], m["vdim"], m["conv"], cfg.norm_eps, dt, dev)
             mlp, n2, n2b = None, None, None
@@ -215,13 +216,13 @@ class BebulornForCausalLM:
         return self.load_weights(lambda n: cache.setdefault(n, make(n)))
 
     @classmethod
-    def from_pretrained(cls, path, device="cuda", dtype=BF16, **unused):
+    def from_pretrained(cls, path, device="cuda", dtype=BF16, cache_dtype=None, **unused):
         from .checkpoint import SafetensorsFile
         cfg = BebulornConfig.from_dict(json.load(open(os.path.join(path, "config.json"))),
                                        name=os.path.basename(os.path.abspath(path)) or "bebulorn")
         f = SafetensorsFile(os.path.join(path, "model.safetensors"))
         try:
-            return cls(cfg, device, dtype).load_weights(f.get)
+            return cls(cfg, device, dtype, cache_dtype).load_weights(f.get)
         finally:
             f.close()
 

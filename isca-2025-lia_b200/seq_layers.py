@@ -413,9 +413,14 @@ class DeltaRuleMixer:
 class WindowAttentionMixer:
     """Softmax attention over the last ``window`` positions, ``kv_heads`` key/value heads shared by groups of query heads, no
     positional rotation.  Values are divided by their per-head root mean square before they are cached; a score is
-    (q . k) * scale * temp_h, then softcap * tanh(score / softcap) (csrc/window_attn.cu); output Wo on the concatenated heads."""
+    (q . k) * scale * temp_h, then softcap * tanh(score / softcap) (csrc/window_attn.cu); output Wo on the concatenated heads.
+    ``cache_dtype`` int8 or float8_e4m3fn: keys and values are cached in 8 bits with a scale per head and token (csrc/kv_8bit.cu, csrc/tree_attn.cu): half the memory, and less of
+    it to read for every token; bf16 layers with heads of 64 or 128 channels."""
 
-    def __init__(self, w, heads, kv_heads, dim, vdim, window, scale, softcap, norm_eps, dtype, device, norm_values=True):
+    def __init__(self, w, heads, kv_heads, dim, vdim, window, scale, softcap, norm_eps, dtype, device, norm_values=True, cache_dtype=None):
+        if cache_dtype is not None and (cache_dtype not in (torch.int8, torch.float8_e4m3fn) or dtype != BF16 or dim not in (64, 128) or vdim not in (64, 128)):
+            raise ValueError(f"caches of 8 bits are int8 or float8_e4m3fn, for bf16 layers with heads of 64 or 128 channels, not {cache_dtype} for {dtype} with heads of {dim} and {vdim}")
+        self.cache_dtype = cache_dtype
         if heads % kv_heads:
             raise ValueError(f"{heads} heads do not divide into {kv_heads} key/value heads")
         self.H, self.G, self.dim, self.vdim, self.window = heads, kv_heads, dim, vdim, int(window)
@@ -426,15 +431,23 @@ class WindowAttentionMixer:
         self.out = Linear([w["o"]], dtype, device)
 
     def new_state(self, slots):
+        if self.cache_dtype is not None:
+            return (*slots.add_rows_8bit(self.G, self.dim, self.cache_dtype), *slots.add_rows_8bit(self.G, self.vdim, self.cache_dtype))
         return (slots.add_rows(self.G * self.dim, self.dtype), slots.add_rows(self.G * self.vdim, self.dtype))
 
     def __call__(self, h, batch, state):
-        kc, vc = state
         M = h.shape[0]
         y = self.proj(h)
         q, k, v = (self.proj.part(y, i) for i in range(3))
-        ops.kv_store(k, v, batch.meta, kc, vc, self.G, self.dim, self.vdim, self.eps, self.norm_values)
         o = torch.empty(M, self.H * self.vdim, dtype=self.dtype, device=h.device)
+        if self.cache_dtype is not None:
+            kc, ks, vc, vs = state
+            ops.kv_store_8bit(k, v, batch.meta, kc, vc, ks, vs, self.G, self.dim, self.vdim, self.eps, self.norm_values)
+            ops.tree_attn(q, kc, vc, batch.segs, o, self.H, self.G, self.dim, self.vdim, self.scale, rows=batch.lengths[1] if batch.lengths else M, max_ctx=batch.max_ctx, temp=self.temp,
+                          window=self.window, softcap=self.softcap, k_scale=ks, v_scale=vs)
+            return self.out(o)
+        kc, vc = state
+        ops.kv_store(k, v, batch.meta, kc, vc, self.G, self.dim, self.vdim, self.eps, self.norm_values)
         ops.window_attn(q, kc, vc, batch.meta, self.temp, o, self.H, self.G, self.dim, self.vdim, self.window, self.scale, self.softcap,
                         nseg=batch.segs.shape[0], segs=batch.segs, max_ctx=batch.max_ctx, form=batch.window_form)
         return self.out(o)

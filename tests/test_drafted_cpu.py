@@ -108,3 +108,42 @@ def test_slots_of_8_bit_rows():
         assert codes.shape == (3, 17, 256) and codes.dtype == dtype and scales.shape == (3, 4, 17) and scales.dtype == F32
     with pytest.raises(ValueError):
         s.add_rows_8bit(4, 64, BF16)
+
+
+def test_scores_are_put_together(lib, monkeypatch):
+    """Engine.score's bookkeeping on a stand-in for a model: the distribution after a token depends on the token and its place alone."""
+    from lia_b200 import ops
+    from lia_b200.engine import Engine
+    from lia_b200.seq_state import SlotState
+
+    class Model:
+        device = torch.device("cpu")
+        config = type("C", (), {"vocab": 11})
+
+        def new_state(self, n, cap):
+            return SlotState(n, cap, "cpu")
+
+        def graph_class(self, n):
+            return n
+
+        def forward_rows(self, ids, batch, want, slots, trace=None):
+            rows = torch.stack([self.logits(int(t), int(p)) for t, (_, p) in zip(ids, batch.meta.tolist())])
+            return None if want is None else rows[want.long()]
+
+        def logits(self, token, place):
+            return torch.sin(torch.arange(11.0) * (token + 2) + place)
+
+    def plain(logits, given, top=0):
+        logp = torch.log_softmax(logits, -1)
+        best, ids = logp.sort(dim=-1, descending=True, stable=True)
+        return logp.gather(1, given.view(-1, 1))[:, 0], -(logp.exp() * logp).sum(-1), best[:, :top], ids[:, :top]
+    monkeypatch.setattr(ops, "token_logprobs", plain)
+    m = Model()
+    texts = [[1, 2, 3, 4, 5, 6, 7], [9], [], [3, 3]]
+    for chunk, rows in ((None, 4096), (2, 4096), (3, 4), (None, 3)):
+        got = Engine(m, 16, max_requests=4, max_rows=rows).score(texts, top=2, chunk=chunk)
+        for text, g in zip(texts, got):
+            want = [torch.log_softmax(m.logits(t, i), -1) for i, t in enumerate(text[:-1])]
+            assert g["logp"] == pytest.approx([float(w[t]) for w, t in zip(want, text[1:])])
+            assert [a[0][0] for a in g["alternatives"]] == [int(w.argmax()) for w in want] and all(len(a) == 2 for a in g["alternatives"])
+            assert g["entropy"] == pytest.approx([float(-(w.exp() * w).sum()) for w in want])
