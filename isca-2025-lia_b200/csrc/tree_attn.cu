@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
   // ---- which keys
   const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + S::ROWS - 1) / a.rep);
   int near = i0, far = i1;                                         // depths of the block's tokens
-  if (a.depth != nullptr) {
+  if (a.depth != nullptr && a.window < 1 << 30) {                  // (without a window depths do not matter)
     near = 1 << 29;
     far = 0;
     for (int i = i0 + lane; i <= i1; i += 32) {

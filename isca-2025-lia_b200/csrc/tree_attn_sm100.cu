@@ -48,6 +48,7 @@ struct Tail {
   float ks[8][KEYS], lv[8][KEYS], rv[8][KEYS];                     // of a stage's keys: scale; of its values: log2 of what is left of the scale, and the inverse of that
   uint64_t odd[8];                                                 // of a stage: a byte for every warp that has brought a value with a scale far from REF
   float2 ml[ROWS];
+  float row_f[2 * ROWS];                                           // what a row's products with keys are multiplied by
   uint64_t full[8], empty[8], s_full[2][2], p_full[2][2], o_done[2], q_full, drain;
   uint32_t tmem;
   int dead;
@@ -104,21 +105,21 @@ __device__ __forceinline__ uint32_t seen32(const TreeArgs& a, const Portion& p, 
   return bits;
 }
 
+__device__ __forceinline__ void put8(uint32_t addr, const uint2& u) { asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(u.x), "r"(u.y) : "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the eight softmax warps
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-// REF, as an exponent: of the largest finite scale of `n` <= 64 positions
-__device__ __forceinline__ int ref_of(const float* scale, int n) {
+// REF, as an exponent: of the largest finite scale of `n` <= 64 positions, two of them a lane
+__device__ __forceinline__ void ask_ref(const float* scale, int n, uint32_t (&u)[2]) {
   const int lane = threadIdx.x & 31;
-  uint32_t top = 0;
 #pragma unroll
-  for (int x = 0; x < 64; x += 32) {
-    const uint32_t u = x + lane < n ? __float_as_uint(__ldcg(scale + x + lane)) : 0u;
-    if (u < 0x7f800000u) top = max(top, u);                        // (not a negative one either)
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
+  for (int x = 0; x < 2; ++x) u[x] = x * 32 + lane < n ? __float_as_uint(__ldcg(scale + x * 32 + lane)) : 0u;
+}
+__device__ __forceinline__ int ref_of(const uint32_t (&u)[2]) {
+  const uint32_t top = __reduce_max_sync(0xffffffffu, max(u[0] < 0x7f800000u ? u[0] : 0u, u[1] < 0x7f800000u ? u[1] : 0u));   // (not a negative one either)
   return top >= 0x00800000u ? min((int)(top >> 23) - 127, 100) : 0;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
       }
       mbar_init(smem_u32(&sm.o_done[i]), 1);
     }
-    mbar_init(smem_u32(&sm.q_full), PAIR ? 8 : 4);
+    mbar_init(smem_u32(&sm.q_full), 8);
     mbar_init(smem_u32(&sm.drain), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
   // ---- which keys
   const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + TILE - 1) / a.rep);
   int near = i0, far = i1;
-  if (a.depth != nullptr) {
+  if (a.depth != nullptr && a.window < 1 << 30) {                  // (without a window depths do not matter)
     near = 1 << 29;
     far = 0;
     for (int i = i0 + lane; i <= i1; i += 32) {
@@ -201,52 +202,62 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     const bool there = row < R, warp_there = row - lane < R;
     const int i = there ? row / a.rep : p.n - 1, h = there ? g * a.rep + row - i * a.rep : g * a.rep;
     const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
-    float rf = a.scale * (a.temp != nullptr ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
-    const bool flip = rf < 0.f;                                    // (so that the largest product is the largest score)
-    {                                                              // queries go to shared memory (those of both groups' rows from the first), and their factor is known
-      const bf16* src = a.q + (long long)(p.row + i) * a.ldq + h * DIM;
-      uint32_t top = 0;
-      uint2 u[DIM / 4];
+    uint32_t scales[2] = {0u, 0u};
+    if constexpr (BITS8) ask_ref(a.v.scale_at(p.slot, g) + start, n > 0 ? min(hi - start, KEYS) : 0, scales);
+    // ---- queries go to shared memory, a row a warp at a time, and what a row's products are multiplied by to sm.row_f
+    constexpr int SHARE = TILE / 8;
+    const int c4 = lane * 4, place = BITS8 ? place_of<DIM>(c4 >> 4, (c4 >> 3) & 1) + (c4 & 7) : c4;     // a lane's four channels, and where they go
+    const uint32_t lane_at = queries + (place >> 6) * C::Q_SLAB + (place & 7) * 2;
+    const int chunk = (place & 63) >> 3;
+    const float factor_all = a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
+    int rr = warp * SHARE, qi = (r0 + rr) / a.rep, qh = r0 + rr - qi * a.rep;                            // the row in the tile, its token and its head of the group's
+#pragma unroll 1
+    for (int x0 = 0; x0 < SHARE && (r0 + rr) / 32 * 32 < R; x0 += 8) {                                  // (warps without a row need none)
+      uint2 u[8];
+      float f[8];
 #pragma unroll
-      for (int c = 0; c < DIM / 4; ++c) {
-        u[c] = there ? *reinterpret_cast<const uint2*>(src + c * 4) : make_uint2(0u, 0u);
-        top = max(top, max(max(u[c].x & 0x7fffu, (u[c].x >> 16) & 0x7fffu), max(u[c].y & 0x7fffu, (u[c].y >> 16) & 0x7fffu)));
-      }
-      const Down down = down_of(top);
-      const float by = flip ? -down.by : down.by;
-      if constexpr (BITS8) rf *= down.back;
-      rf = fabsf(rf);
-      if (PAIR || s == 0) {
-        const uint32_t to = queries + (PAIR ? s * C::Q_BYTES : 0) + r * 128;
-#pragma unroll
-        for (int e = 0; e < DIM / 8; ++e) {                        // eight of the products' columns
-          uint4 q;
-          if constexpr (BITS8) {
-            const int at = e * 8, c = DIM == 128 ? (at & 63) / 8 * 16 + (at >> 6) * 8 : at;
-            float x[8];
-            unpack_bf16x2(u[c / 4].x, x[0], x[1]);
-            unpack_bf16x2(u[c / 4].y, x[2], x[3]);
-            unpack_bf16x2(u[c / 4 + 1].x, x[4], x[5]);
-            unpack_bf16x2(u[c / 4 + 1].y, x[6], x[7]);
-            q = make_uint4(pack_f16x2(x[0] * by, x[1] * by), pack_f16x2(x[2] * by, x[3] * by), pack_f16x2(x[4] * by, x[5] * by), pack_f16x2(x[6] * by, x[7] * by));
-          } else {
-            const uint32_t sign = flip ? 0x80008000u : 0u;
-            q = make_uint4(u[2 * e].x ^ sign, u[2 * e].y ^ sign, u[2 * e + 1].x ^ sign, u[2 * e + 1].y ^ sign);
-          }
-          put16(to + (e >> 3) * C::Q_SLAB + (((e & 7) ^ (r & 7)) << 4), q);
+      for (int x = 0; x < 8; ++x) {
+        const bool in = r0 + rr + x < R;
+        u[x] = in && lane < DIM / 4 ? *reinterpret_cast<const uint2*>(a.q + (long long)(p.row + qi) * a.ldq + (g * a.rep + qh) * DIM + c4) : make_uint2(0u, 0u);
+        f[x] = a.temp != nullptr && in ? a.temp[g * a.rep + qh] * factor_all : factor_all;
+        if (++qh == a.rep) {
+          qh = 0;
+          ++qi;
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full));
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x, ++rr) {
+        const bool flip = f[x] < 0.f;                              // (so that the largest product is the largest score)
+        uint2 w;
+        if constexpr (BITS8) {
+          const uint32_t m = __vmaxu2(u[x].x & 0x7fff7fffu, u[x].y & 0x7fff7fffu);
+          const Down down = down_of(__reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16)));
+          const float by = flip ? -down.by : down.by;
+          float y[4];
+          unpack_bf16x2(u[x].x, y[0], y[1]);
+          unpack_bf16x2(u[x].y, y[2], y[3]);
+          w = make_uint2(pack_f16x2(y[0] * by, y[1] * by), pack_f16x2(y[2] * by, y[3] * by));
+          f[x] *= down.back;
+        } else {
+          const uint32_t sign = flip ? 0x80008000u : 0u;
+          w = make_uint2(u[x].x ^ sign, u[x].y ^ sign);
+        }
+        if (lane < DIM / 4) put8(lane_at + (PAIR ? (rr >> 7) * C::Q_BYTES : 0) + (rr & 127) * 128 + ((chunk ^ (rr & 7)) << 4), w);
+        if (lane == 0) sm.row_f[rr] = fabsf(f[x]);
       }
     }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sm.q_full));
+    softmax_sync();
+    const float rf = sm.row_f[PAIR ? s * ROWS + r : r];
     const int first = first_key(a, p, depth_of(a, p, i));
     const float two_by_cap = a.softcap > 0.f ? 2.f * LOG2E / a.softcap : 0.f;
     const uint32_t values = lanes + VALUES + s * 128;
     float m = -1e30f, l = 0.f;
     bool alive = true;
     int done = 0;                                                  // of the group's blocks
-    const int ref = BITS8 && n > 0 ? ref_of(a.v.scale_at(p.slot, g) + start, min(hi - start, KEYS)) : 0;
+    const int ref = BITS8 ? ref_of(scales) : 0;
     const float ref_l = (float)ref, ref_inv = pow2(-ref);
     // (a row's first block sees to a maximum; -1e30 stands for none, so that nothing is less than it but -inf)
 #pragma unroll 1
@@ -418,8 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     float top = m, sum = l, f0 = n > 0 ? 1.f : 0.f, f1 = 0.f;
     const bool two = !PAIR && n > 1;
     if constexpr (!PAIR) {
-      auto groups_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-      groups_sync();
+      softmax_sync();
       if (s == 1) {
         sm.ml[r] = make_float2(m, l);
         if (two) {
@@ -433,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
           }
         }
       }
-      groups_sync();
+      softmax_sync();
       const float2 ml = sm.ml[r];
       top = fmaxf(m, ml.x);
       f0 = n > 0 ? ex2(m - top) : 0.f;
@@ -498,8 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     // the lane's places in the next block to ask for
     const uint8_t *kp = a.k.at(p.slot, start + k0, g) + kt * 16, *vp = a.v.at(p.slot, start + v0, g) + vt * 16;
     const float *ksp = BITS8 ? a.k.scale_at(p.slot, g) + start : nullptr, *vsp = BITS8 ? a.v.scale_at(p.slot, g) + start : nullptr;
-    const int ref = BITS8 && n > 0 ? ref_of(vsp, min(hi - start, KEYS)) : 0;
-    const float ref_inv = pow2(-ref);
+    uint32_t scales[2] = {0u, 0u};
     uint4 kr[C::AHEAD][C::KN], vr[C::AHEAD][C::VN];
     float ks[C::AHEAD], vs[C::AHEAD][C::VN];                       // of key th < 64, and of the lane's values
     auto ask = [&](int j, int x) {
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
         if constexpr (BITS8) {
           if (th < KEYS) ks[x] = th < left ? __ldcg(ksp + th) : 0.f;
 #pragma unroll
-          for (int c = 0; c < C::VN; ++c) vs[x][c] = v0 + c * VSTEP < left ? __ldcg(vsp + v0 + c * VSTEP) : pow2(ref);
+          for (int c = 0; c < C::VN; ++c) vs[x][c] = v0 + c * VSTEP < left ? __ldcg(vsp + v0 + c * VSTEP) : -1.f;     // (none)
         }
       }
       kp += KEYS * a.k.pos;
@@ -545,6 +554,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     };
 #pragma unroll
     for (int x = 0; x < C::AHEAD; ++x) ask(x, x);
+    if constexpr (BITS8) ask_ref(a.v.scale_at(p.slot, g) + start, n > 0 ? min(hi - start, KEYS) : 0, scales);
+    const int ref = BITS8 ? ref_of(scales) : 0;
+    const float ref_inv = pow2(-ref);
     bool alive = true;
 #pragma unroll 1
     for (int j0 = 0; j0 < n && alive; j0 += C::AHEAD) {
@@ -568,10 +580,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
             uint4 lo16, hi16;
             widen<KIND>(vr[x][c], lo16, hi16);
             const float f = vs[x][c] * ref_inv;
-            const bool near = f >= 0x1p-8f && f < 64.f;
+            const bool near = (f >= 0x1p-8f && f < 64.f) || vs[x][c] == -1.f;
             odd |= !near;
             const __half2 f2 = __float2half2_rn(near ? f : 1.f);
-            scale4(lo16, f2);
+            scale4(lo16, f2);                                      // (zeros, where there is none)
             scale4(hi16, f2);
             put(at + v_at + c * VSTEP * 128, VDIM == 128, lo16, hi16);
             if (vt == 0) {
