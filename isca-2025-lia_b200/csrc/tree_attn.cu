@@ -17,7 +17,7 @@ int lia_tree_attn_tc(const void* args, int type, int rows, int nseg, lia_stream_
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, MAX_SPLITS = 64;
+constexpr int WARPS = 4, THREADS = WARPS * 32, MAX_SPLITS = 64, CLUSTER = 8;   // CLUSTER: up to so many blocks share a history as a cluster, more by way of a workspace
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
   pdl_wait();
   const Portion p = portion_of(a, blockIdx.z);
   if (!p.held) {
-    if (a.splits == 1 && blockIdx.y == 0) nan_rows<VDIM>(a, p);
+    if (a.splits <= CLUSTER && blockIdx.x == 0 && blockIdx.y == 0) nan_rows<VDIM>(a, p);
     return;
   }
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, gq = lane >> 2, t4 = lane & 3;   // (known to be the same in all lanes)
@@ -376,6 +376,10 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     }
     if (a.splits == 1) {
       put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
+    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read)
+#pragma unroll
+      for (int c = 0; c < N; ++c) os[r * VDIM + lane * N + c] = y[c];
+      if (lane == 0) part[r] = make_float2(top, sum);
     } else {
       const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;
 #pragma unroll
@@ -383,6 +387,35 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
       if (lane == 0) reinterpret_cast<float2*>(a.ws + a.splits * rows * VDIM)[at] = make_float2(top, sum);
     }
   }
+  if (a.splits == 1 || a.splits > CLUSTER) return;
+  // ---- the blocks that share a history are a cluster: each joins some of the rows, always in the same order
+  cluster_barrier();
+  for (int r = warp * a.splits + blockIdx.x; r < S::ROWS && r0 + r < R; r += WARPS * a.splits) {
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    float2 ml[CLUSTER];
+    float w[CLUSTER][N], top = NONE, sum = 0.f, y[N] = {};
+#pragma unroll
+    for (int q = 0; q < CLUSTER; ++q) {
+      if (q < a.splits) {
+        ml[q] = cluster_ld_f2(cluster_place(&part[r], q));
+        const uint32_t from = cluster_place(&os[r * VDIM + lane * N], q);
+        if constexpr (N == 4) *reinterpret_cast<float4*>(w[q]) = cluster_ld_f4(from);
+        else *reinterpret_cast<float2*>(w[q]) = cluster_ld_f2(from);
+        top = fmaxf(top, ml[q].x);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < CLUSTER; ++q) {
+      if (q < a.splits) {
+        const float f = ex2(ml[q].x - top);
+        sum = fmaf(ml[q].y, f, sum);
+#pragma unroll
+        for (int c = 0; c < N; ++c) y[c] = fmaf(w[q][c], f, y[c]);
+      }
+    }
+    put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
+  }
+  cluster_barrier();                                               // (no block leaves while it is read)
 }
 
 // How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history
@@ -406,7 +439,7 @@ Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type
   p.splits = s < 1 ? 1 : (int)s;
   return p;
 }
-size_t floats_of(const Plan& p, int M, int H, int vdim) { return p.splits > 1 ? (size_t)p.splits * M * H * (vdim + 2) : 0; }
+size_t floats_of(const Plan& p, int M, int H, int vdim) { return p.splits > (p.nr >= 16 ? 1 : CLUSTER) ? (size_t)p.splits * M * H * (vdim + 2) : 0; }
 
 template <int DIM, int VDIM, int KIND, int NR> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
   using S = Shape<DIM, VDIM, KIND, NR>;
@@ -417,14 +450,16 @@ template <int DIM, int VDIM, int KIND, int NR> int launch(const TreeArgs& a, int
     LIA_CUDA(cudaFuncSetAttribute(tree_attn_kernel<DIM, VDIM, KIND, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     if (dev < 64) configured[dev] = true;
   }
-  LIA_CUDA(lia_launch(tree_attn_kernel<DIM, VDIM, KIND, NR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), S::SMEM, stream, a));
+  const dim3 grid(a.splits, a.tiles * a.G, nseg);
+  if (a.splits > 1 && a.splits <= CLUSTER) LIA_CUDA(lia_launch_cluster(a.splits, tree_attn_kernel<DIM, VDIM, KIND, NR>, grid, dim3(THREADS), S::SMEM, stream, a));
+  else LIA_CUDA(lia_launch(tree_attn_kernel<DIM, VDIM, KIND, NR>, grid, dim3(THREADS), S::SMEM, stream, a));
   return LIA_OK;
 }
 template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
   const int rc = nr >= 16 ? lia_tree_attn_tc(&a, KIND, nr * 8, nseg, stream)
                  : nr == 4 ? launch<DIM, VDIM, KIND, 4>(a, nseg, stream)
                  : nr == 2 ? launch<DIM, VDIM, KIND, 2>(a, nseg, stream) : launch<DIM, VDIM, KIND, 1>(a, nseg, stream);
-  if (rc == LIA_OK && a.splits > 1) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
+  if (rc == LIA_OK && a.splits > (nr >= 16 ? 1 : CLUSTER)) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
   return rc;
 }
 template <int KIND> int launch_dims(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
@@ -454,7 +489,7 @@ extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* k
   LIA_CHECK_ARG(mask == nullptr || rows <= 64 * words, "lia_tree_attn: %d words of mask do not hold %d tokens", words, rows);
   const Plan plan = plan_of(nseg, rows, max_ctx, H, G, window, kc->type);
   LIA_CHECK_ARG(nseg <= 65535 && (long long)plan.tiles * G <= 65535, "lia_tree_attn: too many portions, or rows of one");
-  LIA_CHECK_ARG(plan.splits == 1 || (ws && ws_floats >= floats_of(plan, M, H, vc->dim) && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_tree_attn: needs a workspace of %zu floats",
+  LIA_CHECK_ARG(floats_of(plan, M, H, vc->dim) == 0 || (ws && ws_floats >= floats_of(plan, M, H, vc->dim) && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_tree_attn: needs a workspace of %zu floats",
                 floats_of(plan, M, H, vc->dim));
   const TreeArgs a{reinterpret_cast<const bf16*>(q), ldq, cache8(kc), cache8(vc), segs, reinterpret_cast<const unsigned long long*>(mask), words, depth, temp,
                    reinterpret_cast<bf16*>(out), ws, M, H, G, H / G, rows, window > 0 ? window : 1 << 30, plan.splits, plan.tiles, scale, softcap};

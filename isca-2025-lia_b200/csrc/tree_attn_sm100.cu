@@ -41,7 +41,7 @@ struct Tc {
   static constexpr int ALL_Q = (PAIR ? 2 : 1) * Q_BYTES, ROOM = (221184 - ALL_Q) / STAGE, STAGES = ROOM > 8 ? 8 : ROOM;
   static constexpr int KT = DIM * (BITS8 ? 1 : 2) / 16, VT = VDIM * (BITS8 ? 1 : 2) / 16;      // lanes of a key, of a value
   static constexpr int KN = KEYS * KT / LOADERS, VN = KEYS * VT / LOADERS;                       // vectors of a lane
-  static constexpr int AHEAD = BITS8 ? 3 : 2;                      // blocks on their way from memory
+  static constexpr int AHEAD = BITS8 ? 2 : 1;                      // blocks of 16 or 32 KB on their way from memory (more: more instructions to bring, 5 to 30 % slower with four)
   static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // weights are 2^(x - maximum + LIFT): below 2^15 in fp16
 };
 struct Tail {
@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     far = __reduce_max_sync(0xffffffffu, far);
   }
   const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = a.mask != nullptr ? p.p0 : p.p0 + i0 + 1;
-  const int nb = (hi - lo + KEYS - 1) / KEYS, b0 = (int)((long long)nb * blockIdx.x / a.splits), n = (int)((long long)nb * (blockIdx.x + 1) / a.splits) - b0;
+  const int nb = (hi - lo + KEYS - 1) / KEYS, b0 = __shfl_sync(0xffffffffu, (int)((long long)nb * blockIdx.x / a.splits), 0),
+            n = __shfl_sync(0xffffffffu, (int)((long long)nb * (blockIdx.x + 1) / a.splits), 0) - b0;
   const int start = lo + b0 * KEYS;
 
   if (warp < 8) {

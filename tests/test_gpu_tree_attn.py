@@ -449,3 +449,19 @@ def test_many_blocks_and_no_wait_runs_out(ops, kind, n, G, past):
     outs = [ops.tree_attn(q, kc, vc, segs, torch.empty_like(q), G, G, 128, 128, 128 ** -0.5, rows=n, max_ctx=past + n, k_scale=ks, v_scale=vs) for _ in range(12)]
     assert _lib.load().lia_moe_timeouts() == before
     assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("kind", ["int8", "bf16"])
+@pytest.mark.parametrize("nseg", [9, 10, 12, 14, 18, 24, 37, 75])
+def test_blocks_that_share_a_history(ops, kind, nseg):
+    """One to eight blocks of a cluster, whichever the number of requests leaves room for, with portions of no tokens and of slots that are not there among them."""
+    portions = [(i, 2500 - 61 * (i % 30), 0 if i == 5 else 2) for i in range(nseg)]
+    c = Case(portions, 16, 8, 64, 64, kind)
+    c.check(c.run(ops), kind)
+    lost = c.segs[3]
+    c.segs[3] = (nseg + 7, *lost[1:])
+    out = c.run(ops, out=torch.full_like(c.out, 77.0))
+    assert torch.isnan(out[lost[2]:lost[2] + 2].float()).all()
+    out[lost[2]:lost[2] + 2] = 77.0
+    del c.segs[3]
+    c.check(out, kind)
