@@ -3,8 +3,8 @@
 //   with m = max x, L = sum e^(x - m), A = sum e^(x - m) (x - m):   log p(t) = x_t - m - ln L,   entropy = ln L - A / L
 //
 // One pass over the logits: every thread keeps a running maximum with its L and A (a larger maximum multiplies both by a power and moves A by L times the step).  The largest ones are
-// found from what that leaves: the top-th largest of the 256 threads' maxima is reached by at least `top` logits and, as the largest ones seldom share a thread, by few more; the threads
-// that have one are known by their maxima, so that only their logits are read again (a tenth of the row, from L2), by all lanes of their warps.  What reaches the bound is sorted across a warp's lanes,
+// found from what that leaves: the top-th largest of the 256 threads' maxima is reached by at least `top` logits and, as the largest ones seldom share a thread, by few more; every thread
+// knows the maxima of four parts of its logits, so that only the parts that reach it are read again (a fortieth of the row, from L2), by all lanes of their warps.  What reaches the bound is sorted across a warp's lanes,
 // as whole numbers that order by value and then by lower id.  (A list of the largest ones kept by every warp through the pass took 34 instructions a logit instead of 7.)
 // Few rows share out a row over a cluster of up to eight blocks of threads, whose first one joins the parts (in the same order each time).
 //
@@ -69,7 +69,6 @@ __device__ __forceinline__ u64 sort_up(u64 v, int lane) {
     for (int o = k >> 1; o > 0; o >>= 1) v = exchange(v, o, ((lane & k) == 0) == ((lane & o) != 0));
   return v;
 }
-__device__ __forceinline__ u64 sort_down(u64 v, int lane) { return sort_up(v, lane ^ 31); }
 // list falls with the lane, more rises: the 32 largest of both, falling
 __device__ __forceinline__ u64 merge_down(u64 list, u64 more, int lane) {
   u64 v = list > more ? list : more;
@@ -78,6 +77,26 @@ __device__ __forceinline__ u64 merge_down(u64 list, u64 more, int lane) {
   return v;
 }
 
+// the same of plain whole numbers, for bounds
+__device__ __forceinline__ uint32_t sort_down32(uint32_t v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int o = k >> 1; o > 0; o >>= 1) {
+      const uint32_t w = __shfl_xor_sync(0xffffffffu, v, o);
+      v = ((lane & k) == 0) == ((lane & o) == 0) ? max(v, w) : min(v, w);
+    }
+  return v;
+}
+__device__ __forceinline__ uint32_t merge_down32(uint32_t list, uint32_t more, int lane) {
+  uint32_t v = max(list, more);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint32_t w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = (lane & o) == 0 ? max(v, w) : min(v, w);
+  }
+  return v;
+}
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4, U = 4;                               // logits of a vector; vectors of a lane's share of a block
@@ -130,12 +149,13 @@ template <int W> __device__ __forceinline__ u64 join_lists(u64 list, u64 (*lists
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a) {
-  constexpr int N = Vec<T>::N, U = Vec<T>::U, SHARE = N * U, ROOM = 1024;
+  constexpr int N = Vec<T>::N, U = Vec<T>::U, SHARE = N * U, ROOM = 1024, PARTS = 4;
   __shared__ u64 found[ROOM];                                      // the logits that reach the bound
   __shared__ u64 lists[WARPS][32];
   __shared__ int count;
   __shared__ uint32_t bound;
-  __shared__ uint8_t hot[WARPS][32];
+  __shared__ uint8_t hot[WARPS][32 * PARTS];
+  __shared__ uint32_t bounds[WARPS][32];
   __shared__ Sums warp_sums[WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
   pdl_launch_dependents();
@@ -166,9 +186,12 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
 
   // ---- sums, and every thread's maximum
   Sums s{-INFINITY, 0.f, 0.f};
+  float parts[PARTS];                                              // the maximum of every fourth of the thread's shares
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) parts[q] = -INFINITY;
   uint4 u[U], next[U];
   load(b0 + warp, u);
-  for (int b = b0 + warp; b < b1; b += WARPS) {
+  for (int b = b0 + warp, turn = 0; b < b1; b += WARPS, turn = (turn + 1) & (PARTS - 1)) {
     load(b + WARPS, next);
     float f[SHARE], m = -INFINITY;
 #pragma unroll
@@ -176,6 +199,8 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
 #pragma unroll
     for (int i = 0; i < SHARE; ++i) m = fmaxf(m, f[i]);
     if (m > s.m) raise_to(s, m);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) parts[q] = turn == q ? fmaxf(parts[q], m) : parts[q];
     const float base = s.m == -INFINITY ? 0.f : s.m;
     f32x2 L = 0ull, A = 0ull;
 #pragma unroll
@@ -201,22 +226,33 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   if (a.top > 0) {
     // ---- the top-th largest of the threads' maxima bounds what can be among the top
     if (threadIdx.x == 0) count = 0;
-    const uint32_t most = (uint32_t)(key_of(s.m, 0) >> 32);
-    list = join_lists<WARPS>(sort_down((u64)most << 32 | 1u, lane), lists, warp, lane);
-    if (threadIdx.x == a.top - 1) bound = (uint32_t)(list >> 32);
+    uint32_t best = sort_down32((uint32_t)(key_of(s.m, 0) >> 32), lane);
+#pragma unroll
+    for (int half = WARPS / 2; half > 0; half >>= 1) {
+      if (warp >= half && warp < 2 * half) bounds[warp][31 - lane] = best;                // rising
+      __syncthreads();
+      if (warp < half) best = merge_down32(best, bounds[warp + half][lane], lane);
+    }
+    if (threadIdx.x == a.top - 1) bound = best;
     __syncthreads();
-    // ---- the threads that have something that reaches it: their vectors once more, by all lanes of their warp
-    const unsigned who = __ballot_sync(0xffffffffu, most >= bound);
-    if (most >= bound) hot[warp][__popc(who & ((1u << lane) - 1u))] = (uint8_t)lane;
+    // ---- the shares that hold something that reaches it, once more by all lanes of their warp
+    int shares = 0;
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      const bool in = (uint32_t)(key_of(parts[q], 0) >> 32) >= bound;
+      const unsigned who = __ballot_sync(0xffffffffu, in);
+      if (in) hot[warp][shares + __popc(who & ((1u << lane) - 1u))] = (uint8_t)(lane + 32 * q);
+      shares += __popc(who);
+    }
     __syncwarp();
-    const int mine = b0 + warp < b1 ? (b1 - b0 - warp + WARPS - 1) / WARPS * U : 0, items = __popc(who) * mine;
+    const int turns = b0 + warp < b1 ? (b1 - b0 - warp + WARPS - 1) / WARPS : 0, each = (turns + PARTS - 1) / PARTS * U, items = shares * each;
     for (int t0 = lane; t0 < items; t0 += 128) {
       uint4 w[4];
       int v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int t = t0 + j * 32, h = t / mine, r = t - h * mine;
-        v[j] = t < items ? (b0 + warp + r / U * WARPS) * 32 * U + r % U * 32 + hot[warp][h] : nv;
+        const int t = t0 + j * 32, h = t / each, r = t - h * each, from = t < items ? hot[warp][h] : 0, turn = r / U * PARTS + (from >> 5);
+        v[j] = t < items && turn < turns ? (b0 + warp + turn * WARPS) * 32 * U + r % U * 32 + (from & 31) : nv;
         w[j] = vector(v[j]);
       }
 #pragma unroll
@@ -226,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const u64 k = key_of(f[i], v[j] * N - skew + i);
-          if ((uint32_t)(k >> 32) >= bound && id_of(k) >= 0 && id_of(k) < a.V && t0 + j * 32 < items) {
+          if ((uint32_t)(k >> 32) >= bound && id_of(k) >= 0 && id_of(k) < a.V && v[j] < nv) {
             const int at = atomicAdd(&count, 1);                   // (in any order: they are sorted)
             if (at < ROOM) found[at] = k;
           }
