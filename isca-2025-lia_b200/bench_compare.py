@@ -94,6 +94,13 @@ def _cost(name, a, kw):
         keys = float(kw.get("_wkeys", 0))                                          # sum over rows of keys inside the window
         kind = "tc" if kc.dtype == BF16 and dim in (64, 128) and vdim in (64, 128, 256) else "f32"             # csrc/window_attn_mma.cu
         return 2.0 * keys * H * (dim + vdim), _nbytes(q, out) + kw.get("_wctx", 0) * G * (dim + vdim) * kc.element_size(), kind
+    if name == "tree_attn":
+        q, kc, out, H, G, dim, vdim = a[0], a[1], a[4], a[5], a[6], a[7], a[8]
+        per_key = dim + vdim + 8 if kc.element_size() == 1 else 2 * (dim + vdim)
+        return 2.0 * float(kw.get("_wkeys", 0)) * H * (dim + vdim), _nbytes(q, out) + kw.get("_wctx", 0) * G * per_key, "tc"
+    if name == "kv_store_8bit":
+        k, v, M, G = a[0], a[1], a[0].shape[0], a[7]
+        return 0.0, float(M * ((k.shape[1] + v.shape[1]) * (k.element_size() + 1) + 8 * G)), "mem"
     if name == "qkv_prep":
         y, q_out, kc, vc = a[0], a[3], a[4], a[5]
         M = y.shape[0]
@@ -161,7 +168,7 @@ def _cost(name, a, kw):
 class Instrument:
     NAMES = ("gemm", "linear", "linear_plain", "linear_small", "mlstm_scan", "headnorm_gate", "latent_prep", "latent_attn", "latent_attn_expanded", "clamped_glu",
              "rms_add_norm", "embed_rmsnorm", "rms_gather", "layernorm", "attn_prefill", "attn_decode", "embed", "argmax", "argmax_f32",
-             "linear_scan", "conv_prep", "conv_state_update", "kv_store", "window_attn", "ln_add_norm", "embed_rows", "ln_gather", "gated_act",
+             "linear_scan", "conv_prep", "conv_state_update", "kv_store", "window_attn", "kv_store_8bit", "tree_attn", "ln_add_norm", "embed_rows", "ln_gather", "gated_act",
              "router_topk", "moe_plan", "moe_gemm", "moe_gemm_tc", "moe_gather", "moe_expert_gemms", "moe_combine", "qkv_prep", "gated_rms_add", "poly_norm",
              "embed_scale_pos", "residual_norm", "rms_norm_rows", "sigmoid_mul", "softcap", "forget_gate_prep", "forget_scan", "diff_combine",
              "latent_store", "embed_bigram_pos", "streams_update", "streams_embed", "streams_gather", "conv_act", "ssd_scan", "rglru_scan", "silu_gate_norm")
