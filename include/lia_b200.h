@@ -579,8 +579,8 @@ int lia_moe_plan_rows(const int* idx, int pairs, int E, int tile_rows, int n_til
  * lia_moe_tc_rows() rows; A [n_tiles * rows][K]: the rows in the plan's order.  up: C [n_tiles * rows][N] bf16 = act(sum), or gated (weights [E][2N][K], gate
  * rows before up rows): act(gate) * up, both sums in fp32; weigh_in: the sums are first multiplied by their pair's wt.  down: C bf16 in the plan's
  * order, unweighted, or (c_f32) C [pairs][N] fp32 by pair, times wt unless weigh_in.  Tiles of experts >= E are skipped.  K, N multiples of 8.
- * A wait inside that does not end within seconds ends its CTA, which leaves NaN where its results should be and is counted, as are those of the state-space scan and of prompt
- * attention over windows and expanded latents: lia_moe_timeouts_seen() reads the count
+ * A wait inside that does not end within seconds ends its CTA, which leaves NaN where its results should be and is counted, as are those of the state-space scan, of prompt
+ * attention over windows and expanded latents and of attention of drafted tokens (which forms its rows again, key by key): lia_moe_timeouts_seen() reads the count
  * as far as launches have ended, lia_moe_timeouts() synchronises first. */
 int lia_moe_tc_rows(void);
 int lia_moe_timeouts(void);
@@ -675,9 +675,9 @@ int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const LiaCacheView
  * tokens: without mask those up to its own (under the same window), else those whose bits are set in its `words` 64-bit words of mask (bit j: the portion's token j).  depth_i:
  * depth[row + i], or i where depth is NULL.  A score is temp[h] * scale * (q . k), then softcap * tanh(score / softcap) if softcap > 0; query head h reads key/value head
  * h / (H / G).  A row that sees nothing is 0; what it does not see has no effect, whatever its bits.  Scales are 0 or more, values' up to 2^29 (values with a smaller one
- * than 2^-80 are off by 2^-71 at most).  Rows of no portion stay as they are; a portion that its slot, the M rows, the mask's
+ * than 2^-80 are off by 2^-71 at most).  No two portions share a row.  Rows of no portion stay as they are; a portion that its slot, the M rows, the mask's
  * words or `rows` cannot hold gives NaN rows.  rows: the most rows of a portion; max_ctx: about the longest p0 + n (it decides how many blocks share a history, no more).
- * q and out: bf16, ldq apart and [M, H * vdim].  Heads of 64 or 128 channels.  ws: lia_tree_attn_workspace_floats() floats (0: NULL will do). */
+ * q and out: bf16, ldq apart and [M, H * vdim].  Heads of 64 or 128 channels, 2^29 positions at most.  ws: lia_tree_attn_workspace_floats() floats (0: NULL will do). */
 size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx, int M, int H, int G, int dim, int vdim, int window, int type);
 int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
                   const float* temp, void* out, float* ws, size_t ws_floats, int M, int H, int G, int rows, int max_ctx, int window, float scale, float softcap, lia_stream_t stream);

@@ -8,7 +8,8 @@
 // as whole numbers that order by value and then by lower id.  (A list of the largest ones kept by every warp through the pass took 34 instructions a logit instead of 7.)
 // Few rows share out a row over a cluster of up to eight blocks of threads, whose first one joins the parts (in the same order each time).
 //
-// Memory bounds it for many rows (a logit is read once, eight instructions each), the latency of one block of logits and of sorting for few.
+// Bound, at 4096 rows of 50272 logits: fp32 by memory, 131 us without the largest ones (96 % of the rate of a copy) and 156 with the 20 largest; bf16, half the bytes, by instructions (eight a logit, a
+// power among them): 96 and 150 us.  Few rows by the latency of one block of logits and of sorting: four rows 9 us.
 #include "pairs.cuh"
 
 namespace {

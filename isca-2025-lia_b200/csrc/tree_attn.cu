@@ -3,13 +3,22 @@
 //   s_ij = cap tanh(temp_h scale ks_j (q_i . k_j) / cap),   o_i = sum_j p_ij vs_j v_j / sum_j p_ij,   p_ij = e^(s_ij - max) over the j that row i sees
 //
 // Few rows see a long history: what counts is that the history is read once, whatever the number of rows and of query heads that share a key head.  So a block has up to 32 of the
-// portion's (token, head) rows of one key head, its four warps take 16 keys each in turn, and the history is split over as many blocks as fill the GPU.  Keys and values go
+// portion's (token, head) rows of one key head, its four warps take 16 keys each in turn, and the history is split over as many blocks as fill the GPU: up to eight of them are a cluster and
+// read one another's sums, more leave theirs in a workspace for a second launch.  (With the workspace for these too, a token each of 16 sequences behind 1901 positions took 27 us instead of 23.)
+//
+// The keys are the rows of a product (16 of them) and the queries its columns (8), so that one token of up to eight query heads wastes little.  Keys and values go
 // from memory to the lanes that multiply them, without shared memory between: a product sums over channels in any order, so a lane's 16 neighbouring bytes of a key
-// are four steps' operands, and a product's columns may be any channels, so the 16 neighbouring bytes of four values are its operands for 16 (bf16: 8) products.
+// are four steps' operands, and a product's rows may be any channels, so the 16 neighbouring bytes of a value are its operands for 16 (bf16: 8) of them.  Weights come out of the
+// first product with keys along rows and go into the second with keys along the sum: eight by eight of them are transposed across the warp (movmatrix).
 //
 // 8-bit codes are exact in fp16 and so are multiplied there: q goes to fp16 by a power of two of its own for each row (its 8 bits fit; what is 2^-29 of the row's largest is
-// less exact), a key's scale is multiplied into its scores, and a value's into its weight -- in the exponent, s + log2 vs, so that the running maximum bounds the product and no scale is
-// too large or small: weights are 2^(s + log2 vs - max + 14) in fp16, 11 bits, and their sum takes p = weight / vs in fp32.  With bf16 caches weights are two bf16 parts: 16 bits.
+// less exact), a key's scale is multiplied into its scores, and a value's into its weight -- in the exponent, x = s + log2 vs, so that the maximum bounds the product and no scale is
+// too large or small: weights are 2^(x - max + 7) in fp16, 11 bits, and their sum takes p = weight / vs in fp32.  With bf16 caches weights are two bf16 parts: 16 bits.
+// The maximum moves only when a key exceeds it by 2^8, which the 7 leaves room for; the rows' sums are multiplied only then.
+//
+// Bound: bf16 caches by memory, 8-bit ones by instructions too (a byte is widened, half of them after two codes change places; a score takes some fifteen).  A token of 16 heads on 8 for each of 16
+// histories of 60000 positions: bf16 571 us (6.9 TB/s, what a copy reaches at the most), int8 438 (4.6), e4m3 390 (5.2).  Behind 1901 positions, int8: 23 us, of which memory 10; the rest is
+// one block's way from its first load to its last sum.
 #include "mma.cuh"
 #include "tree_attn.cuh"
 
@@ -422,9 +431,9 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 struct Plan {
   int nr, tiles, splits;                                           // nr: eights of rows; 16 and 32 of them on tcgen05
 };
-#ifndef TC_ROWS
-#define TC_ROWS 32
-#endif
+// Rows of a key head from which tcgen05 takes over: above 32 a history would be read a second time here.  us, tcgen05 | here: 58 rows behind 4099 positions, 8 sequences, int8 50 | 57, bf16
+// 48 | 98; 64 rows behind 131003 144 | 230 (bf16 167 | 445); 64 heads of keys with chains of 33 390 | 669.  With 32 rows and fewer this kernel's are the smaller, down to a half.
+constexpr int TC_ROWS = 32;
 Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
   const long long R = (long long)rows * (H / G);
   Plan p;
@@ -482,6 +491,7 @@ extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* k
   LIA_CHECK_ARG(!(wrong = cache8_wrong(kc, 16)) && !(wrong = cache8_wrong(vc, 16)), "lia_tree_attn: %s", wrong);
   LIA_CHECK_ARG((kc->dim == 64 || kc->dim == 128) && (vc->dim == 64 || vc->dim == 128), "lia_tree_attn: heads have 64 or 128 channels, not %d and %d", kc->dim, vc->dim);
   LIA_CHECK_ARG(kc->type == vc->type && kc->slots == vc->slots && kc->capacity == vc->capacity, "lia_tree_attn: caches of different types or sizes");
+  LIA_CHECK_ARG(kc->capacity <= 1 << 29, "lia_tree_attn: more than 2^29 positions");               // (positions, depths and windows are added up in 32 bits)
   LIA_CHECK_ARG(M >= 0 && nseg >= 0 && rows >= 0 && max_ctx >= 0 && G > 0 && H > 0 && H % G == 0, "lia_tree_attn: bad sizes");
   if (M == 0 || nseg == 0 || rows == 0) return LIA_OK;
   LIA_CHECK_ARG(q && segs && out && (mask == nullptr || words > 0), "lia_tree_attn: null pointer");

@@ -6,8 +6,8 @@
 //                    become zeros, so that nothing unwritten is multiplied.
 //   warp 16          the products (three more are there for their registers)
 // TMEM, 512 columns: group s has the scores of two blocks, one being worked on and the next one, at 128 s and 128 s + 64, in their place its weights (fp16, or two bf16 parts), and its
-// weighted values at 256 + 128 s.  (With one block's scores and the queries in TMEM too, a group waited 40 % of its time for scores that are issued behind its weights' products: an instruction
-// takes 65 clocks to issue, and a block 12.  The queries in shared memory cost nothing: 6 KB a product of 65 clocks are less than it takes in that time.)
+// weighted values at 256 + 128 s.  (With one block's scores and the queries in TMEM too, a group waited for scores that are issued behind its weights' products; the queries in shared memory
+// cost nothing: 6 KB a product are less than shared memory gives in that time.)
 // The weighted values stay in TMEM from block to block.  Weights are relative to a maximum that moves only when a row has exceeded it by 2^8 (they fit fp16 up to there); only then
 // its group multiplies what it has, behind the products of its last block.
 //
@@ -15,8 +15,11 @@
 // (rounded to 11 bits twice: 2^-11 each, as the weights are), which leaves the softmax one instruction less in three.  A value whose scale is not within 2^-8 to 2^6 of REF, one of nothing or NaN
 // among them, stays as it is and its scale joins the exponent (tree_attn.cu); a block with one takes a slower way.
 //
-// What bounds it at 128 rows and more: the powers (one a score, 16 a clock and SM: 512 clocks for 64 keys of 128 rows) as well as the tensor cores (512 with 8-bit codes, 768 with bf16 and its two
-// parts of weights) and, with 8 bits, the instructions that widen the codes; with fewer rows memory (700 clocks for 64 keys of 8 bits, 1400 of bf16).
+// What bounds it: at 128 rows and more the softmax -- a row of 64 scores is one thread's chain of loads from TMEM, a maximum, powers, sums and stores, and two groups of four warps hide little of
+// one another's (with the products halved the time stays as it is, and sixteen warps of it had too few registers) -- at 2.7 times the 512 clocks that 64 x 128 powers take; with fewer rows
+// memory (700 clocks for 64 keys of 8 bits, 1400 of bf16).  A block of threads begins and ends in 19 000 clocks, whatever its keys: loads of programs and of what depends on the portion, one behind
+// the other.  A tree of 64 tokens behind 131003 positions, int8, 32 heads on 8: 228 us; its products would take 83 at the tensor cores' rate, its bytes 42.
+// The issuing warp's block numbers are made uniform by a shuffle: without, each product took twice its instructions.
 #include "pairs.cuh"
 #include "tree_attn.cuh"
 #include "umma.cuh"
@@ -112,7 +115,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-// REF, as an exponent: of the largest finite scale of `n` <= 64 positions, two of them a lane
+// REF, as an exponent: of the largest finite scale of `n` <= 64 positions, two of them a lane.  Not below LEAST_SCALE: a weight / scale is at most 2^(15 + 80), whose sums stay finite
+// (with 2^-107, which a head of zeros is stored with, 2^14 of them did not, and what came behind them was lost)
 __device__ __forceinline__ void ask_ref(const float* scale, int n, uint32_t (&u)[2]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -120,7 +124,7 @@ __device__ __forceinline__ void ask_ref(const float* scale, int n, uint32_t (&u)
 }
 __device__ __forceinline__ int ref_of(const uint32_t (&u)[2]) {
   const uint32_t top = __reduce_max_sync(0xffffffffu, max(u[0] < 0x7f800000u ? u[0] : 0u, u[1] < 0x7f800000u ? u[1] : 0u));   // (not a negative one either)
-  return top >= 0x00800000u ? min((int)(top >> 23) - 127, 100) : 0;
+  return top >= 0x00800000u ? min(max((int)(top >> 23) - 127, -80), 100) : 0;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
 

@@ -1480,7 +1480,7 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
 
     Caches: bf16, or int8 / float8_e4m3fn with ``k_scale`` and ``v_scale`` [slots, G, capacity] (``kv_store_8bit``), [slots, capacity, G * dim] or [slots, capacity, G, dim] with
     neighbouring channels; heads of 64 or 128 channels.  ``q`` [M, H * dim] and ``out`` [M, H * vdim] are bf16.  ``rows``: the most tokens of a portion; ``max_ctx``: the longest p0 + n,
-    about (it decides how many blocks share a history, not what is read).  A row that sees nothing is 0; rows of no portion are left as they are; a portion that does not fit its slot, the
+    about (it decides how many blocks share a history, not what is read).  A row that sees nothing is 0; no two portions share a row; rows of no portion are left as they are; a portion that does not fit its slot, the
     rows, ``rows`` or the mask's words gives NaN rows."""
     dev, M, nseg = _device(q, "tree_attn"), q.shape[0], segs.shape[0]
     qp, ldq = _rows_of(q, BF16, (M, H * dim), dev, "tree_attn: q")

@@ -465,3 +465,34 @@ def test_blocks_that_share_a_history(ops, kind, nseg):
     out[lost[2]:lost[2] + 2] = 77.0
     del c.segs[3]
     c.check(out, kind)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_many_zeros_before_the_first_value(ops, kind):
+    """A head of zeros is stored with a scale near 2^-107: sums of weights over scales stay finite, and values behind 40000 such tokens count."""
+    z = 40000
+    c = Case([(0, z, 40)] * 150, 1, 1, 64, 64, kind)
+    c.q.zero_()
+    c.vc.view(torch.uint8)[0, :z] = 0
+    c.vs[0, 0, :z] = 2.0 ** -107
+    out = c.run(ops)
+    c.check(out, kind)
+    assert (out.float().abs().amax(1) > 0).all()
+
+
+def test_a_capacity_whose_positions_do_not_fit(ops):
+    from lia_b200._lib import LiaError
+    far = torch.zeros(1, 1, 64, dtype=BF16, device="cuda").expand(1, (1 << 29) + 1, 64)
+    q = torch.zeros(1, 64, dtype=BF16, device="cuda")
+    with pytest.raises(LiaError):
+        ops.tree_attn(q, far, far, torch.zeros(1, 4, dtype=torch.int32, device="cuda"), torch.empty_like(q), 1, 1, 64, 64, 1.0, rows=1, max_ctx=1)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("H,n", [(2, 1), (2, 9), (2, 40), (8, 40)])
+def test_depths_behind_the_window(ops, kind, H, n):
+    """Without a mask, tokens whose depth is so far behind that their window ends before the keys do see nothing, whether or not others of the call see something."""
+    c = Case([(0, 4000, n), (1, 300, n), (0, 10, n)], H, 2, 64, 128, kind, depth=[[1000 + i for i in range(n)], list(range(n)), [60 + 2 * i for i in range(n)]], window=50)
+    out = c.run(ops)
+    c.check(out, kind)
+    assert (out[:n] == 0).all()

@@ -1,0 +1,24 @@
+"""Attention of drafted tokens on tcgen05 (csrc/tree_attn_sm100.cu) whose waits run out at once: a launch ends and counts its blocks, and every row is formed again from the keys that it sees, so that
+results are right all the same."""
+import pytest
+import torch
+
+from test_gpu_tree_attn import Case, KINDS, family
+from test_gpu_wait_limits import given_up, nowait  # noqa: F401
+from lia_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("H", [4, 8])                               # rows of a key head: 128, 80 and 66, or twice as many
+@pytest.mark.parametrize("masked", [False, True])
+def test_rows_are_formed_again(nowait, monkeypatch, kind, H, masked):  # noqa: F811
+    sizes = (64, 40, 33)
+    mask = [family(n, lambda i: (i - 1) // 2 if i else -1) for n in sizes] if masked else None
+    c = Case([(0, 300, sizes[0]), (1, 70, sizes[1]), (2, 5, sizes[2])], H, 2, 128, 64, kind, mask=mask, gap=1)
+    again = torch.full_like(c.out, 77.0)
+    assert given_up(nowait, monkeypatch, lambda: c.run(ops, out=again)) == 3 * 2
+    torch.cuda.synchronize()
+    c.check(again, kind)
+    c.check(c.run(ops), kind)
