@@ -59,7 +59,7 @@ struct Shape {
 constexpr float NONE = -1e30f, SLACK = 8.f;                        // a maximum of no keys; how far, in powers of two, weights may exceed 1
 
 template <int DIM, int VDIM, int KIND, int NR>
-__global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   using S = Shape<DIM, VDIM, KIND, NR>;
   constexpr bool BITS8 = S::BITS8;
   constexpr int RQ = BITS8 ? 1 : 2;
@@ -434,10 +434,9 @@ struct Plan {
 // Rows of a key head from which tcgen05 takes over: above 32 a history would be read a second time here.  us, tcgen05 | here: 58 rows behind 4099 positions, 8 sequences, int8 50 | 57, bf16
 // 48 | 98; 64 rows behind 131003 144 | 230 (bf16 167 | 445); 64 heads of keys with chains of 33 390 | 669.  With 32 rows and fewer this kernel's are the smaller, down to a half.
 constexpr int TC_ROWS = 32;
-Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
-  const long long R = (long long)rows * (H / G);
+Plan cut(int nr, long long R, int nseg, int rows, int max_ctx, int G, int window, int type) {
   Plan p;
-  p.nr = R > TC_ROWS ? (R > 128 ? 32 : 16) : R > 16 ? 4 : R > 8 ? 2 : 1;
+  p.nr = nr;
   p.tiles = (int)((R + 8 * p.nr - 1) / (8 * p.nr));
   const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.nr >= 16 ? 1 : blocks_an_sm(type, p.nr));
   const long long span = window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx;
@@ -447,6 +446,26 @@ Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   p.splits = s < 1 ? 1 : (int)s;
   return p;
+}
+// About how long a plan takes on tcgen05, in us, fitted to 13 measured calls (within a fifth, most of them): a block of threads with up to 128 rows 8 and 0.75 for 64 keys, one with 256 rows 20 and
+// 1.2; the first tiles of a portion see fewer keys than the last ones; a second launch 4.
+float tc_time(const Plan& p, long long R, int nseg, int rows, int max_ctx, int G, int window) {
+  const float tile = 8.f * p.nr, tokens = fminf(rows, rows * tile / R), hidden = window > 0 ? 0.f : rows - tokens, span = window > 0 ? fminf(max_ctx, window + tokens) : max_ctx;
+  auto of = [&](bool large, float keys) { return (large ? 20.f : 8.f) + (large ? 1.2f : 0.75f) * fmaxf(keys, 0.f) / (64.f * p.splits); };
+  const float longest = of(p.nr == 32, span), last = of(p.nr == 32 && (R - 1) % 256 >= 128, span), shortest = of(p.nr == 32, span - hidden);
+  const float mean = ((p.tiles - 1) * 0.5f * (longest + shortest) + last) / p.tiles, rounds = (float)nseg * G * p.tiles * p.splits / lia_sm_count();
+  return (rounds <= 1.f ? longest : fmaxf(longest, rounds * mean)) + (p.splits > 1 ? 4.f : 0.f);
+}
+// Of more than 128 rows tiles of 256 bring keys once instead of twice, tiles of 128 share the SMs out more evenly and leave less of the last one empty.  us, 256 | 128, two portions behind 512
+// positions and some, 16 heads on 8, int8: of 200 tokens 29 | 20, 400 34 | 22, 1003 51 | 43, 2000 98 | 105, 4001 258 | 278; of 333 behind 4000 62 | 71; one of 1003 43 | 30.
+Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
+  const long long R = (long long)rows * (H / G);
+  auto of = [&](int nr) { return cut(nr, R, nseg, rows, max_ctx, G, window, type); };
+  if (R <= TC_ROWS) return of(R > 16 ? 4 : R > 8 ? 2 : 1);
+  const Plan one = of(16);
+  if (R <= 128) return one;
+  const Plan two = of(32);
+  return tc_time(two, R, nseg, rows, max_ctx, G, window) <= tc_time(one, R, nseg, rows, max_ctx, G, window) ? two : one;
 }
 size_t floats_of(const Plan& p, int M, int H, int vdim) { return p.splits > (p.nr >= 16 ? 1 : CLUSTER) ? (size_t)p.splits * M * H * (vdim + 2) : 0; }
 

@@ -158,7 +158,7 @@ template <int DIM, int VDIM, int KIND> __device__ __forceinline__ void put_row(c
 }
 
 // The parts of a split history joined, always in the same order.  Warp per (row, head)
-template <int DIM, int VDIM, int KIND> __global__ void __launch_bounds__(128) tree_attn_join_kernel(const TreeArgs a) {
+template <int DIM, int VDIM, int KIND> __global__ void __launch_bounds__(128) tree_attn_join_kernel(const __grid_constant__ TreeArgs a) {
   constexpr int N = VDIM / 32;
   pdl_launch_dependents();
   pdl_wait();

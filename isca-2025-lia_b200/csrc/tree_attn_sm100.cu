@@ -129,7 +129,7 @@ __device__ __forceinline__ int ref_of(const uint32_t (&u)[2]) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
 
 template <int DIM, int VDIM, int KIND, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs a, int* __restrict__ timeouts) {
+__global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_constant__ TreeArgs a, int* __restrict__ timeouts) {
   using C = Tc<DIM, VDIM, KIND, PAIR>;
   constexpr bool BITS8 = C::BITS8;
   constexpr int TILE = PAIR ? 2 * ROWS : ROWS, STAGES = C::STAGES;
@@ -269,10 +269,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
     for (int j = PAIR ? 0 : s; j < n && s < groups; j += PAIR ? 1 : 2, ++done) {
       const int st = j % STAGES, buf = done & 1;
       const uint32_t scores = lanes + s * 128 + buf * KEYS;
-      float4 k4[BITS8 ? 8 : 1];                                    // half of the keys' scales, asked for together
+      float4 k4[BITS8 ? 4 : 1];                                    // a quarter of the keys' scales, asked for together
       auto ask_scales = [&](int half) {
 #pragma unroll
-        for (int c = 0; c < (BITS8 ? 8 : 0); ++c) k4[c] = *reinterpret_cast<const float4*>(&sm.ks[st][half * 32 + c * 4]);
+        for (int c = 0; c < (BITS8 ? 4 : 0); ++c) k4[c] = *reinterpret_cast<const float4*>(&sm.ks[st][half * 16 + c * 4]);
       };
       if constexpr (BITS8) {
         if (!(alive = warp_wait(smem_u32(&sm.full[st]), (j / STAGES) & 1, dead))) break;
@@ -289,14 +289,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const TreeArgs
         tmem_ld_wait();
         if constexpr (BITS8) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float4 f4[8];
+          for (int half = 0; half < 4; ++half) {
+            float4 f4[4];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) f4[c] = k4[c];
-            if (half == 0) ask_scales(1);
+            for (int c = 0; c < 4; ++c) f4[c] = k4[c];
+            if (half < 3) ask_scales(half + 1);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const int x = half * 32 + c * 4;
+            for (int c = 0; c < 4; ++c) {
+              const int x = half * 16 + c * 4;
               float a0, a1;
               unpack2(mul2(pack2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), pack2(f4[c].x, f4[c].y)), a0, a1);
               v[x] = __float_as_uint(a0);
@@ -703,7 +703,7 @@ template <int DIM, int VDIM, int KIND, bool PAIR> int launch(const TreeArgs& a, 
   LIA_CHECK_ARG(split_fits, "lia_tree_attn: the kernel was built with too few registers");
   int* timeouts = lia_timeout_word();
   LIA_CHECK_ARG(timeouts, "lia_tree_attn: no memory for the count of waits that ran out");
-  LIA_CUDA(lia_launch_after(tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), SMEM, stream, a, timeouts));
+  LIA_CUDA(lia_launch(tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), SMEM, stream, a, timeouts));
   return LIA_OK;
 }
 template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int rows, int nseg, cudaStream_t stream) {

@@ -13,12 +13,13 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("H", [4, 8])                               # rows of a key head: 128, 80 and 66, or twice as many
 @pytest.mark.parametrize("masked", [False, True])
-def test_rows_are_formed_again(nowait, monkeypatch, kind, H, masked):  # noqa: F811
+@pytest.mark.parametrize("max_ctx", [364, 100000])                  # how many blocks share a history, and with which rows, goes by it
+def test_rows_are_formed_again(nowait, monkeypatch, kind, H, masked, max_ctx):  # noqa: F811
     sizes = (64, 40, 33)
     mask = [family(n, lambda i: (i - 1) // 2 if i else -1) for n in sizes] if masked else None
     c = Case([(0, 300, sizes[0]), (1, 70, sizes[1]), (2, 5, sizes[2])], H, 2, 128, 64, kind, mask=mask, gap=1)
     again = torch.full_like(c.out, 77.0)
-    assert given_up(nowait, monkeypatch, lambda: c.run(ops, out=again)) == 3 * 2
+    assert given_up(nowait, monkeypatch, lambda: c.run(ops, out=again, max_ctx=max_ctx)) >= 3 * 2      # a block at least for each portion and key head
     torch.cuda.synchronize()
     c.check(again, kind)
-    c.check(c.run(ops), kind)
+    c.check(c.run(ops, max_ctx=max_ctx), kind)
