@@ -17,8 +17,8 @@
 // The maximum moves only when a key exceeds it by 2^8, which the 7 leaves room for; the rows' sums are multiplied only then.
 //
 // Bound: bf16 caches by memory, 8-bit ones by instructions too (a byte is widened, half of them after two codes change places; a score takes some fifteen).  A token of 16 heads on 8 for each of 16
-// histories of 60000 positions: bf16 571 us (6.9 TB/s, what a copy reaches at the most), int8 438 (4.6), e4m3 390 (5.2).  Behind 1901 positions, int8: 23 us, of which memory 10; the rest is
-// one block's way from its first load to its last sum.
+// histories of 60000 positions: bf16 563 us (7.0 TB/s, what a copy reaches at the most), int8 419 (4.8), e4m3 377 (5.4).  Behind 1901 positions, int8: 21 us, of which memory 10; the rest is
+// one block's way from its first load to its last sum.  (Arguments are taken where the launch put them: copied to each thread's stack, for rows that are formed again, they cost 2 us a block.)
 #include "mma.cuh"
 #include "tree_attn.cuh"
 
@@ -431,15 +431,18 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 struct Plan {
   int nr, tiles, splits;                                           // nr: eights of rows; 16 and 32 of them on tcgen05
 };
-// Rows of a key head from which tcgen05 takes over: above 32 a history would be read a second time here.  us, tcgen05 | here: 58 rows behind 4099 positions, 8 sequences, int8 50 | 57, bf16
-// 48 | 98; 64 rows behind 131003 144 | 230 (bf16 167 | 445); 64 heads of keys with chains of 33 390 | 669.  With 32 rows and fewer this kernel's are the smaller, down to a half.
-constexpr int TC_ROWS = 32;
+// Rows of a key head up to which this file's kernel is taken: above 32 a history would be read a second time here, and with bf16 caches the 32 rows' products, in two parts each, take longer than the
+// history's bytes where it is long.  us, tcgen05 | here: 58 rows behind 4099 positions, 8 sequences and 8 key heads, e4m3 62 | 73, bf16 65 | 114; 64 rows behind 131003, one sequence, int8 121 | 213, bf16 137 | 366;
+// 33 rows behind 280, 64 sequences and 56 key heads, int8 340 | 407, bf16 326 | 541; 17 of them 341 | 230, 322 | 311; 28 behind 1000, 30 sequences and 8 key heads, int8 47 | 41, bf16 51 | 68;
+// 32 behind 131003 int8 121 | 122, bf16 138 | 213; 16 behind as many int8 120 | 86, bf16 136 | 102.
+int rows_here(int type, long long span) { return type == LIA_CACHE_BF16 && span > 512 ? 16 : 32; }
+long long span_of(int rows, int max_ctx, int window) { return window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx; }
 Plan cut(int nr, long long R, int nseg, int rows, int max_ctx, int G, int window, int type) {
   Plan p;
   p.nr = nr;
   p.tiles = (int)((R + 8 * p.nr - 1) / (8 * p.nr));
   const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.nr >= 16 ? 1 : blocks_an_sm(type, p.nr));
-  const long long span = window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx;
+  const long long span = span_of(rows, max_ctx, window);
   const long long least = p.nr >= 16 ? 512 : 256;                   // keys of a block of threads: eight blocks of 64, or four of 16 a warp
   long long s = room / blocks, most = (span + least - 1) / least;
   if (s > most) s = most;
@@ -461,7 +464,7 @@ float tc_time(const Plan& p, long long R, int nseg, int rows, int max_ctx, int G
 Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
   const long long R = (long long)rows * (H / G);
   auto of = [&](int nr) { return cut(nr, R, nseg, rows, max_ctx, G, window, type); };
-  if (R <= TC_ROWS) return of(R > 16 ? 4 : R > 8 ? 2 : 1);
+  if (R <= rows_here(type, span_of(rows, max_ctx, window))) return of(R > 16 ? 4 : R > 8 ? 2 : 1);
   const Plan one = of(16);
   if (R <= 128) return one;
   const Plan two = of(32);

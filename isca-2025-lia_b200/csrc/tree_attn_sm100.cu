@@ -17,8 +17,9 @@
 //
 // What bounds it: at 128 rows and more the softmax -- a row of 64 scores is one thread's chain of loads from TMEM, a maximum, powers, sums and stores, and two groups of four warps hide little of
 // one another's (with the products halved the time stays as it is, and sixteen warps of it had too few registers) -- at 2.7 times the 512 clocks that 64 x 128 powers take; with fewer rows
-// memory (700 clocks for 64 keys of 8 bits, 1400 of bf16).  A block of threads begins and ends in 19 000 clocks, whatever its keys: loads of programs and of what depends on the portion, one behind
-// the other.  A tree of 64 tokens behind 131003 positions, int8, 32 heads on 8: 228 us; its products would take 83 at the tensor cores' rate, its bytes 42.
+// memory (700 clocks for 64 keys of 8 bits, 1400 of bf16).  A call behind a single position takes 16 us with 256 rows a block, 10 with up to 128: programs are loaded, and what depends on the portion, one
+// behind the other.  A tree of 64 tokens behind 131003 positions, 32 heads on 8: int8 212 us, bf16 205; its products would take 83 at the tensor cores' rate, its bytes 42 and 82.
+// Keys' scales are held 16 at a time (32: 240 us, for registers).
 // The issuing warp's block numbers are made uniform by a shuffle: without, each product took twice its instructions.
 #include "pairs.cuh"
 #include "tree_attn.cuh"
