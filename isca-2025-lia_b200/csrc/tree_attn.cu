@@ -17,7 +17,7 @@
 // The maximum moves only when a key exceeds it by 2^8, which the 7 leaves room for; the rows' sums are multiplied only then.
 //
 // Bound: bf16 caches by memory, 8-bit ones by instructions too (a byte is widened, half of them after two codes change places; a score takes some fifteen).  A token of 16 heads on 8 for each of 16
-// histories of 60000 positions: bf16 563 us (7.0 TB/s, what a copy reaches at the most), int8 419 (4.8), e4m3 377 (5.4).  Behind 1901 positions, int8: 21 us, of which memory 10; the rest is
+// histories of 60000 positions: bf16 563 us (7.0 TB/s, what a copy reaches at the most), int8 398 to 419 (5.1 to 4.8), e4m3 377 to 391 (5.4 to 5.2).  Behind 1901 positions, int8: 19.5 us, of which memory 10; the rest is
 // one block's way from its first load to its last sum.  (Arguments are taken where the launch put them: copied to each thread's stack, for rows that are formed again, they cost 2 us a block.)
 #include "mma.cuh"
 #include "tree_attn.cuh"
@@ -78,38 +78,6 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
   const int tile = blockIdx.y / a.G, g = blockIdx.y - tile * a.G, r0 = tile * S::ROWS, R = p.n * a.rep;
   if (r0 >= R) return;
 
-  // ---- queries: rows (token, head) in the order of the products' operands
-  for (int r = warp; r < S::ROWS; r += WARPS) {
-    const bool there = r0 + r < R;
-    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
-    uint2 u = make_uint2(0u, 0u);
-    if (there && lane < DIM / 4) u = *reinterpret_cast<const uint2*>(a.q + (p.row + i) * a.ldq + h * DIM + lane * 4);
-    float f = a.scale * (a.temp != nullptr && there ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
-    uint2 w = u;
-    if constexpr (BITS8) {
-      uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
-      const Down down = down_of(__reduce_max_sync(0xffffffffu, top));
-      float x[4];
-      unpack_bf16x2(u.x, x[0], x[1]);
-      unpack_bf16x2(u.y, x[2], x[3]);
-      w = make_uint2(pack_f16x2(x[0] * down.by, x[1] * down.by), pack_f16x2(x[2] * down.by, x[3] * down.by));
-      f *= down.back;
-    }
-    if (lane < DIM / 4) {                                          // four neighbouring channels are a lane's operand of one step
-      const int c = lane * 4, t = BITS8 ? (c >> 4) & 3 : (c >> 3) & 3, step = BITS8 ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
-      qs[((r >> 3) * S::STEPS + step) * 32 + (r & 7) * 4 + t] = w;
-    }
-    if (lane == 0) row_f[r] = f;
-  }
-  __syncthreads();
-  uint2 qa[NR <= RQ ? NR : 1][NR <= RQ ? S::STEPS : 1];            // few rows' queries stay in registers, the others' in shared memory
-  if constexpr (NR <= RQ) {
-#pragma unroll
-    for (int r = 0; r < NR; ++r)
-#pragma unroll
-      for (int s = 0; s < S::STEPS; ++s) qa[r][s] = qs[(r * S::STEPS + s) * 32 + lane];
-  }
-
   // ---- which keys
   const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + S::ROWS - 1) / a.rep);
   int near = i0, far = i1;                                         // depths of the block's tokens
@@ -126,23 +94,6 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
   }
   const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = min(hi, a.mask != nullptr ? p.p0 : p.p0 + i0 + 1);
   const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
-
-  float rf[NR][2], m[NR][2], l[NR][2];                             // of the lane's rows 2 t4 and 2 t4 + 1 of every eight
-#pragma unroll
-  for (int r = 0; r < NR; ++r)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      rf[r][e] = row_f[r * 8 + t4 * 2 + e];
-      m[r][e] = NONE;
-      l[r][e] = 0.f;
-    }
-  float o[NR][S::MT][4];                                           // [..][0]: a lane's first channel of a pair and row 2 t4, [1]: row 2 t4 + 1, [2], [3]: its second channel
-#pragma unroll
-  for (int r = 0; r < NR; ++r)
-#pragma unroll
-    for (int n = 0; n < S::MT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[r][n][e] = 0.f;
 
   const uint8_t *kbase = a.k.at(p.slot, 0, g) + t4 * 16, *vbase = a.v.at(p.slot, 0, g) + gq * (BITS8 ? S::VB : 16);
   const float *ksc = BITS8 ? a.k.scale_at(p.slot, g) : nullptr, *vsc = BITS8 ? a.v.scale_at(p.slot, g) : nullptr;
@@ -177,10 +128,60 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     }
   };
 
-  if (b0 + warp < b1) {
+  if (b0 + warp < b1) {                                            // (on their way while the queries are brought: chains of 8 behind 280 119 -> 113 us)
     load_k(b0 + warp);
     load_v(b0 + warp);
   }
+
+  // ---- queries: rows (token, head) in the order of the products' operands
+  for (int r = warp; r < S::ROWS; r += WARPS) {
+    const bool there = r0 + r < R;
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    uint2 u = make_uint2(0u, 0u);
+    if (there && lane < DIM / 4) u = *reinterpret_cast<const uint2*>(a.q + (p.row + i) * a.ldq + h * DIM + lane * 4);
+    float f = a.scale * (a.temp != nullptr && there ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
+    uint2 w = u;
+    if constexpr (BITS8) {
+      uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
+      const Down down = down_of(__reduce_max_sync(0xffffffffu, top));
+      float x[4];
+      unpack_bf16x2(u.x, x[0], x[1]);
+      unpack_bf16x2(u.y, x[2], x[3]);
+      w = make_uint2(pack_f16x2(x[0] * down.by, x[1] * down.by), pack_f16x2(x[2] * down.by, x[3] * down.by));
+      f *= down.back;
+    }
+    if (lane < DIM / 4) {                                          // four neighbouring channels are a lane's operand of one step
+      const int c = lane * 4, t = BITS8 ? (c >> 4) & 3 : (c >> 3) & 3, step = BITS8 ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
+      qs[((r >> 3) * S::STEPS + step) * 32 + (r & 7) * 4 + t] = w;
+    }
+    if (lane == 0) row_f[r] = f;
+  }
+  __syncthreads();
+  uint2 qa[NR <= RQ ? NR : 1][NR <= RQ ? S::STEPS : 1];            // few rows' queries stay in registers, the others' in shared memory
+  if constexpr (NR <= RQ) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int s = 0; s < S::STEPS; ++s) qa[r][s] = qs[(r * S::STEPS + s) * 32 + lane];
+  }
+
+  float rf[NR][2], m[NR][2], l[NR][2];                             // of the lane's rows 2 t4 and 2 t4 + 1 of every eight
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      rf[r][e] = row_f[r * 8 + t4 * 2 + e];
+      m[r][e] = NONE;
+      l[r][e] = 0.f;
+    }
+  float o[NR][S::MT][4];                                           // [..][0]: a lane's first channel of a pair and row 2 t4, [1]: row 2 t4 + 1, [2], [3]: its second channel
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int n = 0; n < S::MT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[r][n][e] = 0.f;
+
   const float two_by_cap = a.softcap > 0.f ? 2.f * LOG2E / a.softcap : 0.f;
 #pragma unroll 1
   for (int b = b0 + warp; b < b1; b += WARPS) {
@@ -433,7 +434,7 @@ struct Plan {
 };
 // Rows of a key head up to which this file's kernel is taken: above 32 a history would be read a second time here, and with bf16 caches the 32 rows' products, in two parts each, take longer than the
 // history's bytes where it is long.  us, tcgen05 | here: 58 rows behind 4099 positions, 8 sequences and 8 key heads, e4m3 62 | 73, bf16 65 | 114; 64 rows behind 131003, one sequence, int8 121 | 213, bf16 137 | 366;
-// 33 rows behind 280, 64 sequences and 56 key heads, int8 340 | 407, bf16 326 | 541; 17 of them 341 | 230, 322 | 311; 28 behind 1000, 30 sequences and 8 key heads, int8 47 | 41, bf16 51 | 68;
+// 33 rows behind 280, 64 sequences and 56 key heads, int8 340 | 407, bf16 326 | 541; 17 of them 341 | 225, 322 | 301; 28 behind 1000, 30 sequences and 8 key heads, int8 47 | 41, bf16 51 | 68;
 // 32 behind 131003 int8 121 | 122, bf16 138 | 213; 16 behind as many int8 120 | 86, bf16 136 | 102.
 int rows_here(int type, long long span) { return type == LIA_CACHE_BF16 && span > 512 ? 16 : 32; }
 long long span_of(int rows, int max_ctx, int window) { return window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx; }
