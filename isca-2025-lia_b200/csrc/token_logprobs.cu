@@ -33,9 +33,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 struct alignas(16) Sums {
   float m, L, A;
 };
+// (a step counts as 200 at most, where its power is 0 already: of sums whose maximum is a mask of the type's least number, d or d * L would be infinite, and 0 times that NaN)
 __device__ __forceinline__ void raise_to(Sums& s, float m) {
   if (s.m != -INFINITY) {
-    const float d = s.m - m, f = ex2(d * LOG2E);
+    const float d = fmaxf(s.m - m, -200.f), f = ex2(d * LOG2E);
     s.A = f * fmaf(d, s.L, s.A);
     s.L *= f;
   }

@@ -136,3 +136,22 @@ def test_replayed_and_on_another_stream(ops):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(ops.token_logprobs(x, t, 4), got))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("fill,most", [(None, 5.0), (-1e37, 5.0), (-3e38, 3e38)], ids=["least", "1e37", "3e38"])
+@pytest.mark.parametrize("M,V", [(1, 40), (2, 600), (3, 9000), (4, 50265), (700, 4100)])
+def test_finite_masks(ops, dtype, fill, most, M, V):
+    """Banned tokens with the type's least number, or another far below the rest, instead of -inf: before the others, behind them, around them, all but one, in every second place, all of them.
+    Their distances to the maximum, and those distances times their number, leave 32 bits; a distance that does is minus infinity in the results too."""
+    fill = torch.finfo(dtype).min if fill is None else fill
+    i = torch.arange(V, device="cuda")
+    masks = [i < V // 2, i >= V // 3, (i < V // 3) | (i >= V // 2), i != V - 1, i != 0, i % 2 == 0, (i // 16) % 2 == 0, i >= 0]
+    x = rnd(M * len(masks), V, seed=V, dtype=dtype)
+    x[:, V - 1], x[:, 0] = most, most
+    x = torch.where(torch.stack(masks).repeat(M, 1), torch.full_like(x, fill), x)
+    tokens = torch.tensor([[V - 1, 0, V // 2]] * len(x), device="cuda")
+    got, want = ops.token_logprobs(x, tokens, 5), reference(x, tokens, 5)
+    for a, b, what in zip(got, want, ("given", "entropy", "alternatives")):
+        close(a, b.float().double(), what)
+    assert torch.isfinite(got[1]).all() and torch.equal(got[3], want[3])
