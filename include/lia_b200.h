@@ -677,7 +677,7 @@ int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const LiaCacheView
  * h / (H / G).  A row that sees nothing is 0; what it does not see has no effect, whatever its bits.  Scales are 0 or more, values' up to 2^29 (values with a smaller one
  * than 2^-80 are off by 2^-71 at most).  No two portions share a row.  Rows of no portion stay as they are; a portion that its slot, the M rows, the mask's
  * words or `rows` cannot hold gives NaN rows.  rows: the most rows of a portion; max_ctx: about the longest p0 + n (it decides how many blocks share a history, no more).
- * q and out: bf16, ldq apart and [M, H * vdim].  Heads of 64 or 128 channels, 2^29 positions at most.  ws: lia_tree_attn_workspace_floats() floats (0: NULL will do). */
+ * q and out: bf16, ldq apart and [M, H * vdim], on 8-byte boundaries.  Heads of 64 or 128 channels, 2^29 positions at most.  ws: lia_tree_attn_workspace_floats() floats (0: NULL will do). */
 size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx, int M, int H, int G, int dim, int vdim, int window, int type);
 int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
                   const float* temp, void* out, float* ws, size_t ws_floats, int M, int H, int G, int rows, int max_ctx, int window, float scale, float softcap, lia_stream_t stream);

@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
     }
     if ((PAIR || s == 0) && warp_there) {
       const long long rows = (long long)a.M * a.H, at = (long long)(p.row + i) * a.H + h;
-      const bool whole = a.splits == 1;
+      const bool whole = a.splits == 1, wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0;       // (rows are whole 16-byte vectors; where they begin may be on an 8-byte boundary)
       const float inv = whole ? 1.f / sum : 1.f;
       float probe = 0.f;
 #pragma unroll 1
@@ -482,7 +482,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
           const int col = c + e, ch = BITS8 && VDIM == 128 ? (col & 63) / 8 * 16 + (col >> 6) * 8 : col;
           if (there) {
             if (whole) {
-              *reinterpret_cast<uint4*>(a.out + at * VDIM + ch) = pack8(y);
+              const uint4 u = pack8(y);
+              bf16* dst = a.out + at * VDIM + ch;
+              if (wide) {
+                *reinterpret_cast<uint4*>(dst) = u;
+              } else {
+                reinterpret_cast<uint2*>(dst)[0] = make_uint2(u.x, u.y);
+                reinterpret_cast<uint2*>(dst)[1] = make_uint2(u.z, u.w);
+              }
             } else {
               float4* dst = reinterpret_cast<float4*>(a.ws + (blockIdx.x * rows + at) * VDIM + ch);
               dst[0] = make_float4(y[0], y[1], y[2], y[3]);

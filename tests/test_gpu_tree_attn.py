@@ -496,3 +496,18 @@ def test_depths_behind_the_window(ops, kind, H, n):
     out = c.run(ops)
     c.check(out, kind)
     assert (out[:n] == 0).all()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dim,vdim", DIMS)
+@pytest.mark.parametrize("n,past,max_ctx", [(1, 90, 91), (40, 30, 70), (40, 30, 100000), (200, 70, 270), (20, 1500, 1520)])
+def test_outputs_on_8_byte_boundaries(ops, kind, dim, vdim, n, past, max_ctx):
+    """Part of a buffer that begins four numbers into it: the same bits, and nothing beside them, whichever kernel takes the rows."""
+    c = Case([(0, past, n), (1, past // 2, max(1, n - 3))], 4, 2, dim, vdim, kind)
+    want = c.run(ops, max_ctx=max_ctx).clone()
+    c.check(want, kind)
+    buffer = torch.full((4 + want.numel() + 4,), 77.0, dtype=BF16, device="cuda")
+    out = buffer[4:4 + want.numel()].view(want.shape)
+    assert out.data_ptr() % 16 == 8
+    assert torch.equal(c.run(ops, max_ctx=max_ctx, out=out), want)
+    assert (buffer[:4] == 77).all() and (buffer[-4:] == 77).all()
