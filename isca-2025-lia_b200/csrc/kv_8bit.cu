@@ -285,7 +285,7 @@ int head_blocks(const Side& s, int M, int G) { return (int)((((long long)M * G <
 
 const char* sides_wrong(const void* k, const void* v, const void* meta, const LiaCacheView* kc, const LiaCacheView* vc, long long ldk, long long ldv, int M, int G) {
   const char* w = nullptr;
-  if (!k || !v || !meta || M < 0 || G <= 0) return "null pointer or no heads";
+  if (M < 0 || G <= 0 || (M > 0 && (!k || !v || !meta))) return "null pointer or no heads";     // (no rows have no address)
   if ((w = cache8_wrong(kc, 8)) || (w = cache8_wrong(vc, 8))) return w;
   if (kc->type == LIA_CACHE_BF16 || kc->type != vc->type) return "both caches have to be int8, or both e4m3";
   if (kc->slots != vc->slots || kc->capacity != vc->capacity) return "caches of different sizes";

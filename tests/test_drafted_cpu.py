@@ -147,3 +147,12 @@ def test_scores_are_put_together(lib, monkeypatch):
             assert g["logp"] == pytest.approx([float(w[t]) for w, t in zip(want, text[1:])])
             assert [a[0][0] for a in g["alternatives"]] == [int(w.argmax()) for w in want] and all(len(a) == 2 for a in g["alternatives"])
             assert g["entropy"] == pytest.approx([float(-(w.exp() * w).sum()) for w in want])
+
+
+def test_no_rows_have_no_addresses(lib):
+    """What an empty tensor is at the C ABI: a null pointer and no rows; caches and sizes are checked all the same."""
+    L, v = lib.load(), view(lib)
+    assert L.lia_kv_store_8bit(None, 1024, None, 1024, 0, None, v, v, 0, 8, 0.0, 0, None) == 0
+    assert L.lia_kv_load_8bit(None, v, v, None, 1024, None, 1024, 0, 0, 8, None) == 0
+    assert L.lia_kv_store_8bit(None, 1024, None, 1024, 0, None, view(lib, data=None), v, 0, 8, 0.0, 0, None) == -1 and "null cache" in lib.last_error()
+    assert L.lia_kv_load_8bit(None, v, v, None, 1024, None, 1024, 0, 1, 8, None) == -1 and "null pointer" in lib.last_error()

@@ -199,3 +199,15 @@ def test_replayed_on_another_stream(ops):
     both()
     assert torch.equal(got[0], ko) and torch.equal(got[1], vo)
     check_codes(kc, ks, k.double().view(M, G, dim), meta, G, E4M3, True, "keys")
+
+
+@pytest.mark.parametrize("kind", [torch.int8, E4M3], ids=["int8", "e4m3"])
+def test_no_rows(ops, kind):
+    """A step without tokens stores and reads nothing (an empty tensor has no address)."""
+    (kc, ks), (vc, vs) = caches(2, 8, 3, 64, kind), caches(2, 8, 3, 128, kind)
+    before = [x.clone() for x in (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)]
+    k, v, meta = torch.empty(0, 3 * 64, dtype=BF16, device="cuda"), torch.empty(0, 3 * 128, dtype=BF16, device="cuda"), torch.empty(0, 2, dtype=torch.int32, device="cuda")
+    ops.kv_store_8bit(k, v, meta, kc, vc, ks, vs, 3, 64, 128)
+    ops.kv_load_8bit(meta, kc, vc, ks, vs, k, v, 3, 64, 128)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)))
