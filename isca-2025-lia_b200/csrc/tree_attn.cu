@@ -386,9 +386,10 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     }
     if (a.splits == 1) {
       put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
-    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read)
+    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read: with all lanes, before one of them writes)
 #pragma unroll
       for (int c = 0; c < N; ++c) os[r * VDIM + lane * N + c] = y[c];
+      __syncwarp();
       if (lane == 0) part[r] = make_float2(top, sum);
     } else {
       const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;

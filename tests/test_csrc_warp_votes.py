@@ -46,3 +46,12 @@ def test_loads_under_way_are_waited_for_after_the_last_wait():
         assert text.index("wait_in_flight(") > last or name in ("attn_sm100.cuh", "ssd_chunk_sm100.cu"), name      # (one holds functions, the other several kernels without such loads)
         found += "tma_load_2d(" in text
     assert found == 3
+
+
+def test_sums_are_replaced_after_all_lanes_have_read_them():
+    """Where one lane writes a row's joined maximum and sum over a part that all lanes of its warp have just read, the warp meets between: lanes need not run together."""
+    text = SOURCES["tree_attn.cu"]
+    writes = [m.start() for m in re.finditer(r"if \(lane == 0\) part\[r\] =", text)]
+    assert len(writes) == 1
+    read = text.rindex("= part[", 0, writes[0])
+    assert "__syncwarp();" in text[read:writes[0]]
