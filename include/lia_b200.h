@@ -681,6 +681,8 @@ int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const LiaCacheView
 size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx, int M, int H, int G, int dim, int vdim, int window, int type);
 int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
                   const float* temp, void* out, float* ws, size_t ws_floats, int M, int H, int G, int rows, int max_ctx, int window, float scale, float softcap, lia_stream_t stream);
+/* A number (0: bad sizes) that is the same for calls that launch alike, whatever their max_ctx: what was captured of one may be replayed in the place of the other. */
+int lia_tree_attn_plan(int nseg, int rows, int max_ctx, int H, int G, int window, int type);
 
 /* Of every row of logits [M, V] (bf16 or fp32, ld apart): logp[n] of the n given tokens (an id outside [0, V) has NaN), the entropy of the distribution in nats, and the `top` <= 32
  * largest logits' ids (int64; of equal ones the lowest first, NaN counts as -inf) and log probabilities.  Rows that hold NaN or +inf, or -inf alone, have NaN for all but the ids. */

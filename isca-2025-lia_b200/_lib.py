@@ -238,6 +238,7 @@ _PROTOTYPES = {
     "lia_kv_store_8bit": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_int, c_int, c_float, c_int,
                                   c_void_p]),
     "lia_kv_load_8bit": (c_int, [c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p]),
+    "lia_tree_attn_plan": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "lia_tree_attn_workspace_floats": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "lia_tree_attn": (c_int, [c_void_p, c_longlong, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                               c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p]),

@@ -508,6 +508,12 @@ extern "C" size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx
   return floats_of(plan_of(nseg, rows, max_ctx, H, G, window, type), M, H, vdim);
 }
 
+extern "C" int lia_tree_attn_plan(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
+  if (nseg <= 0 || rows <= 0 || G <= 0 || H <= 0 || H % G) return 0;
+  const Plan p = plan_of(nseg, rows, max_ctx, H, G, window, type);
+  return p.splits << 8 | p.nr;
+}
+
 extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
                              const float* temp, void* out, float* ws, size_t ws_floats, int M, int H, int G, int rows, int max_ctx, int window, float scale, float softcap, lia_stream_t stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);

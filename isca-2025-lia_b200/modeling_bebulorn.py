@@ -279,6 +279,16 @@ class BebulornForCausalLM:
         attention layer splits the longest history's window into."""
         return tuple(sorted({ops.window_attn_split_class(max_ctx, l.mixer.window) for l in self.layers if isinstance(l.mixer, WindowAttentionMixer)}))
 
+    def graph_plan(self, requests, max_ctx):
+        """The same for a pass of ``requests`` single tokens, over whichever caches there are: with 8-bit ones how many blocks share a history goes by the number of requests too."""
+        if self.cache_dtype is None:
+            return self.graph_class(max_ctx)
+        plans = {}
+        for l in self.layers:
+            if isinstance(l.mixer, WindowAttentionMixer):
+                l.mixer.step_plans(requests, max_ctx, plans)
+        return tuple(plans.values())
+
     def generate(self, input_ids, max_new_tokens=32, chunk=None, **unused):
         """Greedy generation of a batch of prompts through the step engine; returns ids [B, S + new] on the input's device."""
         from .engine import Engine

@@ -1502,6 +1502,11 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
     return out
 
 
+def tree_attn_plan(nseg, rows, max_ctx, H, G, window, dtype):
+    """All that a call of ``tree_attn`` over caches of ``dtype`` launches by: two lengths ``max_ctx`` of one plan launch alike, so that one's captured launches serve the other."""
+    return _lib.load().lia_tree_attn_plan(nseg, rows, max_ctx, H, G, window, _CACHE_TYPES[dtype])
+
+
 def token_logprobs(logits, tokens=None, top=0):
     """Of every row of ``logits`` [M, V] (bf16 or fp32; rows may lie apart): the log probability of its ``tokens`` (int64 [M] or [M, n]; NaN for an id outside the vocabulary), the
     entropy of its distribution in nats, and its ``top`` <= 32 most likely tokens (csrc/token_logprobs.cu).  Returns (logp, entropy [M], top_logp [M, top], top_ids int64 [M, top]), fp32, logp

@@ -20,7 +20,7 @@ import os
 import torch
 
 from . import ops
-from .ops import _sm_count as sm_count, window_step_form
+from .ops import _sm_count as sm_count, tree_attn_plan, window_step_form
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -429,6 +429,12 @@ class WindowAttentionMixer:
         temp = w.get("temp")
         self.temp = (temp if temp is not None else torch.ones(heads)).to(device=device, dtype=F32).contiguous()
         self.out = Linear([w["o"]], dtype, device)
+
+    def step_plans(self, requests, max_ctx, seen):
+        """What a decode step of ``requests`` tokens launches over an 8-bit cache by, into ``seen`` by what layers share."""
+        shape = (self.H, self.G, self.window)
+        if shape not in seen:
+            seen[shape] = tree_attn_plan(requests, 1, max_ctx, *shape, self.cache_dtype)
 
     def new_state(self, slots):
         if self.cache_dtype is not None:

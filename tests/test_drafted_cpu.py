@@ -156,3 +156,37 @@ def test_no_rows_have_no_addresses(lib):
     assert L.lia_kv_load_8bit(None, v, v, None, 1024, None, 1024, 0, 0, 8, None) == 0
     assert L.lia_kv_store_8bit(None, 1024, None, 1024, 0, None, view(lib, data=None), v, 0, 8, 0.0, 0, None) == -1 and "null cache" in lib.last_error()
     assert L.lia_kv_load_8bit(None, v, v, None, 1024, None, 1024, 0, 1, 8, None) == -1 and "null pointer" in lib.last_error()
+
+
+@pytest.mark.parametrize("cache_dtype", [torch.int8, E4M3], ids=["int8", "e4m3"])
+def test_graphs_of_decode_steps_go_by_what_is_launched(lib, cache_dtype):
+    """The engine's key of a step of single tokens over 8-bit caches: another one wherever the number of blocks that share a history is another, however long the history, and no other."""
+    import types
+
+    from lia_b200.engine import Engine
+    from lia_b200.modeling_bebulorn import BebulornForCausalLM
+    from lia_b200.seq_layers import WindowAttentionMixer
+    H, G, dim, L = 4, 2, 64, lib.load()
+
+    def key(requests, max_ctx, windows):
+        m = object.__new__(BebulornForCausalLM)
+        m.cache_dtype, m.layers = cache_dtype, []
+        for w in windows:
+            x = object.__new__(WindowAttentionMixer)
+            x.H, x.G, x.dim, x.vdim, x.window, x.cache_dtype = H, G, dim, dim, w, cache_dtype
+            m.layers.append(types.SimpleNamespace(mixer=x))
+        e = object.__new__(Engine)
+        e.model, e.graphs = m, True
+        return e._graph_key([(i, [1], []) for i in range(requests)], [(i, max_ctx - 1, i, 1) for i in range(requests)], [])
+
+    def splits(requests, max_ctx, window):
+        floats = lambda M: L.lia_tree_attn_workspace_floats(requests, 1, max_ctx, M, H, G, dim, dim, window, 1 if cache_dtype == torch.int8 else 2)  # noqa: E731
+        return floats(requests) // (requests * H * (dim + 2))       # (0 up to eight blocks)
+    for requests, windows in ((1, [1 << 20]), (3, [1 << 20, 900]), (30, [6000]), (200, [1 << 20])):
+        lengths = [1, 255, 256, 257, 512, 513, 2048, 2049, 2304, 2305, 4000, 9000, 20000, 60000]
+        for a, b in zip(lengths, lengths[1:]):
+            if any(splits(requests, a, w) != splits(requests, b, w) for w in windows):
+                assert key(requests, a, windows) != key(requests, b, windows), (requests, a, b)
+        assert key(requests, 1, windows) == key(requests, 256, windows) and key(requests, 2049, windows) == key(requests, 2304, windows)
+    assert key(1, 256, [5000]) != key(1, 257, [5000]) and key(1, 256, [100]) == key(1, 257, [100]) == key(1, 60000, [100])
+    assert key(1, 3000, [1 << 20]) != key(1, 60000, [1 << 20]) and key(200, 3000, [1 << 20]) == key(200, 60000, [1 << 20])

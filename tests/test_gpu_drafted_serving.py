@@ -189,3 +189,17 @@ def test_waits_that_run_out(nowait, monkeypatch, kind, n, past, splits):
     # both are within 2^-8 of themselves, and of 3 * 2^-11 + 2^-10 of weighted magnitudes below 2 (int8: below 2.6 times the scale's 0.11 * 127 / 2.6)
     assert ((got - want).abs() <= 2.0 ** -7 * want.abs() + (0.006 if kind == BF16 else 0.03)).all(), (got - want).abs().max()
     assert torch.equal(call().double(), want)
+
+
+@pytest.mark.parametrize("cache_dtype", [torch.int8, E4M3], ids=["int8", "e4m3"])
+def test_graphs_launch_what_a_step_would(cache_dtype):
+    """A step that is replayed from a graph gives the bits of one that is launched, wherever the number of blocks that share a history changes: 256 positions, and far behind 2048."""
+    m = small(11, cache_dtype, window=5000)
+    text = tokens(3600, 5)
+    launched, replayed = (Engine(m, 3600, max_requests=1, graphs=g) for g in (False, True))
+    for n in (256, 256, 256, 257, 300, 2100, 2100, 2100, 2600, 3600):
+        got = []
+        for e in (launched, replayed):
+            e.step([{"id": 0, "tokens": text[:n - 1], "want": []}])
+            got.append(e.step([{"id": 0, "tokens": text[n - 1:n], "want": [0]}], end=[0]))
+        assert torch.equal(*got), n
