@@ -580,8 +580,8 @@ int lia_moe_plan_rows(const int* idx, int pairs, int E, int tile_rows, int n_til
  * rows before up rows): act(gate) * up, both sums in fp32; weigh_in: the sums are first multiplied by their pair's wt.  down: C bf16 in the plan's
  * order, unweighted, or (c_f32) C [pairs][N] fp32 by pair, times wt unless weigh_in.  Tiles of experts >= E are skipped.  K, N multiples of 8.
  * A wait inside that does not end within seconds ends its CTA, which leaves NaN where its results should be and is counted, as are those of the state-space scan, of prompt
- * attention over windows and expanded latents and of attention of drafted tokens (which forms its rows again, key by key): lia_moe_timeouts_seen() reads the count
- * as far as launches have ended, lia_moe_timeouts() synchronises first. */
+ * attention over windows and expanded latents: lia_moe_timeouts_seen() reads the count as far as launches have ended.  lia_moe_timeouts() synchronises first, and adds those of
+ * attention of drafted tokens, which forms its rows again, key by key, and leaves no NaN. */
 int lia_moe_tc_rows(void);
 int lia_moe_timeouts(void);
 int lia_moe_timeouts_seen(void);

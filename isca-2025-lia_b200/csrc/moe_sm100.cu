@@ -288,7 +288,7 @@ template <int MODE> int launch(const void* W, uint64_t w_rows, int K, const CUte
 
 extern "C" int lia_moe_tc_rows(void) { return ROWS; }
 
-// The word that counts CTAs whose wait ran out: host memory that every GPU can write, allocated with the first launch and kept.
+// The words that count CTAs whose wait ran out, those that left NaN and those whose rows were formed again: host memory that every GPU can write, allocated with the first launch and kept.
 static int* timeout_word(bool make) {
   static std::mutex m;
   static int* word = nullptr;
@@ -297,26 +297,31 @@ static int* timeout_word(bool make) {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;     // the first launch may be part of a capture
     cudaThreadExchangeStreamCaptureMode(&mode);
     void* p = nullptr;
-    if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+    if (cudaHostAlloc(&p, 2 * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
       word = static_cast<int*>(p);
-      *word = 0;
+      word[0] = word[1] = 0;
     }
     cudaThreadExchangeStreamCaptureMode(&mode);
   }
   return word;
 }
 int* lia_timeout_word() { return timeout_word(true); }             // for the kernels of other files
-
-/* CTAs of the tcgen05 kernels with bounded waits (lia_moe_gemm_tc, lia_ssd_scan_chunks, prompts of lia_window_attn_mma and lia_latent_attn_expanded) that gave up one, as far as launches have ended, since the library was loaded */
-extern "C" int lia_moe_timeouts_seen(void) {
-  const volatile int* word = timeout_word(false);
-  return word ? *word : 0;
+int* lia_formed_again_word() {                                     // for those that make good what a wait cost them
+  int* word = timeout_word(true);
+  return word ? word + 1 : nullptr;
 }
 
-/* the same after all launches (synchronises) */
+/* CTAs of the tcgen05 kernels with bounded waits (lia_moe_gemm_tc, lia_ssd_scan_chunks, prompts of lia_window_attn_mma and lia_latent_attn_expanded) that gave up one and left NaN, as far as launches have ended, since the library was loaded */
+extern "C" int lia_moe_timeouts_seen(void) {
+  const volatile int* word = timeout_word(false);
+  return word ? word[0] : 0;
+}
+
+/* those and lia_tree_attn's, whose rows are right, after all launches (synchronises) */
 extern "C" int lia_moe_timeouts(void) {
   LIA_CUDA(cudaDeviceSynchronize());
-  return lia_moe_timeouts_seen();
+  const volatile int* word = timeout_word(false);
+  return word ? word[0] + word[1] : 0;
 }
 
 extern "C" int lia_moe_gemm_tc(const void* A, const void* W, void* C, int c_f32, const int* perm, const int* tile_expert, int n_tiles, const float* wt, int N,

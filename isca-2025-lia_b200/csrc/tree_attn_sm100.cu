@@ -25,7 +25,7 @@
 #include "tree_attn.cuh"
 #include "umma.cuh"
 
-int* lia_timeout_word();                                           // moe_sm100.cu
+int* lia_formed_again_word();                                      // moe_sm100.cu
 
 namespace {
 
@@ -709,7 +709,7 @@ template <int DIM, int VDIM, int KIND, bool PAIR> int launch(const TreeArgs& a, 
     return cudaFuncGetAttributes(&at, tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>) == cudaSuccess && at.numRegs == LAUNCH_REGS;
   }();
   LIA_CHECK_ARG(split_fits, "lia_tree_attn: the kernel was built with too few registers");
-  int* timeouts = lia_timeout_word();
+  int* timeouts = lia_formed_again_word();
   LIA_CHECK_ARG(timeouts, "lia_tree_attn: no memory for the count of waits that ran out");
   LIA_CUDA(lia_launch(tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), SMEM, stream, a, timeouts));
   return LIA_OK;

@@ -23,3 +23,12 @@ def test_rows_are_formed_again(nowait, monkeypatch, kind, H, masked, max_ctx):  
     torch.cuda.synchronize()
     c.check(again, kind)
     c.check(c.run(ops, max_ctx=max_ctx), kind)
+
+
+def test_rows_that_are_right_raise_nothing(nowait, monkeypatch):  # noqa: F811
+    """What the engine asks about are waits that left NaN: those of drafted tokens leave rows that are right, and are counted apart."""
+    c = Case([(0, 300, 64)], 4, 2, 128, 64, "int8")
+    seen = nowait.lia_moe_timeouts_seen()
+    assert given_up(nowait, monkeypatch, lambda: c.run(ops)) >= 2
+    c.check(c.out, "int8")
+    assert nowait.lia_moe_timeouts_seen() == seen
