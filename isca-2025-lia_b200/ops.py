@@ -1482,12 +1482,13 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
     neighbouring channels; heads of 64 or 128 channels.  ``q`` [M, H * dim] and ``out`` [M, H * vdim] are bf16.  ``rows``: the most tokens of a portion; ``max_ctx``: the longest p0 + n,
     about (it decides how many blocks share a history, not what is read).  A row that sees nothing is 0; no two portions share a row; rows of no portion are left as they are; a portion that does not fit its slot, the
     rows, ``rows`` or the mask's words gives NaN rows."""
+    words, mp, dp, tp = mask.shape[-1] if mask is not None else 0, None, None, None
+    if mask is not None and 64 * words < rows:                      # (one of no words has no address, and would be none)
+        raise _lib.LiaError(f"tree_attn: {words} words of mask do not hold {rows} tokens")
     dev, M, nseg = _device(q, "tree_attn"), q.shape[0], segs.shape[0]
     qp, ldq = _rows_of(q, BF16, (M, H * dim), dev, "tree_attn: q")
     op, sp = _need(out, BF16, (M, H * vdim), dev, "tree_attn: out"), _need(segs, I32, (nseg, 4), dev, "tree_attn: segs")
-    words, mp, dp, tp = 0, None, None, None
     if mask is not None:
-        words = mask.shape[-1]
         mp = _need(mask, torch.int64, (M, words), dev, "tree_attn: mask")
     if depth is not None:
         dp = _need(depth, I32, (M,), dev, "tree_attn: depth")

@@ -190,3 +190,12 @@ def test_graphs_of_decode_steps_go_by_what_is_launched(lib, cache_dtype):
         assert key(requests, 1, windows) == key(requests, 256, windows) and key(requests, 2049, windows) == key(requests, 2304, windows)
     assert key(1, 256, [5000]) != key(1, 257, [5000]) and key(1, 256, [100]) == key(1, 257, [100]) == key(1, 60000, [100])
     assert key(1, 3000, [1 << 20]) != key(1, 60000, [1 << 20]) and key(200, 3000, [1 << 20]) == key(200, 60000, [1 << 20])
+
+
+@pytest.mark.parametrize("words,rows", [(0, 1), (0, 3), (1, 65), (2, 129)])
+def test_masks_that_hold_too_few_tokens(lib, words, rows):
+    """A mask of no words, whose tensor has no address, is not taken for no mask."""
+    from lia_b200 import ops
+    z, kv = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype), torch.zeros(1, 200, 128, dtype=BF16)  # noqa: E731
+    with pytest.raises(lib.LiaError, match=f"{words} words"):
+        ops.tree_attn(z(rows, 128), kv, kv, z(1, 4, dtype=torch.int32), z(rows, 128), 1, 1, 128, 128, 1.0, rows=rows, max_ctx=rows, mask=z(rows, words, dtype=torch.int64))
