@@ -47,6 +47,12 @@ class CheckpointError(RuntimeError):
     pass
 
 
+def no_cache_dtype(cls, options):
+    """Refuse ``cache_dtype`` among the options of a model whose caches have its own type: it would get one of twice the size."""
+    if options.get("cache_dtype") is not None:
+        raise ValueError(f"{cls.__name__} has no caches of {options['cache_dtype']}: cache_dtype is for Bebulorn's attention layers")
+
+
 # ------------------------------------------------------------------------------------------------
 # safetensors container
 # ------------------------------------------------------------------------------------------------

@@ -597,6 +597,7 @@ class OPTForCausalLM:
         writes) or this build's native slab directory (checkpoint.py), whose layers are read straight into
         HBM / the pinned arena without repacking."""
         from . import checkpoint
+        checkpoint.no_cache_dtype(cls, unused)
         ck = checkpoint.open_checkpoint(path)
         cfg = config or ck.config
         native = isinstance(ck, checkpoint.SlabCheckpoint)

@@ -236,7 +236,8 @@ class SekenexForCausalLM:
 
     @classmethod
     def from_pretrained(cls, path, device="cuda", dtype=BF16, **unused):
-        from .checkpoint import SafetensorsFile
+        from .checkpoint import SafetensorsFile, no_cache_dtype
+        no_cache_dtype(cls, unused)
         cfg = SekenexConfig.from_dict(json.load(open(os.path.join(path, "config.json"))), name=os.path.basename(os.path.abspath(path)) or "sekenex")
         f = SafetensorsFile(os.path.join(path, "model.safetensors"))
         try:

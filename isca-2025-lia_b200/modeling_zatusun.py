@@ -222,7 +222,8 @@ class ZatusunForCausalLM:
 
     @classmethod
     def from_pretrained(cls, path, device="cuda", dtype=BF16, **unused):
-        from .checkpoint import SafetensorsFile
+        from .checkpoint import SafetensorsFile, no_cache_dtype
+        no_cache_dtype(cls, unused)
         c = json.load(open(os.path.join(path, "config.json")))
         f = SafetensorsFile(os.path.join(path, "model.safetensors"))
         if "max_positions" not in c and "pos" in f.header:         # the table's own height says how far positions go

@@ -199,3 +199,19 @@ def test_masks_that_hold_too_few_tokens(lib, words, rows):
     z, kv = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype), torch.zeros(1, 200, 128, dtype=BF16)  # noqa: E731
     with pytest.raises(lib.LiaError, match=f"{words} words"):
         ops.tree_attn(z(rows, 128), kv, kv, z(1, 4, dtype=torch.int32), z(rows, 128), 1, 1, 128, 128, 1.0, rows=rows, max_ctx=rows, mask=z(rows, words, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("name", ["OPTForCausalLM", "Davasun", "Bizetar", "Zatusun", "Pazivik", "Sekenex"])
+def test_models_without_8_bit_caches_say_so(lib, tmp_path, name):
+    """Asked for a cache of 8 bits, a model that has none refuses, before it reads anything; None asks for nothing."""
+    import json
+
+    from lia_b200 import registry
+    (tmp_path / "config.json").write_text(json.dumps({"architecture": name}))
+    with pytest.raises(ValueError, match="no caches of torch.int8"):
+        registry.load_model(str(tmp_path), device="cpu", cache_dtype=torch.int8)
+    with pytest.raises(ValueError, match="no caches of torch.float8_e4m3fn"):
+        registry.model_class(str(tmp_path)).from_pretrained("nowhere", cache_dtype=E4M3)
+    with pytest.raises(Exception) as e:                             # (there is no checkpoint to read)
+        registry.load_model(str(tmp_path), device="cpu", cache_dtype=None)
+    assert "caches of" not in str(e.value)
