@@ -523,6 +523,7 @@ extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* k
   LIA_CHECK_ARG(kc->type == vc->type && kc->slots == vc->slots && kc->capacity == vc->capacity, "lia_tree_attn: caches of different types or sizes");
   LIA_CHECK_ARG(kc->capacity <= 1 << 29, "lia_tree_attn: more than 2^29 positions");               // (positions, depths and windows are added up in 32 bits)
   LIA_CHECK_ARG(M >= 0 && nseg >= 0 && rows >= 0 && max_ctx >= 0 && G > 0 && H > 0 && H % G == 0, "lia_tree_attn: bad sizes");
+  LIA_CHECK_ARG(!(softcap > MOST_SOFTCAP), "lia_tree_attn: a soft cap of %g is more than %g", softcap, MOST_SOFTCAP);
   if (M == 0 || nseg == 0 || rows == 0) return LIA_OK;
   LIA_CHECK_ARG(q && segs && out && (mask == nullptr || words > 0), "lia_tree_attn: null pointer");
   LIA_CHECK_ARG(ldq >= (long long)H * kc->dim && ldq % 4 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0, "lia_tree_attn: queries and outputs have to be whole 8-byte vectors");

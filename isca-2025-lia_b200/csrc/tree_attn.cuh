@@ -97,7 +97,9 @@ __device__ __forceinline__ Down down_of(uint32_t top) {
   return {__uint_as_float((268 - e) << 23), __uint_as_float((e - 14) << 23)};
 }
 
-// cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))): off by a rounding of cap
+// cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))): off by up to 2^-21 of cap (the power 2^-22 of itself, the sum half a step, the quotient two), whatever x is, so that caps end where
+// that is 2^-11, what weights of 11 bits are off by
+constexpr float MOST_SOFTCAP = 1024.f;
 __device__ __forceinline__ float capped(float x, float cap, float two_log2e_by_cap) { return cap - __fdividef(2.f * cap, 1.f + ex2(x * two_log2e_by_cap)); }
 
 template <int KIND> __device__ __forceinline__ float cached(const uint8_t* head, int c) {

@@ -1476,7 +1476,7 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
     row .. row + n - 1 have their keys and values at positions p0 .. p0 + n - 1 already.  Every token sees the p0 positions of history and, without ``mask``, the new tokens up to itself
     (n = 1: a decoded token; a chain of drafted tokens; a portion of a prompt); with ``mask`` int64 [M, words] the new tokens j whose bit j is set in its row (a tree of drafted tokens:
     its ancestors and itself).  ``window`` > 0: of the history, and without ``mask`` of the new tokens, only the last window - 1 positions before its own, which is p0 + ``depth``
-    (int32 [M]; None: its number in the portion).  Scores are temp[h] * scale * (q . k), then softcap * tanh(score / softcap) if ``softcap`` > 0.
+    (int32 [M]; None: its number in the portion).  Scores are temp[h] * scale * (q . k), then softcap * tanh(score / softcap) if ``softcap`` > 0 (1024 at most).
 
     Caches: bf16, or int8 / float8_e4m3fn with ``k_scale`` and ``v_scale`` [slots, G, capacity] (``kv_store_8bit``), [slots, capacity, G * dim] or [slots, capacity, G, dim] with
     neighbouring channels; heads of 64 or 128 channels.  ``q`` [M, H * dim] and ``out`` [M, H * vdim] are bf16.  ``rows``: the most tokens of a portion; ``max_ctx``: the longest p0 + n,

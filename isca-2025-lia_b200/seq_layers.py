@@ -415,11 +415,13 @@ class WindowAttentionMixer:
     positional rotation.  Values are divided by their per-head root mean square before they are cached; a score is
     (q . k) * scale * temp_h, then softcap * tanh(score / softcap) (csrc/window_attn.cu); output Wo on the concatenated heads.
     ``cache_dtype`` int8 or float8_e4m3fn: keys and values are cached in 8 bits with a scale per head and token (csrc/kv_8bit.cu, csrc/tree_attn.cu): half the memory, and less of
-    it to read for every token; bf16 layers with heads of 64 or 128 channels."""
+    it to read for every token; bf16 layers with heads of 64 or 128 channels, and soft caps up to 1024."""
 
     def __init__(self, w, heads, kv_heads, dim, vdim, window, scale, softcap, norm_eps, dtype, device, norm_values=True, cache_dtype=None):
         if cache_dtype is not None and (cache_dtype not in (torch.int8, torch.float8_e4m3fn) or dtype != BF16 or dim not in (64, 128) or vdim not in (64, 128)):
             raise ValueError(f"caches of 8 bits are int8 or float8_e4m3fn, for bf16 layers with heads of 64 or 128 channels, not {cache_dtype} for {dtype} with heads of {dim} and {vdim}")
+        if cache_dtype is not None and softcap > 1024:
+            raise ValueError(f"caches of 8 bits: scores are capped at 1024 at most, not {softcap}")
         self.cache_dtype = cache_dtype
         if heads % kv_heads:
             raise ValueError(f"{heads} heads do not divide into {kv_heads} key/value heads")

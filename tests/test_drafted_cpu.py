@@ -215,3 +215,15 @@ def test_models_without_8_bit_caches_say_so(lib, tmp_path, name):
     with pytest.raises(Exception) as e:                             # (there is no checkpoint to read)
         registry.load_model(str(tmp_path), device="cpu", cache_dtype=None)
     assert "caches of" not in str(e.value)
+
+
+def test_soft_caps_end_where_scores_would_be_lost(lib):
+    """A capped score is off by up to 2^-21 of the cap, whatever the score: of a cap of 10^8 nothing is left of scores of 8, and all would weigh the same."""
+    from lia_b200.seq_layers import WindowAttentionMixer
+    L, v = lib.load(), view(lib)
+    attend = lambda softcap, M: L.lia_tree_attn(256, 2048, v, v, 256, 2, None, 0, None, None, 256, None, 0, M, 16, 8, 4, 40, 0, 1.0, softcap, None)  # noqa: E731
+    for softcap in (1025.0, 1e8, float("inf")):
+        assert attend(softcap, 8) == -1 and "soft cap" in lib.last_error()
+    assert attend(1024.0, 0) == attend(0.0, 0) == attend(-1.0, 0) == 0
+    with pytest.raises(ValueError, match="1024"):
+        WindowAttentionMixer({}, 4, 2, 64, 64, 40, 0.1, 2000.0, 1e-5, BF16, "cpu", cache_dtype=torch.int8)
