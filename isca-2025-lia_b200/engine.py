@@ -225,6 +225,8 @@ class Engine:
         """How likely each token of ``prompts`` (lists of ids, any lengths) was after those before it, as one batch: prompts in portions of ``chunk`` tokens (None: as many as fill a pass).
         Returns a dict per prompt with lists over its tokens but the first: ``logp``, the ``entropy`` of the distribution that the token came from (nats), and the ``top`` <= 32 most likely
         tokens there, as (id, log probability) pairs in ``alternatives``."""
+        if chunk is not None and chunk < 0:
+            raise ValueError(f"portions of {chunk} tokens")
         prompts = [[int(t) for t in p] for p in prompts]
         keys = [("score", i) for i in range(len(prompts))]
         out = [{"logp": [], "entropy": [], "alternatives": []} for _ in prompts]

@@ -227,3 +227,14 @@ def test_soft_caps_end_where_scores_would_be_lost(lib):
     assert attend(1024.0, 0) == attend(0.0, 0) == attend(-1.0, 0) == 0
     with pytest.raises(ValueError, match="1024"):
         WindowAttentionMixer({}, 4, 2, 64, 64, 40, 0.1, 2000.0, 1e-5, BF16, "cpu", cache_dtype=torch.int8)
+
+
+def test_scores_of_portions_of_less_than_nothing(lib):
+    """A negative portion is refused: no step would be made, and every text would be scored as one without tokens."""
+    import types
+
+    from lia_b200.engine import Engine
+    from lia_b200.seq_state import SlotState
+    m = types.SimpleNamespace(device=torch.device("cpu"), config=types.SimpleNamespace(vocab=11), new_state=lambda n, cap: SlotState(n, cap, "cpu"))
+    with pytest.raises(ValueError, match="-2"):
+        Engine(m, 16).score([[1, 2, 3]], chunk=-2)
