@@ -674,7 +674,8 @@ int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const LiaCacheView
  * p0 .. p0 + n - 1 of the slot, behind p0 cached positions.  Row i of a portion sees the history -- with window > 0 its positions above p0 + depth_i - window -- and of the n new
  * tokens: without mask those up to its own (under the same window), else those whose bits are set in its `words` 64-bit words of mask (bit j: the portion's token j).  depth_i:
  * depth[row + i], or i where depth is NULL.  A score is temp[h] * scale * (q . k), then softcap * tanh(score / softcap) if softcap > 0 (1024 at most; off by up to 2^-21 of softcap); query head h reads key/value head
- * h / (H / G).  A row that sees nothing is 0; what it does not see has no effect, whatever its bits.  Scales are 0 or more, values' up to 2^29 (values with a smaller one
+ * h / (H / G).  A row that sees nothing is 0; what it does not see has no effect, whatever its bits (but on time: rows that meet a
+ * NaN or an infinity are formed again key by key, 1.3 us for each key of each, so that a request whose cache holds one is better ended).  Scales are 0 or more, values' up to 2^29 (values with a smaller one
  * than 2^-80 are off by 2^-71 at most).  No two portions share a row.  Rows of no portion stay as they are; a portion that its slot, the M rows, the mask's
  * words or `rows` cannot hold gives NaN rows.  rows: the most rows of a portion; max_ctx: about the longest p0 + n (it decides how many blocks share a history, no more).
  * q and out: bf16, ldq apart and [M, H * vdim], on 8-byte boundaries.  Heads of 64 or 128 channels, 2^29 positions at most.  ws: lia_tree_attn_workspace_floats() floats (0: NULL will do). */

@@ -5,9 +5,12 @@
 //          loses nothing against a / 448 down to a / 28672, and makes scaling and reading back exact.
 // One scale for each head of each token: a token that comes later changes nothing that is there, and attention multiplies scores and weights by scales instead of channels by them.
 //
-// Both kernels move each number once; storing computes ten operations on it, so that instructions would bound it before memory does if each lane had few numbers: a lane has 32
-// neighbouring channels of a head (four lanes a head of 128), which divides the addresses, the scale and the steps of finding the largest magnitude among them.  Magnitudes of bf16 numbers
-// are compared as pairs of whole numbers, and a normed head's largest is the largest before, times the norm's factor, because rounding keeps order.
+// Both kernels move each number once.  A lane has 32 neighbouring channels of a head (four lanes a head of 128), which divides the addresses, the scale and the steps of finding the largest magnitude
+// among them.  Magnitudes of bf16 numbers are compared as pairs of whole numbers, and a normed head's largest is the largest before, divided as it is, because rounding keeps order.
+//
+// What bounds them, by counters: storing normed values instructions, some 25 issued a number (7169 tokens of 8 heads of 128 to e4m3 11.5 us, issue slots 71 % busy, memory 25 %); reading back the SMs' own
+// way to memory (86 % of its peak, memory 49 %: 16 histories of 8191 tokens 136 us): a lane's vectors are neighbours, so that one instruction of a warp touches 16 bytes of every 64, half of
+// each sector.
 #include <cuda_fp8.h>
 
 #include "cache8.cuh"
@@ -85,8 +88,9 @@ template <bool INT8> struct Coder {
     const float a = fmaxf(largest, LEAST);
     const int e = (int)(__float_as_uint(a) >> 23) - 127;           // a = 1.m 2^e, -100 <= e <= 127
     if constexpr (INT8) {
-      // 127 x / a, correctly rounded (a quotient's estimate and one correction by its exact remainder), so that a tie is a tie: x = a / 2 is 63.5 whatever 1 / a rounds to.
-      // Both sides are divided by 128 and by a power of two near a, which is exact and keeps 127 x and 1 / a among the normal numbers.
+      // 127 x / a, correctly rounded by Markstein's method (1990: an estimate of the quotient from the rounded reciprocal, and one correction by its exact remainder), so that a tie is a tie: x = a / 2
+      // is 63.5 whatever 1 / a rounds to.  Both sides are divided by 128 and by a power of two near a, which keeps 127 x and 1 / a among the normal numbers.  127 x is exact for bf16 numbers; of fp32 ones it is
+      // rounded once before, so that a code may be the neighbour's where the exact quotient is within 2^-23 of itself from a border.
       const float down = __uint_as_float((uint32_t)(127 - min(e, 126)) << 23);
       scale = a / 127.f;
       as = a * down;
@@ -124,7 +128,7 @@ template <bool INT8> struct Coder {
   }
 };
 
-// x / root, with inv = 1 / root: the estimate and one correction by its exact remainder.  (x * inv behind squares summed in one chain moved more normed values across a border between codes: the
+// x / root, with inv = 1 / root, by the same method.  (x * inv behind squares summed in one chain moved more normed values across a border between codes: the
 // codes of 8 million were off by 1.8e-4 of their size, root mean square, instead of 2e-5.)
 __device__ __forceinline__ float quotient(float x, float root, float inv) {
   const float q = x * inv;

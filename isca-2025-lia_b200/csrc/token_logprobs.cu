@@ -5,11 +5,11 @@
 // One pass over the logits: every thread keeps a running maximum with its L and A (a larger maximum multiplies both by a power and moves A by L times the step).  The largest ones are
 // found from what that leaves: the top-th largest of the 256 threads' maxima is reached by at least `top` logits and, as the largest ones seldom share a thread, by few more; every thread
 // knows the maxima of four parts of its logits, so that only the parts that reach it are read again (a fortieth of the row, from L2), by all lanes of their warps.  What reaches the bound is sorted across a warp's lanes,
-// as whole numbers that order by value and then by lower id.  (A list of the largest ones kept by every warp through the pass took 34 instructions a logit instead of 7.)
+// as whole numbers that order by value and then by lower id.  (With lists of the largest ones kept by every warp through the pass 4096 rows took 577 us instead of 172.)
 // Few rows share out a row over a cluster of up to eight blocks of threads, whose first one joins the parts (in the same order each time).
 //
-// Bound, at 4096 rows of 50272 logits: fp32 by memory, 131 us without the largest ones (96 % of the rate of a copy) and 156 with the 20 largest; bf16, half the bytes, by instructions (eight a logit, a
-// power among them): 96 and 150 us.  Few rows by the latency of one block of logits and of sorting: four rows 9 us.
+// Bound, at 4096 rows of 50272 logits: fp32 by memory, 131 us without the largest ones (96 % of the rate of a copy) and 156 with the 20 largest; bf16, half the bytes, by instructions:
+// 96 and 150 us.  (Issued are some 17 a logit, counted with fp32 and the 20 largest, issue slots 61 % busy.)  Few rows by the latency of one block of logits and of sorting: four rows 9 us.
 #include "pairs.cuh"
 
 namespace {

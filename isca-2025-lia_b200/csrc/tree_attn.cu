@@ -17,7 +17,7 @@
 // The maximum moves only when a key exceeds it by 2^8, which the 7 leaves room for; the rows' sums are multiplied only then.
 //
 // Bound: bf16 caches by memory, 8-bit ones by instructions too (a byte is widened, half of them after two codes change places; a score takes some fifteen).  A token of 16 heads on 8 for each of 16
-// histories of 60000 positions: bf16 563 us (7.0 TB/s, what a copy reaches at the most), int8 398 to 419 (5.1 to 4.8), e4m3 377 to 391 (5.4 to 5.2).  Behind 1901 positions, int8: 19.5 us, of which memory 10; the rest is
+// histories of 60000 positions: bf16 563 us (7.0 TB/s; a copy, which writes half of what it moves, has 6.55), int8 398 to 419 (5.1 to 4.8), e4m3 377 to 391 (5.4 to 5.2).  Behind 1901 positions, int8: 19.5 us, of which memory 10; the rest is
 // one block's way from its first load to its last sum.  (Arguments are taken where the launch put them: copied to each thread's stack, for rows that are formed again, they cost 2 us a block.)
 #include "mma.cuh"
 #include "tree_attn.cuh"

@@ -1479,7 +1479,8 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
     (int32 [M]; None: its number in the portion).  Scores are temp[h] * scale * (q . k), then softcap * tanh(score / softcap) if ``softcap`` > 0 (1024 at most).
 
     Caches: bf16, or int8 / float8_e4m3fn with ``k_scale`` and ``v_scale`` [slots, G, capacity] (``kv_store_8bit``), [slots, capacity, G * dim] or [slots, capacity, G, dim] with
-    neighbouring channels; heads of 64 or 128 channels.  ``q`` [M, H * dim] and ``out`` [M, H * vdim] are bf16.  ``rows``: the most tokens of a portion; ``max_ctx``: the longest p0 + n,
+    neighbouring channels; heads of 64 or 128 channels; values' scales up to 2^29.  A NaN or an infinity among keys or values that a tile of rows reads has its rows formed again key by key, about a
+    thousand times slower.  ``q`` [M, H * dim] and ``out`` [M, H * vdim] are bf16.  ``rows``: the most tokens of a portion; ``max_ctx``: the longest p0 + n,
     about (it decides how many blocks share a history, not what is read).  A row that sees nothing is 0; no two portions share a row; rows of no portion are left as they are; a portion that does not fit its slot, the
     rows, ``rows`` or the mask's words gives NaN rows."""
     words, mp, dp, tp = mask.shape[-1] if mask is not None else 0, None, None, None
