@@ -13,7 +13,7 @@
 //
 // 8-bit codes are exact in fp16 and so are multiplied there: q goes to fp16 by a power of two of its own for each row (its 8 bits fit; what is 2^-29 of the row's largest is
 // less exact), a key's scale is multiplied into its scores, and a value's into its weight -- in the exponent, x = s + log2 vs, so that the maximum bounds the product and no scale is
-// too large or small: weights are 2^(x - max + 7) in fp16, 11 bits, and their sum takes p = weight / vs in fp32.  With bf16 caches weights are two bf16 parts: 16 bits.
+// too large or small: weights are 2^(x - max + 7) in fp16, 11 bits (fewer below 2^-21 of the row's largest, none below 2^-32), and their sum takes p = weight / vs in fp32.  With bf16 caches weights are two bf16 parts: 16 bits.
 // The maximum moves only when a key exceeds it by 2^8, which the 7 leaves room for; the rows' sums are multiplied only then.
 //
 // Bound: bf16 caches by memory, 8-bit ones by instructions too (a byte is widened, half of them after two codes change places; a score takes some fifteen).  A token of 16 heads on 8 for each of 16
