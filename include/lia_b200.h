@@ -646,15 +646,18 @@ int lia_router_topk_grouped(const float* logits, int ldl, const float* correctio
  * Serving with drafted tokens: caches of 8 bits, attention of several new tokens behind a history, log probabilities.
  * (Not in the reference, which caches bf16 and decodes one token per sequence.)
  * ---------------------------------------------------------------------------------------------------------------- */
-enum { LIA_CACHE_BF16 = 0, LIA_CACHE_INT8 = 1, LIA_CACHE_E4M3 = 2 };
+enum { LIA_CACHE_BF16 = 0, LIA_CACHE_INT8 = 1, LIA_CACHE_E4M3 = 2, LIA_CACHE_INT4 = 3 };
 
 /* One side (keys or values) of a cache of heads of `dim` channels: the number of (slot, position, head, channel) lies at
  * data[slot * slot_stride + position * pos_stride + head * head_stride + channel], strides in numbers; with 8 bits the numbers of a
  * (slot, position, head) stand for themselves times scale[slot * scale_slot_stride + head * scale_head_stride + position].  data and all its
- * strides: whole 16-byte vectors (8 bytes for lia_kv_store_8bit and lia_kv_load_8bit). */
+ * strides: whole 16-byte vectors (8 bytes for lia_kv_store_8bit, lia_kv_load_8bit, lia_kv_store_4bit and lia_kv_load_4bit).
+ * With 4 bits a head is dim / 2 bytes (strides of data count bytes), dim a multiple of 32: channel c is in byte 2 * ((c % 32 / 4) * (dim / 32) + c / 32) + c % 4 / 2, as code + 8 in the lower four
+ * bits for an even c, the upper four for an odd one.  It stands for code times the bf16 number scale[slot * scale_slot_stride + head * scale_head_stride + position * (dim / 32) + c / 32]; a position's
+ * scales are read together, so that scale and its strides are whole vectors of 8 bytes (4, 2) where dim / 32 is a multiple of 4 (of 2, neither). */
 typedef struct LiaCacheView {
   void* data;
-  float* scale;                  /* NULL with bf16 */
+  void* scale;                   /* fp32, with 4 bits bf16; NULL with bf16 */
   int64_t slot_stride, pos_stride, head_stride, scale_slot_stride, scale_head_stride;
   int32_t slots, capacity, type, dim;
 } LiaCacheView;
@@ -668,6 +671,13 @@ int lia_kv_store_8bit(const void* k, long long ldk, const void* v, long long ldv
                       float eps, int norm_values, lia_stream_t stream);
 /* The reverse: code * scale of the rows at meta into k [M, G * dim] and v [M, G * vdim]; NaN for a row whose slot or position the caches do not have */
 int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, void* k, long long ldk, void* v, long long ldv, int out_f32, int M, int G,
+                     lia_stream_t stream);
+
+/* The same with caches of 4 bits, every 32 channels of a head with a scale of their own: scale = a / 7 rounded to fp32 and then to bf16, with a the largest magnitude of the 32 numbers (counted as 2^-100
+ * at least); code = rint(x / scale), -7 to 7, of the exact quotient.  A group with an infinity or NaN gets scale NaN and codes 0; the head's other groups do not depend on it.  Heads of up to 1024 channels. */
+int lia_kv_store_4bit(const void* k, long long ldk, const void* v, long long ldv, int act_f32, const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, int M, int G,
+                      float eps, int norm_values, lia_stream_t stream);
+int lia_kv_load_4bit(const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, void* k, long long ldk, void* v, long long ldv, int out_f32, int M, int G,
                      lia_stream_t stream);
 
 /* Attention of portions of new tokens behind their histories.  segs[i] = (slot, p0, row, n): the n tokens of rows row .. row + n - 1 have their keys and values at positions

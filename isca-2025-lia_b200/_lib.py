@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(_HERE, "libliab200.so")
 
 EPI_BIAS, EPI_BIAS_RELU, EPI_BIAS_RESIDUAL, EPI_QKV = 0, 1, 2, 3
 ABI_VERSION = 11
-CACHE_BF16, CACHE_INT8, CACHE_E4M3 = 0, 1, 2
+CACHE_BF16, CACHE_INT8, CACHE_E4M3, CACHE_INT4 = 0, 1, 2, 3
 TP_MAX_WORLD = 8
 P2P_HANDLE_BYTES = 64
 
@@ -238,6 +238,9 @@ _PROTOTYPES = {
     "lia_kv_store_8bit": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_int, c_int, c_float, c_int,
                                   c_void_p]),
     "lia_kv_load_8bit": (c_int, [c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p]),
+    "lia_kv_store_4bit": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_int, c_int, c_float, c_int,
+                                  c_void_p]),
+    "lia_kv_load_4bit": (c_int, [c_void_p, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p]),
     "lia_tree_attn_plan": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "lia_tree_attn_workspace_floats": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "lia_tree_attn": (c_int, [c_void_p, c_longlong, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,

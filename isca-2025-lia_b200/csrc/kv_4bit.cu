@@ -1,0 +1,249 @@
+// Keys and values in 4 bits: quantised as they are written into a cache, and read back.
+//
+//   a = max |x| over 32 channels of a head of one token, s = bf16(a / 7), code = rint(x / s) in -7 .. 7, x stands for code * s: 4.5 bits a number
+//
+// An even grid without an offset: a group's zero is a zero, and a score is a sum of whole numbers times one scale.  Groups of 32: of normal numbers they leave 1 / 11 of their size as error, whole heads of
+// 128 1 / 9, and a channel that is ten times the others takes the bits of 31 others instead of 127.
+//
+// Eight lanes have a head: lane q takes the channels 4 q .. 4 q + 3 of every group, which are 64 neighbouring bytes of bf16 activations for the eight, and whose codes are neighbours in the cache (byte4()).  Up
+// to four groups at a time, so that a lane's codes of 128 channels are one 8-byte store.
+#include "cache8.cuh"
+
+namespace {
+
+constexpr int THREADS = 256, LANES = 8, AT_ONCE = 4;               // lanes of a head, groups that a lane takes at a time
+constexpr float LEAST = 7.888609052210118e-31f;                    // 2^-100: keeps scales and their inverses normal numbers
+
+struct Side {
+  const void* x;                                                   // rows of activations (store) or where they go (load)
+  long long ld;
+  Cache8 c;
+  int vec, norm;                                                   // rows' fours are whole vectors apart
+};
+struct Head {
+  bool there;
+  int row, g, q, slot, pos;
+};
+__device__ __forceinline__ Head head_of(unsigned block, const int* meta, int M, int G) {
+  Head h;
+  const unsigned i = block * (THREADS / LANES) + threadIdx.x / LANES;
+  h.there = i < (unsigned)M * G;
+  h.row = h.there ? i / (unsigned)G : 0;
+  h.g = h.there ? i - h.row * (unsigned)G : 0;
+  h.q = threadIdx.x % LANES;
+  h.slot = h.there ? meta[2ll * h.row] : -1;
+  h.pos = h.there ? meta[2ll * h.row + 1] : -1;
+  return h;
+}
+
+template <typename T> __device__ __forceinline__ void load4(const T* p, bool vec, float* x) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec) {
+      const uint2 u = __ldcg(reinterpret_cast<const uint2*>(p));
+      unpack_bf16x2(u.x, x[0], x[1]);
+      unpack_bf16x2(u.y, x[2], x[3]);
+      return;
+    }
+  } else if (vec) {
+    *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(p));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (float)p[i];
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, bool vec, const float* x) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+      return;
+    }
+  } else if (vec) {
+    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = (T)x[i];
+}
+
+// x / d, correctly rounded, with inv = 1 / d correctly rounded (Markstein 1990: the estimate and one correction by its exact remainder)
+__device__ __forceinline__ float quotient(float x, float d, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-d, q, x), inv, q);
+}
+
+// `n` numbers of 16 bits, as wide as a lane's n groups of ng lie; eight lanes' are neighbours
+__device__ __forceinline__ void put_units(uint16_t* dst, int ng, int n, const uint32_t* u) {
+  if ((ng & 3) == 0) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
+  } else if ((ng & 1) == 0) {
+    *reinterpret_cast<uint32_t*>(dst) = u[0] | u[1] << 16;
+    if (n > 2) *reinterpret_cast<uint32_t*>(dst + 2) = u[2] | u[3] << 16;
+  } else {
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+      if (i < n) dst[i] = (uint16_t)u[i];
+  }
+}
+__device__ __forceinline__ void get_units(const uint16_t* src, int ng, int n, uint32_t* u) {
+  if ((ng & 3) == 0) {
+    const uint2 w = __ldcg(reinterpret_cast<const uint2*>(src));
+    u[0] = w.x & 0xffffu, u[1] = w.x >> 16, u[2] = w.y & 0xffffu, u[3] = w.y >> 16;
+  } else if ((ng & 1) == 0) {
+    const uint32_t a = __ldcg(reinterpret_cast<const uint32_t*>(src)), b = n > 2 ? __ldcg(reinterpret_cast<const uint32_t*>(src + 2)) : 0u;
+    u[0] = a & 0xffffu, u[1] = a >> 16, u[2] = b & 0xffffu, u[3] = b >> 16;
+  } else {
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) u[i] = i < n ? __ldcg(src + i) : 0u;
+  }
+}
+
+// Grid: blocks of heads of k and, behind them, of v
+template <typename T>
+__global__ void __launch_bounds__(THREADS) kv_store_4bit_kernel(const __grid_constant__ Side k, const __grid_constant__ Side v, const int* __restrict__ meta, int M, int G, int blocks, float eps) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const bool is_v = (int)blockIdx.x >= blocks;
+  const Side& s = is_v ? v : k;
+  const Head h = head_of(is_v ? blockIdx.x - blocks : blockIdx.x, meta, M, G);
+  const int ng = s.c.dim / GROUP4;
+  const T* src = reinterpret_cast<const T*>(s.x) + h.row * s.ld + h.g * s.c.dim + h.q * 4;
+  float x[AT_ONCE][4];
+  auto load = [&](int g0) {
+#pragma unroll
+    for (int g = 0; g < AT_ONCE; ++g) {
+      x[g][0] = x[g][1] = x[g][2] = x[g][3] = 0.f;
+      if (h.there && g0 + g < ng) load4(src + (g0 + g) * GROUP4, s.vec, x[g]);
+    }
+  };
+  load(0);
+  float root = 1.f, inv_root = 1.f;
+  if (s.norm) {
+    float sum = 0.f;
+    for (int g0 = 0; g0 < ng; g0 += AT_ONCE) {
+      if (g0 > 0) load(g0);
+      float part[AT_ONCE];
+#pragma unroll
+      for (int g = 0; g < AT_ONCE; ++g) part[g] = fmaf(x[g][0], x[g][0], x[g][1] * x[g][1]) + fmaf(x[g][2], x[g][2], x[g][3] * x[g][3]);
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    root = sqrtf(sum / (float)s.c.dim + eps);
+    inv_root = 1.f / root;
+    if (ng > AT_ONCE) load(0);
+  }
+  const bool held = s.c.holds(h.slot, h.pos);
+  uint16_t* codes = held ? reinterpret_cast<uint16_t*>(s.c.at(h.slot, h.pos, h.g)) + h.q * ng : nullptr;
+  uint16_t* scales = held ? reinterpret_cast<uint16_t*>(s.c.scale4_at(h.slot, h.g)) + (long long)h.pos * ng : nullptr;
+  for (int g0 = 0; g0 < ng; g0 += AT_ONCE) {
+    if (g0 > 0) load(g0);
+    uint32_t most[AT_ONCE], units[AT_ONCE], sc[AT_ONCE];
+#pragma unroll
+    for (int g = 0; g < AT_ONCE; ++g) {
+      if (s.norm) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[g][i] = root > 3.402823466e38f ? x[g][i] * 0.f : quotient(x[g][i], root, inv_root);
+      }
+      most[g] = 0u;                                                // magnitudes as whole numbers: NaN is above infinity and that above the rest
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most[g] = max(most[g], __float_as_uint(x[g][i]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) most[g] = max(most[g], __shfl_xor_sync(0xffffffffu, most[g], o));
+      const bool bad = most[g] >= 0x7f800000u;
+      const __nv_bfloat16 s16 = __float2bfloat16_rn(fmaxf(__uint_as_float(most[g]), LEAST) / 7.f);
+      const float scale = bad ? 1.f : __bfloat162float(s16), inv = __frcp_rn(scale);
+      sc[g] = bad ? 0x7fc0u : (uint32_t)__bfloat16_as_ushort(s16);
+      uint32_t u = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // rint of the quotient that is rounded to 24 bits; where that made a tie of it, the exact rest (12 bits times 8, below x: no rounding) tells on which side it was
+        float c = rintf(quotient(x[g][i], scale, inv));
+        const float rest = fmaf(-c, scale, x[g][i]);
+        if (sizeof(T) == 4 || s.norm) c += fabsf(rest) > 0.5f * scale ? copysignf(1.f, rest) : 0.f;
+        u |= (uint32_t)((bad ? 0 : (int)c) + 8) << (4 * i);
+      }
+      units[g] = u;
+    }
+    if (!held) continue;
+    const int n = min(AT_ONCE, ng - g0);
+    put_units(codes + g0, ng, n, units);
+    if (h.q == 0) put_units(scales + g0, ng, n, sc);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) kv_load_4bit_kernel(const __grid_constant__ Side k, const __grid_constant__ Side v, const int* __restrict__ meta, int M, int G, int blocks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const bool is_v = (int)blockIdx.x >= blocks;
+  const Side& s = is_v ? v : k;
+  const Head h = head_of(is_v ? blockIdx.x - blocks : blockIdx.x, meta, M, G);
+  if (!h.there) return;
+  const int ng = s.c.dim / GROUP4;
+  const bool held = s.c.holds(h.slot, h.pos);
+  const uint16_t* codes = held ? reinterpret_cast<const uint16_t*>(s.c.at(h.slot, h.pos, h.g)) + h.q * ng : nullptr;
+  const uint16_t* scales = held ? reinterpret_cast<const uint16_t*>(s.c.scale4_at(h.slot, h.g)) + (long long)h.pos * ng : nullptr;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(s.x)) + h.row * s.ld + h.g * s.c.dim + h.q * 4;
+  for (int g0 = 0; g0 < ng; g0 += AT_ONCE) {
+    const int n = min(AT_ONCE, ng - g0);
+    uint32_t u[AT_ONCE] = {}, sc[AT_ONCE] = {0x7fc0u, 0x7fc0u, 0x7fc0u, 0x7fc0u};
+    if (held) {
+      get_units(codes + g0, ng, n, u);
+      get_units(scales + g0, ng, n, sc);
+    }
+#pragma unroll
+    for (int g = 0; g < AT_ONCE; ++g) {
+      if (g >= n) break;
+      const float scale = __uint_as_float(sc[g] << 16);
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (float)((int)(u[g] >> (4 * i) & 15u) - 8) * scale;
+      store4(dst + (g0 + g) * GROUP4, s.vec, x);
+    }
+  }
+}
+
+Side make_side(const void* x, long long ld, int act_f32, const LiaCacheView* view, int norm) {
+  const int bytes = act_f32 ? 16 : 8;
+  return {x, ld, cache8(view), reinterpret_cast<uintptr_t>(x) % bytes == 0 && ld % 4 == 0, norm};
+}
+
+const char* sides_wrong(const void* k, const void* v, const void* meta, const LiaCacheView* kc, const LiaCacheView* vc, long long ldk, long long ldv, int M, int G) {
+  const char* w = nullptr;
+  if (M < 0 || G <= 0 || (M > 0 && (!k || !v || !meta))) return "null pointer or no heads";     // (no rows have no address)
+  if ((w = cache8_wrong(kc, 8)) || (w = cache8_wrong(vc, 8))) return w;
+  if (kc->type != LIA_CACHE_INT4 || vc->type != LIA_CACHE_INT4) return "both caches have to be of 4 bits";
+  if (kc->slots != vc->slots || kc->capacity != vc->capacity) return "caches of different sizes";
+  if (kc->dim > 1024 || vc->dim > 1024) return "heads have 1024 channels at most";
+  if ((long long)M * G >= 1ll << 31) return "too many rows";
+  if (ldk < (long long)G * kc->dim || ldv < (long long)G * vc->dim) return "rows shorter than their heads";
+  return w;
+}
+
+}  // namespace
+
+extern "C" int lia_kv_store_4bit(const void* k, long long ldk, const void* v, long long ldv, int act_f32, const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, int M, int G,
+                                 float eps, int norm_values, lia_stream_t stream_) {
+  const char* wrong = sides_wrong(k, v, meta, kc, vc, ldk, ldv, M, G);
+  LIA_CHECK_ARG(!wrong, "lia_kv_store_4bit: %s", wrong);
+  if (M == 0) return LIA_OK;
+  const Side a = make_side(k, ldk, act_f32, kc, 0), b = make_side(v, ldv, act_f32, vc, norm_values != 0);
+  const int blocks = (int)(((long long)M * G * LANES + THREADS - 1) / THREADS);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  if (act_f32) LIA_CUDA(lia_launch(kv_store_4bit_kernel<float>, dim3(2 * blocks), dim3(THREADS), 0, stream, a, b, meta, M, G, blocks, eps));
+  else LIA_CUDA(lia_launch(kv_store_4bit_kernel<bf16>, dim3(2 * blocks), dim3(THREADS), 0, stream, a, b, meta, M, G, blocks, eps));
+  return LIA_OK;
+}
+
+extern "C" int lia_kv_load_4bit(const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, void* k, long long ldk, void* v, long long ldv, int out_f32, int M, int G,
+                                lia_stream_t stream_) {
+  const char* wrong = sides_wrong(k, v, meta, kc, vc, ldk, ldv, M, G);
+  LIA_CHECK_ARG(!wrong, "lia_kv_load_4bit: %s", wrong);
+  if (M == 0) return LIA_OK;
+  const Side a = make_side(k, ldk, out_f32, kc, 0), b = make_side(v, ldv, out_f32, vc, 0);
+  const int blocks = (int)(((long long)M * G * LANES + THREADS - 1) / THREADS);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  if (out_f32) LIA_CUDA(lia_launch(kv_load_4bit_kernel<float>, dim3(2 * blocks), dim3(THREADS), 0, stream, a, b, meta, M, G, blocks));
+  else LIA_CUDA(lia_launch(kv_load_4bit_kernel<bf16>, dim3(2 * blocks), dim3(THREADS), 0, stream, a, b, meta, M, G, blocks));
+  return LIA_OK;
+}

@@ -291,7 +291,7 @@ const char* sides_wrong(const void* k, const void* v, const void* meta, const Li
   const char* w = nullptr;
   if (M < 0 || G <= 0 || (M > 0 && (!k || !v || !meta))) return "null pointer or no heads";     // (no rows have no address)
   if ((w = cache8_wrong(kc, 8)) || (w = cache8_wrong(vc, 8))) return w;
-  if (kc->type == LIA_CACHE_BF16 || kc->type != vc->type) return "both caches have to be int8, or both e4m3";
+  if ((kc->type != LIA_CACHE_INT8 && kc->type != LIA_CACHE_E4M3) || kc->type != vc->type) return "both caches have to be int8, or both e4m3";
   if (kc->slots != vc->slots || kc->capacity != vc->capacity) return "caches of different sizes";
   if (kc->dim % 8 || vc->dim % 8 || kc->dim > 1024 || vc->dim > 1024) return "heads have to be multiples of 8 channels, 1024 at most";
   if ((long long)M * G >= 1ll << 31) return "too many rows";

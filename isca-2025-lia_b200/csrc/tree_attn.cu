@@ -44,25 +44,26 @@ constexpr int blocks_an_sm(int kind, int nr) { return nr == 1 ? (kind == LIA_CAC
 
 template <int DIM, int VDIM, int KIND, int NR>
 struct Shape {
-  static constexpr bool BITS8 = KIND != LIA_CACHE_BF16;
+  static constexpr bool SCALED = KIND != LIA_CACHE_BF16, FOUR = KIND == LIA_CACHE_INT4;
   static constexpr int STEPS = DIM / 16;                           // products of a block of 16 keys with 8 rows' queries
   static constexpr int MT = VDIM / 16;                             // products of 16 channels of a block's values with 8 rows' weights
-  static constexpr int KV = DIM * (BITS8 ? 1 : 2) / 64;            // 16-byte vectors of a key in a lane
-  static constexpr int VB = VDIM * (BITS8 ? 1 : 2) / 8;            // bytes of a value in a lane
+  static constexpr int KB = DIM * (FOUR ? 1 : SCALED ? 2 : 4) / 8;  // bytes of a key in a lane
+  static constexpr int VB = VDIM * (FOUR ? 1 : SCALED ? 2 : 4) / 16;                           // bytes of a value in a lane
+  static constexpr int KG = FOUR ? DIM / GROUP4 : 2, VG = FOUR ? VDIM / GROUP4 : 2;             // scales of a position with 4 bits (else: not used)
   static constexpr int ROWS = 8 * NR;
   static constexpr int Q_BYTES = NR * STEPS * 32 * 8, O_BYTES = WARPS * ROWS * VDIM * 4, BIG = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
   static constexpr int SMEM = BIG + ROWS * 4 + WARPS * ROWS * 8;
-  static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // a weight of the maximum is 2^LIFT, one that is just not outgrown 2^15 in fp16
+  static constexpr float LIFT = SCALED ? 7.f : 0.f;                // a weight of the maximum is 2^LIFT, one that is just not outgrown 2^15 in fp16
   // the channel of the first of a lane's pair in the i-th product with the values
-  static __device__ __forceinline__ int channel(int i, int gq) { return BITS8 ? gq * (VDIM / 8) + 2 * i : (i >> 2) * 64 + gq * 8 + (i & 3) * 2; }
+  static __device__ __forceinline__ int channel(int i, int gq) { return FOUR ? (i >> 1) * GROUP4 + gq * 4 + (i & 1) * 2 : SCALED ? gq * (VDIM / 8) + 2 * i : (i >> 2) * 64 + gq * 8 + (i & 3) * 2; }
 };
 constexpr float NONE = -1e30f, SLACK = 8.f;                        // a maximum of no keys; how far, in powers of two, weights may exceed 1
 
 template <int DIM, int VDIM, int KIND, int NR>
 __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   using S = Shape<DIM, VDIM, KIND, NR>;
-  constexpr bool BITS8 = S::BITS8;
-  constexpr int RQ = BITS8 ? 1 : 2;
+  constexpr bool SCALED = S::SCALED, FOUR = S::FOUR;
+  constexpr int RQ = SCALED ? 1 : 2;
   extern __shared__ uint4 smem[];
   float* row_f = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + S::BIG);        // [ROWS] what a row's products with keys are multiplied by
   float2* part = reinterpret_cast<float2*>(row_f + S::ROWS);       // [WARPS][ROWS] maximum, sum
@@ -95,19 +96,28 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
   const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = min(hi, a.mask != nullptr ? p.p0 : p.p0 + i0 + 1);
   const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
 
-  const uint8_t *kbase = a.k.at(p.slot, 0, g) + t4 * 16, *vbase = a.v.at(p.slot, 0, g) + gq * (BITS8 ? S::VB : 16);
-  const float *ksc = BITS8 ? a.k.scale_at(p.slot, g) : nullptr, *vsc = BITS8 ? a.v.scale_at(p.slot, g) : nullptr;
-  uint4 kr[2][S::KV];                                              // keys gq and gq + 8
+  const uint8_t *kbase = a.k.at(p.slot, 0, g) + t4 * (FOUR ? S::KB : 16), *vbase = a.v.at(p.slot, 0, g) + gq * (SCALED ? S::VB : 16);
+  const float *ksc = SCALED ? a.k.scale_at(p.slot, g) : nullptr, *vsc = SCALED ? a.v.scale_at(p.slot, g) : nullptr;
+  const bf16 *ksc4 = FOUR ? a.k.scale4_at(p.slot, g) : nullptr, *vsc4 = FOUR ? a.v.scale4_at(p.slot, g) : nullptr;
+  uint32_t kr[2][S::KB / 4];                                       // keys gq and gq + 8
   uint32_t vr[4][S::VB / 4];                                       // values 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4
   float ks[2], vs[2];                                              // of keys gq and gq + 8
+  uint32_t ks4[2][S::KG / 2], vs4[2][S::VG / 2];                   // of the same, with 4 bits
   auto load_k = [&](int b) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int key = min(lo + b * 16 + j * 8 + gq, hi - 1);
       const uint8_t* src = kbase + (long long)key * a.k.pos;
+      if constexpr (S::KB == 8) {
+        *reinterpret_cast<uint2*>(kr[j]) = __ldcg(reinterpret_cast<const uint2*>(src));
+      } else {
 #pragma unroll
-      for (int c = 0; c < S::KV; ++c) kr[j][c] = ldg_act(src + c * 64);
-      if constexpr (BITS8) {
+        for (int c = 0; c < S::KB / 16; ++c) *reinterpret_cast<uint4*>(&kr[j][c * 4]) = ldg_act(src + c * 64);
+      }
+      if constexpr (FOUR) {
+        ask_scales4<S::KG>(ksc4 + (long long)key * S::KG, ks4[j]);
+        ask_scales4<S::VG>(vsc4 + (long long)key * S::VG, vs4[j]);
+      } else if constexpr (SCALED) {
         ks[j] = __ldcg(ksc + key);
         vs[j] = __ldcg(vsc + key);
       }
@@ -117,7 +127,9 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint8_t* src = vbase + (long long)min(lo + b * 16 + (c >> 1) * 8 + t4 * 2 + (c & 1), hi - 1) * a.v.pos;
-      if constexpr (S::VB == 8) {
+      if constexpr (S::VB == 4) {
+        vr[c][0] = __ldcg(reinterpret_cast<const uint32_t*>(src));
+      } else if constexpr (S::VB == 8) {
         const uint2 u = __ldcg(reinterpret_cast<const uint2*>(src));
         vr[c][0] = u.x;
         vr[c][1] = u.y;
@@ -141,7 +153,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     if (there && lane < DIM / 4) u = *reinterpret_cast<const uint2*>(a.q + (p.row + i) * a.ldq + h * DIM + lane * 4);
     float f = a.scale * (a.temp != nullptr && there ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
     uint2 w = u;
-    if constexpr (BITS8) {
+    if constexpr (SCALED) {
       uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
       const Down down = down_of(__reduce_max_sync(0xffffffffu, top));
       float x[4];
@@ -150,8 +162,9 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
       w = make_uint2(pack_f16x2(x[0] * down.by, x[1] * down.by), pack_f16x2(x[2] * down.by, x[3] * down.by));
       f *= down.back;
     }
+    if constexpr (FOUR) w = in_code_order(w);
     if (lane < DIM / 4) {                                          // four neighbouring channels are a lane's operand of one step
-      const int c = lane * 4, t = BITS8 ? (c >> 4) & 3 : (c >> 3) & 3, step = BITS8 ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
+      const int c = lane * 4, t = SCALED && !FOUR ? (c >> 4) & 3 : (c >> 3) & 3, step = SCALED && !FOUR ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
       qs[((r >> 3) * S::STEPS + step) * 32 + (r & 7) * 4 + t] = w;
     }
     if (lane == 0) row_f[r] = f;
@@ -191,14 +204,38 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
+    if constexpr (FOUR) {                                          // group by group, whose sums are multiplied by their scales
+      float kg[2][S::KG];
 #pragma unroll
-    for (int st = 0; st < S::STEPS; ++st) {
+      for (int j = 0; j < 2; ++j) scales4_of<S::KG>(ks4[j], kg[j]);
+#pragma unroll
+      for (int gr = 0; gr < S::KG; ++gr) {
+        uint32_t codes[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) int4x2(__byte_perm(kr[j][gr >> 1], kr[j][S::KB / 8 + (gr >> 1)], gr & 1 ? 0x7632 : 0x5410), codes[j]);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          float part[4] = {};
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const uint32_t ka[4] = {codes[0][2 * st], codes[1][2 * st], codes[0][2 * st + 1], codes[1][2 * st + 1]};
+            uint2 q;
+            if constexpr (NR <= RQ) q = qa[r][gr * 2 + st];
+            else q = qs[(r * S::STEPS + gr * 2 + st) * 32 + lane];
+            mma_f16(part, ka, q.x, q.y);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[r][e] = fmaf(part[e], kg[e >> 1][gr], s[r][e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < (FOUR ? 0 : S::STEPS); ++st) {
       uint32_t ka[4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if constexpr (BITS8) {
-          const uint4& u = kr[j][st >> 2];
-          uint32_t w = (st & 3) == 0 ? u.x : (st & 3) == 1 ? u.y : (st & 3) == 2 ? u.z : u.w;
+        if constexpr (SCALED) {
+          uint32_t w = kr[j][st];
           if constexpr (KIND == LIA_CACHE_INT8) {
             w ^= 0x80808080u;
             ka[j] = int8x2(__byte_perm(w, 0x64646464u, 0x4140));
@@ -208,9 +245,8 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
             ka[2 + j] = e4m3x2(w >> 16);
           }
         } else {
-          const uint4& u = kr[j][st >> 1];
-          ka[j] = st & 1 ? u.z : u.x;
-          ka[2 + j] = st & 1 ? u.w : u.y;
+          ka[j] = kr[j][2 * st];
+          ka[2 + j] = kr[j][2 * st + 1];
         }
       }
 #pragma unroll
@@ -218,18 +254,30 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
         uint2 q;
         if constexpr (NR <= RQ) q = qa[r][st];
         else q = qs[(r * S::STEPS + st) * 32 + lane];
-        if constexpr (BITS8) mma_f16(s[r], ka, q.x, q.y);
+        if constexpr (SCALED) mma_f16(s[r], ka, q.x, q.y);
         else mma_bf16(s[r], ka, q.x, q.y);
       }
     }
     float kf[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f}, rv[2] = {1.f, 1.f};
-    if constexpr (BITS8) {
+    float ratio[2][S::VG];                                         // with 4 bits: a group's scale relative to the value's largest, which goes into the exponent
+    if constexpr (SCALED) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        kf[j] = ks[j];
+        if constexpr (FOUR) {
+          scales4_of<S::VG>(vs4[j], ratio[j]);
+          vs[j] = ratio[j][0];
+#pragma unroll
+          for (int gr = 1; gr < S::VG; ++gr) vs[j] = max_nan(vs[j], ratio[j][gr]);
+        } else {
+          kf[j] = ks[j];
+        }
         const float y = max_nan(vs[j], LEAST_SCALE);
         lv[j] = lg2(y);
         rv[j] = __fdividef(1.f, y);
+        if constexpr (FOUR) {
+#pragma unroll
+          for (int gr = 0; gr < S::VG; ++gr) ratio[j][gr] *= rv[j];
+        }
       }
     }
     if (b + WARPS < b1) load_k(b + WARPS);
@@ -244,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[r][e] = BITS8 ? fmaf(s[r][e] * kf[e >> 1], rf[r][e & 1], lv[e >> 1]) : s[r][e] * rf[r][e & 1];
+        for (int e = 0; e < 4; ++e) s[r][e] = SCALED ? fmaf(s[r][e] * kf[e >> 1], rf[r][e & 1], lv[e >> 1]) : s[r][e] * rf[r][e & 1];
     }
     if (key0 < all_lo || key0 + 16 > all_hi) {
 #pragma unroll
@@ -285,37 +333,55 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
         }
     }
     // ---- weights, turned into the products' other operand
-    uint32_t pb[BITS8 ? 1 : 2][NR][2];
+    constexpr int PARTS = FOUR ? S::VG : SCALED ? 1 : 2;           // with 4 bits a group's weights each, with bf16 two parts of a weight
+    uint32_t pb[PARTS][NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       float w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         w[e] = ex2(s[r][e] - m[r][e & 1]);
-        l[r][e & 1] = BITS8 ? fmaf(w[e], rv[e >> 1], l[r][e & 1]) : l[r][e & 1] + w[e];
+        l[r][e & 1] = SCALED ? fmaf(w[e], rv[e >> 1], l[r][e & 1]) : l[r][e & 1] + w[e];
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if constexpr (BITS8) {
+        if constexpr (FOUR) {
+#pragma unroll
+          for (int gr = 0; gr < S::VG; ++gr) pb[gr][r][j] = transposed(pack_f16x2(w[2 * j] * ratio[j][gr], w[2 * j + 1] * ratio[j][gr]));
+        } else if constexpr (SCALED) {
           pb[0][r][j] = transposed(pack_f16x2(w[2 * j], w[2 * j + 1]));
         } else {
           const uint32_t hi2 = pack_bf16x2(w[2 * j], w[2 * j + 1]);
           float x, y;
           unpack_bf16x2(hi2, x, y);
           pb[0][r][j] = transposed(hi2);
-          pb[BITS8 ? 0 : 1][r][j] = transposed(pack_bf16x2(w[2 * j] - x, w[2 * j + 1] - y));
+          pb[PARTS - 1][r][j] = transposed(pack_bf16x2(w[2 * j] - x, w[2 * j + 1] - y));
         }
       }
     }
     // ---- weighted values
+    if constexpr (FOUR) {
 #pragma unroll
-    for (int w = 0; w < S::VB / 4; ++w) {
-      constexpr int PER = BITS8 ? 4 : 2;                           // channels of a word
+      for (int gr = 0; gr < S::VG; ++gr) {
+        uint32_t va[2][4];                                         // a lane's four channels of the group, of keys 2 t4 and 2 t4 + 1, and of those 8 on
+#pragma unroll
+        for (int c = 0; c < 2; ++c) int4x2(__byte_perm(vr[2 * c][gr >> 1], vr[2 * c + 1][gr >> 1], gr & 1 ? 0x7632 : 0x5410), va[c]);
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          const uint32_t v4[4] = {va[0][c], va[0][c + 1], va[1][c], va[1][c + 1]};
+#pragma unroll
+          for (int r = 0; r < NR; ++r) mma_f16(o[r][gr * 2 + (c >> 1)], v4, pb[gr][r][0], pb[gr][r][1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < (FOUR ? 0 : S::VB / 4); ++w) {
+      constexpr int PER = SCALED ? 4 : 2;                           // channels of a word
       uint32_t va[PER][2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const uint32_t u0 = vr[2 * c][w], u1 = vr[2 * c + 1][w];
-        if constexpr (BITS8) {
+        if constexpr (SCALED) {
           uint32_t x = __byte_perm(u0, u1, 0x5140), y = __byte_perm(u0, u1, 0x7362);
           if constexpr (KIND == LIA_CACHE_INT8) {
             x ^= 0x80808080u;
@@ -341,11 +407,11 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
         const int n = (w * PER + c) >> 1;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          if constexpr (BITS8) {
+          if constexpr (SCALED) {
             mma_f16(o[r][n], v4, pb[0][r][0], pb[0][r][1]);
           } else {
             mma_bf16(o[r][n], v4, pb[0][r][0], pb[0][r][1]);
-            mma_bf16(o[r][n], v4, pb[BITS8 ? 0 : 1][r][0], pb[BITS8 ? 0 : 1][r][1]);
+            mma_bf16(o[r][n], v4, pb[PARTS - 1][r][0], pb[PARTS - 1][r][1]);
           }
         }
       }
@@ -537,6 +603,7 @@ extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* k
   switch (kc->type) {
     case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, plan.nr, nseg, stream);
     case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, plan.nr, nseg, stream);
+    case LIA_CACHE_INT4: return launch_dims<LIA_CACHE_INT4>(a, plan.nr, nseg, stream);
     default: return launch_dims<LIA_CACHE_E4M3>(a, plan.nr, nseg, stream);
   }
 }

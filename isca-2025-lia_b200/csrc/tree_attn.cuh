@@ -84,6 +84,39 @@ __device__ __forceinline__ uint32_t int8x2(uint32_t u) {
   const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// of 4-bit caches: two units (byte4()) as a word of eight codes + 8, of which the j-th of both (j = 0 .. 3) become fp16: 1024 + u - 1032, and (1024 + 16 u) / 16 - 72
+__device__ __forceinline__ void int4x2(uint32_t w, uint32_t (&r)[4]) {
+  const uint32_t m32 = 0x64086408u, sixteenth = 0x2c002c00u, m72 = 0xd480d480u;                // 1032, 1 / 16, -72
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = i == 0 ? w : w >> 8;
+    const uint32_t a = (x & 0x000f000fu) | 0x64006400u, b = (x & 0x00f000f0u) | 0x64006400u;
+    const __half2 lo = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&m32));
+    const __half2 hi = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&sixteenth), *reinterpret_cast<const __half2*>(&m72));
+    r[2 * i] = *reinterpret_cast<const uint32_t*>(&lo);
+    r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+  }
+}
+// a position's scales, NG of them
+template <int NG> __device__ __forceinline__ void ask_scales4(const bf16* p, uint32_t (&w)[NG / 2]) {
+  if constexpr (NG == 4) {
+    const uint2 u = __ldcg(reinterpret_cast<const uint2*>(p));
+    w[0] = u.x;
+    w[1] = u.y;
+  } else {
+    w[0] = __ldcg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+template <int NG> __device__ __forceinline__ void scales4_of(const uint32_t (&w)[NG / 2], float (&s)[NG]) {
+#pragma unroll
+  for (int i = 0; i < NG / 2; ++i) unpack_bf16x2(w[i], s[2 * i], s[2 * i + 1]);
+}
+// The queries of a 4-bit head, lane l with the channels 4 l .. 4 l + 3 as two pairs: every eight channels 0 .. 7 are to be in the order 0 4 1 5 | 2 6 3 7 in which codes are unpacked
+__device__ __forceinline__ uint2 in_code_order(const uint2& w) {
+  const bool odd = threadIdx.x & 1;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w.x : w.y, 1), a = odd ? other : w.x, b = odd ? w.y : other;
+  return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -102,8 +135,10 @@ __device__ __forceinline__ Down down_of(uint32_t top) {
 constexpr float MOST_SOFTCAP = 1024.f;
 __device__ __forceinline__ float capped(float x, float cap, float two_log2e_by_cap) { return cap - __fdividef(2.f * cap, 1.f + ex2(x * two_log2e_by_cap)); }
 
-template <int KIND> __device__ __forceinline__ float cached(const uint8_t* head, int c) {
-  if constexpr (KIND == LIA_CACHE_BF16) return __bfloat162float(reinterpret_cast<const bf16*>(head)[c]);
+// channel c of a head, without its scale but with 4 bits
+template <int KIND, int D> __device__ __forceinline__ float cached(const uint8_t* head, const bf16* scales4, int c) {
+  if constexpr (KIND == LIA_CACHE_INT4) return (float)((int)(head[byte4(c, D)] >> (c % 2 * 4) & 15) - 8) * __bfloat162float(scales4[c / GROUP4]);
+  else if constexpr (KIND == LIA_CACHE_BF16) return __bfloat162float(reinterpret_cast<const bf16*>(head)[c]);
   else if constexpr (KIND == LIA_CACHE_INT8) return (float)reinterpret_cast<const int8_t*>(head)[c];
   else return __half2float(__half(__nv_cvt_fp8_to_halfraw(head[c], __NV_E4M3)));
 }
@@ -114,6 +149,7 @@ template <int KIND> __device__ __forceinline__ float cached(const uint8_t* head,
 // 131003 160 ms, 64 tokens behind 2000 whose tile is one block's 60 ms (a warp's 32 rows one after the other).
 template <int DIM, int VDIM, int KIND> __device__ __noinline__ void form_again(const TreeArgs& a, const Portion p, int i, int h, float* y) {
   constexpr int KN = DIM / 32, VN = VDIM / 32;
+  constexpr bool HEAD_SCALE = KIND == LIA_CACHE_INT8 || KIND == LIA_CACHE_E4M3, FOUR = KIND == LIA_CACHE_INT4;
   const int lane = threadIdx.x & 31, g = h / a.rep, deep = depth_of(a, p, i);
   const float nan = __uint_as_float(0x7fc00000u), f = a.scale * (a.temp != nullptr ? a.temp[h] : 1.f);
   float q[KN], o[VN], m = -INFINITY, l = 0.f;
@@ -125,15 +161,16 @@ template <int DIM, int VDIM, int KIND> __device__ __noinline__ void form_again(c
     if (!sees(a, p, i, deep, t)) continue;
     any = true;
     const uint8_t *kh = a.k.at(p.slot, t, g), *vh = a.v.at(p.slot, t, g);
+    const bf16 *k4 = FOUR ? a.k.scale4_at(p.slot, g) + t * (long long)(DIM / GROUP4) : nullptr, *v4 = FOUR ? a.v.scale4_at(p.slot, g) + t * (long long)(VDIM / GROUP4) : nullptr;
     float s = 0.f;
-    for (int c = 0; c < KN; ++c) s = fmaf(q[c], cached<KIND>(kh, c * 32 + lane), s);
+    for (int c = 0; c < KN; ++c) s = fmaf(q[c], cached<KIND, DIM>(kh, k4, c * 32 + lane), s);
     s = warp_sum(s) * f;
-    if (KIND != LIA_CACHE_BF16) s *= a.k.scale_at(p.slot, g)[t];
+    if (HEAD_SCALE) s *= a.k.scale_at(p.slot, g)[t];
     if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
     const float mn = fmaxf(m, s), keep = m == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : expf(m - mn), w = s == -INFINITY ? 0.f : expf(s - mn);
-    const float vs = KIND != LIA_CACHE_BF16 ? a.v.scale_at(p.slot, g)[t] : 1.f;
+    const float vs = HEAD_SCALE ? a.v.scale_at(p.slot, g)[t] : 1.f;
     l = l * keep + w;
-    for (int c = 0; c < VN; ++c) o[c] = o[c] * keep + w * (cached<KIND>(vh, c * 32 + lane) * vs);
+    for (int c = 0; c < VN; ++c) o[c] = o[c] * keep + w * (cached<KIND, VDIM>(vh, v4, c * 32 + lane) * vs);
     m = mn;
   }
   for (int c = 0; c < VN; ++c) y[c] = !any ? 0.f : l > 0.f ? o[c] / l : nan;      // (all scores -inf, or NaN)

@@ -25,6 +25,8 @@
 #include "tree_attn.cuh"
 #include "umma.cuh"
 
+#include <type_traits>
+
 int* lia_formed_again_word();                                      // moe_sm100.cu
 
 namespace {
@@ -34,19 +36,21 @@ constexpr int SOFTMAX_REGS = 128, LOADER_REGS = 96, OTHER_REGS = 32; // of a thr
 constexpr int LAUNCH_REGS = 96;
 static_assert(SOFTMAX_REGS >= LAUNCH_REGS && LOADER_REGS <= LAUNCH_REGS && OTHER_REGS <= LAUNCH_REGS && 2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS <= THREADS / 128 * LAUNCH_REGS, "shares");
 constexpr uint32_t VALUES = 256;
+constexpr float LEAST_KEY_SCALE = 0x1p-110f;                       // a 4-bit key's largest scale counts as that at least, so that its inverse is finite
 constexpr float SLACK = 8.f;                                       // how far, in powers of two, weights may exceed 1
 
 template <int DIM, int VDIM, int KIND, bool PAIR>
 struct Tc {
-  static constexpr bool BITS8 = KIND != LIA_CACHE_BF16;
+  static constexpr bool SCALED = KIND != LIA_CACHE_BF16, FOUR = KIND == LIA_CACHE_INT4;
   static constexpr int SLAB = KEYS * 128;                          // 64 channels of 16 bits of a block's keys
   static constexpr int K_BYTES = DIM / 64 * SLAB, V_BYTES = VDIM / 64 * SLAB, STAGE = K_BYTES + V_BYTES;
   static constexpr int Q_SLAB = ROWS * 128, Q_BYTES = DIM / 64 * Q_SLAB;                        // a group's queries
   static constexpr int ALL_Q = (PAIR ? 2 : 1) * Q_BYTES, ROOM = (221184 - ALL_Q) / STAGE, STAGES = ROOM > 8 ? 8 : ROOM;
-  static constexpr int KT = DIM * (BITS8 ? 1 : 2) / 16, VT = VDIM * (BITS8 ? 1 : 2) / 16;      // lanes of a key, of a value
+  static constexpr int KT = FOUR ? 4 : DIM * (SCALED ? 1 : 2) / 16, VT = FOUR ? 4 : VDIM * (SCALED ? 1 : 2) / 16;      // lanes of a key, of a value
   static constexpr int KN = KEYS * KT / LOADERS, VN = KEYS * VT / LOADERS;                       // vectors of a lane
-  static constexpr int AHEAD = BITS8 ? 2 : 1;                      // blocks of 16 or 32 KB on their way from memory (more: more instructions to bring, 5 to 30 % slower with four)
-  static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // weights are 2^(x - maximum + LIFT): below 2^15 in fp16
+  static constexpr int KG = FOUR ? DIM / GROUP4 : 2, VG = FOUR ? VDIM / GROUP4 : 2;             // scales of a position with 4 bits (else: not used)
+  static constexpr int AHEAD = SCALED ? 2 : 1;                      // blocks of 16 or 32 KB on their way from memory (more: more instructions to bring, 5 to 30 % slower with four)
+  static constexpr float LIFT = SCALED ? 7.f : 0.f;                 // weights are 2^(x - maximum + LIFT): below 2^15 in fp16
 };
 struct Tail {
   float ks[8][KEYS], lv[8][KEYS], rv[8][KEYS];                     // of a stage's keys: scale; of its values: log2 of what is left of the scale, and the inverse of that
@@ -123,6 +127,21 @@ __device__ __forceinline__ void ask_ref(const float* scale, int n, uint32_t (&u)
 #pragma unroll
   for (int x = 0; x < 2; ++x) u[x] = x * 32 + lane < n ? __float_as_uint(__ldcg(scale + x * 32 + lane)) : 0u;
 }
+// the same of 4 bits: the largest finite scale of each position's
+template <int NG> __device__ __forceinline__ void ask_ref4(const bf16* scale, int n, uint32_t (&u)[2]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint32_t w[NG / 2] = {}, m = 0u;
+    if (x * 32 + lane < n) ask_scales4<NG>(scale + (x * 32 + lane) * NG, w);
+#pragma unroll
+    for (int i = 0; i < NG / 2; ++i) {
+      const uint32_t lo = w[i] << 16, hi = w[i] & 0xffff0000u;
+      m = max(m, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+    }
+    u[x] = m;
+  }
+}
 __device__ __forceinline__ int ref_of(const uint32_t (&u)[2]) {
   const uint32_t top = __reduce_max_sync(0xffffffffu, max(u[0] < 0x7f800000u ? u[0] : 0u, u[1] < 0x7f800000u ? u[1] : 0u));   // (not a negative one either)
   return top >= 0x00800000u ? min(max((int)(top >> 23) - 127, -80), 100) : 0;
@@ -132,7 +151,7 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 template <int DIM, int VDIM, int KIND, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_constant__ TreeArgs a, int* __restrict__ timeouts) {
   using C = Tc<DIM, VDIM, KIND, PAIR>;
-  constexpr bool BITS8 = C::BITS8;
+  constexpr bool SCALED = C::SCALED, FOUR = C::FOUR;
   constexpr int TILE = PAIR ? 2 * ROWS : ROWS, STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -209,10 +228,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
     const int i = there ? row / a.rep : p.n - 1, h = there ? g * a.rep + row - i * a.rep : g * a.rep;
     const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
     uint32_t scales[2] = {0u, 0u};
-    if constexpr (BITS8) ask_ref(a.v.scale_at(p.slot, g) + start, n > 0 ? min(hi - start, KEYS) : 0, scales);
+    if constexpr (FOUR) ask_ref4<C::VG>(a.v.scale4_at(p.slot, g) + (long long)start * C::VG, n > 0 ? min(hi - start, KEYS) : 0, scales);
+    else if constexpr (SCALED) ask_ref(a.v.scale_at(p.slot, g) + start, n > 0 ? min(hi - start, KEYS) : 0, scales);
     // ---- queries go to shared memory, a row a warp at a time, and what a row's products are multiplied by to sm.row_f
     constexpr int SHARE = TILE / 8;
-    const int c4 = lane * 4, place = BITS8 ? place_of<DIM>(c4 >> 4, (c4 >> 3) & 1) + (c4 & 7) : c4;     // a lane's four channels, and where they go
+    const int c4 = lane * 4, place = SCALED && !FOUR ? place_of<DIM>(c4 >> 4, (c4 >> 3) & 1) + (c4 & 7) : c4;     // a lane's four channels, and where they go
     const uint32_t lane_at = queries + (place >> 6) * C::Q_SLAB + (place & 7) * 2;
     const int chunk = (place & 63) >> 3;
     const float factor_all = a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
@@ -235,7 +255,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
       for (int x = 0; x < 8; ++x, ++rr) {
         const bool flip = f[x] < 0.f;                              // (so that the largest product is the largest score)
         uint2 w;
-        if constexpr (BITS8) {
+        if constexpr (SCALED) {
           const uint32_t m = __vmaxu2(u[x].x & 0x7fff7fffu, u[x].y & 0x7fff7fffu);
           const Down down = down_of(__reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16)));
           const float by = flip ? -down.by : down.by;
@@ -244,6 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
           unpack_bf16x2(u[x].y, y[2], y[3]);
           w = make_uint2(pack_f16x2(y[0] * by, y[1] * by), pack_f16x2(y[2] * by, y[3] * by));
           f[x] *= down.back;
+          if constexpr (FOUR) w = in_code_order(w);
         } else {
           const uint32_t sign = flip ? 0x80008000u : 0u;
           w = make_uint2(u[x].x ^ sign, u[x].y ^ sign);
@@ -263,19 +284,19 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
     float m = -1e30f, l = 0.f;
     bool alive = true;
     int done = 0;                                                  // of the group's blocks
-    const int ref = BITS8 ? ref_of(scales) : 0;
+    const int ref = SCALED ? ref_of(scales) : 0;
     const float ref_l = (float)ref, ref_inv = pow2(-ref);
     // (a row's first block sees to a maximum; -1e30 stands for none, so that nothing is less than it but -inf)
 #pragma unroll 1
     for (int j = PAIR ? 0 : s; j < n && s < groups; j += PAIR ? 1 : 2, ++done) {
       const int st = j % STAGES, buf = done & 1;
       const uint32_t scores = lanes + s * 128 + buf * KEYS;
-      float4 k4[BITS8 ? 4 : 1];                                    // a quarter of the keys' scales, asked for together
+      float4 k4[SCALED ? 4 : 1];                                    // a quarter of the keys' scales, asked for together
       auto ask_scales = [&](int half) {
 #pragma unroll
-        for (int c = 0; c < (BITS8 ? 4 : 0); ++c) k4[c] = *reinterpret_cast<const float4*>(&sm.ks[st][half * 16 + c * 4]);
+        for (int c = 0; c < (SCALED ? 4 : 0); ++c) k4[c] = *reinterpret_cast<const float4*>(&sm.ks[st][half * 16 + c * 4]);
       };
-      if constexpr (BITS8) {
+      if constexpr (SCALED) {
         if (!(alive = warp_wait(smem_u32(&sm.full[st]), (j / STAGES) & 1, dead))) break;
         ask_scales(0);
       }
@@ -288,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
         tmem_ld32(scores, v);
         tmem_ld32(scores + 32, v + 32);
         tmem_ld_wait();
-        if constexpr (BITS8) {
+        if constexpr (SCALED) {
 #pragma unroll
           for (int half = 0; half < 4; ++half) {
             float4 f4[4];
@@ -309,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
           }
         }
         const int t = start + j * KEYS;
-        const bool odd = BITS8 && sm.odd[st] != 0;
+        const bool odd = SCALED && sm.odd[st] != 0;
         float factor = rf, add = ref_l;                            // x = v * factor + add, in powers of two (with the values' scales)
         if (odd || a.softcap > 0.f) {
           factor = 1.f;
@@ -328,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
           each([&](f32x2 x, int c) {
             float x0, x1;
             unpack2(mul2(x, both(rf)), x0, x1);
-            return fma2(pack2(capped(x0, a.softcap, two_by_cap), capped(x1, a.softcap, two_by_cap)), both(LOG2E), BITS8 ? pack2(sm.lv[st][c], sm.lv[st][c + 1]) : both(0.f));
+            return fma2(pack2(capped(x0, a.softcap, two_by_cap), capped(x1, a.softcap, two_by_cap)), both(LOG2E), SCALED ? pack2(sm.lv[st][c], sm.lv[st][c + 1]) : both(0.f));
           });
         } else if (odd) {
           each([&](f32x2 x, int c) { return fma2(x, both(rf), pack2(sm.lv[st][c], sm.lv[st][c + 1])); });
@@ -373,7 +394,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
             w2 = ex2(w2);
             w3 = ex2(w3);
             sum = add2(sum, add2(pack2(w0, w1), pack2(w2, w3)));
-            if constexpr (BITS8) {
+            if constexpr (SCALED) {
               hi16[e / 2] = pack_f16x2(w0, w1);
               hi16[e / 2 + 1] = pack_f16x2(w2, w3);
               v[c + e] = __float_as_uint(w0);
@@ -391,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
             }
           }
           tmem_st8(scores + c / 2, hi16);
-          if constexpr (!BITS8) tmem_st8(scores + 32 + c / 2, lo16);
+          if constexpr (!SCALED) tmem_st8(scores + 32 + c / 2, lo16);
         }
         float s0, s1;
         if (odd) {                                                 // p = weight / what is left of the scale
@@ -479,7 +500,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
             y[x] *= inv;
             probe = fmaf(y[x], 0.f, probe);
           }
-          const int col = c + e, ch = BITS8 && VDIM == 128 ? (col & 63) / 8 * 16 + (col >> 6) * 8 : col;
+          const int col = c + e, ch = SCALED && !FOUR && VDIM == 128 ? (col & 63) / 8 * 16 + (col >> 6) * 8 : col;
+          if constexpr (FOUR) {                                    // (columns have the order in which codes are unpacked: 0 4 1 5 2 6 3 7)
+            const float y1 = y[1], y2 = y[2], y3 = y[3], y5 = y[5], y6 = y[6];
+            float z[8] = {y[0], y2, y[4], y6, y1, y3, y5, y[7]};
+#pragma unroll
+            for (int x = 0; x < 8; ++x) y[x] = z[x];
+          }
           if (there) {
             if (whole) {
               const uint4 u = pack8(y);
@@ -519,20 +546,37 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
     const int th = threadIdx.x - 256, kt = th % C::KT, vt = th % C::VT, k0 = th / C::KT, v0 = th / C::VT;
     constexpr int KSTEP = LOADERS / C::KT, VSTEP = LOADERS / C::VT;                            // a lane's keys are so far apart
     // the lane's places in the next block to ask for
-    const uint8_t *kp = a.k.at(p.slot, start + k0, g) + kt * 16, *vp = a.v.at(p.slot, start + v0, g) + vt * 16;
-    const float *ksp = BITS8 ? a.k.scale_at(p.slot, g) + start : nullptr, *vsp = BITS8 ? a.v.scale_at(p.slot, g) + start : nullptr;
+    const uint8_t *kp = a.k.at(p.slot, start + k0, g) + kt * (FOUR ? DIM / 8 : 16), *vp = a.v.at(p.slot, start + v0, g) + vt * (FOUR ? VDIM / 8 : 16);
+    const float *ksp = SCALED && !FOUR ? a.k.scale_at(p.slot, g) + start : nullptr, *vsp = SCALED && !FOUR ? a.v.scale_at(p.slot, g) + start : nullptr;
+    const bf16 *ks4p = FOUR ? a.k.scale4_at(p.slot, g) + (long long)(start + k0) * C::KG : nullptr, *vs4p = FOUR ? a.v.scale4_at(p.slot, g) + (long long)(start + v0) * C::VG : nullptr;
     uint32_t scales[2] = {0u, 0u};
     uint4 kr[C::AHEAD][C::KN], vr[C::AHEAD][C::VN];
     float ks[C::AHEAD], vs[C::AHEAD][C::VN];                       // of key th < 64, and of the lane's values
+    uint32_t ks4[C::AHEAD][C::KG / 2], vs4[C::AHEAD][C::VG / 2];   // of the lane's key and value, with 4 bits
+    bool there4[C::AHEAD];
     auto ask = [&](int j, int x) {
       if (j >= n) return;
       const int left = hi - start - j * KEYS;                      // keys from the block's first on
-      if (left >= KEYS) {
+      if constexpr (FOUR) {                                        // (a lane has one key and the value beside it)
+        there4[x] = k0 < left;
+        kr[x][0] = vr[x][0] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+        ks4[x][0] = ks4[x][C::KG / 2 - 1] = vs4[x][0] = vs4[x][C::VG / 2 - 1] = 0u;
+        if (there4[x]) {
+          if constexpr (DIM == 128) kr[x][0] = ldg_act(kp);
+          else *reinterpret_cast<uint2*>(&kr[x][0]) = __ldcg(reinterpret_cast<const uint2*>(kp));
+          if constexpr (VDIM == 128) vr[x][0] = ldg_act(vp);
+          else *reinterpret_cast<uint2*>(&vr[x][0]) = __ldcg(reinterpret_cast<const uint2*>(vp));
+          ask_scales4<C::KG>(ks4p, ks4[x]);
+          ask_scales4<C::VG>(vs4p, vs4[x]);
+        }
+        ks4p += KEYS * C::KG;
+        vs4p += KEYS * C::VG;
+      } else if (left >= KEYS) {
 #pragma unroll
         for (int c = 0; c < C::KN; ++c) kr[x][c] = ldg_act(kp + c * KSTEP * a.k.pos);
 #pragma unroll
         for (int c = 0; c < C::VN; ++c) vr[x][c] = ldg_act(vp + c * VSTEP * a.v.pos);
-        if constexpr (BITS8) {
+        if constexpr (SCALED) {
           if (th < KEYS) ks[x] = __ldcg(ksp + th);
 #pragma unroll
           for (int c = 0; c < C::VN; ++c) vs[x][c] = __ldcg(vsp + v0 + c * VSTEP);
@@ -542,7 +586,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
         for (int c = 0; c < C::KN; ++c) kr[x][c] = k0 + c * KSTEP < left ? ldg_act(kp + c * KSTEP * a.k.pos) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int c = 0; c < C::VN; ++c) vr[x][c] = v0 + c * VSTEP < left ? ldg_act(vp + c * VSTEP * a.v.pos) : make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (BITS8) {
+        if constexpr (SCALED) {
           if (th < KEYS) ks[x] = th < left ? __ldcg(ksp + th) : 0.f;
 #pragma unroll
           for (int c = 0; c < C::VN; ++c) vs[x][c] = v0 + c * VSTEP < left ? __ldcg(vsp + v0 + c * VSTEP) : -1.f;     // (none)
@@ -550,14 +594,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
       }
       kp += KEYS * a.k.pos;
       vp += KEYS * a.v.pos;
-      if constexpr (BITS8) {
+      if constexpr (SCALED && !FOUR) {
         ksp += KEYS;
         vsp += KEYS;
       }
     };
     // where the lane's vectors go: the second half of 16 codes beside the first or in the next slab, the vectors of other keys some rows of 128 bytes on
     auto place = [&](int key, int tid, int wide) {
-      const int p0 = BITS8 ? (wide == 128 ? place_of<128>(tid, 0) : place_of<64>(tid, 0)) : tid * 8;
+      const int p0 = SCALED ? (wide == 128 ? place_of<128>(tid, 0) : place_of<64>(tid, 0)) : tid * 8;
       return (uint32_t)((p0 >> 6) * C::SLAB + key * 128 + ((((p0 & 63) >> 3) ^ (key & 7)) << 4));
     };
     const uint32_t k_at = place(k0, kt, DIM), v_at = C::K_BYTES + place(v0, vt, VDIM);
@@ -567,8 +611,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
     };
 #pragma unroll
     for (int x = 0; x < C::AHEAD; ++x) ask(x, x);
-    if constexpr (BITS8) ask_ref(a.v.scale_at(p.slot, g) + start, n > 0 ? min(hi - start, KEYS) : 0, scales);
-    const int ref = BITS8 ? ref_of(scales) : 0;
+    if constexpr (FOUR) ask_ref4<C::VG>(a.v.scale4_at(p.slot, g) + (long long)start * C::VG, n > 0 ? min(hi - start, KEYS) : 0, scales);
+    else if constexpr (SCALED) ask_ref(a.v.scale_at(p.slot, g) + start, n > 0 ? min(hi - start, KEYS) : 0, scales);
+    const int ref = SCALED ? ref_of(scales) : 0;
     const float ref_inv = pow2(-ref);
     bool alive = true;
 #pragma unroll 1
@@ -579,7 +624,46 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
         if (j >= n) break;
         if (!(alive = warp_wait(smem_u32(&sm.empty[st]), ((j / STAGES) & 1) ^ 1u, dead))) break;
         const uint32_t at = smem + st * C::STAGE;
-        if constexpr (BITS8) {
+        if constexpr (FOUR) {
+          // a group of 32 channels at a time, of which the lane has eight: 16 bytes.  A key's scales relative to its largest, which multiplies its scores; odd keys' groups are
+          // taken in the other order, so that the two keys that are written together go to different banks
+          float kg[C::KG], vg[C::VG];
+          scales4_of<C::KG>(ks4[x], kg);
+          scales4_of<C::VG>(vs4[x], vg);
+          float km = kg[0], vm = vg[0];
+#pragma unroll
+          for (int i = 1; i < C::KG; ++i) km = max_nan(km, kg[i]);
+#pragma unroll
+          for (int i = 1; i < C::VG; ++i) vm = max_nan(vm, vg[i]);
+          km = max_nan(km, LEAST_KEY_SCALE);
+          const float f = vm * ref_inv, y = max_nan(vm, LEAST_SCALE), k_by = __fdividef(1.f, km);
+          const bool near = (f >= 0x1p-8f && f < 64.f) || !there4[x];
+          const float v_by = near ? ref_inv : __fdividef(1.f, y);
+          const uint32_t kw[4] = {kr[x][0].x, kr[x][0].y, kr[x][0].z, kr[x][0].w}, vw[4] = {vr[x][0].x, vr[x][0].y, vr[x][0].z, vr[x][0].w};
+          auto widen4 = [&](uint32_t to, const uint32_t (&w)[4], auto ng, const float* s, float by, int i) {
+            constexpr int NG = decltype(ng)::value;
+            const bool other = k0 & 1;
+            uint32_t r[4];
+            int4x2(__byte_perm(w[i >> 1], w[NG / 2 + (i >> 1)], other == (i & 1) ? 0x5410 : 0x7632), r);
+            const __half2 f2 = __float2half2_rn((other ? s[i ^ 1] : s[i]) * by);
+            uint4 u = make_uint4(r[0], r[1], r[2], r[3]);
+            scale4(u, f2);
+            const int chunk = ((i ^ (other ? 1 : 0)) & 1) * 4 + kt;
+            put16(to + (i >> 1) * C::SLAB + k0 * 128 + ((chunk ^ (k0 & 7)) << 4), u);
+          };
+#pragma unroll
+          for (int i = 0; i < C::KG; ++i) widen4(at, kw, std::integral_constant<int, C::KG>{}, kg, k_by, i);
+#pragma unroll
+          for (int i = 0; i < C::VG; ++i) widen4(at + C::K_BYTES, vw, std::integral_constant<int, C::VG>{}, vg, v_by, i);
+          if (kt == 0) {
+            sm.ks[st][k0] = km;
+            const float z = near ? pow2(ref) : y;
+            sm.lv[st][k0] = lg2(z);
+            sm.rv[st][k0] = __fdividef(1.f, z);
+          }
+          const bool odd = __any_sync(0xffffffffu, !near);
+          if (lane == 0) reinterpret_cast<uint8_t*>(&sm.odd[st])[warp - 8] = odd;
+        } else if constexpr (SCALED) {
 #pragma unroll
           for (int c = 0; c < C::KN; ++c) {
             uint4 lo16, hi16;
@@ -624,7 +708,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
     if (warp == ISSUER) {
       const uint32_t one = elect_one();
-      constexpr uint32_t types = BITS8 ? 0u : (1u << 7) | (1u << 10);
+      constexpr uint32_t types = SCALED ? 0u : (1u << 7) | (1u << 10);
       constexpr uint32_t idesc_qk = (1u << 4) | types | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       constexpr uint32_t idesc_pv = (1u << 4) | types | (1u << 16) | ((uint32_t)(VDIM >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);      // (the values lie with the keys as rows)
       bool alive = n > 0 && warp_wait(smem_u32(&sm.q_full), 0, dead);
@@ -645,7 +729,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_c
         tcgen05_fence_after();
         const uint32_t at = smem + st * C::STAGE + C::K_BYTES;
 #pragma unroll
-        for (int part = 0; part < (BITS8 ? 1 : 2); ++part)
+        for (int part = 0; part < (SCALED ? 1 : 2); ++part)
 #pragma unroll
           for (int k = 0; k < KEYS / 16; ++k)
             mma_tmem_a_if(one, tmem + VALUES + s * 128, tmem + s * 128 + buf * KEYS + part * 32 + k * 8, make_smem_desc_mn(at + k * 16 * 128, C::SLAB), idesc_pv,
@@ -731,6 +815,7 @@ int lia_tree_attn_tc(const void* args, int type, int rows, int nseg, lia_stream_
   switch (type) {
     case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, rows, nseg, stream);
     case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, rows, nseg, stream);
+    case LIA_CACHE_INT4: return launch_dims<LIA_CACHE_INT4>(a, rows, nseg, stream);
     default: return launch_dims<LIA_CACHE_E4M3>(a, rows, nseg, stream);
   }
 }

@@ -139,7 +139,7 @@ class BebulornForCausalLM:
     step_serving = True          # served through engine.Engine (requests, slots, portions)
 
     def __init__(self, config, device="cuda", dtype=BF16, cache_dtype=None):
-        """``cache_dtype``: int8 or float8_e4m3fn for the attention layers' keys and values (None: ``dtype``)."""
+        """``cache_dtype``: int8, float8_e4m3fn or int4 for the attention layers' keys and values (None: ``dtype``)."""
         _lib.load()
         if dtype not in (BF16, F32):
             raise ValueError("dtype must be torch.bfloat16 or torch.float32")

@@ -1391,10 +1391,11 @@ def rglru_scan(u, z, z_bias, c, y, y_bias, state, segs, blocks, out):
 
 
 # ------------------------------------------------------------------------------------------------------------------
-# Serving with drafted tokens: keys and values in 8 bits, attention of several new tokens behind a history, log
+# Serving with drafted tokens: keys and values in 8 or 4 bits, attention of several new tokens behind a history, log
 # probabilities of tokens.  (Not in the reference either.)
 # ------------------------------------------------------------------------------------------------------------------
-_CACHE_TYPES = {BF16: _lib.CACHE_BF16, torch.int8: _lib.CACHE_INT8, torch.float8_e4m3fn: _lib.CACHE_E4M3}
+_CACHE_TYPES = {BF16: _lib.CACHE_BF16, torch.int8: _lib.CACHE_INT8, torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int4: _lib.CACHE_INT4, torch.uint8: _lib.CACHE_INT4}
+GROUP4 = 32                                                   # channels of a head that share a scale in a cache of 4 bits
 
 
 def _device(t, what):
@@ -1421,11 +1422,14 @@ def _rows_of(t, dtype, shape, dev, what):
 
 
 def _cache_view(what, cache, scale, heads, dim, dev):
-    """A cache [slots, capacity, heads * dim] or [slots, capacity, heads, dim] with neighbouring channels (any strides else) and its scales [slots, heads, capacity]."""
+    """A cache [slots, capacity, heads * dim] or [slots, capacity, heads, dim] with neighbouring channels (any strides else) and its scales [slots, heads, capacity]; with 4 bits half the
+    numbers as bytes and scales [slots, heads, capacity, dim / 32]."""
     shape, strides = cache.shape, cache.stride()
     kind = _CACHE_TYPES.get(cache.dtype)
     if kind is None or cache.get_device() != dev:
-        raise _lib.LiaError(f"{what} has to be bf16, int8 or float8_e4m3fn on the current CUDA device, not {cache.dtype} on {cache.device}")
+        raise _lib.LiaError(f"{what} has to be bf16, int8, float8_e4m3fn or uint8 (4 bits) on the current CUDA device, not {cache.dtype} on {cache.device}")
+    if kind == _lib.CACHE_INT4:
+        return _cache4_view(what, cache, scale, heads, dim, dev, shape, strides)
     if len(shape) == 3 and shape[2] == heads * dim:
         head = dim
     elif len(shape) == 4 and shape[2] == heads and shape[3] == dim:
@@ -1445,6 +1449,26 @@ def _cache_view(what, cache, scale, heads, dim, dev):
     if capacity > 1 and apart[2] != 1:
         raise _lib.LiaError(f"{what}: the positions of its scales have to be neighbours, strides are {apart}")
     return _lib.LiaCacheView(cache.data_ptr(), scale.data_ptr(), strides[0], strides[1], head, apart[0], apart[1], slots, capacity, kind, dim)
+
+
+def _cache4_view(what, cache, scale, heads, dim, dev, shape, strides):
+    if dim % GROUP4:
+        raise _lib.LiaError(f"{what}: heads of 4 bits are multiples of {GROUP4} channels, not {dim}")
+    if len(shape) == 3 and shape[2] == heads * dim // 2:
+        head = dim // 2
+    elif len(shape) == 4 and shape[2] == heads and shape[3] == dim // 2:
+        head = strides[2]
+    else:
+        raise _lib.LiaError(f"{what} has to be [slots, capacity, {heads} * {dim // 2}] or [slots, capacity, {heads}, {dim // 2}] bytes, not {tuple(shape)}")
+    slots, capacity, groups = shape[0], shape[1], dim // GROUP4
+    if strides[-1] != 1:
+        raise _lib.LiaError(f"{what}: its channels have to be neighbours, strides are {strides}")
+    if scale is None or scale.dtype is not BF16 or scale.get_device() != dev or tuple(scale.shape) != (slots, heads, capacity, groups):
+        raise _lib.LiaError(f"{what} is of 4 bits and needs bf16 scales [slots, {heads}, capacity, {groups}] on the current CUDA device")
+    apart = scale.stride()
+    if (groups > 1 and apart[3] != 1) or (capacity > 1 and apart[2] != groups):
+        raise _lib.LiaError(f"{what}: the scales of a head have to be neighbours, strides are {apart}")
+    return _lib.LiaCacheView(cache.data_ptr(), scale.data_ptr(), strides[0], strides[1], head, apart[0], apart[1], slots, capacity, _lib.CACHE_INT4, dim)
 
 
 def _cache_rows(what, k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim):
@@ -1471,6 +1495,23 @@ def kv_load_8bit(meta, kcache, vcache, k_scale, v_scale, k, v, G, dim, vdim):
     count_launches()
 
 
+def kv_store_4bit(k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim, eps=0.0, norm_values=False):
+    """``kv_store_8bit`` into caches of 4 bits (csrc/kv_4bit.cu): uint8 [slots, capacity, G * dim // 2] (or [slots, capacity, G, dim // 2]), two codes of -7 to 7 a byte, with a scale for every 32
+    channels of each head of each row in ``k_scale`` / ``v_scale``, bf16 [slots, G, capacity, dim // 32]: 4.5 bits a number.  The largest magnitude a of 32 channels gives the scale a / 7, rounded to
+    bf16; code = round(x / scale).  32 channels that hold an infinity or NaN read back as NaN.  Heads are multiples of 32 channels."""
+    kp, ldk, vp, ldv, f32, at, kc, vc, M = _cache_rows("kv_store_4bit", k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim)
+    check(_lib.load().lia_kv_store_4bit(kp, ldk, vp, ldv, f32, at, kc, vc, M, G, eps, norm_values, _stream()), "lia_kv_store_4bit")
+    count_launches()
+
+
+def kv_load_4bit(meta, kcache, vcache, k_scale, v_scale, k, v, G, dim, vdim):
+    """The rows at ``meta`` of 4-bit caches as numbers, code * scale rounded once, into ``k`` [M, G * dim] and ``v`` [M, G * vdim] (bf16 or fp32; column slices are fine).  NaN for a
+    row whose slot or position the caches lack."""
+    kp, ldk, vp, ldv, f32, at, kc, vc, M = _cache_rows("kv_load_4bit", k, v, meta, kcache, vcache, k_scale, v_scale, G, dim, vdim)
+    check(_lib.load().lia_kv_load_4bit(at, kc, vc, kp, ldk, vp, ldv, f32, M, G, _stream()), "lia_kv_load_4bit")
+    count_launches()
+
+
 def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ctx, mask=None, depth=None, temp=None, window=0, softcap=0.0, k_scale=None, v_scale=None):
     """Attention of portions of new tokens behind their cached histories (csrc/tree_attn.cu): ``segs`` int32 [nseg, 4] on the device, (slot, p0, row, n) each -- the n tokens of rows
     row .. row + n - 1 have their keys and values at positions p0 .. p0 + n - 1 already.  Every token sees the p0 positions of history and, without ``mask``, the new tokens up to itself
@@ -1479,7 +1520,7 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
     (int32 [M]; None: its number in the portion).  Scores are temp[h] * scale * (q . k), then softcap * tanh(score / softcap) if ``softcap`` > 0 (1024 at most).
 
     Caches: bf16, or int8 / float8_e4m3fn with ``k_scale`` and ``v_scale`` [slots, G, capacity] (``kv_store_8bit``), [slots, capacity, G * dim] or [slots, capacity, G, dim] with
-    neighbouring channels; heads of 64 or 128 channels; values' scales up to 2^29.  A NaN or an infinity among keys or values that a tile of rows reads has its rows formed again key by key, about a
+    neighbouring channels, or uint8 of 4 bits with bf16 scales (``kv_store_4bit``); heads of 64 or 128 channels; values' scales up to 2^29.  A NaN or an infinity among keys or values that a tile of rows reads has its rows formed again key by key, about a
     thousand times slower.  ``q`` [M, H * dim] and ``out`` [M, H * vdim] are bf16.  ``rows``: the most tokens of a portion; ``max_ctx``: the longest p0 + n,
     about (it decides how many blocks share a history, not what is read).  A row that sees nothing is 0; no two portions share a row; rows of no portion are left as they are; a portion that does not fit its slot, the
     rows, ``rows`` or the mask's words gives NaN rows."""
@@ -1505,7 +1546,7 @@ def tree_attn(q, kcache, vcache, segs, out, H, G, dim, vdim, scale, rows, max_ct
 
 
 def tree_attn_plan(nseg, rows, max_ctx, H, G, window, dtype):
-    """All that a call of ``tree_attn`` over caches of ``dtype`` launches by: two lengths ``max_ctx`` of one plan launch alike, so that one's captured launches serve the other."""
+    """All that a call of ``tree_attn`` over caches of ``dtype`` (torch.int4 for 4 bits) launches by: two lengths ``max_ctx`` of one plan launch alike, so that one's captured launches serve the other."""
     return _lib.load().lia_tree_attn_plan(nseg, rows, max_ctx, H, G, window, _CACHE_TYPES[dtype])
 
 

@@ -415,11 +415,11 @@ class WindowAttentionMixer:
     positional rotation.  Values are divided by their per-head root mean square before they are cached; a score is
     (q . k) * scale * temp_h, then softcap * tanh(score / softcap) (csrc/window_attn.cu); output Wo on the concatenated heads.
     ``cache_dtype`` int8 or float8_e4m3fn: keys and values are cached in 8 bits with a scale per head and token (csrc/kv_8bit.cu, csrc/tree_attn.cu): half the memory, and less of
-    it to read for every token; bf16 layers with heads of 64 or 128 channels, and soft caps up to 1024."""
+    it to read for every token; int4: in 4 bits with a scale per 32 channels (csrc/kv_4bit.cu), 0.28 of the memory; bf16 layers with heads of 64 or 128 channels, and soft caps up to 1024."""
 
     def __init__(self, w, heads, kv_heads, dim, vdim, window, scale, softcap, norm_eps, dtype, device, norm_values=True, cache_dtype=None):
-        if cache_dtype is not None and (cache_dtype not in (torch.int8, torch.float8_e4m3fn) or dtype != BF16 or dim not in (64, 128) or vdim not in (64, 128)):
-            raise ValueError(f"caches of 8 bits are int8 or float8_e4m3fn, for bf16 layers with heads of 64 or 128 channels, not {cache_dtype} for {dtype} with heads of {dim} and {vdim}")
+        if cache_dtype is not None and (cache_dtype not in (torch.int8, torch.float8_e4m3fn, torch.int4) or dtype != BF16 or dim not in (64, 128) or vdim not in (64, 128)):
+            raise ValueError(f"caches of 8 bits are int8 or float8_e4m3fn (of 4 int4), for bf16 layers with heads of 64 or 128 channels, not {cache_dtype} for {dtype} with heads of {dim} and {vdim}")
         if cache_dtype is not None and softcap > 1024:
             raise ValueError(f"caches of 8 bits: scores are capped at 1024 at most, not {softcap}")
         self.cache_dtype = cache_dtype
@@ -439,6 +439,8 @@ class WindowAttentionMixer:
             seen[shape] = tree_attn_plan(requests, 1, max_ctx, *shape, self.cache_dtype)
 
     def new_state(self, slots):
+        if self.cache_dtype is torch.int4:
+            return (*slots.add_rows_4bit(self.G, self.dim), *slots.add_rows_4bit(self.G, self.vdim))
         if self.cache_dtype is not None:
             return (*slots.add_rows_8bit(self.G, self.dim, self.cache_dtype), *slots.add_rows_8bit(self.G, self.vdim, self.cache_dtype))
         return (slots.add_rows(self.G * self.dim, self.dtype), slots.add_rows(self.G * self.vdim, self.dtype))
@@ -450,7 +452,8 @@ class WindowAttentionMixer:
         o = torch.empty(M, self.H * self.vdim, dtype=self.dtype, device=h.device)
         if self.cache_dtype is not None:
             kc, ks, vc, vs = state
-            ops.kv_store_8bit(k, v, batch.meta, kc, vc, ks, vs, self.G, self.dim, self.vdim, self.eps, self.norm_values)
+            store = ops.kv_store_4bit if self.cache_dtype is torch.int4 else ops.kv_store_8bit
+            store(k, v, batch.meta, kc, vc, ks, vs, self.G, self.dim, self.vdim, self.eps, self.norm_values)
             ops.tree_attn(q, kc, vc, batch.segs, o, self.H, self.G, self.dim, self.vdim, self.scale, rows=batch.lengths[1] if batch.lengths else M, max_ctx=batch.max_ctx, temp=self.temp,
                           window=self.window, softcap=self.softcap, k_scale=ks, v_scale=vs)
             return self.out(o)

@@ -47,6 +47,15 @@ class SlotState:
         self.rows += [codes, scales]
         return codes, scales
 
+    def add_rows_4bit(self, heads, dim):
+        """A row cache of ``heads`` heads in 4 bits for ``ops.kv_store_4bit``: (bytes of two codes [n_slots, capacity, heads * dim // 2], bf16 scales [n_slots, heads, capacity, dim // 32])."""
+        if dim % 32:
+            raise ValueError(f"heads of 4 bits are multiples of 32 channels, not {dim}")
+        codes = torch.zeros(self.n_slots, self.capacity, int(heads) * int(dim) // 2, dtype=torch.uint8, device=self.device)
+        scales = torch.zeros(self.n_slots, int(heads), self.capacity, int(dim) // 32, dtype=torch.bfloat16, device=self.device)
+        self.rows += [codes, scales]
+        return codes, scales
+
     # ---- requests (scheduler side)
     def slot_of(self, req_id):
         return self.by_id.get(req_id)

@@ -1,0 +1,77 @@
+"""What the operators of serving in fewer bits refuse, and their state's shapes: no GPU, no launch."""
+import pytest
+import torch
+
+BF16, F32, U8 = torch.bfloat16, torch.float32, torch.uint8
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import __graft_entry__ as g
+    g.build()
+    import lia_b200  # noqa: F401
+    from lia_b200 import _lib
+    return _lib
+
+
+def view(_lib, **change):
+    v = dict(data=1 << 20, scale=1 << 21, slot_stride=1 << 15, pos_stride=512, head_stride=64, scale_slot_stride=2048, scale_head_stride=256, slots=2, capacity=64, type=_lib.CACHE_INT4, dim=128)
+    return _lib.LiaCacheView(**(v | change))
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"data": None}, "null cache"), ({"scale": None}, "scales"), ({"type": 7}, "type"), ({"type": 1}, "4 bits"), ({"slots": 0}, "empty"), ({"capacity": 0}, "empty"),
+    ({"data": (1 << 20) + 4}, "vectors"), ({"pos_stride": 516}, "vectors"), ({"head_stride": 68}, "vectors"), ({"dim": 100}, "multiples of 32"), ({"dim": 2048}, "1024"),
+    ({"capacity": 65}, "different sizes"), ({"scale": (1 << 21) + 2}, "scales"), ({"scale_head_stride": 258}, "scales"), ({"scale_slot_stride": 2049}, "scales")])
+def test_store_and_load_of_4_bits_refuse(lib, change, message):
+    L = lib.load()
+    good, bad = view(lib), view(lib, **change)
+    for kc, vc in ((bad, good), (good, bad)):
+        assert L.lia_kv_store_4bit(16, 1024, 16, 1024, 0, 16, kc, vc, 4, 8, 0.0, 0, None) == -1 and message in lib.last_error()
+        assert L.lia_kv_load_4bit(16, kc, vc, 16, 1024, 16, 1024, 0, 4, 8, None) == -1 and message in lib.last_error()
+
+
+def test_store_of_4_bits_refuses_short_rows_and_null_pointers(lib):
+    L, v = lib.load(), view(lib)
+    assert L.lia_kv_store_4bit(16, 1023, 16, 1024, 0, 16, v, v, 4, 8, 0.0, 0, None) == -1 and "shorter" in lib.last_error()
+    assert L.lia_kv_store_4bit(None, 1024, 16, 1024, 0, 16, v, v, 4, 8, 0.0, 0, None) == -1
+    assert L.lia_kv_store_4bit(16, 1024, 16, 1024, 0, None, v, v, 4, 8, 0.0, 0, None) == -1
+    assert L.lia_kv_store_4bit(16, 1024, 16, 1024, 0, 16, v, v, -1, 8, 0.0, 0, None) == -1
+    assert L.lia_kv_store_4bit(16, 1 << 20, 16, 1 << 20, 0, 16, v, v, 1 << 28, 8, 0.0, 0, None) == -1 and "too many" in lib.last_error()
+    assert L.lia_kv_store_4bit(None, 1024, None, 1024, 0, None, v, v, 0, 8, 0.0, 0, None) == 0     # no rows, no launch
+    assert L.lia_kv_store_8bit(16, 1024, 16, 1024, 0, 16, v, v, 4, 8, 0.0, 0, None) == -1 and "int8" in lib.last_error()
+
+
+@pytest.mark.parametrize("change,message", [({"data": (1 << 20) + 8}, "vectors"), ({"dim": 96}, "64 or 128"), ({"dim": 256}, "64 or 128"), ({"type": 1}, "different types"),
+                                            ({"slots": 3}, "different types or sizes"), ({"scale": None}, "scales"), ({"scale": (1 << 21) + 4}, "scales")])
+def test_attention_refuses_caches_of_4_bits(lib, change, message):
+    good, bad = view(lib), view(lib, **change)
+    for kc, vc in ((bad, good), (good, bad)):
+        assert lib.load().lia_tree_attn(256, 2048, kc, vc, 256, 2, None, 0, None, None, 256, None, 0, 8, 16, 8, 4, 40, 0, 1.0, 0.0, None) == -1 and message in lib.last_error()
+
+
+def test_views_of_4_bit_caches(lib):
+    """Tensors of the wrong shape, type, strides or place raise before anything is launched."""
+    from lia_b200 import ops
+    z, E = torch.zeros, lib.LiaError
+    c, s = z(2, 9, 3 * 64, dtype=U8), z(2, 3, 9, 4, dtype=BF16)
+    v = ops._cache_view("x", c, s, 3, 128, -1)
+    assert (v.type, v.dim, v.head_stride, v.pos_stride, v.slot_stride) == (lib.CACHE_INT4, 128, 64, 192, 9 * 192) and (v.scale_slot_stride, v.scale_head_stride) == (108, 36)
+    v = ops._cache_view("x", z(2, 9, 3, 2, 64, dtype=U8)[:, :, :, 1], s, 3, 128, -1)
+    assert (v.head_stride, v.pos_stride) == (128, 384)
+    for cache, scale, dim, message in ((z(2, 9, 3 * 128, dtype=U8), s, 128, "bytes"), (c, None, 128, "bf16 scales"), (c, s.float(), 128, "bf16 scales"), (c, z(2, 3, 9, dtype=BF16), 128, "bf16 scales"),
+                                       (c, z(2, 3, 9, 8, dtype=BF16)[..., ::2], 128, "neighbours"), (c, z(2, 3, 4, 9, dtype=BF16).transpose(2, 3), 128, "neighbours"),
+                                       (z(2, 9, 3 * 24, dtype=U8), s, 48, "multiples of 32"), (z(2, 9, 3 * 128, dtype=U8)[..., ::2], s, 128, "neighbours")):
+        with pytest.raises(E, match=message):
+            ops._cache_view("x", cache, scale, 3, dim, -1)
+    with pytest.raises(E):
+        ops.kv_store_4bit(z(2, 128, dtype=BF16), z(2, 128, dtype=BF16), z(2, 2, dtype=torch.int32), z(1, 4, 64, dtype=U8), z(1, 4, 64, dtype=U8), z(1, 1, 4, 4), z(1, 1, 4, 4), 1, 128, 128)
+
+
+def test_slots_of_4_bit_rows():
+    from lia_b200.seq_state import SlotState
+    s = SlotState(3, 17, "cpu")
+    codes, scales = s.add_rows_4bit(4, 64)
+    assert codes.shape == (3, 17, 128) and codes.dtype == U8 and scales.shape == (3, 4, 17, 2) and scales.dtype == BF16
+    with pytest.raises(ValueError):
+        s.add_rows_4bit(4, 48)
