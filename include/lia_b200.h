@@ -700,6 +700,21 @@ int lia_tree_attn_plan(int nseg, int rows, int max_ctx, int H, int G, int window
 int lia_token_logprobs(const void* logits, int act_f32, long long ld, int M, int V, const int64_t* tokens, int n, float* logp, float* entropy, int top, float* top_logp, int64_t* top_ids,
                        lia_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Projections in 8-bit integers, with a scale for each token and each output channel.  (Not in the reference.)
+ * ---------------------------------------------------------------------------------------------------------------- */
+enum { LIA_X_BF16 = 0, LIA_X_F32 = 1, LIA_X_INT8 = 2 };
+
+/* Rows of x [M, K] (bf16 or fp32, ldx apart) as codes int8 [M, K] (ldc apart; 8-byte vectors) and scale [M]: scale = a / 127, code = rint(127 x / a) with a the row's largest magnitude (counted as 2^-100
+ * at least; 127 x of fp32 numbers is rounded once).  A row with an infinity or NaN gets scale NaN and codes 0.  Weights [N, K] become codes with a scale for each output channel in the same way. */
+int lia_quantize_rows(const void* x, int act_f32, long long ldx, void* codes, long long ldc, float* scale, int M, int K, lia_stream_t stream);
+/* out [M, N] (bf16 or fp32, rows side by side) = x . w^T with codes w int8 [N, K] (ldw bytes apart) times w_scale [N]: x is codes (ldx bytes apart) with x_scale [M], or bf16 or fp32 rows (ldx numbers
+ * apart, x_scale NULL) that are quantised on the way.  Rows of codes: whole 16-byte vectors, 131071 codes at most (sums are exact 32-bit integers).  out = (float(sum) * x_scale[m]) * w_scale[n], rounded to
+ * fp32 at every step and then to out's type.  ws: lia_linear_int8_workspace_bytes() bytes (0: NULL will do), no two calls under way at the same time share it. */
+size_t lia_linear_int8_workspace_bytes(int x_type, int M, int N, int K);
+int lia_linear_int8(const void* x, int x_type, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, void* out, int out_f32, int M, int N, int K,
+                    void* ws, size_t ws_bytes, lia_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libliab200.so")
 EPI_BIAS, EPI_BIAS_RELU, EPI_BIAS_RESIDUAL, EPI_QKV = 0, 1, 2, 3
 ABI_VERSION = 11
 CACHE_BF16, CACHE_INT8, CACHE_E4M3, CACHE_INT4 = 0, 1, 2, 3
+X_BF16, X_F32, X_INT8 = 0, 1, 2
 TP_MAX_WORLD = 8
 P2P_HANDLE_BYTES = 64
 
@@ -246,6 +247,10 @@ _PROTOTYPES = {
     "lia_tree_attn": (c_int, [c_void_p, c_longlong, POINTER(LiaCacheView), POINTER(LiaCacheView), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                               c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p]),
     "lia_token_logprobs": (c_int, [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    # projections in 8-bit integers
+    "lia_quantize_rows": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p]),
+    "lia_linear_int8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "lia_linear_int8": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
 }
 
 EXPORTS = tuple(_PROTOTYPES)

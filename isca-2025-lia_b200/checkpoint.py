@@ -48,9 +48,11 @@ class CheckpointError(RuntimeError):
 
 
 def no_cache_dtype(cls, options):
-    """Refuse ``cache_dtype`` among the options of a model whose caches have its own type: it would get one of twice the size."""
+    """Refuse ``cache_dtype`` and ``weight_dtype`` among the options of a model whose caches and weights have its own type: it would get some of twice the size."""
     if options.get("cache_dtype") is not None:
         raise ValueError(f"{cls.__name__} has no caches of {options['cache_dtype']}: cache_dtype is for Bebulorn's attention layers")
+    if options.get("weight_dtype") is not None:
+        raise ValueError(f"{cls.__name__} has no projections of {options['weight_dtype']}: weight_dtype is for Bebulorn")
 
 
 # ------------------------------------------------------------------------------------------------

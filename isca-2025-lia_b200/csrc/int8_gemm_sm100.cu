@@ -1,0 +1,637 @@
+// Projections in 8-bit integers: out[m, n] = sx[m] sw[n] sum_k cx[m, k] cw[n, k], codes of 8 bits with a scale for each token and each channel, for sm_100a.
+//
+//   tokens   a = max |x[m]|, sx = a / 127, cx = rint(127 x / a)   (quantize_rows_kernel, a block a token; coder8.cuh)
+//   sums     whole numbers of 32 bits, exact for up to 131071 products: whatever order they are added in, the bits are the same
+//
+// tcgen05.mma.kind::i8, both operands K-major from shared memory (TMA, 128-byte swizzle: 128 codes a row), sums in TMEM.  Two forms:
+//   FEW    (up to 128 tokens; bound by the weights' bytes)  the weights' rows are the product's 128 rows, the tokens its 16 to 128 columns.  The list of (row tile, block of K) is cut into as many
+//          spans of equal length as there are CTAs, so that every SM streams the same number of bytes.  A tile that several spans share is finished by whichever of them arrives last: the others leave
+//          their sums in a workspace and count themselves, nobody waits, so that launches on several streams cannot hold one another up.  Weights are on their way while the
+//          tokens are quantised.
+//   MANY   (bound by the tensor cores)  the tokens' rows are the product's rows: CTA pairs on 256 x 256 tiles (cta_group::2), or one CTA on 128 x 256, 128 or 64 where those would leave SMs idle.
+//
+// Every wait is bounded; a CTA that gives one up makes its outputs NaN (a shared tile's by way of its count) and counts itself in lia_moe_timeouts_seen().
+#include <cuda.h>
+
+#include <mutex>
+
+#include "coder8.cuh"
+#include "common.cuh"
+#include "umma.cuh"
+
+int* lia_timeout_word();                                           // moe_sm100.cu
+
+namespace {
+
+constexpr int TILE = 128, KB = 128;                                // rows of a tile, codes (bytes) of a block of K
+constexpr int MOST_K = 131071;                                     // 127 * 127 * K stays below 2^31 (and 128 * 128 * K)
+constexpr int MOST_PIECES = 1 << 16;                               // what a CTA that gave up adds to a tile's count
+
+// ------------------------------------------------------------------ tokens' codes
+struct QuantArgs {
+  const void* x;
+  long long ldx, ldc;
+  int8_t* codes;
+  float* scale;
+  int* counts;                                                     // made zero for the product behind
+  int K, n_counts, vec;
+};
+constexpr int Q_THREADS = 256, Q_HELD = 4;                         // vectors of eight numbers that a thread holds: rows of 8192 numbers are read once
+
+template <typename T> __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_constant__ QuantArgs a) {
+  // In this order: the product behind asks for its weights before it waits, and may not begin before what came before this kernel (the weights' own quantisation, perhaps) has ended
+  pdl_wait();
+  pdl_launch_dependents();
+  __shared__ uint32_t part[Q_THREADS / 32];
+  const int t = threadIdx.x, vecs = (a.K + 7) / 8;
+  const T* src = reinterpret_cast<const T*>(a.x) + (long long)blockIdx.x * a.ldx;
+  for (int i = blockIdx.x * Q_THREADS + t; i < a.n_counts; i += gridDim.x * Q_THREADS) a.counts[i] = 0;
+  auto load = [&](int v) {                                         // numbers behind the row's end are zeros
+    if (v >= vecs) return Raw8<T>{};
+    if (v * 8 + 8 <= a.K) return load8(src + v * 8, a.vec);
+    T r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = v * 8 + i < a.K ? src[v * 8 + i] : (T)0.f;
+    Raw8<T> u;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.u[i] = reinterpret_cast<const uint4*>(r)[i];
+    return u;
+  };
+  Raw8<T> raw[Q_HELD];
+#pragma unroll
+  for (int i = 0; i < Q_HELD; ++i) raw[i] = load(t + i * Q_THREADS);
+  uint32_t most = 0u;
+#pragma unroll
+  for (int i = 0; i < Q_HELD; ++i) most = most_of(raw[i], most);
+  for (int v = t + Q_HELD * Q_THREADS; v < vecs; v += Q_THREADS) most = most_of(load(v), most);
+  if constexpr (sizeof(T) == 2) most = max(most & 0xffffu, most >> 16) << 16;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((t & 31) == 0) part[t >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < Q_THREADS / 32; ++i) most = max(most, part[i]);
+  const Coder<true> code(__uint_as_float(most));
+  int8_t* dst = a.codes + (long long)blockIdx.x * a.ldc;
+  auto put = [&](int v, const Raw8<T>& r) {
+    if (v >= vecs) return;
+    float f[8];
+    numbers_of(r, f);
+    const uint2 c = code(f);
+    if (v * 8 + 8 <= a.K) {
+      *reinterpret_cast<uint2*>(dst + v * 8) = c;
+    } else {
+      for (int i = v * 8; i < a.K; ++i) dst[i] = (int8_t)((i & 4 ? c.y : c.x) >> (8 * (i & 3)));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < Q_HELD; ++i) put(t + i * Q_THREADS, raw[i]);
+  for (int v = t + Q_HELD * Q_THREADS; v < vecs; v += Q_THREADS) put(v, load(v));
+  if (t == 0) a.scale[blockIdx.x] = code.scale;
+}
+
+// ------------------------------------------------------------------ products
+struct Args {
+  const float* sx;
+  const float* sw;
+  void* out;
+  int* pieces;                                                     // FEW: sums of parts of tiles [2 * CTAs][tokens][TILE]
+  int* counts;                                                     // FEW: of a tile's parts that have been left
+  int* timeouts;
+  int M, N, k_blocks, tiles_a, tiles_b, wide;                      // wide: rows of out are whole 16-byte vectors apart
+};
+
+// kind::i8: sums of 32-bit integers, both operands signed and K-major
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+__device__ __forceinline__ void mma_i8_if(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+               "r"(accumulate), "r"(one)
+               : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair_if(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+               "r"(accumulate), "r"(one)
+               : "memory");
+}
+
+template <bool FEW, int BN, bool PAIR> struct Shape {
+  static constexpr int A_BYTES = TILE * KB, B_BYTES = (PAIR ? BN / 2 : BN) * KB, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGING = FEW ? 0 : 4 * 4096;               // 32 rows of 128 bytes for each epilogue warp
+  static constexpr int ROOM = (229376 - STAGING) / STAGE, STAGES = ROOM > 10 ? 10 : ROOM;
+  static constexpr int BARS = STAGES * STAGE + STAGING;
+  static constexpr int SMEM = BARS + (2 * STAGES + 5) * 8 + 32 + 1024;
+  static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;           // of TMEM: two tiles' sums
+};
+
+struct Work {
+  int ta, tb, kb0, kb1;
+};
+// FEW: the CTA's span of the flat list of (tile, block of K).  MANY: tile u = worker + i * workers, in groups of some rows of tiles, so that what runs at the same time shares operands in L2.
+template <bool FEW> struct Sched {
+  int k_blocks, tiles_a, tiles_b, group;
+  unsigned pos, end, step;
+  __device__ __forceinline__ Sched(const Args& p, bool pair) : k_blocks(p.k_blocks), tiles_a(p.tiles_a), tiles_b(p.tiles_b), group(pair ? 8 : 16) {
+    if (FEW) {
+      const unsigned total = (unsigned)tiles_a * (unsigned)k_blocks;                           // (times the CTAs below 2^31: checked on the host)
+      pos = total * blockIdx.x / gridDim.x;
+      end = total * (blockIdx.x + 1) / gridDim.x;
+      step = 0;
+    } else {
+      pos = pair ? blockIdx.x >> 1 : blockIdx.x;
+      step = pair ? gridDim.x >> 1 : gridDim.x;
+      end = (unsigned)tiles_a * (unsigned)tiles_b;
+    }
+  }
+  __device__ __forceinline__ bool next(Work& w) {
+    if (pos >= end) return false;
+    if (FEW) {
+      w.ta = (int)(pos / (unsigned)k_blocks);
+      w.tb = 0;
+      w.kb0 = (int)(pos - (unsigned)w.ta * (unsigned)k_blocks);
+      w.kb1 = min(k_blocks, w.kb0 + (int)(end - pos));
+      pos += (unsigned)(w.kb1 - w.kb0);
+    } else {
+      const int u = (int)pos, size = group * tiles_b, first = u / size * group, gm = min(group, tiles_a - first), r = u % size;
+      w.ta = first + r % gm;
+      w.tb = r / gm;
+      w.kb0 = 0;
+      w.kb1 = k_blocks;
+      pos += step;
+    }
+    return true;
+  }
+};
+
+template <bool OUT32> __device__ __forceinline__ void put_one(void* out, size_t at, float y) {
+  if constexpr (OUT32) reinterpret_cast<float*>(out)[at] = y;
+  else reinterpret_cast<bf16*>(out)[at] = __float2bfloat16_rn(y);
+}
+
+template <bool FEW, int BN, bool PAIR, bool OUT32>
+__global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Args p) {
+  static_assert(!PAIR || (!FEW && BN == 256), "CTA pairs: 256 x 256 tiles");
+  using L = Shape<FEW, BN, PAIR>;
+  constexpr int STAGES = L::STAGES;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;             // of a pair the first issues every product and owns the barriers that loads and epilogues arrive on
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem - smem_u32(smem_raw));
+  const uint32_t bars = smem + L::BARS;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (STAGES + s); };
+  auto tfull = [&](int a) { return bars + 8u * (2 * STAGES + a); };
+  auto tempty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
+  const uint32_t drain = bars + 8u * (2 * STAGES + 4);
+  volatile uint32_t* tmem_at = reinterpret_cast<volatile uint32_t*>(smem_gen + L::BARS + (2 * STAGES + 5) * 8);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_at + 1);
+  volatile int* arrived = reinterpret_cast<volatile int*>(tmem_at + 2);
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
+    *dead = 0;
+  }
+  if (warp == 1 && lane == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull(a), 1);
+      mbar_init(tempty(a), PAIR ? 8 : 4);
+    }
+    mbar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_at)), "r"((uint32_t)L::COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_at)), "r"((uint32_t)L::COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();
+  tcgen05_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+  pdl_launch_dependents();                                         // (only weights are touched before pdl_wait)
+  int issued = 0;                                                  // blocks that the loading lane has asked for
+
+  if (warp == 0) {
+    // ================================================================ loads
+    if (lane == 0) {
+      int early = 0;
+      if (FEW) {                                                   // weights, which no kernel writes, before the tokens' codes are there
+        Sched<FEW> s(p, PAIR);
+        Work w;
+        while (early < STAGES && s.next(w))
+          for (int kb = w.kb0; kb < w.kb1 && early < STAGES; ++kb, ++early) {
+            mbar_expect_tx(full(early), L::STAGE);
+            tma_load_2d(smem + early * L::STAGE, &tmA, kb * KB, w.ta * TILE, full(early));
+          }
+      }
+      pdl_wait();
+      Sched<FEW> s(p, PAIR);
+      Work w;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      while (alive && s.next(w))
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          const uint32_t sa = smem + stage * L::STAGE, sb = sa + L::A_BYTES;
+          if (FEW && issued < early) {
+            tma_load_2d(sb, &tmB, kb * KB, 0, full(stage));
+          } else {
+            if (!(alive = wait_for(empty(stage), phase ^ 1u, dead))) break;
+            if (PAIR) {
+              const uint32_t fb = mapa_u32(full(stage), 0);
+              if (rank == 0) mbar_expect_tx(full(stage), 2 * L::STAGE);
+              tma_load_2d_pair(sa, &tmA, kb * KB, (w.ta * 2 + (int)rank) * TILE, fb);
+              tma_load_2d_pair(sb, &tmB, kb * KB, w.tb * BN + (int)rank * (BN / 2), fb);
+            } else {
+              mbar_expect_tx(full(stage), L::STAGE);
+              tma_load_2d(sa, &tmA, kb * KB, w.ta * TILE, full(stage));
+              tma_load_2d(sb, &tmB, kb * KB, w.tb * BN, full(stage));
+            }
+          }
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+    }
+  } else if (warp == 1) {
+    // ================================================================ products
+    if (rank == 0) {
+      const uint32_t one = elect_one();
+      constexpr uint32_t idesc = idesc_i8(PAIR ? 2 * TILE : TILE, BN);
+      Sched<FEW> s(p, PAIR);
+      Work w;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool alive = true;
+      while (alive && s.next(w)) {
+        if (!(alive = warp_wait(tempty(acc), acc_phase ^ 1u, dead))) break;
+        tcgen05_fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc * BN);
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!(alive = warp_wait(full(stage), phase, dead))) break;
+          tcgen05_fence_after();
+          const uint32_t sa = smem + stage * L::STAGE;
+          const uint64_t da = make_smem_desc(sa), db = make_smem_desc(sa + L::A_BYTES);
+#pragma unroll
+          for (int k = 0; k < KB / 32; ++k) {                      // 32 codes on are 32 bytes inside the swizzled row: + 2 in the address field
+            if (PAIR) mma_i8_pair_if(one, d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb > w.kb0 || k > 0) ? 1u : 0u);
+            else mma_i8_if(one, d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb > w.kb0 || k > 0) ? 1u : 0u);
+          }
+          if (PAIR) {
+            if (one) tcgen05_commit_pair(empty(stage));
+          } else {
+            commit_if(one, empty(stage));
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!alive) break;
+        if (PAIR) {
+          if (one) tcgen05_commit_pair(tfull(acc));
+        } else {
+          commit_if(one, tfull(acc));
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+  } else if (warp >= 4) {
+    // ================================================================ sums to outputs
+    const int ew = warp - 4;                                       // TMEM lanes 32 ew .. 32 ew + 31
+    pdl_wait();
+    Sched<FEW> s(p, PAIR);
+    Work w;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool alive = true;
+    while (s.next(w)) {
+      alive = __all_sync(0xffffffffu, alive && wait_for(tfull(acc), acc_phase, dead));
+      tcgen05_fence_after();
+      const uint32_t taddr = tmem + (uint32_t)(acc * BN) + ((uint32_t)(ew * 32) << 16);
+      auto give_back = [&] {                                       // the sums are read
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(tempty(acc), 0));
+          else mbar_arrive(tempty(acc));
+        }
+      };
+      if constexpr (FEW) {
+        // a lane has one channel, its columns are the tokens
+        const int nl = ew * 32 + lane, n = w.ta * TILE + nl;
+        const bool there = n < p.N;
+        constexpr int CH = BN < 32 ? BN : 32;
+        bool whole = w.kb0 == 0 && w.kb1 == p.k_blocks, good = alive;
+        int c0 = (int)blockIdx.x, c1 = c0;                         // the CTAs that share the tile
+        if (!whole) {
+          const unsigned total = (unsigned)p.tiles_a * (unsigned)p.k_blocks, first = (unsigned)w.ta * (unsigned)p.k_blocks, last = first + (unsigned)p.k_blocks - 1u;
+          c0 = (int)(((first + 1u) * gridDim.x - 1u) / total);     // span c begins at total * c / CTAs, rounded down
+          c1 = (int)(((last + 1u) * gridDim.x - 1u) / total);
+          int* mine = p.pieces + ((size_t)blockIdx.x * 2 + (w.kb0 == 0)) * p.M * TILE + nl;
+          if (alive) {
+#pragma unroll 1
+            for (int c = 0; c < BN && c < p.M; c += CH) {
+              uint32_t v[CH];
+              if constexpr (CH == 32) tmem_ld32(taddr + c, v);
+              else tmem_ld16(taddr + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < CH; ++j)
+                if (c + j < p.M) __stcg(mine + (size_t)(c + j) * TILE, (int)v[j]);
+            }
+          }
+          __threadfence();
+          epi_bar_sync();
+          if (ew == 0 && lane == 0) *arrived = atomicAdd(p.counts + w.ta, *dead ? 1 + MOST_PIECES : 1);
+          epi_bar_sync();
+          const int before = *arrived;
+          epi_bar_sync();                                          // (read by all before it is written again)
+          if ((before & (MOST_PIECES - 1)) != c1 - c0) {           // not the last one
+            if (alive) give_back();
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1u;
+            continue;
+          }
+          __threadfence();
+          good = alive && before < MOST_PIECES;
+        }
+        const float sw = there ? __ldg(p.sw + n) : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < BN && c < p.M; c += CH) {
+          uint32_t v[CH];
+          if (good) {
+            if constexpr (CH == 32) tmem_ld32(taddr + c, v);
+            else tmem_ld16(taddr + c, v);
+            tmem_ld_wait();
+            for (int o = c0; o <= c1; ++o) {
+              if (o == (int)blockIdx.x) continue;
+              const int* piece = p.pieces + ((size_t)o * 2 + (o == c0)) * p.M * TILE + nl;
+#pragma unroll
+              for (int j = 0; j < CH; ++j)
+                if (c + j < p.M) v[j] += (uint32_t)__ldcg(piece + (size_t)(c + j) * TILE);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < CH; ++j)
+            if (there && c + j < p.M) put_one<OUT32>(p.out, (size_t)(c + j) * p.N + n, good ? (float)(int)v[j] * __ldcg(p.sx + c + j) * sw : NAN);
+        }
+        if (alive) give_back();
+      } else {
+        // a lane has one token, its columns are channels: through shared memory to whole rows
+        const int row0 = (w.ta * (PAIR ? 2 : 1) + (int)rank) * TILE + ew * 32, m = row0 + lane;
+        const float sx = m < p.M ? __ldcg(p.sx + m) : 0.f;
+        const uint32_t stg = smem + STAGES * L::STAGE + ew * 4096;
+        constexpr int SLAB = OUT32 ? 32 : 64, PER = OUT32 ? 4 : 8; // columns of 128 bytes, of 16 bytes
+#pragma unroll 1
+        for (int c0 = 0; c0 < BN; c0 += SLAB) {
+#pragma unroll
+          for (int half = 0; half < SLAB / 32; ++half) {
+            uint32_t v[32];
+            float f[32];
+            if (alive) {
+              tmem_ld32(taddr + c0 + half * 32, v);
+              tmem_ld_wait();
+            }
+            const int n0 = w.tb * BN + c0 + half * 32;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = alive ? (float)(int)v[j] * sx * (n0 + j < p.N ? __ldg(p.sw + n0 + j) : 0.f) : NAN;
+#pragma unroll
+            for (int j = 0; j < 32 / PER; ++j) {                   // each row's chunks turned by the row, so that neither side of the transposition collides
+              const int chunk = half * 4 + j;
+              uint4 q;
+              if constexpr (OUT32) q = make_uint4(__float_as_uint(f[4 * j]), __float_as_uint(f[4 * j + 1]), __float_as_uint(f[4 * j + 2]), __float_as_uint(f[4 * j + 3]));
+              else q = pack8(f + 8 * j);
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stg + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+            }
+          }
+          if (c0 + SLAB >= BN && alive) give_back();
+          else __syncwarp();
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int r = it * 4 + (lane >> 3), chunk = lane & 7;
+            uint4 q;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(stg + r * 128 + ((chunk ^ (r & 7)) << 4)));
+            const int n = w.tb * BN + c0 + chunk * PER;
+            if (row0 + r >= p.M || n >= p.N) continue;
+            const size_t at = (size_t)(row0 + r) * p.N + n;
+            if (p.wide && n + PER <= p.N) {
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + at * (OUT32 ? 4 : 2)) = q;
+            } else {
+              const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int i = 0; i < PER; ++i) {
+                if (n + i >= p.N) break;
+                if constexpr (OUT32) reinterpret_cast<uint32_t*>(p.out)[at + i] = u[i];
+                else reinterpret_cast<uint16_t*>(p.out)[at + i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if (*dead) {                                                     // loads and products in flight end before shared memory and TMEM are given back
+    if (threadIdx.x == 0) {
+      atomicAdd_system(p.timeouts, 1);
+      for (int i = 0; i < STAGES && i < issued && rank == 0; ++i) { // (a pair's loads all arrive on the first one's barriers)
+        const int n = issued - 1 - i;
+        wait_in_flight(full(n % STAGES), (uint32_t)(n / STAGES) & 1u);
+      }
+    }
+    if (warp == 1 && rank == 0) {
+      const uint32_t one = elect_one();
+      if (PAIR) {
+        if (one) tcgen05_commit_pair(drain);
+      } else {
+        commit_if(one, drain);
+      }
+      wait_in_flight(drain, 0u);
+    }
+    __syncthreads();
+  }
+  if (PAIR) cluster_sync_all();                                    // nobody leaves while the other may arrive on its barriers
+  if (warp == 2) {
+    tcgen05_fence_after();
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ host
+// codes [rows, K], `ld` bytes from row to row: boxes of 128 codes x box_rows, what lies outside reads as zeros
+int make_tmap(CUtensorMap* map, const void* base, int rows, int K, long long ld, int box_rows) {
+  PFN_encodeTiled enc = get_encode();
+  LIA_CHECK_ARG(enc, "cuTensorMapEncodeTiled entry point not available (no CUDA driver?)");
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)KB, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    lia_set_error("cuTensorMapEncodeTiled failed with CUresult %d (rows=%d K=%d ld=%lld)", (int)r, rows, K, ld);
+    return LIA_ERR_CUDA;
+  }
+  return LIA_OK;
+}
+
+struct Plan {
+  bool few, pair, split;                                           // split: tiles that several CTAs share
+  int bn, grid, tiles_a, tiles_b, k_blocks;
+};
+Plan plan_of(int M, int N, int K) {
+  Plan p{};
+  const int sms = lia_sm_count();
+  p.k_blocks = (K + KB - 1) / KB;
+  p.few = M <= 128;
+  if (p.few) {
+    p.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    p.tiles_a = (N + TILE - 1) / TILE;
+    p.tiles_b = 1;
+    const long long total = (long long)p.tiles_a * p.k_blocks;
+    long long g = total / 4;                                       // spans of four blocks of K at least
+    g = g < 1 ? 1 : g > sms ? sms : g;
+    p.grid = (int)g;
+    p.split = total % g != 0 || total / g % p.k_blocks != 0;
+    return p;
+  }
+  auto tiles = [&](int rows, int cols) { return (long long)((M + rows - 1) / rows) * ((N + cols - 1) / cols); };
+  auto rounds = [&](long long n, int workers) { return (n + workers - 1) / workers; };
+  long long least = -1;
+  auto offer = [&](int bn, bool pair, long long ns) {
+    if (least >= 0 && ns >= least) return;
+    least = ns;
+    p.bn = bn;
+    p.pair = pair;
+  };
+  offer(256, true, rounds(tiles(2 * TILE, 256), sms / 2) * p.k_blocks * 290 + 6200);
+  offer(256, false, rounds(tiles(TILE, 256), sms) * p.k_blocks * 320 + 5900);
+  offer(128, false, rounds(tiles(TILE, 128), sms) * p.k_blocks * 190 + 1800);
+  offer(64, false, rounds(tiles(TILE, 64), sms) * p.k_blocks * 130 + 200);
+  const int rows = p.pair ? 2 * TILE : TILE;
+  p.tiles_a = (M + rows - 1) / rows;
+  p.tiles_b = (N + p.bn - 1) / p.bn;
+  const long long units = (long long)p.tiles_a * p.tiles_b;
+  p.grid = p.pair ? 2 * (int)(units < sms / 2 ? units : sms / 2) : (int)(units < sms ? units : sms);
+  return p;
+}
+// of a workspace: counts, codes and scales of the tokens (unless they are given), parts of tiles
+struct Rooms {
+  size_t codes, scales, pieces, bytes;
+  long long ldc;
+};
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+Rooms rooms_of(const Plan& p, int M, int K, bool given) {
+  Rooms r;
+  r.ldc = ((long long)K + 15) / 16 * 16;
+  r.codes = p.few && p.split ? up((size_t)p.tiles_a * sizeof(int)) : 0;
+  r.scales = r.codes + (given ? 0 : up((size_t)M * r.ldc));
+  r.pieces = r.scales + (given ? 0 : up((size_t)M * sizeof(float)));
+  r.bytes = r.pieces + (p.few && p.split ? (size_t)p.grid * 2 * M * TILE * sizeof(int) : 0);
+  return r;
+}
+
+template <bool FEW, int BN, bool PAIR, bool OUT32> int launch(const Plan& pl, const CUtensorMap& tmA, const CUtensorMap& tmB, const Args& a, bool early, cudaStream_t stream) {
+  using L = Shape<FEW, BN, PAIR>;
+  static_assert(L::SMEM <= 232448 && L::STAGES >= 3, "shared memory");
+  auto kernel = int8_gemm_kernel<FEW, BN, PAIR, OUT32>;
+  static bool configured[64] = {};                                 // per device
+  int dev = 0;
+  LIA_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    LIA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
+    if (dev < 64) configured[dev] = true;
+  }
+  if (PAIR) LIA_CUDA(lia_launch_cluster(2, kernel, dim3(pl.grid), dim3(256), L::SMEM, stream, tmA, tmB, a));
+  else LIA_CUDA(lia_launch_as(early, kernel, dim3(pl.grid), dim3(256), L::SMEM, stream, tmA, tmB, a));
+  return LIA_OK;
+}
+template <bool OUT32> int launch_plan(const Plan& pl, const CUtensorMap& tmA, const CUtensorMap& tmB, const Args& a, bool early, cudaStream_t stream) {
+  if (pl.few) {
+    switch (pl.bn) {
+      case 16: return launch<true, 16, false, OUT32>(pl, tmA, tmB, a, early, stream);
+      case 32: return launch<true, 32, false, OUT32>(pl, tmA, tmB, a, early, stream);
+      case 64: return launch<true, 64, false, OUT32>(pl, tmA, tmB, a, early, stream);
+      default: return launch<true, 128, false, OUT32>(pl, tmA, tmB, a, early, stream);
+    }
+  }
+  if (pl.pair) return launch<false, 256, true, OUT32>(pl, tmA, tmB, a, early, stream);
+  switch (pl.bn) {
+    case 256: return launch<false, 256, false, OUT32>(pl, tmA, tmB, a, early, stream);
+    case 128: return launch<false, 128, false, OUT32>(pl, tmA, tmB, a, early, stream);
+    default: return launch<false, 64, false, OUT32>(pl, tmA, tmB, a, early, stream);
+  }
+}
+
+int quantize(const void* x, int act_f32, long long ldx, int8_t* codes, long long ldc, float* scale, int* counts, int n_counts, int M, int K, cudaStream_t stream) {
+  const QuantArgs q{x, ldx, ldc, codes, scale, counts, K, n_counts, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (act_f32 ? 4 : 8) == 0};
+  if (act_f32) LIA_CUDA(lia_launch(quantize_rows_kernel<float>, dim3(M), dim3(Q_THREADS), 0, stream, q));
+  else LIA_CUDA(lia_launch(quantize_rows_kernel<bf16>, dim3(M), dim3(Q_THREADS), 0, stream, q));
+  return LIA_OK;
+}
+
+}  // namespace
+
+extern "C" int lia_quantize_rows(const void* x, int act_f32, long long ldx, void* codes, long long ldc, float* scale, int M, int K, lia_stream_t stream) {
+  LIA_CHECK_ARG(M >= 0 && K > 0 && ldx >= K && ldc >= K, "lia_quantize_rows: bad sizes");
+  if (M == 0) return LIA_OK;
+  LIA_CHECK_ARG(x && codes && scale, "lia_quantize_rows: null pointer");
+  LIA_CHECK_ARG(reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldc % 8 == 0, "lia_quantize_rows: rows of codes have to be whole 8-byte vectors apart");
+  return quantize(x, act_f32, ldx, static_cast<int8_t*>(codes), ldc, scale, nullptr, 0, M, K, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t lia_linear_int8_workspace_bytes(int x_type, int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > MOST_K) return 0;
+  return rooms_of(plan_of(M, N, K), M, K, x_type == LIA_X_INT8).bytes;
+}
+
+extern "C" int lia_linear_int8(const void* x, int x_type, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, void* out, int out_f32, int M, int N, int K,
+                               void* ws, size_t ws_bytes, lia_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const bool given = x_type == LIA_X_INT8;
+  LIA_CHECK_ARG(x_type >= LIA_X_BF16 && x_type <= LIA_X_INT8, "lia_linear_int8: unknown type %d of tokens", x_type);
+  LIA_CHECK_ARG(M >= 0 && N > 0 && K > 0 && ldx >= K && ldw >= K, "lia_linear_int8: bad sizes");
+  LIA_CHECK_ARG(K <= MOST_K, "lia_linear_int8: sums of %d products do not fit 32 bits (at most %d)", K, MOST_K);
+  if (M == 0) return LIA_OK;
+  LIA_CHECK_ARG(x && w && w_scale && out && (given == (x_scale != nullptr)), "lia_linear_int8: null pointer, or scales of tokens that are not codes");
+  LIA_CHECK_ARG(reinterpret_cast<uintptr_t>(w) % 16 == 0 && ldw % 16 == 0 && (!given || (reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 16 == 0)),
+                "lia_linear_int8: rows of codes have to be whole 16-byte vectors apart");
+  const Plan pl = plan_of(M, N, K);
+  LIA_CHECK_ARG((long long)pl.tiles_a * pl.k_blocks * (pl.grid + 1) < (1ll << 31) && (long long)pl.tiles_a * pl.tiles_b < (1ll << 31), "lia_linear_int8: too large (M=%d N=%d K=%d)", M, N, K);
+  const Rooms r = rooms_of(pl, M, K, given);
+  LIA_CHECK_ARG(r.bytes == 0 || (ws && ws_bytes >= r.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_linear_int8: needs a workspace of %zu bytes", r.bytes);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  const bool split = pl.few && pl.split;
+  const void* codes = given ? x : base + r.codes;
+  const long long ldc = given ? ldx : r.ldc;
+  CUtensorMap tmX, tmW;
+  int rc = make_tmap(&tmX, codes, M, K, ldc, pl.few ? pl.bn : TILE);
+  if (rc == LIA_OK) rc = make_tmap(&tmW, w, N, K, ldw, pl.few ? TILE : pl.pair ? pl.bn / 2 : pl.bn);
+  if (rc != LIA_OK) return rc;
+  Args a{given ? x_scale : reinterpret_cast<float*>(base + r.scales), w_scale, out, reinterpret_cast<int*>(base + r.pieces), reinterpret_cast<int*>(base), lia_timeout_word(), M, N, pl.k_blocks,
+         pl.tiles_a, pl.tiles_b, reinterpret_cast<uintptr_t>(out) % 16 == 0 && (long long)N * (out_f32 ? 4 : 2) % 16 == 0};
+  LIA_CHECK_ARG(a.timeouts, "lia_linear_int8: no memory for the count of waits that ran out");
+  if (!given) rc = quantize(x, x_type == LIA_X_F32, ldx, reinterpret_cast<int8_t*>(base + r.codes), r.ldc, reinterpret_cast<float*>(base + r.scales), a.counts, split ? pl.tiles_a : 0, M, K, stream);
+  else if (split) LIA_CUDA(cudaMemsetAsync(base, 0, (size_t)pl.tiles_a * sizeof(int), stream));
+  if (rc != LIA_OK) return rc;
+  const bool early = !given;                                       // (right behind another kernel, which may have written the weights, the product does not begin before that has ended)
+  return pl.few ? (out_f32 ? launch_plan<true>(pl, tmW, tmX, a, early, stream) : launch_plan<false>(pl, tmW, tmX, a, early, stream))
+                : (out_f32 ? launch_plan<true>(pl, tmX, tmW, a, early, stream) : launch_plan<false>(pl, tmX, tmW, a, early, stream));
+}

@@ -52,7 +52,7 @@ class Engine:
         seen = ops.moe_timeouts_seen()
         if seen != self._timeouts:
             new, self._timeouts = seen - self._timeouts, seen
-            raise _lib.LiaError(f"{new} blocks of an experts' projection, of a state-space scan or of prompt attention gave up waiting: what was computed since the last check holds NaN")
+            raise _lib.LiaError(f"{new} blocks of an experts' or 8-bit projection, of a state-space scan or of prompt attention gave up waiting: what was computed since the last check holds NaN")
 
     # ---- batch assembly: one pinned staging buffer, one H2D copy per pass
     def _upload(self, ids, segs, meta, want, static=None):

@@ -138,11 +138,15 @@ class _Layer:
 class BebulornForCausalLM:
     step_serving = True          # served through engine.Engine (requests, slots, portions)
 
-    def __init__(self, config, device="cuda", dtype=BF16, cache_dtype=None):
-        """``cache_dtype``: int8, float8_e4m3fn or int4 for the attention layers' keys and values (None: ``dtype``)."""
+    def __init__(self, config, device="cuda", dtype=BF16, cache_dtype=None, weight_dtype=None):
+        """``cache_dtype``: int8, float8_e4m3fn or int4 for the attention layers' keys and values (None: ``dtype``).  ``weight_dtype`` int8: the projections of mixers, dense feed-forwards and
+        shared experts hold codes of 8 bits with a scale for each output channel, and quantise their tokens (routers, routed experts, embedding and head keep ``dtype``)."""
         _lib.load()
         if dtype not in (BF16, F32):
             raise ValueError("dtype must be torch.bfloat16 or torch.float32")
+        if weight_dtype not in (None, torch.int8):
+            raise ValueError(f"weight_dtype must be torch.int8 (or None: as dtype), not {weight_dtype}")
+        self.weight_dtype = weight_dtype
         self.config, self.device, self.dtype, self.cache_dtype = config, torch.device(device), dtype, cache_dtype
         self.layers = []
         self.runs = config.layer_runs()
@@ -191,6 +195,11 @@ class BebulornForCausalLM:
                     experts = [{k: fetch(q + f"e{e}." + k) for k in ("up", "down")} for e in range(spec["router"]["experts"])]
                     mlp = MoEFeedForward(fetch(q + "router"), experts, spec["router"]["top"], spec["expert"]["ff"], ops.ACT_GELU_ERF, shared, dt, dev)
                 n2, n2b = norm(p + "norm2"), norm(p + "norm2b")
+            if self.weight_dtype is not None:
+                for part in (mixer, mlp, getattr(mlp, "shared", None)):
+                    for x in (vars(part).values() if part is not None else ()):
+                        if isinstance(x, Linear):
+                            x.to_int8()
             self.layers.append(_Layer(mixer, mlp, (norm(p + "norm1"), norm(p + "norm1b"), n2, n2b)))
         return self
 
@@ -216,13 +225,13 @@ class BebulornForCausalLM:
         return self.load_weights(lambda n: cache.setdefault(n, make(n)))
 
     @classmethod
-    def from_pretrained(cls, path, device="cuda", dtype=BF16, cache_dtype=None, **unused):
+    def from_pretrained(cls, path, device="cuda", dtype=BF16, cache_dtype=None, weight_dtype=None, **unused):
         from .checkpoint import SafetensorsFile
         cfg = BebulornConfig.from_dict(json.load(open(os.path.join(path, "config.json"))),
                                        name=os.path.basename(os.path.abspath(path)) or "bebulorn")
         f = SafetensorsFile(os.path.join(path, "model.safetensors"))
         try:
-            return cls(cfg, device, dtype, cache_dtype).load_weights(f.get)
+            return cls(cfg, device, dtype, cache_dtype, weight_dtype).load_weights(f.get)
         finally:
             f.close()
 

@@ -1570,3 +1570,56 @@ def token_logprobs(logits, tokens=None, top=0):
     check(_lib.load().lia_token_logprobs(xp, f32, ld, M, V, tp, n, lp, entropy.data_ptr(), top, top_logp.data_ptr(), top_ids.data_ptr(), _stream()), "lia_token_logprobs")
     count_launches()
     return logp, entropy, top_logp, top_ids
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# Projections in 8-bit integers.  (Not in the reference.)
+# ------------------------------------------------------------------------------------------------------------------
+_X_TYPES = {BF16: _lib.X_BF16, F32: _lib.X_F32, torch.int8: _lib.X_INT8}
+
+
+def quantize_rows(x, codes=None, scale=None):
+    """Rows of ``x`` [M, K] (bf16 or fp32; they may lie apart) as int8 codes and a scale each (csrc/int8_gemm_sm100.cu): the largest magnitude a of a row is 127, scale = a / 127,
+    code = round(127 x / a).  A row that holds an infinity or NaN gets the scale NaN.  Returns (codes [M, K], scale fp32 [M]), by themselves with rows a multiple of 16 bytes apart, as
+    ``linear_int8`` takes them; of a weight matrix [N, K] they are its codes with a scale for each output channel."""
+    dev, (M, K) = _device(x, "quantize_rows"), x.shape
+    xp, ldx = _rows_of(x, x.dtype, (M, K), dev, "quantize_rows: x")
+    if codes is None:
+        codes = torch.empty(M, (K + 15) // 16 * 16, dtype=torch.int8, device=x.device)[:, :K]
+    if scale is None:
+        scale = torch.empty(M, dtype=F32, device=x.device)
+    cp, ldc = _rows_of(codes, torch.int8, (M, K), dev, "quantize_rows: codes")
+    if M == 1:
+        ldc = (K + 7) // 8 * 8                                  # (one row has no next one)
+    check(_lib.load().lia_quantize_rows(xp, _f32(x), max(ldx, K), cp, ldc, _need(scale, F32, (M,), dev, "quantize_rows: scale"), M, K, _stream()), "lia_quantize_rows")
+    count_launches()
+    return codes, scale
+
+
+def linear_int8(x, w, w_scale, out=None, x_scale=None):
+    """``x`` [M, K] @ w^T in 8-bit integers (csrc/int8_gemm_sm100.cu): ``w`` int8 [N, K] with a scale for each output channel (``quantize_rows`` of the weights); ``x`` int8 with ``x_scale`` [M],
+    or bf16 or fp32 rows, which are quantised on the way as ``quantize_rows`` does.  ``out`` [M, N] bf16 or fp32 (by itself of x's type, bf16 for codes) = sum of the codes' products, exact in
+    32 bits, times x_scale[m] times w_scale[n].  Rows of codes lie a multiple of 16 bytes apart; K is 131071 at most.  The same rows give the same bits whatever is beside them."""
+    dev, (M, K), N = _device(x, "linear_int8"), x.shape, w.shape[0]
+    kind = _X_TYPES.get(x.dtype)
+    if kind is None or (x_scale is None) == (kind == _lib.X_INT8):
+        raise _lib.LiaError(f"linear_int8: tokens are bf16 or fp32, or int8 with their scales, not {x.dtype} {'with' if x_scale is not None else 'without'} scales")
+    if out is None:
+        out = torch.empty(M, N, dtype=F32 if x.dtype is F32 else BF16, device=x.device)
+    elif out.dtype not in (BF16, F32):
+        raise _lib.LiaError(f"linear_int8: the output is bf16 or fp32, not {out.dtype}")
+    xp, ldx = _rows_of(x, x.dtype, (M, K), dev, "linear_int8: x")
+    wp, ldw = _rows_of(w, torch.int8, (N, K), dev, "linear_int8: w")
+    whole = (K + 15) // 16 * 16                                 # (one row has no next one)
+    if M == 1:
+        ldx = whole
+    if N == 1:
+        ldw = whole
+    sp, wsp, op = _need(x_scale, F32, (M,), dev, "linear_int8: x_scale") if x_scale is not None else None, _need(w_scale, F32, (N,), dev, "linear_int8: w_scale"), \
+        _need(out, out.dtype, (M, N), dev, "linear_int8: out")
+    lib = _lib.load()
+    size = lib.lia_linear_int8_workspace_bytes(kind, M, N, K)
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    check(lib.lia_linear_int8(xp, kind, ldx, sp, wp, ldw, wsp, op, _f32(out), M, N, K, _p(ws), size, _stream()), "lia_linear_int8")
+    count_launches(1 if kind == _lib.X_INT8 else 2)
+    return out

@@ -12,7 +12,7 @@ shared expert with or without a gate, experts that hand the token back).  Each o
 registers its per-sequence state with a ``seq_state.SlotState`` and runs one step over a batch of portions
 (``StepBatch``) through the kernels of ``ops``.
 
-Projections go through ``Linear``: for bf16 activations the tensor-core GEMM of the OPT path (csrc/gemm_sm100.cu) and, for few rows and small
+Projections go through ``Linear``: with weights of 8 bits csrc/int8_gemm_sm100.cu; for bf16 activations the tensor-core GEMM of the OPT path (csrc/gemm_sm100.cu) and, for few rows and small
 weights, csrc/linear_rows_mma.cu; ``ops.linear_plain`` for fp32 activations and for shapes that these do not take.
 """
 import os
@@ -55,7 +55,7 @@ class StepBatch:
 class Linear:
     """y = x @ W.T for one or several weight matrices stacked by rows (one launch, outputs side by side; each block's
     first column is a multiple of 8 so that every slice stays 16-byte aligned in bf16).  ``pad``: so does the whole output's width, for outputs
-    that are read slice by slice (the last columns are zeros)."""
+    that are read slice by slice (the last columns are zeros).  After ``to_int8`` the weights are codes of 8 bits with a scale for each output channel, and so are the tokens on their way in."""
 
     _gemm_ws = {}
 
@@ -73,6 +73,7 @@ class Linear:
             self.weight[o:o + w.shape[0]] = w
         self._ws_bytes = {}
         self.dtype = dtype
+        self.scale = None                                        # of every output channel, once the weights are codes
         self.tensor_core = (dtype == BF16 and self.K % 8 == 0 and self.N % 8 == 0 and os.environ.get("LIA_PLAIN_LINEAR", "0") == "0")
 
     def _workspace(self, M, device):
@@ -87,11 +88,16 @@ class Linear:
             ws = Linear._gemm_ws[key] = ops.GemmWorkspace(need, device)
         return ws
 
+    def to_int8(self):
+        self.weight, self.scale = ops.quantize_rows(self.weight)
+
     def __call__(self, x, out=None):
         M = x.shape[0]
         if out is None:
             out = torch.empty(M, self.N, dtype=self.dtype, device=x.device)
-        if self.tensor_core and x.is_contiguous() and x.data_ptr() % 16 == 0:
+        if self.scale is not None:
+            ops.linear_int8(x, self.weight, self.scale, out=out)
+        elif self.tensor_core and x.is_contiguous() and x.data_ptr() % 16 == 0:
             ops.linear(x, self.weight, out=out, workspace=self._workspace(M, x.device))
         else:
             ops.linear_plain(x, self.weight, out, resident=True)

@@ -75,3 +75,46 @@ def test_slots_of_4_bit_rows():
     assert codes.shape == (3, 17, 128) and codes.dtype == U8 and scales.shape == (3, 4, 17, 2) and scales.dtype == BF16
     with pytest.raises(ValueError):
         s.add_rows_4bit(4, 48)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"x_type": 3}, "type"), ({"x_type": -1}, "type"), ({"M": -1}, "sizes"), ({"N": 0}, "sizes"), ({"K": 0}, "sizes"), ({"ldx": 99}, "sizes"), ({"ldw": 99}, "sizes"),
+    ({"K": 131072, "ldx": 131072, "ldw": 131072}, "131071"), ({"x": None}, "null"), ({"w": None}, "null"), ({"w_scale": None}, "null"), ({"out": None}, "null"), ({"x_scale": None}, "null"),
+    ({"x_type": 0}, "not codes"), ({"w": 264}, "vectors"), ({"ldw": 120}, "vectors"), ({"x": 264}, "vectors"), ({"ldx": 120}, "vectors"),
+    ({"ws": None, "N": 1 << 20, "K": 4096, "ldx": 4096, "ldw": 4096}, "workspace"), ({"bytes": 8, "N": 1 << 20, "K": 4096, "ldx": 4096, "ldw": 4096}, "workspace"),
+    ({"ws": 264, "N": 1 << 20, "K": 4096, "ldx": 4096, "ldw": 4096}, "workspace"), ({"N": 1 << 30, "K": 4096, "ldx": 4096, "ldw": 4096}, "too large"),
+    ({"M": 1 << 30, "N": 1 << 30}, "too large")])
+def test_products_refuse(lib, change, message):
+    a = dict(x=256, x_type=2, ldx=112, x_scale=256, w=256, ldw=112, w_scale=256, out=256, f32=0, M=4, N=64, K=100, ws=256, bytes=1 << 30) | change
+    rc = lib.load().lia_linear_int8(a["x"], a["x_type"], a["ldx"], a["x_scale"], a["w"], a["ldw"], a["w_scale"], a["out"], a["f32"], a["M"], a["N"], a["K"], a["ws"], a["bytes"], None)
+    assert rc == -1 and message in lib.last_error()
+
+
+def test_products_of_no_tokens_and_their_workspace(lib):
+    L = lib.load()
+    assert L.lia_linear_int8(None, 0, 100, None, 256, 112, 256, None, 0, 0, 64, 100, None, 0, None) == 0
+    assert L.lia_linear_int8_workspace_bytes(0, 0, 64, 100) == L.lia_linear_int8_workspace_bytes(0, 4, 64, 131072) == 0
+    assert L.lia_linear_int8_workspace_bytes(0, 300, 64, 100) >= 300 * (112 + 4) and L.lia_linear_int8_workspace_bytes(2, 300, 64, 100) == 0
+    assert L.lia_quantize_rows(None, 0, 8, None, 8, None, 0, 8, None) == 0
+    for args, message in (((16, 0, 7, 16, 8, 16, 2, 8), "sizes"), ((16, 0, 8, 16, 7, 16, 2, 8), "sizes"), ((None, 0, 8, 16, 8, 16, 2, 8), "null"), ((16, 0, 8, 20, 8, 16, 2, 8), "vectors"),
+                          ((16, 0, 12, 16, 12, 16, 2, 8), "vectors"), ((16, 0, 8, 16, 8, None, 2, 8), "null")):
+        assert L.lia_quantize_rows(*args, None) == -1 and message in lib.last_error()
+
+
+def test_wrappers_of_products_refuse(lib):
+    from lia_b200 import ops
+    z, E = torch.zeros, lib.LiaError
+    with pytest.raises(E):
+        ops.quantize_rows(z(2, 8, dtype=BF16))                                # not on a GPU
+    with pytest.raises(E):
+        ops.linear_int8(z(2, 8, dtype=BF16), z(4, 8, dtype=torch.int8), z(4))
+
+
+def test_models_say_which_weights_they_can_hold(lib, tmp_path):
+    from lia_b200.checkpoint import no_cache_dtype
+    from lia_b200.modeling_bebulorn import BebulornConfig, BebulornForCausalLM
+    with pytest.raises(ValueError, match="weight_dtype"):
+        BebulornForCausalLM(BebulornConfig(), "cpu", BF16, weight_dtype=torch.float8_e4m3fn)
+    for cls in (BebulornForCausalLM, str):
+        with pytest.raises(ValueError, match="weight_dtype"):
+            no_cache_dtype(cls, {"weight_dtype": torch.int8})
