@@ -715,6 +715,25 @@ size_t lia_linear_int8_workspace_bytes(int x_type, int M, int N, int K);
 int lia_linear_int8(const void* x, int x_type, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, void* out, int out_f32, int M, int N, int K,
                     void* ws, size_t ws_bytes, lia_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Rows of caches copied to other slots, and moved inside one.
+ * ---------------------------------------------------------------------------------------------------------------- */
+/* A tensor of per-request state as bytes: those of (slot, position) are `pieces` runs of piece_bytes at data + slot * slot_stride + position * pos_stride + piece * piece_stride.  state: the tensor has no
+ * positions, a slot is piece_bytes (one piece). */
+typedef struct LiaCacheRows {
+  void* data;
+  int64_t slot_stride, pos_stride, piece_stride, piece_bytes;
+  int32_t pieces, state;
+} LiaCacheRows;
+
+/* copies [n][3] on the device: (from, to, count): the first `count` positions of slot `from` (the capacity's at most) go to slot `to`, in all n_tensors tensors (a host array of tensors of `slots` slots
+ * and `capacity` positions); of states all of the slot.  A copy whose slots are not there, or are one, is left out; no slot may be named by two copies as `to`, or by one as `to` and by another as `from`.
+ * max_count: about the largest count (it decides how many blocks share the work, not what is copied). */
+int lia_cache_fork(const LiaCacheRows* tensors, int n_tensors, int slots, int capacity, const int* copies, int n, int max_count, lia_stream_t stream);
+/* segs[i] = (slot, p0, row, n) as lia_tree_attn takes them, kept [nseg][most] on the device: position p0 + i of the slot gets position p0 + kept[i], for i up to the first kept[i] that is not larger than the one
+ * before, or not in 0 .. n - 1 (a shorter list ends with -1).  A portion that its slot cannot hold is left out; no two portions share positions. */
+int lia_cache_compact(const LiaCacheRows* tensors, int n_tensors, int slots, int capacity, const int* segs, int nseg, const int* kept, int most, lia_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,10 @@ class LiaCacheView(ctypes.Structure):
                 ("scale_slot_stride", c_int64), ("scale_head_stride", c_int64), ("slots", c_int32), ("capacity", c_int32), ("type", c_int32), ("dim", c_int32)]
 
 
+class LiaCacheRows(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("slot_stride", c_int64), ("pos_stride", c_int64), ("piece_stride", c_int64), ("piece_bytes", c_int64), ("pieces", c_int32), ("state", c_int32)]
+
+
 class LiaError(RuntimeError):
     pass
 
@@ -251,6 +255,9 @@ _PROTOTYPES = {
     "lia_quantize_rows": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p]),
     "lia_linear_int8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "lia_linear_int8": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    # rows of caches copied to other slots, and moved inside one
+    "lia_cache_fork": (c_int, [POINTER(LiaCacheRows), c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p]),
+    "lia_cache_compact": (c_int, [POINTER(LiaCacheRows), c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p]),
 }
 
 EXPORTS = tuple(_PROTOTYPES)

@@ -6,7 +6,8 @@ a portion of one, or a single decoded token) and the places among them whose log
 request a slot of the model's per-sequence state (seq_state.SlotState), lays the entries' tokens out as the rows of one
 batch, cuts what exceeds the row budget into further passes, runs the model's ``forward_rows`` and frees the slots of the
 requests named in ``end``.  ``Engine.generate`` is greedy decoding on top of it (argmax on the device), ``Engine.score`` says how
-likely given texts are (log probabilities, entropies and alternatives on the device); the trace runner (bin/trace_run) drives the same ``step``.
+likely given texts are (log probabilities, entropies and alternatives on the device), ``Engine.score_choices`` the same of several answers to one
+prompt, which ``Engine.fork`` hands on to each; the trace runner (bin/trace_run) drives the same ``step``.
 
 A pass in which every request brings ONE token (a decode step) is launch-bound when run eagerly -- some sixty kernels of
 a few microseconds each -- so it is captured as a CUDA graph the second time its shape comes up and replayed from then
@@ -24,6 +25,7 @@ import torch
 
 from . import _lib, graphs, ops
 from .seq_layers import StepBatch
+from .seq_state import SlotError
 
 
 class _StepGraph:
@@ -219,6 +221,48 @@ class Engine:
                 out[i].append(tok)
         for i in ids:
             self.slots.free(i)
+        return out
+
+    def fork(self, req_id, new_ids):
+        """Requests ``new_ids`` go on from where ``req_id`` stands, which goes on too: several answers to one prompt, of which the prompt is processed once."""
+        self.slots.fork(req_id, new_ids)
+
+    def score_choices(self, prompt, choices, top=0):
+        """How likely each of ``choices`` (lists of ids) is behind ``prompt`` (ids): the prompt is processed once and forked to every choice, as many at a time as there are free slots.  Returns a dict
+        per choice as ``score`` does, over all tokens of the choice."""
+        prompt, choices = [int(t) for t in prompt], [[int(t) for t in c] for c in choices]
+        if not prompt or any(not c for c in choices):
+            raise ValueError("a prompt and its choices have at least one token")
+        root, out, at = ("choices", "prompt"), [], 0
+        try:
+            room = self.slots.owner.count(None) - (len(prompt) > 1)
+            if choices and room < 1:
+                raise SlotError("no slots are free for the choices of a prompt")
+            if len(prompt) > 1 and choices:
+                self.step([{"id": root, "tokens": prompt[:-1]}])
+            while at < len(choices):
+                group = choices[at:at + room]
+                keys = [("choices", at + i) for i in range(len(group))]
+                try:
+                    if len(prompt) > 1:
+                        self.fork(root, keys)
+                    logits = self.step([{"id": k, "tokens": prompt[-1:] + c[:-1], "want": list(range(len(c)))} for k, c in zip(keys, group)])
+                    given = [t for c in group for t in c]
+                    logp, entropy, best, ids = (t.tolist() for t in ops.token_logprobs(logits, torch.tensor(given, dtype=torch.int64, device=self.device), top=top))
+                    self.check()
+                finally:
+                    for k in keys:
+                        if self.slots.slot_of(k) is not None:
+                            self.slots.free(k)
+                row = 0
+                for c in group:
+                    rows = range(row, row + len(c))
+                    out.append({"logp": [logp[r] for r in rows], "entropy": [entropy[r] for r in rows], "alternatives": [list(zip(ids[r], best[r])) for r in rows]})
+                    row += len(c)
+                at += len(group)
+        finally:
+            if self.slots.slot_of(root) is not None:
+                self.slots.free(root)
         return out
 
     def score(self, prompts, top=0, chunk=None):

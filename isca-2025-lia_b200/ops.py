@@ -1623,3 +1623,59 @@ def linear_int8(x, w, w_scale, out=None, x_scale=None):
     check(lib.lia_linear_int8(xp, kind, ldx, sp, wp, ldw, wsp, op, _f32(out), M, N, K, _p(ws), size, _stream()), "lia_linear_int8")
     count_launches(1 if kind == _lib.X_INT8 else 2)
     return out
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# Rows of caches copied to other slots, and moved inside one.
+# ------------------------------------------------------------------------------------------------------------------
+class CacheSet:
+    """The tensors of per-request state that ``fork`` and ``compact`` work on together (csrc/cache_move.cu): ``rows`` of shape [slots, capacity, ...], of any types and strides as long as what
+    follows the positions is whole runs of bytes at equal distances (scales [slots, heads, capacity] are given as ``.transpose(1, 2)``), and ``states`` [slots, ...], contiguous inside a slot.
+    All have the same slots, all rows the same capacity.  The tensors are held, not copied."""
+
+    def __init__(self, rows, states=()):
+        self.tensors = [*rows, *states]
+        if not self.tensors:
+            raise _lib.LiaError("CacheSet: no tensors")
+        self.slots, self.capacity, self.states = self.tensors[0].shape[0], rows[0].shape[1] if len(rows) else 1, len(states)
+        self.device = self.tensors[0].device
+        self._rows = (_lib.LiaCacheRows * len(self.tensors))(*[self._of(t, False) for t in rows], *[self._of(t, True) for t in states])
+
+    def _of(self, t, state):
+        if t.device != self.device or t.dim() < 1 + (not state) or t.shape[0] != self.slots or (not state and t.shape[1] != self.capacity) or t.numel() == 0:
+            raise _lib.LiaError(f"CacheSet: need tensors [{self.slots}, {'' if state else f'{self.capacity}, '}...] with something in them on {self.device}, got {list(t.shape)} on {t.device}")
+        size, strides = t.element_size(), t.stride()
+        piece, pieces, apart = size, 1, 0
+        for n, s in reversed(list(zip(t.shape[2 - state:], strides[2 - state:]))):           # what lies side by side is one run; outer dimensions at equal distances are pieces
+            if n == 1:
+                continue
+            if pieces == 1 and s * size == piece:
+                piece *= n
+            elif pieces == 1:
+                pieces, apart = n, s * size
+            elif s * size == apart * pieces:
+                pieces *= n
+            else:
+                raise _lib.LiaError(f"CacheSet: a row of strides {strides} is not runs of bytes at equal distances")
+        if (self.slots > 1 and strides[0] == 0) or (not state and self.capacity > 1 and strides[1] == 0) or (pieces > 1 and apart < piece) or (state and pieces > 1):
+            raise _lib.LiaError(f"CacheSet: rows that share their place, or a state that is not contiguous: strides {strides}")
+        pos = 0 if state else strides[1] * size if self.capacity > 1 else piece
+        return _lib.LiaCacheRows(t.data_ptr(), strides[0] * size, pos, apart, piece, pieces, int(state))
+
+    def fork(self, copies, max_count=0):
+        """``copies`` int32 [n, 3] on the device, (from, to, count) each: the first ``count`` positions of slot ``from`` go to slot ``to`` in every tensor, and the whole of its states.  Copies
+        whose slots are not there are left out; a slot is the target of one copy, and then the source of none.  ``max_count``: about the largest count."""
+        dev, n = _device(self.tensors[0], "CacheSet.fork"), copies.shape[0]
+        check(_lib.load().lia_cache_fork(self._rows, len(self._rows), self.slots, self.capacity, _need(copies, I32, (n, 3), dev, "CacheSet.fork: copies"), n, int(max_count) or self.capacity, _stream()),
+              "lia_cache_fork")
+        count_launches(-(-len(self._rows) // 64) if n else 0)
+
+    def compact(self, segs, kept):
+        """``segs`` int32 [nseg, 4] as ``tree_attn`` takes them, ``kept`` int32 [nseg, most], both on the device: of the portion's tokens those that stay, ascending, -1 behind the last: token
+        kept[i], at position p0 + kept[i] of its slot, moves to position p0 + i.  States have no positions and are not allowed here."""
+        if self.states:
+            raise _lib.LiaError("CacheSet.compact: a state has no positions: make a set of the rows alone")
+        dev, (nseg, most) = _device(self.tensors[0], "CacheSet.compact"), kept.shape
+        check(_lib.load().lia_cache_compact(self._rows, len(self._rows), self.slots, self.capacity, _need(segs, I32, (nseg, 4), dev, "CacheSet.compact: segs"), nseg,
+                                            _need(kept, I32, (nseg, most), dev, "CacheSet.compact: kept"), most, _stream()), "lia_cache_compact")
+        count_launches(-(-len(self._rows) // 64) if nseg and most else 0)

@@ -118,3 +118,98 @@ def test_models_say_which_weights_they_can_hold(lib, tmp_path):
     for cls in (BebulornForCausalLM, str):
         with pytest.raises(ValueError, match="weight_dtype"):
             no_cache_dtype(cls, {"weight_dtype": torch.int8})
+
+
+def test_forks_of_host_resident_state():
+    from lia_b200.seq_state import SlotError, SlotState
+    s = SlotState(4, 9, "cpu")
+    r, (c, a) = s.add_recurrent((2, 3)), s.add_rows_8bit(2, 16, torch.int8)
+    rows, (c4, a4) = s.add_rows(5, F32), s.add_rows_4bit(3, 32)
+    assert s.alloc("x") == 0 and s.alloc("y") == 1 and s.reserve(1, 4) == 0
+    for t in (r, c, a, rows, c4, a4):
+        t[1] = torch.randint(1, 9, t.shape[1:], generator=torch.Generator().manual_seed(1)).to(t.dtype)
+    s.free("x")
+    assert s.fork("y", ["p", "q"]) == [0, 2] and s.length == [4, 4, 4, 0] and s.slot_of("q") == 2
+    for t, axis in ((c, 0), (a, 1), (rows, 0), (c4, 0), (a4, 1)):
+        for to in (0, 2):
+            assert torch.equal(t[to].narrow(axis, 0, 4), t[1].narrow(axis, 0, 4)) and (t[to].narrow(axis, 4, 5) == 0).all()
+    assert torch.equal(r[0], r[1]) and torch.equal(r[2], r[1]) and (r[3] == 0).all()
+    for who, ids in (("z", ["u"]), ("y", ["p"]), ("y", ["u", "u"]), ("y", ["u", "v"])):
+        with pytest.raises(SlotError):
+            s.fork(who, ids)
+    assert s.owner == ["p", "y", "q", None] and s.length == [4, 4, 4, 0]                # nothing of them was done
+    assert s.reserve(2, 5) == 4 and s.fork("q", ["w"]) == [3] and s.length == [4, 4, 9, 9]
+
+
+def rows(_lib, **change):
+    return (_lib.LiaCacheRows * 1)(_lib.LiaCacheRows(**(dict(data=1 << 20, slot_stride=4096, pos_stride=64, piece_stride=0, piece_bytes=64, pieces=1, state=0) | change)))
+
+
+@pytest.mark.parametrize("change,message", [({"data": None}, "null"), ({"pieces": 0}, "bytes"), ({"piece_bytes": 0}, "bytes"), ({"piece_bytes": 1 << 31}, "bytes"), ({"slot_stride": -64}, "share"),
+                                            ({"slot_stride": 0}, "share"), ({"pos_stride": 0}, "share"), ({"state": 1, "pieces": 2}, "pieces")])
+def test_moves_refuse_tensors(lib, change, message):
+    L = lib.load()
+    assert L.lia_cache_fork(rows(lib, **change), 1, 4, 64, 16, 1, 1, None) == -1 and message in lib.last_error()
+    assert L.lia_cache_compact(rows(lib, **change), 1, 4, 64, 16, 1, 16, 1, None) == -1 and message in lib.last_error()
+
+
+def test_moves_refuse_sizes_and_null_pointers(lib):
+    L, r = lib.load(), rows(lib)
+    for args in ((r, -1, 4, 64, 16, 1, 1), (r, 1, 0, 64, 16, 1, 1), (r, 1, 4, 0, 16, 1, 1), (r, 1, 4, 64, 16, -1, 1), (None, 1, 4, 64, 16, 1, 1), (r, 1, 4, 64, None, 1, 1)):
+        assert L.lia_cache_fork(*args, None) == -1
+    for args in ((r, -1, 4, 64, 16, 1, 16, 1), (r, 1, 4, 64, 16, -1, 16, 1), (r, 1, 4, 64, 16, 1, 16, -1), (r, 1, 4, 64, None, 1, 16, 1), (r, 1, 4, 64, 16, 1, None, 1), (r, 1, 4, 64, 16, 70000, 16, 1)):
+        assert L.lia_cache_compact(*args, None) == -1
+    assert L.lia_cache_compact(rows(lib, state=1), 1, 4, 64, 16, 1, 16, 1, None) == -1 and "state" in lib.last_error()
+    assert L.lia_cache_fork(None, 0, 4, 64, None, 0, 0, None) == L.lia_cache_compact(None, 0, 4, 64, None, 0, None, 0, None) == 0
+
+
+def test_choices_are_put_together(lib, monkeypatch):
+    """Engine.score_choices' bookkeeping on a stand-in for a model whose distribution after a token depends on all tokens before it: what a fork carries on is a recurrent sum."""
+    from lia_b200 import ops
+    from lia_b200.engine import Engine
+    from lia_b200.seq_state import SlotState
+
+    class Model:
+        device = torch.device("cpu")
+        config = type("C", (), {"vocab": 11})
+        steps = 0
+
+        def new_state(self, n, cap):
+            s = SlotState(n, cap, "cpu")
+            s.sums = s.add_recurrent(())
+            return s
+
+        def forward_rows(self, ids, batch, want, slots, trace=None):
+            self.steps += len(ids)
+            out = []
+            for t, (slot, _) in zip(ids.tolist(), batch.meta.tolist()):
+                slots.sums[slot] = slots.sums[slot] * 0.5 + t
+                out.append(self.logits(slots.sums[slot]))
+            return None if want is None else torch.stack(out)[want.long()]
+
+        def logits(self, x):
+            return torch.sin(torch.arange(11.0) * (x + 2))
+
+    def plain(logits, given, top=0):
+        logp = torch.log_softmax(logits, -1)
+        best, ids = logp.sort(dim=-1, descending=True, stable=True)
+        return logp.gather(1, given.view(-1, 1))[:, 0], -(logp.exp() * logp).sum(-1), best[:, :top], ids[:, :top]
+    monkeypatch.setattr(ops, "token_logprobs", plain)
+    choices = [[1, 2, 3], [9], [3, 3], [4, 5, 6, 7]]
+    for prompt in ([8, 1, 5, 2], [6]):
+        for requests in (1, 2, 3, 9) if len(prompt) == 1 else (2, 3, 9):
+            m = Model()
+            e = Engine(m, 16, max_requests=requests)
+            got = e.score_choices(prompt, choices, top=2)
+            assert e.slots.live_tokens == 0 and m.steps == len(prompt) - 1 + sum(len(c) for c in choices)      # the prompt once
+            for c, g in zip(choices, got):
+                x = torch.zeros(())
+                logps = []
+                for t in prompt + c[:-1]:
+                    x = x * 0.5 + t
+                    logps.append(torch.log_softmax(m.logits(x), -1))
+                want = [float(w[t]) for w, t in zip(logps[-len(c):], c)]
+                assert g["logp"] == pytest.approx(want) and all(len(a) == 2 for a in g["alternatives"])
+    from lia_b200.seq_state import SlotError
+    with pytest.raises(SlotError):
+        Engine(Model(), 16, max_requests=1).score_choices([8, 1], choices)

@@ -8,6 +8,7 @@ import torch
 
 from cache4 import numbers, packed
 from test_gpu_tree_attn import DIMS, Case, family, rnd
+from test_gpu_wait_limits import given_up, nowait  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 BF16, F32, F64, U8 = torch.bfloat16, torch.float32, torch.float64, torch.uint8
@@ -299,3 +300,16 @@ def test_outputs_on_8_byte_boundaries(ops, dim, vdim, n, past, max_ctx):
     out = buffer[4:4 + want.numel()].view(want.shape)
     assert torch.equal(c.run(ops, max_ctx=max_ctx, out=out), want)
     assert (buffer[:4] == 77).all() and (buffer[-4:] == 77).all()
+
+
+@pytest.mark.parametrize("H", [4, 8])
+@pytest.mark.parametrize("max_ctx", [364, 100000])
+def test_waits_that_run_out(nowait, monkeypatch, ops, H, max_ctx):  # noqa: F811
+    """With a limit of 0 every wait gives up: launches end and are counted, and rows, formed key by key, are right all the same."""
+    sizes = (64, 40, 33)
+    c = Case4([(0, 300, sizes[0]), (1, 70, sizes[1]), (2, 5, sizes[2])], H, 2, 128, 64, mask=[family(n, lambda i: (i - 1) // 2 if i else -1) for n in sizes], gap=1)
+    again = torch.full_like(c.out, 77.0)
+    assert given_up(nowait, monkeypatch, lambda: c.run(ops, out=again, max_ctx=max_ctx)) >= 3 * 2
+    torch.cuda.synchronize()
+    c.check(again)
+    c.check(c.run(ops, max_ctx=max_ctx))
