@@ -67,7 +67,7 @@ inline cudaError_t lia_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
 }
 // With clusters of `cluster` blocks along x (up to 8), which see one another's shared memory
 template <typename... KArgs, typename... Args>
-inline cudaError_t lia_launch_cluster(int cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+inline cudaError_t lia_launch_cluster_as(bool early, int cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                                       Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
@@ -81,8 +81,13 @@ inline cudaError_t lia_launch_cluster(int cluster, void (*kernel)(KArgs...), dim
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = lia_pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = early && lia_pdl_enabled() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t lia_launch_cluster(int cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                      Args&&... args) {
+  return lia_launch_cluster_as(true, cluster, kernel, grid, block, smem, stream, std::forward<Args>(args)...);
 }
 // Without that: for kernels of long-running blocks that fill the GPU once.  Placed while the previous kernel drains, their blocks crowd the SMs
 // that empty first (state-space scan of 2048 tokens: the mixer 495 us instead of 414).
@@ -168,6 +173,11 @@ __device__ __forceinline__ uint32_t cluster_place(const void* addr, uint32_t ran
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(addr)), "r"(rank));
   return r;
+}
+__device__ __forceinline__ uint32_t cluster_ld_u32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
 }
 __device__ __forceinline__ uint64_t cluster_ld64(uint32_t at) {
   uint64_t v;

@@ -4,13 +4,12 @@
 //   sums     whole numbers of 32 bits, exact for up to 131071 products: whatever order they are added in, the bits are the same
 //
 // tcgen05.mma.kind::i8, both operands K-major from shared memory (TMA, 128-byte swizzle: 128 codes a row), sums in TMEM.  Two forms:
-//   FEW    (up to 128 tokens; bound by the weights' bytes)  the weights' rows are the product's 128 rows, the tokens its 16 to 128 columns.  The list of (row tile, block of K) is cut into as many
-//          spans of equal length as there are CTAs, so that every SM streams the same number of bytes.  A tile that several spans share is finished by whichever of them arrives last: the others leave
-//          their sums in a workspace and count themselves, nobody waits, so that launches on several streams cannot hold one another up.  Weights are on their way while the
-//          tokens are quantised.
+//   FEW    (up to 128 tokens; bound by the weights' bytes)  the weights' rows are the product's 128 rows, the tokens its 16 to 128 columns.  A CTA has a tile of 128 channels, or `parts` CTAs that are a
+//          cluster share one along K and add up each other's sums by way of shared memory.  Two CTAs fit an SM, so that one's beginning and end lie under the other's loads, and memory shares itself out
+//          among as many tiles as there are.  Weights are on their way while the tokens are quantised.
 //   MANY   (bound by the tensor cores)  the tokens' rows are the product's rows: CTA pairs on 256 x 256 tiles (cta_group::2), or one CTA on 128 x 256, 128 or 64 where those would leave SMs idle.
 //
-// Every wait is bounded; a CTA that gives one up makes its outputs NaN (a shared tile's by way of its count) and counts itself in lia_moe_timeouts_seen().
+// Every wait is bounded; a CTA that gives one up makes its tile's outputs NaN and counts itself in lia_moe_timeouts_seen().
 #include <cuda.h>
 
 #include <mutex>
@@ -25,7 +24,6 @@ namespace {
 
 constexpr int TILE = 128, KB = 128;                                // rows of a tile, codes (bytes) of a block of K
 constexpr int MOST_K = 131071;                                     // 127 * 127 * K stays below 2^31 (and 128 * 128 * K)
-constexpr int MOST_PIECES = 1 << 16;                               // what a CTA that gave up adds to a tile's count
 
 // ------------------------------------------------------------------ tokens' codes
 struct QuantArgs {
@@ -33,19 +31,17 @@ struct QuantArgs {
   long long ldx, ldc;
   int8_t* codes;
   float* scale;
-  int* counts;                                                     // made zero for the product behind
-  int K, n_counts, vec;
+  int K, vec;
 };
-constexpr int Q_THREADS = 256, Q_HELD = 4;                         // vectors of eight numbers that a thread holds: rows of 8192 numbers are read once
+constexpr int Q_HELD = 4;                                          // vectors of eight numbers that a thread holds: rows of 8192 numbers, or 32768, are read once
 
-template <typename T> __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_constant__ QuantArgs a) {
+template <typename T, int Q_THREADS> __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_constant__ QuantArgs a) {
   // In this order: the product behind asks for its weights before it waits, and may not begin before what came before this kernel (the weights' own quantisation, perhaps) has ended
   pdl_wait();
   pdl_launch_dependents();
   __shared__ uint32_t part[Q_THREADS / 32];
   const int t = threadIdx.x, vecs = (a.K + 7) / 8;
   const T* src = reinterpret_cast<const T*>(a.x) + (long long)blockIdx.x * a.ldx;
-  for (int i = blockIdx.x * Q_THREADS + t; i < a.n_counts; i += gridDim.x * Q_THREADS) a.counts[i] = 0;
   auto load = [&](int v) {                                         // numbers behind the row's end are zeros
     if (v >= vecs) return Raw8<T>{};
     if (v * 8 + 8 <= a.K) return load8(src + v * 8, a.vec);
@@ -94,10 +90,9 @@ struct Args {
   const float* sx;
   const float* sw;
   void* out;
-  int* pieces;                                                     // FEW: sums of parts of tiles [2 * CTAs][tokens][TILE]
-  int* counts;                                                     // FEW: of a tile's parts that have been left
   int* timeouts;
   int M, N, k_blocks, tiles_a, tiles_b, wide;                      // wide: rows of out are whole 16-byte vectors apart
+  int parts;                                                       // FEW: CTAs that share a tile
 };
 
 // kind::i8: sums of 32-bit integers, both operands signed and K-major
@@ -116,24 +111,24 @@ __device__ __forceinline__ void mma_i8_pair_if(uint32_t one, uint32_t d, uint64_
 template <bool FEW, int BN, bool PAIR> struct Shape {
   static constexpr int A_BYTES = TILE * KB, B_BYTES = (PAIR ? BN / 2 : BN) * KB, STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGING = FEW ? 0 : 4 * 4096;               // 32 rows of 128 bytes for each epilogue warp
-  static constexpr int ROOM = (229376 - STAGING) / STAGE, STAGES = ROOM > 10 ? 10 : ROOM;
+  static constexpr int STAGES = ((FEW ? 112640 : 228352) - STAGING) / STAGE > 8 ? 8 : ((FEW ? 112640 : 228352) - STAGING) / STAGE;    // (of FEW's, two blocks fit an SM)
   static constexpr int BARS = STAGES * STAGE + STAGING;
-  static constexpr int SMEM = BARS + (2 * STAGES + 5) * 8 + 32 + 1024;
-  static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;           // of TMEM: two tiles' sums
+  static constexpr int SCALES = (BARS + (2 * STAGES + 5) * 8 + 8 + 15) / 16 * 16, SMEM = SCALES + (FEW ? BN : 2 * BN) * 4 + 1024;   // of the tokens, or of two tiles' channels
+  static constexpr int COLS = FEW ? (BN < 32 ? 32 : BN) : 2 * BN;   // of TMEM: a tile's sums, or two tiles'
 };
 
 struct Work {
   int ta, tb, kb0, kb1;
 };
-// FEW: the CTA's span of the flat list of (tile, block of K).  MANY: tile u = worker + i * workers, in groups of some rows of tiles, so that what runs at the same time shares operands in L2.
+// FEW: one tile, or part of one.  MANY: tile u = worker + i * workers, in groups of some rows of tiles, so that what runs at the same time shares operands in L2.
 template <bool FEW> struct Sched {
   int k_blocks, tiles_a, tiles_b, group;
   unsigned pos, end, step;
   __device__ __forceinline__ Sched(const Args& p, bool pair) : k_blocks(p.k_blocks), tiles_a(p.tiles_a), tiles_b(p.tiles_b), group(pair ? 8 : 16) {
     if (FEW) {
-      const unsigned total = (unsigned)tiles_a * (unsigned)k_blocks;                           // (times the CTAs below 2^31: checked on the host)
-      pos = total * blockIdx.x / gridDim.x;
-      end = total * (blockIdx.x + 1) / gridDim.x;
+      const unsigned tile = blockIdx.x / (unsigned)p.parts, part = blockIdx.x - tile * (unsigned)p.parts;
+      pos = tile * (unsigned)k_blocks + (unsigned)k_blocks * part / (unsigned)p.parts;         // (k_blocks is 1024 at most, and parts 8)
+      end = tile * (unsigned)k_blocks + (unsigned)k_blocks * (part + 1) / (unsigned)p.parts;
       step = 0;
     } else {
       pos = pair ? blockIdx.x >> 1 : blockIdx.x;
@@ -167,7 +162,7 @@ template <bool OUT32> __device__ __forceinline__ void put_one(void* out, size_t 
 }
 
 template <bool FEW, int BN, bool PAIR, bool OUT32>
-__global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(256, FEW ? 2 : 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Args p) {
   static_assert(!PAIR || (!FEW && BN == 256), "CTA pairs: 256 x 256 tiles");
   using L = Shape<FEW, BN, PAIR>;
   constexpr int STAGES = L::STAGES;
@@ -183,7 +178,6 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant
   const uint32_t drain = bars + 8u * (2 * STAGES + 4);
   volatile uint32_t* tmem_at = reinterpret_cast<volatile uint32_t*>(smem_gen + L::BARS + (2 * STAGES + 5) * 8);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_at + 1);
-  volatile int* arrived = reinterpret_cast<volatile int*>(tmem_at + 2);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -312,12 +306,22 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant
     // ================================================================ sums to outputs
     const int ew = warp - 4;                                       // TMEM lanes 32 ew .. 32 ew + 31
     pdl_wait();
+    float* scales_s = reinterpret_cast<float*>(smem_gen + L::SCALES);                          // (read one by one between the outputs' stores they cost an L2 round trip each: 128 tokens 30 us)
+    if (FEW) {
+      const int i = ew * 32 + lane;
+      if (i < BN) scales_s[i] = i < p.M ? __ldcg(p.sx + i) : 0.f;
+      epi_bar_sync();
+    }
     Sched<FEW> s(p, PAIR);
     Work w;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool alive = true;
     while (s.next(w)) {
+      if (!FEW) {                                                  // the channels' scales, while the sums are on their way; zeros behind the last (the buffer before the last tile's has been read)
+        for (int i = ew * 32 + lane; i < BN; i += 128) scales_s[acc * BN + i] = w.tb * BN + i < p.N ? __ldg(p.sw + w.tb * BN + i) : 0.f;
+        epi_bar_sync();
+      }
       alive = __all_sync(0xffffffffu, alive && wait_for(tfull(acc), acc_phase, dead));
       tcgen05_fence_after();
       const uint32_t taddr = tmem + (uint32_t)(acc * BN) + ((uint32_t)(ew * 32) << 16);
@@ -330,65 +334,21 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant
         }
       };
       if constexpr (FEW) {
-        // a lane has one channel, its columns are the tokens
-        const int nl = ew * 32 + lane, n = w.ta * TILE + nl;
-        const bool there = n < p.N;
+        // a lane has one channel, its columns are the tokens: to shared memory where the operands were, [tokens][TILE]
+        int* sums = reinterpret_cast<int*>(smem_gen) + ew * 32 + lane;
         constexpr int CH = BN < 32 ? BN : 32;
-        bool whole = w.kb0 == 0 && w.kb1 == p.k_blocks, good = alive;
-        int c0 = (int)blockIdx.x, c1 = c0;                         // the CTAs that share the tile
-        if (!whole) {
-          const unsigned total = (unsigned)p.tiles_a * (unsigned)p.k_blocks, first = (unsigned)w.ta * (unsigned)p.k_blocks, last = first + (unsigned)p.k_blocks - 1u;
-          c0 = (int)(((first + 1u) * gridDim.x - 1u) / total);     // span c begins at total * c / CTAs, rounded down
-          c1 = (int)(((last + 1u) * gridDim.x - 1u) / total);
-          int* mine = p.pieces + ((size_t)blockIdx.x * 2 + (w.kb0 == 0)) * p.M * TILE + nl;
-          if (alive) {
+        if (alive) {
 #pragma unroll 1
-            for (int c = 0; c < BN && c < p.M; c += CH) {
-              uint32_t v[CH];
-              if constexpr (CH == 32) tmem_ld32(taddr + c, v);
-              else tmem_ld16(taddr + c, v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < CH; ++j)
-                if (c + j < p.M) __stcg(mine + (size_t)(c + j) * TILE, (int)v[j]);
-            }
-          }
-          __threadfence();
-          epi_bar_sync();
-          if (ew == 0 && lane == 0) *arrived = atomicAdd(p.counts + w.ta, *dead ? 1 + MOST_PIECES : 1);
-          epi_bar_sync();
-          const int before = *arrived;
-          epi_bar_sync();                                          // (read by all before it is written again)
-          if ((before & (MOST_PIECES - 1)) != c1 - c0) {           // not the last one
-            if (alive) give_back();
-            acc ^= 1;
-            if (acc == 0) acc_phase ^= 1u;
-            continue;
-          }
-          __threadfence();
-          good = alive && before < MOST_PIECES;
-        }
-        const float sw = there ? __ldg(p.sw + n) : 0.f;
-#pragma unroll 1
-        for (int c = 0; c < BN && c < p.M; c += CH) {
-          uint32_t v[CH];
-          if (good) {
+          for (int c = 0; c < BN && c < p.M; c += CH) {
+            uint32_t v[CH];
             if constexpr (CH == 32) tmem_ld32(taddr + c, v);
             else tmem_ld16(taddr + c, v);
             tmem_ld_wait();
-            for (int o = c0; o <= c1; ++o) {
-              if (o == (int)blockIdx.x) continue;
-              const int* piece = p.pieces + ((size_t)o * 2 + (o == c0)) * p.M * TILE + nl;
 #pragma unroll
-              for (int j = 0; j < CH; ++j)
-                if (c + j < p.M) v[j] += (uint32_t)__ldcg(piece + (size_t)(c + j) * TILE);
-            }
+            for (int j = 0; j < CH; ++j)
+              if (c + j < p.M) sums[(c + j) * TILE] = (int)v[j];
           }
-#pragma unroll
-          for (int j = 0; j < CH; ++j)
-            if (there && c + j < p.M) put_one<OUT32>(p.out, (size_t)(c + j) * p.N + n, good ? (float)(int)v[j] * __ldcg(p.sx + c + j) * sw : NAN);
         }
-        if (alive) give_back();
       } else {
         // a lane has one token, its columns are channels: through shared memory to whole rows
         const int row0 = (w.ta * (PAIR ? 2 : 1) + (int)rank) * TILE + ew * 32, m = row0 + lane;
@@ -405,9 +365,15 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant
               tmem_ld32(taddr + c0 + half * 32, v);
               tmem_ld_wait();
             }
-            const int n0 = w.tb * BN + c0 + half * 32;
+            const float4* sw = reinterpret_cast<const float4*>(scales_s + acc * BN + c0 + half * 32);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = alive ? (float)(int)v[j] * sx * (n0 + j < p.N ? __ldg(p.sw + n0 + j) : 0.f) : NAN;
+            for (int j = 0; j < 32; j += 4) {
+              const float4 w4 = sw[j / 4];
+              f[j] = alive ? (float)(int)v[j] * sx * w4.x : NAN;
+              f[j + 1] = alive ? (float)(int)v[j + 1] * sx * w4.y : NAN;
+              f[j + 2] = alive ? (float)(int)v[j + 2] * sx * w4.z : NAN;
+              f[j + 3] = alive ? (float)(int)v[j + 3] * sx * w4.w : NAN;
+            }
 #pragma unroll
             for (int j = 0; j < 32 / PER; ++j) {                   // each row's chunks turned by the row, so that neither side of the transposition collides
               const int chunk = half * 4 + j;
@@ -449,6 +415,37 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant
 
   tcgen05_fence_before();
   __syncthreads();
+  if (FEW) {
+    // ================================================================ a cluster's parts of a tile: each CTA adds up and writes some of the outputs, four channels a thread at a time
+    pdl_wait();
+    if (p.parts > 1) cluster_barrier();
+    const int rank4 = (int)(blockIdx.x % (unsigned)p.parts), first = (p.M * (TILE / 4) * rank4 / p.parts), last = (p.M * (TILE / 4) * (rank4 + 1) / p.parts), n0 = (int)(blockIdx.x / (unsigned)p.parts) * TILE;
+    const float* sx_s = reinterpret_cast<const float*>(smem_gen + L::SCALES);
+    bool bad = false;
+    for (int o = 0; o < p.parts; ++o) bad |= cluster_ld_u32(cluster_place(const_cast<const int*>(dead), o)) != 0u;
+    for (int i = first + (int)threadIdx.x; i < last; i += 256) {
+      const int m = i / (TILE / 4), n = n0 + i % (TILE / 4) * 4;
+      int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+      for (int o = 0; o < p.parts; ++o) {
+        const float4 f = cluster_ld_f4(cluster_place(smem_gen + (size_t)i * 16, o));
+        sum.x += __float_as_int(f.x), sum.y += __float_as_int(f.y), sum.z += __float_as_int(f.z), sum.w += __float_as_int(f.w);
+      }
+      const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = bad ? NAN : n + j < p.N ? (float)v[j] * sx_s[m] * __ldg(p.sw + n + j) : 0.f;
+      const size_t at = (size_t)m * p.N + n;
+      if (p.wide && n + 4 <= p.N) {
+        if constexpr (OUT32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+        else *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(p.out) + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) put_one<OUT32>(p.out, at + j, y[j]);
+      }
+    }
+  }
   if (*dead) {                                                     // loads and products in flight end before shared memory and TMEM are given back
     if (threadIdx.x == 0) {
       atomicAdd_system(p.timeouts, 1);
@@ -468,7 +465,7 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_kernel(const __grid_constant
     }
     __syncthreads();
   }
-  if (PAIR) cluster_sync_all();                                    // nobody leaves while the other may arrive on its barriers
+  if (PAIR || (FEW && p.parts > 1)) cluster_barrier();             // nobody leaves while others may arrive on its barriers, or read its sums
   if (warp == 2) {
     tcgen05_fence_after();
     if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
@@ -493,8 +490,8 @@ int make_tmap(CUtensorMap* map, const void* base, int rows, int K, long long ld,
 }
 
 struct Plan {
-  bool few, pair, split;                                           // split: tiles that several CTAs share
-  int bn, grid, tiles_a, tiles_b, k_blocks;
+  bool few, pair;
+  int bn, grid, tiles_a, tiles_b, k_blocks, parts;                 // parts: CTAs of a cluster that share a tile
 };
 Plan plan_of(int M, int N, int K) {
   Plan p{};
@@ -506,10 +503,14 @@ Plan plan_of(int M, int N, int K) {
     p.tiles_a = (N + TILE - 1) / TILE;
     p.tiles_b = 1;
     const long long total = (long long)p.tiles_a * p.k_blocks;
-    long long g = total / 4;                                       // spans of four blocks of K at least
-    g = g < 1 ? 1 : g > sms ? sms : g;
-    p.grid = (int)g;
-    p.split = total % g != 0 || total / g % p.k_blocks != 0;
+    // Sharing a tile costs a cluster's meeting, 1 to 2 us, and pays as long as the CTAs fit two an SM; eight of them only where the tiles are few and long.  us with 1 | 2 | 4 | 8 parts, 64 tokens:
+    // 1024 x 1024 9.0 | 8.2 | 7.4 | 7.2; 2560 x 2560 12.1 | 10.2 | 8.8 | 9.6; 1024 x 8192 22.5 | 15.6 | 11.5 | 10.7; 7168 x 7168 24.2 | 19.1 | 17.0 | 23.6; 12288 x 4096 19.3 | 18.0 | 21.4;
+    // 28672 x 7168 41.4 | 46.5.  (As spans of equal length over one CTA an SM, whose shared tiles met by way of global memory, 2560 x 2560 took 18, 28672 x 7168 49.)
+    p.parts = 1;
+    if (p.k_blocks >= 40 && p.tiles_a * 8 <= sms * 11 / 10) p.parts = 8;
+    else if (p.k_blocks >= 4 && p.tiles_a * 4 <= sms * 8 / 5) p.parts = 4;
+    else if (p.k_blocks >= 4 && p.tiles_a * 2 <= sms * 8 / 5) p.parts = 2;
+    p.grid = p.tiles_a * p.parts;
     return p;
   }
   auto tiles = [&](int rows, int cols) { return (long long)((M + rows - 1) / rows) * ((N + cols - 1) / cols); };
@@ -521,10 +522,12 @@ Plan plan_of(int M, int N, int K) {
     p.bn = bn;
     p.pair = pair;
   };
-  offer(256, true, rounds(tiles(2 * TILE, 256), sms / 2) * p.k_blocks * 290 + 6200);
-  offer(256, false, rounds(tiles(TILE, 256), sms) * p.k_blocks * 320 + 5900);
-  offer(128, false, rounds(tiles(TILE, 128), sms) * p.k_blocks * 190 + 1800);
-  offer(64, false, rounds(tiles(TILE, 64), sms) * p.k_blocks * 130 + 200);
+  // ns of a round for each block of K, and once, fitted to 7 matrices from 1024 x 1024 to 28672 x 7168 at 129 to 4096 tokens.  us by pairs | 256 wide | 128 | 64: 256 tokens of 1024 x 1024 10.4 | 10.0 | 7.8
+  // | 7.2; of 7168 x 7168 26.6 | 30.5 | 22.1 | 27.4; 1000 tokens of it 45 | 52 | 55 | 82; 4096 of 28672 x 7168 521 | 566 | 801 | 1364.
+  offer(256, true, rounds(tiles(2 * TILE, 256), sms / 2) * p.k_blocks * 330 + 5000);
+  offer(256, false, rounds(tiles(TILE, 256), sms) * p.k_blocks * 390 + 4300);
+  offer(128, false, rounds(tiles(TILE, 128), sms) * p.k_blocks * 235 + 3200);
+  offer(64, false, rounds(tiles(TILE, 64), sms) * p.k_blocks * 190 + 2900);
   const int rows = p.pair ? 2 * TILE : TILE;
   p.tiles_a = (M + rows - 1) / rows;
   p.tiles_b = (N + p.bn - 1) / p.bn;
@@ -532,25 +535,23 @@ Plan plan_of(int M, int N, int K) {
   p.grid = p.pair ? 2 * (int)(units < sms / 2 ? units : sms / 2) : (int)(units < sms ? units : sms);
   return p;
 }
-// of a workspace: counts, codes and scales of the tokens (unless they are given), parts of tiles
+// of a workspace: codes and scales of the tokens, unless they are given
 struct Rooms {
-  size_t codes, scales, pieces, bytes;
+  size_t scales, bytes;
   long long ldc;
 };
-size_t up(size_t n) { return (n + 255) / 256 * 256; }
-Rooms rooms_of(const Plan& p, int M, int K, bool given) {
-  Rooms r;
+Rooms rooms_of(int M, int K, bool given) {
+  Rooms r{};
   r.ldc = ((long long)K + 15) / 16 * 16;
-  r.codes = p.few && p.split ? up((size_t)p.tiles_a * sizeof(int)) : 0;
-  r.scales = r.codes + (given ? 0 : up((size_t)M * r.ldc));
-  r.pieces = r.scales + (given ? 0 : up((size_t)M * sizeof(float)));
-  r.bytes = r.pieces + (p.few && p.split ? (size_t)p.grid * 2 * M * TILE * sizeof(int) : 0);
+  if (given) return r;
+  r.scales = ((size_t)M * r.ldc + 255) / 256 * 256;
+  r.bytes = r.scales + (size_t)M * sizeof(float);
   return r;
 }
 
 template <bool FEW, int BN, bool PAIR, bool OUT32> int launch(const Plan& pl, const CUtensorMap& tmA, const CUtensorMap& tmB, const Args& a, bool early, cudaStream_t stream) {
   using L = Shape<FEW, BN, PAIR>;
-  static_assert(L::SMEM <= 232448 && L::STAGES >= 3, "shared memory");
+  static_assert(L::SMEM <= (FEW ? 115712 : 232448) && L::STAGES >= 3 && (!FEW || L::STAGES * L::STAGE >= BN * TILE * 4), "shared memory");
   auto kernel = int8_gemm_kernel<FEW, BN, PAIR, OUT32>;
   static bool configured[64] = {};                                 // per device
   int dev = 0;
@@ -559,7 +560,7 @@ template <bool FEW, int BN, bool PAIR, bool OUT32> int launch(const Plan& pl, co
     LIA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
     if (dev < 64) configured[dev] = true;
   }
-  if (PAIR) LIA_CUDA(lia_launch_cluster(2, kernel, dim3(pl.grid), dim3(256), L::SMEM, stream, tmA, tmB, a));
+  if (PAIR || pl.parts > 1) LIA_CUDA(lia_launch_cluster_as(early || PAIR, PAIR ? 2 : pl.parts, kernel, dim3(pl.grid), dim3(256), L::SMEM, stream, tmA, tmB, a));
   else LIA_CUDA(lia_launch_as(early, kernel, dim3(pl.grid), dim3(256), L::SMEM, stream, tmA, tmB, a));
   return LIA_OK;
 }
@@ -580,10 +581,16 @@ template <bool OUT32> int launch_plan(const Plan& pl, const CUtensorMap& tmA, co
   }
 }
 
-int quantize(const void* x, int act_f32, long long ldx, int8_t* codes, long long ldc, float* scale, int* counts, int n_counts, int M, int K, cudaStream_t stream) {
-  const QuantArgs q{x, ldx, ldc, codes, scale, counts, K, n_counts, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (act_f32 ? 4 : 8) == 0};
-  if (act_f32) LIA_CUDA(lia_launch(quantize_rows_kernel<float>, dim3(M), dim3(Q_THREADS), 0, stream, q));
-  else LIA_CUDA(lia_launch(quantize_rows_kernel<bf16>, dim3(M), dim3(Q_THREADS), 0, stream, q));
+int quantize(const void* x, int act_f32, long long ldx, int8_t* codes, long long ldc, float* scale, int M, int K, cudaStream_t stream) {
+  const QuantArgs q{x, ldx, ldc, codes, scale, K, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (act_f32 ? 4 : 8) == 0};
+  // a block of 256 threads holds a row of 8192 numbers, one of 1024 four times that; longer rows are read twice
+  if (K > 8 * Q_HELD * 256) {
+    if (act_f32) LIA_CUDA(lia_launch(quantize_rows_kernel<float, 1024>, dim3(M), dim3(1024), 0, stream, q));
+    else LIA_CUDA(lia_launch(quantize_rows_kernel<bf16, 1024>, dim3(M), dim3(1024), 0, stream, q));
+  } else {
+    if (act_f32) LIA_CUDA(lia_launch(quantize_rows_kernel<float, 256>, dim3(M), dim3(256), 0, stream, q));
+    else LIA_CUDA(lia_launch(quantize_rows_kernel<bf16, 256>, dim3(M), dim3(256), 0, stream, q));
+  }
   return LIA_OK;
 }
 
@@ -594,12 +601,12 @@ extern "C" int lia_quantize_rows(const void* x, int act_f32, long long ldx, void
   if (M == 0) return LIA_OK;
   LIA_CHECK_ARG(x && codes && scale, "lia_quantize_rows: null pointer");
   LIA_CHECK_ARG(reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldc % 8 == 0, "lia_quantize_rows: rows of codes have to be whole 8-byte vectors apart");
-  return quantize(x, act_f32, ldx, static_cast<int8_t*>(codes), ldc, scale, nullptr, 0, M, K, reinterpret_cast<cudaStream_t>(stream));
+  return quantize(x, act_f32, ldx, static_cast<int8_t*>(codes), ldc, scale, M, K, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t lia_linear_int8_workspace_bytes(int x_type, int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0 || K > MOST_K) return 0;
-  return rooms_of(plan_of(M, N, K), M, K, x_type == LIA_X_INT8).bytes;
+  return rooms_of(M, K, x_type == LIA_X_INT8).bytes;
 }
 
 extern "C" int lia_linear_int8(const void* x, int x_type, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, void* out, int out_f32, int M, int N, int K,
@@ -614,22 +621,20 @@ extern "C" int lia_linear_int8(const void* x, int x_type, long long ldx, const f
   LIA_CHECK_ARG(reinterpret_cast<uintptr_t>(w) % 16 == 0 && ldw % 16 == 0 && (!given || (reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 16 == 0)),
                 "lia_linear_int8: rows of codes have to be whole 16-byte vectors apart");
   const Plan pl = plan_of(M, N, K);
-  LIA_CHECK_ARG((long long)pl.tiles_a * pl.k_blocks * (pl.grid + 1) < (1ll << 31) && (long long)pl.tiles_a * pl.tiles_b < (1ll << 31), "lia_linear_int8: too large (M=%d N=%d K=%d)", M, N, K);
-  const Rooms r = rooms_of(pl, M, K, given);
+  LIA_CHECK_ARG((long long)pl.tiles_a * pl.k_blocks < (1ll << 31) && (long long)pl.tiles_a * pl.tiles_b < (1ll << 31), "lia_linear_int8: too large (M=%d N=%d K=%d)", M, N, K);
+  const Rooms r = rooms_of(M, K, given);
   LIA_CHECK_ARG(r.bytes == 0 || (ws && ws_bytes >= r.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_linear_int8: needs a workspace of %zu bytes", r.bytes);
   uint8_t* base = static_cast<uint8_t*>(ws);
-  const bool split = pl.few && pl.split;
-  const void* codes = given ? x : base + r.codes;
+  const void* codes = given ? x : base;
   const long long ldc = given ? ldx : r.ldc;
   CUtensorMap tmX, tmW;
   int rc = make_tmap(&tmX, codes, M, K, ldc, pl.few ? pl.bn : TILE);
   if (rc == LIA_OK) rc = make_tmap(&tmW, w, N, K, ldw, pl.few ? TILE : pl.pair ? pl.bn / 2 : pl.bn);
   if (rc != LIA_OK) return rc;
-  Args a{given ? x_scale : reinterpret_cast<float*>(base + r.scales), w_scale, out, reinterpret_cast<int*>(base + r.pieces), reinterpret_cast<int*>(base), lia_timeout_word(), M, N, pl.k_blocks,
-         pl.tiles_a, pl.tiles_b, reinterpret_cast<uintptr_t>(out) % 16 == 0 && (long long)N * (out_f32 ? 4 : 2) % 16 == 0};
+  Args a{given ? x_scale : reinterpret_cast<float*>(base + r.scales), w_scale, out, lia_timeout_word(), M, N, pl.k_blocks,
+         pl.tiles_a, pl.tiles_b, reinterpret_cast<uintptr_t>(out) % 16 == 0 && (long long)N * (out_f32 ? 4 : 2) % 16 == 0, pl.parts};
   LIA_CHECK_ARG(a.timeouts, "lia_linear_int8: no memory for the count of waits that ran out");
-  if (!given) rc = quantize(x, x_type == LIA_X_F32, ldx, reinterpret_cast<int8_t*>(base + r.codes), r.ldc, reinterpret_cast<float*>(base + r.scales), a.counts, split ? pl.tiles_a : 0, M, K, stream);
-  else if (split) LIA_CUDA(cudaMemsetAsync(base, 0, (size_t)pl.tiles_a * sizeof(int), stream));
+  if (!given) rc = quantize(x, x_type == LIA_X_F32, ldx, reinterpret_cast<int8_t*>(base), r.ldc, reinterpret_cast<float*>(base + r.scales), M, K, stream);
   if (rc != LIA_OK) return rc;
   const bool early = !given;                                       // (right behind another kernel, which may have written the weights, the product does not begin before that has ended)
   return pl.few ? (out_f32 ? launch_plan<true>(pl, tmW, tmX, a, early, stream) : launch_plan<false>(pl, tmW, tmX, a, early, stream))

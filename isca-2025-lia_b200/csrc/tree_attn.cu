@@ -1,4 +1,5 @@
-// Attention of portions of new tokens -- a decoded token, a chain or a tree of drafted ones, a part of a prompt -- behind their cached histories, over caches of bf16, int8 or e4m3.
+// Attention of portions of new tokens -- a decoded token, a chain or a tree of drafted ones, a part of a prompt -- behind their cached histories, over caches of bf16, int8 or e4m3 (and,
+// by way of tree_attn_4bit.cu, of 4 bits).
 //
 //   s_ij = cap tanh(temp_h scale ks_j (q_i . k_j) / cap),   o_i = sum_j p_ij vs_j v_j / sum_j p_ij,   p_ij = e^(s_ij - max) over the j that row i sees
 //
@@ -23,47 +24,34 @@
 #include "tree_attn.cuh"
 
 int lia_tree_attn_tc(const void* args, int type, int rows, int nseg, lia_stream_t stream);      // tree_attn_sm100.cu
+int lia_tree_attn_4bit(const void* args, int nr, int nseg, lia_stream_t stream);                // tree_attn_4bit.cu
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, MAX_SPLITS = 64, CLUSTER = 8;   // CLUSTER: up to so many blocks share a history as a cluster, more by way of a workspace
-
-__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transposed(uint32_t x) {       // of 8 x 8 numbers of 16 bits, a row's two neighbours a lane
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
+constexpr int MAX_SPLITS = 64;
 
 // blocks of an SM, by the registers that the rows' sums and the keys and values on their way take
-constexpr int blocks_an_sm(int kind, int nr) { return nr == 1 ? (kind == LIA_CACHE_BF16 ? 3 : 4) : nr == 2 ? (kind == LIA_CACHE_BF16 ? 2 : 3) : 2; }
+constexpr int blocks_an_sm(int kind, int nr) { return kind == LIA_CACHE_INT4 ? tree_attn4_blocks(nr) : nr == 1 ? (kind == LIA_CACHE_BF16 ? 3 : 4) : nr == 2 ? (kind == LIA_CACHE_BF16 ? 2 : 3) : 2; }
 
 template <int DIM, int VDIM, int KIND, int NR>
 struct Shape {
-  static constexpr bool SCALED = KIND != LIA_CACHE_BF16, FOUR = KIND == LIA_CACHE_INT4;
+  static constexpr bool BITS8 = KIND != LIA_CACHE_BF16;
   static constexpr int STEPS = DIM / 16;                           // products of a block of 16 keys with 8 rows' queries
   static constexpr int MT = VDIM / 16;                             // products of 16 channels of a block's values with 8 rows' weights
-  static constexpr int KB = DIM * (FOUR ? 1 : SCALED ? 2 : 4) / 8;  // bytes of a key in a lane
-  static constexpr int VB = VDIM * (FOUR ? 1 : SCALED ? 2 : 4) / 16;                           // bytes of a value in a lane
-  static constexpr int KG = FOUR ? DIM / GROUP4 : 2, VG = FOUR ? VDIM / GROUP4 : 2;             // scales of a position with 4 bits (else: not used)
+  static constexpr int KV = DIM * (BITS8 ? 1 : 2) / 64;            // 16-byte vectors of a key in a lane
+  static constexpr int VB = VDIM * (BITS8 ? 1 : 2) / 8;            // bytes of a value in a lane
   static constexpr int ROWS = 8 * NR;
   static constexpr int Q_BYTES = NR * STEPS * 32 * 8, O_BYTES = WARPS * ROWS * VDIM * 4, BIG = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
   static constexpr int SMEM = BIG + ROWS * 4 + WARPS * ROWS * 8;
-  static constexpr float LIFT = SCALED ? 7.f : 0.f;                // a weight of the maximum is 2^LIFT, one that is just not outgrown 2^15 in fp16
+  static constexpr float LIFT = BITS8 ? 7.f : 0.f;                 // a weight of the maximum is 2^LIFT, one that is just not outgrown 2^15 in fp16
   // the channel of the first of a lane's pair in the i-th product with the values
-  static __device__ __forceinline__ int channel(int i, int gq) { return FOUR ? (i >> 1) * GROUP4 + gq * 4 + (i & 1) * 2 : SCALED ? gq * (VDIM / 8) + 2 * i : (i >> 2) * 64 + gq * 8 + (i & 3) * 2; }
+  static __device__ __forceinline__ int channel(int i, int gq) { return BITS8 ? gq * (VDIM / 8) + 2 * i : (i >> 2) * 64 + gq * 8 + (i & 3) * 2; }
 };
-constexpr float NONE = -1e30f, SLACK = 8.f;                        // a maximum of no keys; how far, in powers of two, weights may exceed 1
-
 template <int DIM, int VDIM, int KIND, int NR>
 __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   using S = Shape<DIM, VDIM, KIND, NR>;
-  constexpr bool SCALED = S::SCALED, FOUR = S::FOUR;
-  constexpr int RQ = SCALED ? 1 : 2;
+  constexpr bool BITS8 = S::BITS8;
+  constexpr int RQ = BITS8 ? 1 : 2;
   extern __shared__ uint4 smem[];
   float* row_f = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + S::BIG);        // [ROWS] what a row's products with keys are multiplied by
   float2* part = reinterpret_cast<float2*>(row_f + S::ROWS);       // [WARPS][ROWS] maximum, sum
@@ -96,28 +84,19 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
   const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = min(hi, a.mask != nullptr ? p.p0 : p.p0 + i0 + 1);
   const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
 
-  const uint8_t *kbase = a.k.at(p.slot, 0, g) + t4 * (FOUR ? S::KB : 16), *vbase = a.v.at(p.slot, 0, g) + gq * (SCALED ? S::VB : 16);
-  const float *ksc = SCALED ? a.k.scale_at(p.slot, g) : nullptr, *vsc = SCALED ? a.v.scale_at(p.slot, g) : nullptr;
-  const bf16 *ksc4 = FOUR ? a.k.scale4_at(p.slot, g) : nullptr, *vsc4 = FOUR ? a.v.scale4_at(p.slot, g) : nullptr;
-  uint32_t kr[2][S::KB / 4];                                       // keys gq and gq + 8
+  const uint8_t *kbase = a.k.at(p.slot, 0, g) + t4 * 16, *vbase = a.v.at(p.slot, 0, g) + gq * (BITS8 ? S::VB : 16);
+  const float *ksc = BITS8 ? a.k.scale_at(p.slot, g) : nullptr, *vsc = BITS8 ? a.v.scale_at(p.slot, g) : nullptr;
+  uint4 kr[2][S::KV];                                              // keys gq and gq + 8
   uint32_t vr[4][S::VB / 4];                                       // values 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4
   float ks[2], vs[2];                                              // of keys gq and gq + 8
-  uint32_t ks4[2][S::KG / 2], vs4[2][S::VG / 2];                   // of the same, with 4 bits
   auto load_k = [&](int b) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int key = min(lo + b * 16 + j * 8 + gq, hi - 1);
       const uint8_t* src = kbase + (long long)key * a.k.pos;
-      if constexpr (S::KB == 8) {
-        *reinterpret_cast<uint2*>(kr[j]) = __ldcg(reinterpret_cast<const uint2*>(src));
-      } else {
 #pragma unroll
-        for (int c = 0; c < S::KB / 16; ++c) *reinterpret_cast<uint4*>(&kr[j][c * 4]) = ldg_act(src + c * 64);
-      }
-      if constexpr (FOUR) {
-        ask_scales4<S::KG>(ksc4 + (long long)key * S::KG, ks4[j]);
-        ask_scales4<S::VG>(vsc4 + (long long)key * S::VG, vs4[j]);
-      } else if constexpr (SCALED) {
+      for (int c = 0; c < S::KV; ++c) kr[j][c] = ldg_act(src + c * 64);
+      if constexpr (BITS8) {
         ks[j] = __ldcg(ksc + key);
         vs[j] = __ldcg(vsc + key);
       }
@@ -127,9 +106,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint8_t* src = vbase + (long long)min(lo + b * 16 + (c >> 1) * 8 + t4 * 2 + (c & 1), hi - 1) * a.v.pos;
-      if constexpr (S::VB == 4) {
-        vr[c][0] = __ldcg(reinterpret_cast<const uint32_t*>(src));
-      } else if constexpr (S::VB == 8) {
+      if constexpr (S::VB == 8) {
         const uint2 u = __ldcg(reinterpret_cast<const uint2*>(src));
         vr[c][0] = u.x;
         vr[c][1] = u.y;
@@ -153,7 +130,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     if (there && lane < DIM / 4) u = *reinterpret_cast<const uint2*>(a.q + (p.row + i) * a.ldq + h * DIM + lane * 4);
     float f = a.scale * (a.temp != nullptr && there ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
     uint2 w = u;
-    if constexpr (SCALED) {
+    if constexpr (BITS8) {
       uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
       const Down down = down_of(__reduce_max_sync(0xffffffffu, top));
       float x[4];
@@ -162,9 +139,8 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
       w = make_uint2(pack_f16x2(x[0] * down.by, x[1] * down.by), pack_f16x2(x[2] * down.by, x[3] * down.by));
       f *= down.back;
     }
-    if constexpr (FOUR) w = in_code_order(w);
     if (lane < DIM / 4) {                                          // four neighbouring channels are a lane's operand of one step
-      const int c = lane * 4, t = SCALED && !FOUR ? (c >> 4) & 3 : (c >> 3) & 3, step = SCALED && !FOUR ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
+      const int c = lane * 4, t = BITS8 ? (c >> 4) & 3 : (c >> 3) & 3, step = BITS8 ? (c >> 6) * 4 + ((c >> 2) & 3) : (c >> 5) * 2 + ((c >> 2) & 1);
       qs[((r >> 3) * S::STEPS + step) * 32 + (r & 7) * 4 + t] = w;
     }
     if (lane == 0) row_f[r] = f;
@@ -204,38 +180,14 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
-    if constexpr (FOUR) {                                          // group by group, whose sums are multiplied by their scales
-      float kg[2][S::KG];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) scales4_of<S::KG>(ks4[j], kg[j]);
-#pragma unroll
-      for (int gr = 0; gr < S::KG; ++gr) {
-        uint32_t codes[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) int4x2(__byte_perm(kr[j][gr >> 1], kr[j][S::KB / 8 + (gr >> 1)], gr & 1 ? 0x7632 : 0x5410), codes[j]);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          float part[4] = {};
-#pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            const uint32_t ka[4] = {codes[0][2 * st], codes[1][2 * st], codes[0][2 * st + 1], codes[1][2 * st + 1]};
-            uint2 q;
-            if constexpr (NR <= RQ) q = qa[r][gr * 2 + st];
-            else q = qs[(r * S::STEPS + gr * 2 + st) * 32 + lane];
-            mma_f16(part, ka, q.x, q.y);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[r][e] = fmaf(part[e], kg[e >> 1][gr], s[r][e]);
-        }
-      }
-    }
-#pragma unroll
-    for (int st = 0; st < (FOUR ? 0 : S::STEPS); ++st) {
+    for (int st = 0; st < S::STEPS; ++st) {
       uint32_t ka[4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if constexpr (SCALED) {
-          uint32_t w = kr[j][st];
+        if constexpr (BITS8) {
+          const uint4& u = kr[j][st >> 2];
+          uint32_t w = (st & 3) == 0 ? u.x : (st & 3) == 1 ? u.y : (st & 3) == 2 ? u.z : u.w;
           if constexpr (KIND == LIA_CACHE_INT8) {
             w ^= 0x80808080u;
             ka[j] = int8x2(__byte_perm(w, 0x64646464u, 0x4140));
@@ -245,8 +197,9 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
             ka[2 + j] = e4m3x2(w >> 16);
           }
         } else {
-          ka[j] = kr[j][2 * st];
-          ka[2 + j] = kr[j][2 * st + 1];
+          const uint4& u = kr[j][st >> 1];
+          ka[j] = st & 1 ? u.z : u.x;
+          ka[2 + j] = st & 1 ? u.w : u.y;
         }
       }
 #pragma unroll
@@ -254,30 +207,18 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
         uint2 q;
         if constexpr (NR <= RQ) q = qa[r][st];
         else q = qs[(r * S::STEPS + st) * 32 + lane];
-        if constexpr (SCALED) mma_f16(s[r], ka, q.x, q.y);
+        if constexpr (BITS8) mma_f16(s[r], ka, q.x, q.y);
         else mma_bf16(s[r], ka, q.x, q.y);
       }
     }
     float kf[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f}, rv[2] = {1.f, 1.f};
-    float ratio[2][S::VG];                                         // with 4 bits: a group's scale relative to the value's largest, which goes into the exponent
-    if constexpr (SCALED) {
+    if constexpr (BITS8) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if constexpr (FOUR) {
-          scales4_of<S::VG>(vs4[j], ratio[j]);
-          vs[j] = ratio[j][0];
-#pragma unroll
-          for (int gr = 1; gr < S::VG; ++gr) vs[j] = max_nan(vs[j], ratio[j][gr]);
-        } else {
-          kf[j] = ks[j];
-        }
+        kf[j] = ks[j];
         const float y = max_nan(vs[j], LEAST_SCALE);
         lv[j] = lg2(y);
         rv[j] = __fdividef(1.f, y);
-        if constexpr (FOUR) {
-#pragma unroll
-          for (int gr = 0; gr < S::VG; ++gr) ratio[j][gr] *= rv[j];
-        }
       }
     }
     if (b + WARPS < b1) load_k(b + WARPS);
@@ -292,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[r][e] = SCALED ? fmaf(s[r][e] * kf[e >> 1], rf[r][e & 1], lv[e >> 1]) : s[r][e] * rf[r][e & 1];
+        for (int e = 0; e < 4; ++e) s[r][e] = BITS8 ? fmaf(s[r][e] * kf[e >> 1], rf[r][e & 1], lv[e >> 1]) : s[r][e] * rf[r][e & 1];
     }
     if (key0 < all_lo || key0 + 16 > all_hi) {
 #pragma unroll
@@ -333,55 +274,37 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
         }
     }
     // ---- weights, turned into the products' other operand
-    constexpr int PARTS = FOUR ? S::VG : SCALED ? 1 : 2;           // with 4 bits a group's weights each, with bf16 two parts of a weight
-    uint32_t pb[PARTS][NR][2];
+    uint32_t pb[BITS8 ? 1 : 2][NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       float w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         w[e] = ex2(s[r][e] - m[r][e & 1]);
-        l[r][e & 1] = SCALED ? fmaf(w[e], rv[e >> 1], l[r][e & 1]) : l[r][e & 1] + w[e];
+        l[r][e & 1] = BITS8 ? fmaf(w[e], rv[e >> 1], l[r][e & 1]) : l[r][e & 1] + w[e];
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if constexpr (FOUR) {
-#pragma unroll
-          for (int gr = 0; gr < S::VG; ++gr) pb[gr][r][j] = transposed(pack_f16x2(w[2 * j] * ratio[j][gr], w[2 * j + 1] * ratio[j][gr]));
-        } else if constexpr (SCALED) {
+        if constexpr (BITS8) {
           pb[0][r][j] = transposed(pack_f16x2(w[2 * j], w[2 * j + 1]));
         } else {
           const uint32_t hi2 = pack_bf16x2(w[2 * j], w[2 * j + 1]);
           float x, y;
           unpack_bf16x2(hi2, x, y);
           pb[0][r][j] = transposed(hi2);
-          pb[PARTS - 1][r][j] = transposed(pack_bf16x2(w[2 * j] - x, w[2 * j + 1] - y));
+          pb[BITS8 ? 0 : 1][r][j] = transposed(pack_bf16x2(w[2 * j] - x, w[2 * j + 1] - y));
         }
       }
     }
     // ---- weighted values
-    if constexpr (FOUR) {
 #pragma unroll
-      for (int gr = 0; gr < S::VG; ++gr) {
-        uint32_t va[2][4];                                         // a lane's four channels of the group, of keys 2 t4 and 2 t4 + 1, and of those 8 on
-#pragma unroll
-        for (int c = 0; c < 2; ++c) int4x2(__byte_perm(vr[2 * c][gr >> 1], vr[2 * c + 1][gr >> 1], gr & 1 ? 0x7632 : 0x5410), va[c]);
-#pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          const uint32_t v4[4] = {va[0][c], va[0][c + 1], va[1][c], va[1][c + 1]};
-#pragma unroll
-          for (int r = 0; r < NR; ++r) mma_f16(o[r][gr * 2 + (c >> 1)], v4, pb[gr][r][0], pb[gr][r][1]);
-        }
-      }
-    }
-#pragma unroll
-    for (int w = 0; w < (FOUR ? 0 : S::VB / 4); ++w) {
-      constexpr int PER = SCALED ? 4 : 2;                           // channels of a word
+    for (int w = 0; w < S::VB / 4; ++w) {
+      constexpr int PER = BITS8 ? 4 : 2;                           // channels of a word
       uint32_t va[PER][2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const uint32_t u0 = vr[2 * c][w], u1 = vr[2 * c + 1][w];
-        if constexpr (SCALED) {
+        if constexpr (BITS8) {
           uint32_t x = __byte_perm(u0, u1, 0x5140), y = __byte_perm(u0, u1, 0x7362);
           if constexpr (KIND == LIA_CACHE_INT8) {
             x ^= 0x80808080u;
@@ -407,11 +330,11 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
         const int n = (w * PER + c) >> 1;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          if constexpr (SCALED) {
+          if constexpr (BITS8) {
             mma_f16(o[r][n], v4, pb[0][r][0], pb[0][r][1]);
           } else {
             mma_bf16(o[r][n], v4, pb[0][r][0], pb[0][r][1]);
-            mma_bf16(o[r][n], v4, pb[PARTS - 1][r][0], pb[PARTS - 1][r][1]);
+            mma_bf16(o[r][n], v4, pb[BITS8 ? 0 : 1][r][0], pb[BITS8 ? 0 : 1][r][1]);
           }
         }
       }
@@ -435,64 +358,7 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
       for (int n = 0; n < S::MT; ++n) *reinterpret_cast<float2*>(os + at * VDIM + S::channel(n, gq)) = make_float2(o[r][n][e], o[r][n][2 + e]);
     }
   __syncthreads();
-  constexpr int N = VDIM / 32;
-  const long long rows = (long long)a.M * a.H;
-  for (int r = warp; r < S::ROWS && r0 + r < R; r += WARPS) {
-    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
-    float top = NONE, sum = 0.f, y[N] = {};
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w * S::ROWS + r].x);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float2 x = part[w * S::ROWS + r];
-      const float f = ex2(x.x - top);
-      sum = fmaf(x.y, f, sum);
-#pragma unroll
-      for (int c = 0; c < N; ++c) y[c] = fmaf(os[(w * S::ROWS + r) * VDIM + lane * N + c], f, y[c]);
-    }
-    if (a.splits == 1) {
-      put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
-    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read: with all lanes, before one of them writes)
-#pragma unroll
-      for (int c = 0; c < N; ++c) os[r * VDIM + lane * N + c] = y[c];
-      __syncwarp();
-      if (lane == 0) part[r] = make_float2(top, sum);
-    } else {
-      const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;
-#pragma unroll
-      for (int c = 0; c < N; ++c) a.ws[at * VDIM + lane * N + c] = y[c];
-      if (lane == 0) reinterpret_cast<float2*>(a.ws + a.splits * rows * VDIM)[at] = make_float2(top, sum);
-    }
-  }
-  if (a.splits == 1 || a.splits > CLUSTER) return;
-  // ---- the blocks that share a history are a cluster: each joins some of the rows, always in the same order
-  cluster_barrier();
-  for (int r = warp * a.splits + blockIdx.x; r < S::ROWS && r0 + r < R; r += WARPS * a.splits) {
-    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
-    float2 ml[CLUSTER];
-    float w[CLUSTER][N], top = NONE, sum = 0.f, y[N] = {};
-#pragma unroll
-    for (int q = 0; q < CLUSTER; ++q) {
-      if (q < a.splits) {
-        ml[q] = cluster_ld_f2(cluster_place(&part[r], q));
-        const uint32_t from = cluster_place(&os[r * VDIM + lane * N], q);
-        if constexpr (N == 4) *reinterpret_cast<float4*>(w[q]) = cluster_ld_f4(from);
-        else *reinterpret_cast<float2*>(w[q]) = cluster_ld_f2(from);
-        top = fmaxf(top, ml[q].x);
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < CLUSTER; ++q) {
-      if (q < a.splits) {
-        const float f = ex2(ml[q].x - top);
-        sum = fmaf(ml[q].y, f, sum);
-#pragma unroll
-        for (int c = 0; c < N; ++c) y[c] = fmaf(w[q][c], f, y[c]);
-      }
-    }
-    put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
-  }
-  cluster_barrier();                                               // (no block leaves while it is read)
+  meet<DIM, VDIM, KIND, S::ROWS>(a, p, r0, R, g, os, part);
 }
 
 // How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history
@@ -555,9 +421,10 @@ template <int DIM, int VDIM, int KIND, int NR> int launch(const TreeArgs& a, int
   return LIA_OK;
 }
 template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
-  const int rc = nr >= 16 ? lia_tree_attn_tc(&a, KIND, nr * 8, nseg, stream)
-                 : nr == 4 ? launch<DIM, VDIM, KIND, 4>(a, nseg, stream)
-                 : nr == 2 ? launch<DIM, VDIM, KIND, 2>(a, nseg, stream) : launch<DIM, VDIM, KIND, 1>(a, nseg, stream);
+  int rc;
+  if (nr >= 16) rc = lia_tree_attn_tc(&a, KIND, nr * 8, nseg, stream);
+  else if constexpr (KIND == LIA_CACHE_INT4) rc = lia_tree_attn_4bit(&a, nr, nseg, stream);
+  else rc = nr == 4 ? launch<DIM, VDIM, KIND, 4>(a, nseg, stream) : nr == 2 ? launch<DIM, VDIM, KIND, 2>(a, nseg, stream) : launch<DIM, VDIM, KIND, 1>(a, nseg, stream);
   if (rc == LIA_OK && a.splits > (nr >= 16 ? 1 : CLUSTER)) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
   return rc;
 }

@@ -232,4 +232,84 @@ template <int DIM, int VDIM, int KIND> __global__ void __launch_bounds__(128) tr
   put_row<DIM, VDIM, KIND>(a, p, i, h, o, l);
 }
 
+constexpr int WARPS = 4, THREADS = WARPS * 32;                    // of the kernels for few rows of a key head
+constexpr int CLUSTER = 8;                                         // up to so many blocks share a history as a cluster, more by way of a workspace
+constexpr float NONE = -1e30f, SLACK = 8.f;                        // a maximum of no keys; how far, in powers of two, weights may exceed 1
+// blocks of an SM that tree_attn_4bit.cu's kernel is built for, by its eights of rows
+constexpr int tree_attn4_blocks(int nr) { return nr == 1 ? 4 : nr == 2 ? 3 : 2; }
+
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {       // of 8 x 8 numbers of 16 bits, a row's two neighbours a lane
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// A block's parts, in shared memory as [WARPS][ROWS], to outputs: os the weighted values [..][VDIM], part maximum and sum of weights
+template <int DIM, int VDIM, int KIND, int ROWS> __device__ __forceinline__ void meet(const TreeArgs& a, const Portion& p, int r0, int R, int g, float* os, float2* part) {
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr int N = VDIM / 32;
+  const long long rows = (long long)a.M * a.H;
+  for (int r = warp; r < ROWS && r0 + r < R; r += WARPS) {
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    float top = NONE, sum = 0.f, y[N] = {};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w * ROWS + r].x);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 x = part[w * ROWS + r];
+      const float f = ex2(x.x - top);
+      sum = fmaf(x.y, f, sum);
+#pragma unroll
+      for (int c = 0; c < N; ++c) y[c] = fmaf(os[(w * ROWS + r) * VDIM + lane * N + c], f, y[c]);
+    }
+    if (a.splits == 1) {
+      put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
+    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read: with all lanes, before one of them writes)
+#pragma unroll
+      for (int c = 0; c < N; ++c) os[r * VDIM + lane * N + c] = y[c];
+      __syncwarp();
+      if (lane == 0) part[r] = make_float2(top, sum);
+    } else {
+      const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;
+#pragma unroll
+      for (int c = 0; c < N; ++c) a.ws[at * VDIM + lane * N + c] = y[c];
+      if (lane == 0) reinterpret_cast<float2*>(a.ws + a.splits * rows * VDIM)[at] = make_float2(top, sum);
+    }
+  }
+  if (a.splits == 1 || a.splits > CLUSTER) return;
+  // ---- the blocks that share a history are a cluster: each joins some of the rows, always in the same order
+  cluster_barrier();
+  for (int r = warp * a.splits + blockIdx.x; r < ROWS && r0 + r < R; r += WARPS * a.splits) {
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    float2 ml[CLUSTER];
+    float w[CLUSTER][N], top = NONE, sum = 0.f, y[N] = {};
+#pragma unroll
+    for (int q = 0; q < CLUSTER; ++q) {
+      if (q < a.splits) {
+        ml[q] = cluster_ld_f2(cluster_place(&part[r], q));
+        const uint32_t from = cluster_place(&os[r * VDIM + lane * N], q);
+        if constexpr (N == 4) *reinterpret_cast<float4*>(w[q]) = cluster_ld_f4(from);
+        else *reinterpret_cast<float2*>(w[q]) = cluster_ld_f2(from);
+        top = fmaxf(top, ml[q].x);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < CLUSTER; ++q) {
+      if (q < a.splits) {
+        const float f = ex2(ml[q].x - top);
+        sum = fmaf(ml[q].y, f, sum);
+#pragma unroll
+        for (int c = 0; c < N; ++c) y[c] = fmaf(w[q][c], f, y[c]);
+      }
+    }
+    put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
+  }
+  cluster_barrier();                                               // (no block leaves while it is read)
+}
+
 }  // namespace

@@ -31,13 +31,12 @@ int* lia_formed_again_word();                                      // moe_sm100.
 
 namespace {
 
-constexpr int ROWS = 128, KEYS = 64, THREADS = 640, LOADERS = 256, ISSUER = 16;
+constexpr int ROWS = 128, KEYS = 64, TC_THREADS = 640, LOADERS = 256, ISSUER = 16;
 constexpr int SOFTMAX_REGS = 128, LOADER_REGS = 96, OTHER_REGS = 32; // of a thread, by what its four warps do (setmaxnreg: multiples of 8); the launch gives 96
 constexpr int LAUNCH_REGS = 96;
-static_assert(SOFTMAX_REGS >= LAUNCH_REGS && LOADER_REGS <= LAUNCH_REGS && OTHER_REGS <= LAUNCH_REGS && 2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS <= THREADS / 128 * LAUNCH_REGS, "shares");
+static_assert(SOFTMAX_REGS >= LAUNCH_REGS && LOADER_REGS <= LAUNCH_REGS && OTHER_REGS <= LAUNCH_REGS && 2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS <= TC_THREADS / 128 * LAUNCH_REGS, "shares");
 constexpr uint32_t VALUES = 256;
 constexpr float LEAST_KEY_SCALE = 0x1p-110f;                       // a 4-bit key's largest scale counts as that at least, so that its inverse is finite
-constexpr float SLACK = 8.f;                                       // how far, in powers of two, weights may exceed 1
 
 template <int DIM, int VDIM, int KIND, bool PAIR>
 struct Tc {
@@ -149,7 +148,7 @@ __device__ __forceinline__ int ref_of(const uint32_t (&u)[2]) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
 
 template <int DIM, int VDIM, int KIND, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) tree_attn_tc_kernel(const __grid_constant__ TreeArgs a, int* __restrict__ timeouts) {
+__global__ void __launch_bounds__(TC_THREADS, 1) tree_attn_tc_kernel(const __grid_constant__ TreeArgs a, int* __restrict__ timeouts) {
   using C = Tc<DIM, VDIM, KIND, PAIR>;
   constexpr bool SCALED = C::SCALED, FOUR = C::FOUR;
   constexpr int TILE = PAIR ? 2 * ROWS : ROWS, STAGES = C::STAGES;
@@ -795,7 +794,7 @@ template <int DIM, int VDIM, int KIND, bool PAIR> int launch(const TreeArgs& a, 
   LIA_CHECK_ARG(split_fits, "lia_tree_attn: the kernel was built with too few registers");
   int* timeouts = lia_formed_again_word();
   LIA_CHECK_ARG(timeouts, "lia_tree_attn: no memory for the count of waits that ran out");
-  LIA_CUDA(lia_launch(tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(THREADS), SMEM, stream, a, timeouts));
+  LIA_CUDA(lia_launch(tree_attn_tc_kernel<DIM, VDIM, KIND, PAIR>, dim3(a.splits, a.tiles * a.G, nseg), dim3(TC_THREADS), SMEM, stream, a, timeouts));
   return LIA_OK;
 }
 template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int rows, int nseg, cudaStream_t stream) {

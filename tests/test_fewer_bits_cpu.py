@@ -81,8 +81,8 @@ def test_slots_of_4_bit_rows():
     ({"x_type": 3}, "type"), ({"x_type": -1}, "type"), ({"M": -1}, "sizes"), ({"N": 0}, "sizes"), ({"K": 0}, "sizes"), ({"ldx": 99}, "sizes"), ({"ldw": 99}, "sizes"),
     ({"K": 131072, "ldx": 131072, "ldw": 131072}, "131071"), ({"x": None}, "null"), ({"w": None}, "null"), ({"w_scale": None}, "null"), ({"out": None}, "null"), ({"x_scale": None}, "null"),
     ({"x_type": 0}, "not codes"), ({"w": 264}, "vectors"), ({"ldw": 120}, "vectors"), ({"x": 264}, "vectors"), ({"ldx": 120}, "vectors"),
-    ({"ws": None, "N": 1 << 20, "K": 4096, "ldx": 4096, "ldw": 4096}, "workspace"), ({"bytes": 8, "N": 1 << 20, "K": 4096, "ldx": 4096, "ldw": 4096}, "workspace"),
-    ({"ws": 264, "N": 1 << 20, "K": 4096, "ldx": 4096, "ldw": 4096}, "workspace"), ({"N": 1 << 30, "K": 4096, "ldx": 4096, "ldw": 4096}, "too large"),
+    ({"x_type": 0, "x_scale": None, "ws": None}, "workspace"), ({"x_type": 0, "x_scale": None, "bytes": 400}, "workspace"), ({"x_type": 1, "x_scale": None, "ws": 264}, "workspace"),
+    ({"N": 1 << 30, "K": 131071, "ldx": 131072, "ldw": 131072}, "too large"),
     ({"M": 1 << 30, "N": 1 << 30}, "too large")])
 def test_products_refuse(lib, change, message):
     a = dict(x=256, x_type=2, ldx=112, x_scale=256, w=256, ldw=112, w_scale=256, out=256, f32=0, M=4, N=64, K=100, ws=256, bytes=1 << 30) | change
