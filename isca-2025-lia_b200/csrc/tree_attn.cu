@@ -364,15 +364,21 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
 // How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history
 struct Plan {
   int nr, tiles, splits;                                           // nr: eights of rows; 16 and 32 of them on tcgen05
+  int spans;                                                       // 4 bits, up to eight rows: blocks that share all histories alike (0: `splits` blocks for each)
 };
 // Rows of a key head up to which this file's kernel is taken: above 32 a history would be read a second time here, and with bf16 caches the 32 rows' products, in two parts each, take longer than the
 // history's bytes where it is long.  us, tcgen05 | here: 58 rows behind 4099 positions, 8 sequences and 8 key heads, e4m3 62 | 73, bf16 65 | 114; 64 rows behind 131003, one sequence, int8 121 | 213, bf16 137 | 366;
 // 33 rows behind 280, 64 sequences and 56 key heads, int8 340 | 407, bf16 326 | 541; 17 of them 341 | 225, 322 | 301; 28 behind 1000, 30 sequences and 8 key heads, int8 47 | 41, bf16 51 | 68;
-// 32 behind 131003 int8 121 | 122, bf16 138 | 213; 16 behind as many int8 120 | 86, bf16 136 | 102.
+// 32 behind 131003 int8 121 | 122, bf16 138 | 213; 16 behind as many int8 120 | 86, bf16 136 | 102.  4 bits: 32 behind 131003 128 | 99, 32 behind 8000, 16 sequences and 8 key heads, 131 | 103, 31 behind
+// 280, 64 sequences and 56 key heads, 347 | 232.
 int rows_here(int type, long long span) { return type == LIA_CACHE_BF16 && span > 512 ? 16 : 32; }
 long long span_of(int rows, int max_ctx, int window) { return window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx; }
+// Histories of four bits: up to eight rows of a key head in equal spans of all histories together, which no block has more of than another, and a second launch that joins; or so many blocks a history,
+// and a cluster that joins.  us, spans | splits: a token of 16 requests behind 30001 positions, 16 heads on 8, 135 | 145, of requests behind 21000 to 30001 117 | 136, behind 3000 to 30001 85 | 131; of 32
+// behind 8000, 8 heads on 8 (3459 keys a block) 79 | 82; of 64 behind 2000, 32 heads on 8 (1729) 54 | 49; of 16 behind 1901 (411) 22 | 16.
+constexpr long long SPAN_KEYS = 3000;                              // of a block, from which on
 Plan cut(int nr, long long R, int nseg, int rows, int max_ctx, int G, int window, int type) {
-  Plan p;
+  Plan p{};
   p.nr = nr;
   p.tiles = (int)((R + 8 * p.nr - 1) / (8 * p.nr));
   const long long blocks = (long long)nseg * G * p.tiles, room = (long long)lia_sm_count() * (p.nr >= 16 ? 1 : blocks_an_sm(type, p.nr));
@@ -382,6 +388,7 @@ Plan cut(int nr, long long R, int nseg, int rows, int max_ctx, int G, int window
   if (s > most) s = most;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   p.splits = s < 1 ? 1 : (int)s;
+  if (type == LIA_CACHE_INT4 && nr == 1 && blocks * span >= room * SPAN_KEYS) p.spans = (int)(room / G);
   return p;
 }
 // About how long a plan takes on tcgen05, in us, fitted to 13 measured calls (within a fifth, most of them): a block of threads with up to 128 rows 8 and 0.75 for 64 keys, one with 256 rows 20 and
@@ -404,7 +411,10 @@ Plan plan_of(int nseg, int rows, int max_ctx, int H, int G, int window, int type
   const Plan two = of(32);
   return tc_time(two, R, nseg, rows, max_ctx, G, window) <= tc_time(one, R, nseg, rows, max_ctx, G, window) ? two : one;
 }
-size_t floats_of(const Plan& p, int M, int H, int vdim) { return p.splits > (p.nr >= 16 ? 1 : CLUSTER) ? (size_t)p.splits * M * H * (vdim + 2) : 0; }
+size_t floats_of(const Plan& p, int nseg, int rows, int M, int H, int G, int vdim) {
+  if (p.spans > 0) return ((size_t)nseg + p.spans) * G * rows * (H / G) * (vdim + 2);
+  return p.splits > (p.nr >= 16 ? 1 : CLUSTER) ? (size_t)p.splits * M * H * (vdim + 2) : 0;
+}
 
 template <int DIM, int VDIM, int KIND, int NR> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
   using S = Shape<DIM, VDIM, KIND, NR>;
@@ -425,7 +435,7 @@ template <int DIM, int VDIM, int KIND> int launch_rows(const TreeArgs& a, int nr
   if (nr >= 16) rc = lia_tree_attn_tc(&a, KIND, nr * 8, nseg, stream);
   else if constexpr (KIND == LIA_CACHE_INT4) rc = lia_tree_attn_4bit(&a, nr, nseg, stream);
   else rc = nr == 4 ? launch<DIM, VDIM, KIND, 4>(a, nseg, stream) : nr == 2 ? launch<DIM, VDIM, KIND, 2>(a, nseg, stream) : launch<DIM, VDIM, KIND, 1>(a, nseg, stream);
-  if (rc == LIA_OK && a.splits > (nr >= 16 ? 1 : CLUSTER)) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
+  if (rc == LIA_OK && a.spans == 0 && a.splits > (nr >= 16 ? 1 : CLUSTER)) LIA_CUDA(lia_launch(tree_attn_join_kernel<DIM, VDIM, KIND>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
   return rc;
 }
 template <int KIND> int launch_dims(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
@@ -438,13 +448,13 @@ template <int KIND> int launch_dims(const TreeArgs& a, int nr, int nseg, cudaStr
 extern "C" size_t lia_tree_attn_workspace_floats(int nseg, int rows, int max_ctx, int M, int H, int G, int dim, int vdim, int window, int type) {
   (void)dim;
   if (nseg <= 0 || rows <= 0 || M <= 0 || G <= 0 || H <= 0 || H % G || vdim <= 0) return 0;
-  return floats_of(plan_of(nseg, rows, max_ctx, H, G, window, type), M, H, vdim);
+  return floats_of(plan_of(nseg, rows, max_ctx, H, G, window, type), nseg, rows, M, H, G, vdim);
 }
 
 extern "C" int lia_tree_attn_plan(int nseg, int rows, int max_ctx, int H, int G, int window, int type) {
   if (nseg <= 0 || rows <= 0 || G <= 0 || H <= 0 || H % G) return 0;
   const Plan p = plan_of(nseg, rows, max_ctx, H, G, window, type);
-  return p.splits << 8 | p.nr;
+  return (p.spans > 0 ? 1 << 30 | p.spans << 8 : p.splits << 8) | p.nr;
 }
 
 extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* kc, const LiaCacheView* vc, const int* segs, int nseg, const long long* mask, int words, const int* depth,
@@ -463,10 +473,10 @@ extern "C" int lia_tree_attn(const void* q, long long ldq, const LiaCacheView* k
   LIA_CHECK_ARG(mask == nullptr || rows <= 64 * words, "lia_tree_attn: %d words of mask do not hold %d tokens", words, rows);
   const Plan plan = plan_of(nseg, rows, max_ctx, H, G, window, kc->type);
   LIA_CHECK_ARG(nseg <= 65535 && (long long)plan.tiles * G <= 65535, "lia_tree_attn: too many portions, or rows of one");
-  LIA_CHECK_ARG(floats_of(plan, M, H, vc->dim) == 0 || (ws && ws_floats >= floats_of(plan, M, H, vc->dim) && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_tree_attn: needs a workspace of %zu floats",
-                floats_of(plan, M, H, vc->dim));
+  LIA_CHECK_ARG(floats_of(plan, nseg, rows, M, H, G, vc->dim) == 0 || (ws && ws_floats >= floats_of(plan, nseg, rows, M, H, G, vc->dim) && reinterpret_cast<uintptr_t>(ws) % 16 == 0), "lia_tree_attn: needs a workspace of %zu floats",
+                floats_of(plan, nseg, rows, M, H, G, vc->dim));
   const TreeArgs a{reinterpret_cast<const bf16*>(q), ldq, cache8(kc), cache8(vc), segs, reinterpret_cast<const unsigned long long*>(mask), words, depth, temp,
-                   reinterpret_cast<bf16*>(out), ws, M, H, G, H / G, rows, window > 0 ? window : 1 << 30, plan.splits, plan.tiles, scale, softcap};
+                   reinterpret_cast<bf16*>(out), ws, M, H, G, H / G, rows, window > 0 ? window : 1 << 30, plan.splits, plan.tiles, scale, softcap, nseg, plan.spans};
   switch (kc->type) {
     case LIA_CACHE_BF16: return launch_dims<LIA_CACHE_BF16>(a, plan.nr, nseg, stream);
     case LIA_CACHE_INT8: return launch_dims<LIA_CACHE_INT8>(a, plan.nr, nseg, stream);

@@ -25,6 +25,7 @@ struct TreeArgs {
   float* ws;                                                       // weighted values [splits][M * H][VDIM], then (maximum, sum of weights) [splits][M * H]
   int M, H, G, rep, rows, window, splits, tiles;
   float scale, softcap;
+  int nseg, spans;                                                 // tree_attn_4bit.cu: blocks that share all portions' histories alike (0: `splits` a history)
 };
 
 struct Portion {

@@ -11,7 +11,8 @@
 //   * One or two rows (PACKED; a decoded token of up to two query heads): the eight columns are four quarters of the channels times two rows.  A column's query is nothing but in its quarter, whose
 //     group is one, so that a lane has one scale a key instead of four, and a weight goes into the second product once, not once a group.
 //
-// 16 tokens behind 30001 positions and fewer, 16 heads on 8 (475 MB): 212 us with the 8-bit kernel's structure.
+// 16 tokens behind 21000 to 30001 positions, 16 heads on 8 (475 MB): 117 us, 4.1 TB/s, 62 % of the copy rate; with the 8-bit kernel's structure 207.  What bounds it: instructions, some 350 a warp for 16
+// keys (488 before), half of them on the integer pipe (59 % busy, issue slots 61 %); a fifth block an SM changes nothing.
 #include "mma.cuh"
 #include "tree_attn.cuh"
 
@@ -32,6 +33,11 @@ __device__ __forceinline__ void small4x2(uint32_t w, uint32_t (&r)[4]) {
   const uint32_t x = w >> 8;
   r[2] = x & 0x000f000fu;
   r[3] = x & 0x00f000f0u;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 template <int BYTES> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
@@ -73,70 +79,74 @@ template <int VROW> __device__ __forceinline__ int value_at(int i, int c) {
   return VROW == 64 ? r * 64 + ((c ^ (r & 2)) << 4) : r * VROW + (c << 4);
 }
 
-template <int DIM, int VDIM, int NR, bool PACKED>
-__global__ void __launch_bounds__(THREADS, tree_attn4_blocks(NR)) tree_attn4_kernel(const __grid_constant__ TreeArgs a) {
+// What a block of threads works on: rows r0 .. of a portion and a key head, blocks b0 .. b1 - 1 of 16 keys from position lo on
+struct Piece {
+  int g, r0, lo, hi, all_lo, all_hi, b0, b1;
+};
+template <int DIM, int VDIM, int NR> struct Shared {
+  using S = Four<DIM, VDIM, NR>;
+  float* row_f;                                                    // [ROWS] what a row's products with keys are multiplied by
+  float2* part;                                                    // [WARPS][ROWS] maximum, sum
+  float* row_q;                                                    // [ROWS][KG] -8 2^-24 times the sum of a group's queries
+  uint2* qs;                                                       // [NR][STEPS][32]
+  float* os;                                                       // [WARPS][ROWS][VDIM] weighted values, where queries and rings were
+  __device__ __forceinline__ explicit Shared(uint4* smem) {
+    row_f = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + S::BIG);
+    part = reinterpret_cast<float2*>(row_f + S::ROWS);
+    row_q = reinterpret_cast<float*>(part + WARPS * S::ROWS);
+    qs = reinterpret_cast<uint2*>(smem);
+    os = reinterpret_cast<float*>(smem);
+  }
+};
+
+// leaves the warps' sums in sh.os and sh.part, behind a barrier
+template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ void run_piece(const TreeArgs& a, const Portion& p, const Piece& pc, const Shared<DIM, VDIM, NR>& sh) {
   using S = Four<DIM, VDIM, NR>;
   constexpr bool SMALL = NR == 1;                                  // keys' codes as subnormal numbers
   static_assert(!PACKED || NR == 1, "one or two rows");
-  extern __shared__ uint4 smem[];
-  uint8_t* behind = reinterpret_cast<uint8_t*>(smem) + S::BIG;
-  float* row_f = reinterpret_cast<float*>(behind);                 // [ROWS] what a row's products with keys are multiplied by
-  float2* part = reinterpret_cast<float2*>(row_f + S::ROWS);       // [WARPS][ROWS] maximum, sum
-  float* row_q = reinterpret_cast<float*>(part + WARPS * S::ROWS); // [ROWS][KG] -8 2^-24 times the sum of a group's queries
-  uint2* qs = reinterpret_cast<uint2*>(smem);                      // [NR][STEPS][32]
-  pdl_launch_dependents();
-  pdl_wait();
-  const Portion p = portion_of(a, blockIdx.z);
-  if (!p.held) {
-    if (a.splits <= CLUSTER && blockIdx.x == 0 && blockIdx.y == 0) nan_rows<VDIM>(a, p);
-    return;
-  }
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, gq = lane >> 2, t4 = lane & 3;   // (known to be the same in all lanes)
-  const int tile = blockIdx.y / a.G, g = blockIdx.y - tile * a.G, r0 = tile * S::ROWS, R = p.n * a.rep;
-  if (r0 >= R) return;
-
-  // ---- which keys
-  const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + S::ROWS - 1) / a.rep);
-  int near = i0, far = i1;                                         // depths of the block's tokens
-  if (a.depth != nullptr && a.window < 1 << 30) {                  // (without a window depths do not matter)
-    near = 1 << 29;
-    far = 0;
-    for (int i = i0 + lane; i <= i1; i += 32) {
-      const int d = depth_of(a, p, i);
-      near = min(near, d);
-      far = max(far, d);
-    }
-    near = __reduce_min_sync(0xffffffffu, near);
-    far = __reduce_max_sync(0xffffffffu, far);
-  }
-  const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = min(hi, a.mask != nullptr ? p.p0 : p.p0 + i0 + 1);
-  const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
+  const int g = pc.g, r0 = pc.r0, lo = pc.lo, hi = pc.hi, all_lo = pc.all_lo, all_hi = pc.all_hi, b0 = pc.b0, b1 = pc.b1, R = p.n * a.rep;
+  float* row_f = sh.row_f;
+  float2* part = sh.part;
+  float* row_q = sh.row_q;
+  uint2* qs = sh.qs;
 
   // ---- the ring: a lane brings 16-byte chunks of keys and values lane / CH (and 8 more, where a row has four chunks), lanes 0 .. 15 a key's scales, the others a value's
-  const uint32_t ring = smem_u32(smem) + S::Q_BYTES + warp * DEPTH * S::STAGE;
+  const uint32_t ring = smem_u32(sh.qs) + S::Q_BYTES + warp * DEPTH * S::STAGE;
   constexpr int KCH = S::KROW / 16, VCH = S::VROW / 16, KN = 16 * KCH / 32, VN = 16 * VCH / 32;  // chunks of a row; copies of a lane
-  const uint8_t *kbase = a.k.at(p.slot, 0, g) + lane % KCH * 16, *vbase = a.v.at(p.slot, 0, g) + lane % VCH * 16;
-  const bf16* sbase = lane < 16 ? a.k.scale4_at(p.slot, g) : a.v.scale4_at(p.slot, g);
-  const int sgroups = lane < 16 ? S::KG : S::VG;
+  const int sgroups = lane < 16 ? S::KG : S::VG, start = lo + (b0 + warp) * 16;                // the warp's first block
+  const uint8_t *kp = a.k.at(p.slot, start, g) + lane / KCH * a.k.pos + lane % KCH * 16, *vp = a.v.at(p.slot, start, g) + lane / VCH * a.v.pos + lane % VCH * 16;
+  const bf16* sp = (lane < 16 ? a.k.scale4_at(p.slot, g) : a.v.scale4_at(p.slot, g)) + (long long)(start + (lane & 15)) * sgroups;
+  const long long k_step = WARPS * 16 * a.k.pos, v_step = WARPS * 16 * a.v.pos;
   const uint32_t k_to = lane * 16, s_to = lane < 16 ? S::KS_AT + lane * S::KG * 2 : S::VS_AT + (lane - 16) * S::VG * 2;
   auto bring = [&](int b, int stage) {
     if (b < b1) {
       const uint32_t at = ring + stage * S::STAGE;
-      const int first = lo + b * 16, last = hi - 1 - first;        // keys behind the last one are that one again
+      const int last = hi - 1 - (lo + b * 16);                     // of the block: keys behind it are that one again
+      if (last >= 15) {
 #pragma unroll
-      for (int n = 0; n < KN; ++n) cp_async16(at + k_to + n * 512, kbase + (long long)(first + min(lane / KCH + n * 8, last)) * a.k.pos, 16);
+        for (int n = 0; n < KN; ++n) cp_async16(at + k_to + n * 512, kp + n * 8 * a.k.pos, 16);
 #pragma unroll
-      for (int n = 0; n < VN; ++n) {
-        const int i = lane / VCH + n * 8;
-        cp_async16(at + 16 * S::KROW + value_at<S::VROW>(i, lane % VCH), vbase + (long long)(first + min(i, last)) * a.v.pos, 16);
+        for (int n = 0; n < VN; ++n) cp_async16(at + 16 * S::KROW + value_at<S::VROW>(lane / VCH + n * 8, lane % VCH), vp + n * 8 * a.v.pos, 16);
+      } else {
+#pragma unroll
+        for (int n = 0; n < KN; ++n) cp_async16(at + k_to + n * 512, kp + (long long)(min(lane / KCH + n * 8, last) - lane / KCH) * a.k.pos, 16);
+#pragma unroll
+        for (int n = 0; n < VN; ++n) {
+          const int i = lane / VCH + n * 8;
+          cp_async16(at + 16 * S::KROW + value_at<S::VROW>(i, lane % VCH), vp + (long long)(min(i, last) - lane / VCH) * a.v.pos, 16);
+        }
       }
-      const bf16* src = sbase + (long long)(first + min(lane & 15, last)) * sgroups;
+      const bf16* src = sp + (min(lane & 15, last) - (lane & 15)) * sgroups;
       if constexpr (S::KG == S::VG) {
         cp_async_small<S::KG * 2>(at + s_to, src);
       } else {
         if (lane < 16) cp_async_small<S::KG * 2>(at + s_to, src);
         else cp_async_small<S::VG * 2>(at + s_to, src);
       }
+      kp += k_step;
+      vp += v_step;
+      sp += WARPS * 16 * sgroups;
     }
     cp_async_commit();
   };
@@ -309,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, tree_attn4_blocks(NR)) tree_attn4_ker
       const uint32_t two = S::VG == 4 ? __vmaxu2(vs4[0], vs4[S::VG / 2 - 1]) : vs4[0];
       const float y = max_nan(__uint_as_float(max(two << 16, two & 0xffff0000u)), LEAST_SCALE);
       lv[j] = lg2(y);
-      rv[j] = __fdividef(1.f, y);
+      rv[j] = rcp(y);
       if constexpr (PACKED) {
         ratio[j][0] = lds_bf16(from_at + t4 / (4 / S::VG) * 2) * rv[j];
       } else {
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, tree_attn4_blocks(NR)) tree_attn4_ker
 
   // ---- the warps' parts meet in shared memory
   __syncthreads();                                                 // (queries and rings have been read)
-  float* os = reinterpret_cast<float*>(smem);
+  float* os = sh.os;
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -428,7 +438,181 @@ __global__ void __launch_bounds__(THREADS, tree_attn4_blocks(NR)) tree_attn4_ker
           *reinterpret_cast<float2*>(os + at * VDIM + (n >> 1) * GROUP4 + gq * 4 + (n & 1) * 2) = make_float2(o[r][n][e], o[r][n][2 + e]);
     }
   __syncthreads();
-  meet<DIM, VDIM, LIA_CACHE_INT4, S::ROWS>(a, p, r0, R, g, os, part);
+}
+
+template <int DIM, int VDIM, int NR, bool PACKED>
+__global__ void __launch_bounds__(THREADS, tree_attn4_blocks(NR)) tree_attn4_kernel(const __grid_constant__ TreeArgs a) {
+  using S = Four<DIM, VDIM, NR>;
+  extern __shared__ uint4 smem[];
+  const Shared<DIM, VDIM, NR> sh(smem);
+  pdl_launch_dependents();
+  pdl_wait();
+  const Portion p = portion_of(a, blockIdx.z);
+  if (!p.held) {
+    if (a.splits <= CLUSTER && blockIdx.x == 0 && blockIdx.y == 0) nan_rows<VDIM>(a, p);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const int tile = blockIdx.y / a.G, g = blockIdx.y - tile * a.G, r0 = tile * S::ROWS, R = p.n * a.rep;
+  if (r0 >= R) return;
+
+  // ---- which keys
+  const int i0 = r0 / a.rep, i1 = min(p.n - 1, (r0 + S::ROWS - 1) / a.rep);
+  int near = i0, far = i1;                                         // depths of the block's tokens
+  if (a.depth != nullptr && a.window < 1 << 30) {                  // (without a window depths do not matter)
+    near = 1 << 29;
+    far = 0;
+    for (int i = i0 + lane; i <= i1; i += 32) {
+      const int d = depth_of(a, p, i);
+      near = min(near, d);
+      far = max(far, d);
+    }
+    near = __reduce_min_sync(0xffffffffu, near);
+    far = __reduce_max_sync(0xffffffffu, far);
+  }
+  const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = min(hi, a.mask != nullptr ? p.p0 : p.p0 + i0 + 1);
+  const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
+  run_piece<DIM, VDIM, NR, PACKED>(a, p, Piece{g, r0, lo, hi, all_lo, all_hi, b0, b1}, sh);
+  meet<DIM, VDIM, LIA_CACHE_INT4, S::ROWS>(a, p, r0, R, g, sh.os, sh.part);
+}
+
+// ---- All histories as one list of units of 64 keys (16 for each warp), of which every block of a key head has the same number, whatever the histories' lengths: its span may end one history and begin
+// others.  (The heads' blocks of the same span are neighbours: they bring the same positions at the same time, and with them whole lines of memory.)  Span c of head g leaves what it has of portion z in
+// slot (z + c) G + g of the workspace, which no other pair (z, c) has, and a second launch joins.
+__device__ __forceinline__ int units_of(const TreeArgs& a, int z, int& lo) {
+  const Portion p = portion_of(a, z);
+  lo = p.held && p.n > 0 ? first_key(a, p, 0) : 0;                 // (of the least depth there can be)
+  return p.held && p.n > 0 ? (p.p0 + p.n - lo + WARPS * 16 - 1) / (WARPS * 16) : 0;
+}
+// by a warp: the portion that unit `u` of the list lies in (a.nseg: behind all of them), how many units come before its first, and how many its history has; u < 0: all units together in `before`
+struct Place {
+  int z, units;
+  long long before;
+};
+__device__ __forceinline__ Place place_in_list(const TreeArgs& a, long long u) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int z0 = 0; z0 < a.nseg; z0 += 32) {
+    int lo;
+    const int mine = z0 + lane < a.nseg ? units_of(a, z0 + lane, lo) : 0;
+    long long sum = mine;                                          // up to and with this lane's portion
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    const unsigned behind = u < 0 ? 0u : __ballot_sync(0xffffffffu, before + sum > u);
+    if (behind) {
+      const int l = __ffs(behind) - 1, n = __shfl_sync(0xffffffffu, mine, l);
+      return {z0 + l, n, before + __shfl_sync(0xffffffffu, sum, l) - n};
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {a.nseg, 0, before};
+}
+
+template <int DIM, int VDIM, bool PACKED> __global__ void __launch_bounds__(THREADS, tree_attn4_blocks(1)) tree_attn4_spans_kernel(const __grid_constant__ TreeArgs a) {
+  using S = Four<DIM, VDIM, 1>;
+  constexpr int N = VDIM / 32;
+  extern __shared__ uint4 smem[];
+  const Shared<DIM, VDIM, 1> sh(smem);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, most = a.rows * a.rep;
+  const long long total = place_in_list(a, -1).before, blocks = min((long long)a.spans, total);       // (no block without a unit)
+  const int span = blockIdx.x / a.G, g = blockIdx.x - span * a.G;
+  if (span >= blocks) return;
+  const long long end = total * (span + 1) / blocks;
+  long long u = total * span / blocks;
+  while (u < end) {
+    const Place at = place_in_list(a, u);
+    const int z = __shfl_sync(0xffffffffu, at.z, 0), units = __shfl_sync(0xffffffffu, at.units, 0), from = (int)(u - at.before), to = (int)min((long long)units, from + (end - u));
+    const Portion p = portion_of(a, z);
+    int lo;
+    units_of(a, z, lo);
+    {
+      const int hi = p.p0 + p.n, last = p.n - 1;
+      int far = last;
+      if (a.depth != nullptr && a.window < 1 << 30) {
+        far = lane <= last ? depth_of(a, p, min(lane, last)) : 0;  // (eight tokens at most)
+        far = __reduce_max_sync(0xffffffffu, far);
+      }
+      const int nb = (hi - lo + 15) >> 4;
+      run_piece<DIM, VDIM, 1, PACKED>(a, p, Piece{g, 0, lo, hi, first_key(a, p, far), min(hi, a.mask != nullptr ? p.p0 : p.p0 + 1), from * WARPS, min(nb, to * WARPS)}, sh);
+      // the warps' sums together, into the slot
+      const long long slot = (long long)(z + span) * a.G + g, slots = (long long)(a.nseg + a.spans) * a.G;
+      for (int r = warp; r < p.n * a.rep; r += WARPS) {
+        float top = NONE, sum = 0.f, y[N] = {};
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sh.part[w * S::ROWS + r].x);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float2 x = sh.part[w * S::ROWS + r];
+          const float f = ex2(x.x - top);
+          sum = fmaf(x.y, f, sum);
+#pragma unroll
+          for (int c = 0; c < N; ++c) y[c] = fmaf(sh.os[(w * S::ROWS + r) * VDIM + lane * N + c], f, y[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < N; ++c) a.ws[(slot * most + r) * VDIM + lane * N + c] = y[c];
+        if (lane == 0) reinterpret_cast<float2*>(a.ws + slots * most * VDIM)[slot * most + r] = make_float2(top, sum);
+      }
+      __syncthreads();                                             // (before the next piece's rings and queries)
+      u += to - from;
+    }
+  }
+}
+
+// Warp per (row, head): the parts that blocks c0 .. c1 have left of its history, always in the same order
+template <int DIM, int VDIM> __global__ void __launch_bounds__(128) tree_attn4_join_kernel(const __grid_constant__ TreeArgs a) {
+  constexpr int N = VDIM / 32;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int z = blockIdx.y, lane = threadIdx.x & 31, at = blockIdx.x * 4 + (threadIdx.x >> 5), i = at / a.H, h = at - i * a.H, most = a.rows * a.rep;
+  const Portion p = portion_of(a, z);
+  if (!p.held) {
+    if (blockIdx.x == 0) nan_rows<VDIM>(a, p);
+    return;
+  }
+  if (i >= p.n) return;
+  const int g = h / a.rep, r = i * a.rep + h - g * a.rep;
+  int lo;
+  const int units = units_of(a, z, lo);
+  long long before = 0, total = 0;                                 // units of the portions before, and of all
+  for (int x = lane; x < a.nseg; x += 32) {
+    int unused;
+    const int n = units_of(a, x, unused);
+    total += n;
+    if (x < z) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  const long long blocks = min((long long)a.spans, total);
+  const int c0 = (int)(((before + 1) * blocks - 1) / total), c1 = (int)(((before + units) * blocks - 1) / total);            // (block c begins with unit total * c / blocks, rounded down)
+  const long long slots = (long long)(a.nseg + a.spans) * a.G;
+  auto slot = [&](int c) { return ((long long)(z + c) * a.G + g) * most + r; };
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + slots * most * VDIM);
+  float top = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, ml[slot(c)].x);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float o[N] = {}, l = 0.f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const float2 x = ml[slot(c)];
+    const float f = ex2(x.x - base);
+    const float* src = a.ws + slot(c) * VDIM + lane * N;
+    l = fmaf(x.y, f, l);
+    float w[N];
+    if constexpr (N == 4) *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(src);
+    else *reinterpret_cast<float2*>(w) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = fmaf(w[e], f, o[e]);
+  }
+  put_row<DIM, VDIM, LIA_CACHE_INT4>(a, p, i, h, o, l);
 }
 
 template <int DIM, int VDIM, int NR, bool PACKED> int launch(const TreeArgs& a, int nseg, cudaStream_t stream) {
@@ -446,10 +630,18 @@ template <int DIM, int VDIM, int NR, bool PACKED> int launch(const TreeArgs& a, 
   else LIA_CUDA(lia_launch(tree_attn4_kernel<DIM, VDIM, NR, PACKED>, grid, dim3(THREADS), S::SMEM, stream, a));
   return LIA_OK;
 }
+template <int DIM, int VDIM, bool PACKED> int launch_spans(const TreeArgs& a, int nseg, cudaStream_t stream) {
+  static_assert(Four<DIM, VDIM, 1>::SMEM <= 48 * 1024, "shared memory");
+  LIA_CUDA(lia_launch(tree_attn4_spans_kernel<DIM, VDIM, PACKED>, dim3(a.spans * a.G), dim3(THREADS), (size_t)Four<DIM, VDIM, 1>::SMEM, stream, a));
+  LIA_CUDA(lia_launch(tree_attn4_join_kernel<DIM, VDIM>, dim3((unsigned)(((long long)a.rows * a.H + 3) / 4), nseg), dim3(128), 0, stream, a));
+  return LIA_OK;
+}
 template <int DIM, int VDIM> int launch_rows(const TreeArgs& a, int nr, int nseg, cudaStream_t stream) {
+  const bool packed = a.rows * a.rep <= 2;
   if (nr == 4) return launch<DIM, VDIM, 4, false>(a, nseg, stream);
   if (nr == 2) return launch<DIM, VDIM, 2, false>(a, nseg, stream);
-  return a.rows * a.rep <= 2 ? launch<DIM, VDIM, 1, true>(a, nseg, stream) : launch<DIM, VDIM, 1, false>(a, nseg, stream);
+  if (a.spans > 0) return packed ? launch_spans<DIM, VDIM, true>(a, nseg, stream) : launch_spans<DIM, VDIM, false>(a, nseg, stream);
+  return packed ? launch<DIM, VDIM, 1, true>(a, nseg, stream) : launch<DIM, VDIM, 1, false>(a, nseg, stream);
 }
 
 }  // namespace

@@ -313,3 +313,54 @@ def test_waits_that_run_out(nowait, monkeypatch, ops, H, max_ctx):  # noqa: F811
     torch.cuda.synchronize()
     c.check(again)
     c.check(c.run(ops, max_ctx=max_ctx))
+
+
+@pytest.mark.parametrize("dim,vdim", DIMS)
+@pytest.mark.parametrize("H,G,n,masked,window", [(8, 8, 1, False, 0), (16, 8, 1, False, 0), (32, 8, 2, False, 0), (8, 8, 8, True, 0), (16, 8, 4, True, 700), (24, 8, 1, False, 1500), (56, 56, 1, False, 0)])
+def test_histories_of_unequal_lengths_in_equal_spans(ops, dim, vdim, H, G, n, masked, window):
+    """Long histories of up to eight rows are cut into equal spans over all requests: spans that end one history and begin the next, portions of no tokens, a slot that is not there, histories of nothing,
+    rows that see nothing; and the same bits again, and from a graph with other lengths in it."""
+    past = [7003, 0, 64, 2000, 1, 12345, 63, 65, 300, 4097, 0]
+    portions = [(i, p, 0 if i == 6 else max(1, n - i % 3)) for i, p in enumerate(past)]
+    tree = lambda m: family(m, lambda i: (i - 1) // 2 if i else -1)  # noqa: E731
+    deep = [[int(tree(m)[i].sum()) - 1 for i in range(m)] for _, _, m in portions] if masked else None
+    c = Case4(portions, H, G, dim, vdim, mask=[tree(m) for _, _, m in portions] if masked else None, depth=deep, window=window, gap=1)
+    if masked:
+        c.mask[c.segs[10][2]] = 0                                           # without history: this row sees nothing
+        c.sees[10][0] = False
+    long = 3_000_000 // (G * len(portions)) * 2                             # enough for spans, whatever is there
+    from lia_b200 import _lib
+    assert _lib.load().lia_tree_attn_plan(len(portions), n, long, H, G, window, 3) >> 30 or window
+    out = c.run(ops, rows=n, max_ctx=long).clone()
+    c.check(out)
+    assert torch.equal(out, c.run(ops, rows=n, max_ctx=long, out=torch.full_like(out, 77.0)))
+    lost = c.segs[3]
+    c.segs[3] = (99, *lost[1:])
+    gone = c.run(ops, rows=n, max_ctx=long, out=torch.full_like(out, 77.0))
+    assert torch.isnan(gone[lost[2]:lost[2] + lost[3]].float()).all()
+    gone[lost[2]:lost[2] + lost[3]] = out[lost[2]:lost[2] + lost[3]]
+    c.segs[3] = lost
+    c.check(gone)
+    segs, again = torch.tensor(c.segs, dtype=torch.int32, device="cuda"), torch.full_like(out, 77.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.tree_attn(c.q, c.kc, c.vc, segs, again, H, G, dim, vdim, c.scale, rows=n, max_ctx=long, mask=c.mask, depth=c.depth, window=window, k_scale=c.ks, v_scale=c.vs)
+    order = torch.randperm(len(portions), generator=torch.Generator().manual_seed(1)).tolist()
+    segs.copy_(torch.tensor([c.segs[i] for i in order], dtype=torch.int32))  # (in another order, spans are others: sums of the same numbers)
+    graph.replay()
+    torch.cuda.synchronize()
+    c.check(again)
+    segs.copy_(torch.tensor([(s, 0, r, 0) for s, _, r, _ in c.segs], dtype=torch.int32))      # nothing at all
+    again.fill_(77.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (again == 77).all()
+
+
+@pytest.mark.parametrize("n", [1, 4])
+def test_weights_that_average_out(ops, n):
+    """40000 keys of nearly equal weight: what their values average out to is a hundredth of the values, and as exact."""
+    c = Case4([(0, 40000, n), (1, 39000, n)], 4, 2, 128, 128)
+    c.q *= 0.02
+    c.check(c.run(ops))
+    c.check(c.run(ops, max_ctx=4_000_000))
