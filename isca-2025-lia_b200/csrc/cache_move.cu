@@ -2,7 +2,7 @@
 // all layers in one launch (in groups of MOST tensors), of any type and with positions anywhere among their dimensions, as bytes.
 //
 //   fork      slot `to` gets positions 0 .. count - 1 of slot `from`, and its whole state where a tensor has no positions.  A block brings 16 KB of a source once and writes it to every slot that is to
-//             get it, four vectors a thread on their way at a time.
+//             get it, two vectors a thread on their way at a time, four blocks an SM (with four vectors two blocks fit, 54 us instead of 48 for a prompt of 2049 tokens to 7 slots, 268 MB).
 //   compact   position p0 + i of a portion's slot gets position p0 + kept[i], for ascending kept.  A thread has a column of the rows and takes them in order, eight at a time: kept[i] >= i, so what is
 //             written (up to the i-th place) lies before all that is still to be read, and no two threads share a byte.
 //
@@ -11,7 +11,8 @@
 
 namespace {
 
-constexpr int MOST = 64, THREADS = 256, HELD = 4, CHUNK = THREADS * HELD * 16, BATCH = 8;
+constexpr int MOST = 64, THREADS = 256, HELD = 2, CHUNK = 16384, BATCH = 8;
+constexpr int COLUMNS = 64;                                        // threads of a block that compacts: a row is 32 to 128 vectors, scales 8 (with 256 threads 64 portions of 60 tensors took 9.9 us)
 
 struct Tensor {
   uint8_t* data;
@@ -25,7 +26,7 @@ struct Tensors {
 };
 
 template <typename V>
-__device__ __forceinline__ void fork_chunk(const Tensor& t, const int* copies, int c, int n, int slots, int most, int capacity, long long first) {
+__device__ __forceinline__ void fork_chunk_of(const Tensor& t, const int* copies, int c, int n, int slots, int most, int capacity, long long first) {
   const int end = (int)min((long long)t.per, (long long)most - first);                         // positions of this chunk
   const unsigned vpp = (unsigned)(t.bytes / sizeof(V)), run = t.pos == t.bytes ? (unsigned)end * vpp : vpp, outer = t.pos == t.bytes ? (unsigned)t.pieces : (unsigned)(end * t.pieces);
   const uint8_t* src = t.data + copies[3 * c] * t.slot + first * t.pos;
@@ -60,8 +61,13 @@ __device__ __forceinline__ void fork_chunk(const Tensor& t, const int* copies, i
   }
 }
 
+// (apart, so that the narrow ones do not cost the wide one registers)
+template <typename V> __device__ __noinline__ void fork_chunk(const Tensor& t, const int* copies, int c, int n, int slots, int most, int capacity, long long first) {
+  fork_chunk_of<V>(t, copies, c, n, slots, most, capacity, first);
+}
+
 // Grid: copies, chunks of positions, tensors
-__global__ void __launch_bounds__(THREADS) cache_fork_kernel(const __grid_constant__ Tensors all, const int* __restrict__ copies, int n, int slots, int capacity) {
+__global__ void __launch_bounds__(THREADS, 4) cache_fork_kernel(const __grid_constant__ Tensors all, const int* __restrict__ copies, int n, int slots, int capacity) {
   pdl_launch_dependents();
   pdl_wait();
   const Tensor& t = all.t[blockIdx.z];
@@ -75,7 +81,7 @@ __global__ void __launch_bounds__(THREADS) cache_fork_kernel(const __grid_consta
       if (copies[3 * j] == from) most = max(most, min(copies[3 * j + 2], capacity));
   for (long long first = (long long)blockIdx.y * t.per; first < most; first += (long long)gridDim.y * t.per) {
     switch (t.vec) {
-      case 16: fork_chunk<uint4>(t, copies, c, n, slots, most, capacity, first); break;
+      case 16: fork_chunk_of<uint4>(t, copies, c, n, slots, most, capacity, first); break;
       case 8: fork_chunk<uint2>(t, copies, c, n, slots, most, capacity, first); break;
       case 4: fork_chunk<uint32_t>(t, copies, c, n, slots, most, capacity, first); break;
       case 2: fork_chunk<uint16_t>(t, copies, c, n, slots, most, capacity, first); break;
@@ -113,14 +119,14 @@ __device__ __forceinline__ void compact_column(const Tensor& t, uint8_t* base, c
 }
 
 // Grid: columns of the rows, tensors, portions
-__global__ void __launch_bounds__(THREADS) cache_compact_kernel(const __grid_constant__ Tensors all, const int* __restrict__ segs, const int* __restrict__ kept, int most, int slots, int capacity) {
+__global__ void __launch_bounds__(COLUMNS) cache_compact_kernel(const __grid_constant__ Tensors all, const int* __restrict__ segs, const int* __restrict__ kept, int most, int slots, int capacity) {
   pdl_launch_dependents();
   pdl_wait();
   const Tensor& t = all.t[blockIdx.y];
   const int* s = segs + 4ll * blockIdx.z;
   const int slot = s[0], p0 = s[1], n = s[3];
   if ((unsigned)slot >= (unsigned)slots || p0 < 0 || n <= 0 || n > capacity || p0 > capacity - n) return;
-  const unsigned column = blockIdx.x * THREADS + threadIdx.x;
+  const unsigned column = blockIdx.x * COLUMNS + threadIdx.x;
   if (column >= (unsigned)(t.bytes / t.vec) * (unsigned)t.pieces) return;
   uint8_t* base = t.data + slot * t.slot + p0 * t.pos;
   const int* list = kept + (long long)blockIdx.z * most;
@@ -190,7 +196,7 @@ extern "C" int lia_cache_compact(const LiaCacheRows* tensors, int n_tensors, int
       const long long c = all.t[i].bytes / all.t[i].vec * all.t[i].pieces;
       if (c > columns) columns = c;
     }
-    LIA_CUDA(lia_launch(cache_compact_kernel, dim3((unsigned)((columns + THREADS - 1) / THREADS), m, nseg), dim3(THREADS), 0, reinterpret_cast<cudaStream_t>(stream), all, segs, kept, most, slots,
+    LIA_CUDA(lia_launch(cache_compact_kernel, dim3((unsigned)((columns + COLUMNS - 1) / COLUMNS), m, nseg), dim3(COLUMNS), 0, reinterpret_cast<cudaStream_t>(stream), all, segs, kept, most, slots,
                         capacity));
   }
   return LIA_OK;

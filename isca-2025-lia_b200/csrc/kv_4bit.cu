@@ -36,20 +36,57 @@ __device__ __forceinline__ Head head_of(unsigned block, const int* meta, int M, 
   return h;
 }
 
-template <typename T> __device__ __forceinline__ void load4(const T* p, bool vec, float* x) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec) {
-      const uint2 u = __ldcg(reinterpret_cast<const uint2*>(p));
-      unpack_bf16x2(u.x, x[0], x[1]);
-      unpack_bf16x2(u.y, x[2], x[3]);
-      return;
-    }
-  } else if (vec) {
-    *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(p));
-    return;
-  }
+// Four numbers as they come
+template <typename T> struct Raw4 {
+  uint32_t w[sizeof(T)];
+};
+template <typename T> __device__ __forceinline__ Raw4<T> load4(const T* p, bool vec) {
+  Raw4<T> r;
+  if (vec) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(r.w) = __ldcg(reinterpret_cast<const uint2*>(p));
+    else *reinterpret_cast<uint4*>(r.w) = ldg_act(p);
+  } else {
+    T t[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (float)p[i];
+    for (int i = 0; i < 4; ++i) t[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) r.w[i] = reinterpret_cast<const uint32_t*>(t)[i];
+  }
+  return r;
+}
+template <typename T> __device__ __forceinline__ void numbers_of(const Raw4<T>& r, float* x) {
+  if constexpr (sizeof(T) == 2) {
+    unpack_bf16x2(r.w[0], x[0], x[1]);
+    unpack_bf16x2(r.w[1], x[2], x[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r.w[i]);
+  }
+}
+// The bits of four groups' largest magnitudes, for the eight lanes of a head (as whole numbers NaN is above infinity and that above the rest)
+template <typename T> __device__ __forceinline__ void most_of(const Raw4<T>* raw, uint32_t* most) {
+  if constexpr (sizeof(T) == 2) {                                  // two groups of 16 bits at a time
+    uint32_t m[AT_ONCE];
+#pragma unroll
+    for (int g = 0; g < AT_ONCE; ++g) m[g] = __vmaxu2(raw[g].w[0] & 0x7fff7fffu, raw[g].w[1] & 0x7fff7fffu);
+#pragma unroll
+    for (int g = 0; g < AT_ONCE; g += 2) {
+      uint32_t two = __vmaxu2(__byte_perm(m[g], m[g + 1], 0x5410), __byte_perm(m[g], m[g + 1], 0x7632));
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, o));
+      most[g] = two << 16;
+      most[g + 1] = two & 0xffff0000u;
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < AT_ONCE; ++g) {
+      most[g] = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most[g] = max(most[g], raw[g].w[i] & 0x7fffffffu);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) most[g] = max(most[g], __shfl_xor_sync(0xffffffffu, most[g], o));
+    }
+  }
 }
 template <typename T> __device__ __forceinline__ void store4(T* p, bool vec, const float* x) {
   if constexpr (sizeof(T) == 2) {
@@ -69,6 +106,13 @@ template <typename T> __device__ __forceinline__ void store4(T* p, bool vec, con
 __device__ __forceinline__ float quotient(float x, float d, float inv) {
   const float q = x * inv;
   return fmaf(fmaf(-d, q, x), inv, q);
+}
+
+// 1 / d of a number of 8 bits, correctly rounded (an inverse of 8 bits is further than 2^-33 of itself from a border between numbers of 24)
+__device__ __forceinline__ float inverse(float d) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d));
+  return fmaf(fmaf(-d, y, 1.f), y, y);
 }
 
 // `n` numbers of 16 bits, as wide as a lane's n groups of ng lie; eight lanes' are neighbours
@@ -97,6 +141,8 @@ __device__ __forceinline__ void get_units(const uint16_t* src, int ng, int n, ui
   }
 }
 
+constexpr float ROUND = 12582912.f;                                // 1.5 * 2^23: what is added to it is rounded to a whole number
+
 // Grid: blocks of heads of k and, behind them, of v
 template <typename T>
 __global__ void __launch_bounds__(THREADS) kv_store_4bit_kernel(const __grid_constant__ Side k, const __grid_constant__ Side v, const int* __restrict__ meta, int M, int G, int blocks, float eps) {
@@ -107,12 +153,12 @@ __global__ void __launch_bounds__(THREADS) kv_store_4bit_kernel(const __grid_con
   const Head h = head_of(is_v ? blockIdx.x - blocks : blockIdx.x, meta, M, G);
   const int ng = s.c.dim / GROUP4;
   const T* src = reinterpret_cast<const T*>(s.x) + h.row * s.ld + h.g * s.c.dim + h.q * 4;
-  float x[AT_ONCE][4];
+  Raw4<T> raw[AT_ONCE];
   auto load = [&](int g0) {
 #pragma unroll
     for (int g = 0; g < AT_ONCE; ++g) {
-      x[g][0] = x[g][1] = x[g][2] = x[g][3] = 0.f;
-      if (h.there && g0 + g < ng) load4(src + (g0 + g) * GROUP4, s.vec, x[g]);
+      raw[g] = Raw4<T>{};
+      if (h.there && g0 + g < ng) raw[g] = load4(src + (g0 + g) * GROUP4, s.vec);
     }
   };
   load(0);
@@ -123,13 +169,18 @@ __global__ void __launch_bounds__(THREADS) kv_store_4bit_kernel(const __grid_con
       if (g0 > 0) load(g0);
       float part[AT_ONCE];
 #pragma unroll
-      for (int g = 0; g < AT_ONCE; ++g) part[g] = fmaf(x[g][0], x[g][0], x[g][1] * x[g][1]) + fmaf(x[g][2], x[g][2], x[g][3] * x[g][3]);
+      for (int g = 0; g < AT_ONCE; ++g) {
+        float x[4];
+        numbers_of(raw[g], x);
+        part[g] = fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]);
+      }
       sum += (part[0] + part[1]) + (part[2] + part[3]);
     }
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     root = sqrtf(sum / (float)s.c.dim + eps);
     inv_root = 1.f / root;
+    if (root > 3.402823466e38f) root = 0.f;                        // (quotients are 0, and stay so)
     if (ng > AT_ONCE) load(0);
   }
   const bool held = s.c.holds(h.slot, h.pos);
@@ -138,31 +189,35 @@ __global__ void __launch_bounds__(THREADS) kv_store_4bit_kernel(const __grid_con
   for (int g0 = 0; g0 < ng; g0 += AT_ONCE) {
     if (g0 > 0) load(g0);
     uint32_t most[AT_ONCE], units[AT_ONCE], sc[AT_ONCE];
+    most_of(raw, most);
 #pragma unroll
     for (int g = 0; g < AT_ONCE; ++g) {
-      if (s.norm) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[g][i] = root > 3.402823466e38f ? x[g][i] * 0.f : quotient(x[g][i], root, inv_root);
-      }
-      most[g] = 0u;                                                // magnitudes as whole numbers: NaN is above infinity and that above the rest
-#pragma unroll
-      for (int i = 0; i < 4; ++i) most[g] = max(most[g], __float_as_uint(x[g][i]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) most[g] = max(most[g], __shfl_xor_sync(0xffffffffu, most[g], o));
-      const bool bad = most[g] >= 0x7f800000u;
-      const __nv_bfloat16 s16 = __float2bfloat16_rn(fmaxf(__uint_as_float(most[g]), LEAST) / 7.f);
-      const float scale = bad ? 1.f : __bfloat162float(s16), inv = __frcp_rn(scale);
+      float a = __uint_as_float(most[g]), x[4], c[4];
+      if (s.norm) a = quotient(a, root, inv_root);                 // (the largest before, divided as it is: rounding keeps order)
+      const bool bad = !(a <= 3.402823466e38f);
+      a = bad ? 1.f : fmaxf(a, LEAST);
+      const __nv_bfloat16 s16 = __float2bfloat16_rn(quotient(a, 7.f, 1.f / 7.f));
+      const float scale = __bfloat162float(s16), inv = inverse(scale);
       sc[g] = bad ? 0x7fc0u : (uint32_t)__bfloat16_as_ushort(s16);
-      uint32_t u = 0u;
+      numbers_of(raw[g], x);
+      if (s.norm) {                                                // (the root is off by more than these two products)
+        const float f = inv_root * inv;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // rint of the quotient that is rounded to 24 bits; where that made a tie of it, the exact rest (12 bits times 8, below x: no rounding) tells on which side it was
-        float c = rintf(quotient(x[g][i], scale, inv));
-        const float rest = fmaf(-c, scale, x[g][i]);
-        if (sizeof(T) == 4 || s.norm) c += fabsf(rest) > 0.5f * scale ? copysignf(1.f, rest) : 0.f;
-        u |= (uint32_t)((bad ? 0 : (int)c) + 8) << (4 * i);
+        for (int i = 0; i < 4; ++i) c[i] = fmaf(x[i], f, ROUND) - ROUND;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          c[i] = (quotient(x[i], scale, inv) + ROUND) - ROUND;
+          // where rounding the quotient to 24 bits made a tie of it, the exact rest (a code times 8 bits) tells on which side it was; of two numbers of 8 bits it is a tie or far from one
+          if (sizeof(T) == 4) {
+            const float rest = fmaf(-c[i], scale, x[i]);
+            c[i] += fabsf(rest) > 0.5f * scale ? copysignf(1.f, rest) : 0.f;
+          }
+        }
       }
-      units[g] = u;
+      // four codes + 8 as the lowest 16 bits of a float
+      const float sum = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + (8388608.f + 0x8888);
+      units[g] = bad ? 0x8888u : __float_as_uint(sum) & 0xffffu;
     }
     if (!held) continue;
     const int n = min(AT_ONCE, ng - g0);

@@ -1463,10 +1463,10 @@ def _cache4_view(what, cache, scale, heads, dim, dev, shape, strides):
     slots, capacity, groups = shape[0], shape[1], dim // GROUP4
     if strides[-1] != 1:
         raise _lib.LiaError(f"{what}: its channels have to be neighbours, strides are {strides}")
-    if scale is None or scale.dtype is not BF16 or scale.get_device() != dev or tuple(scale.shape) != (slots, heads, capacity, groups):
+    if scale is None or scale.dtype is not BF16 or scale.shape != (slots, heads, capacity, groups) or scale.get_device() != dev:
         raise _lib.LiaError(f"{what} is of 4 bits and needs bf16 scales [slots, {heads}, capacity, {groups}] on the current CUDA device")
     apart = scale.stride()
-    if (groups > 1 and apart[3] != 1) or (capacity > 1 and apart[2] != groups):
+    if (apart[3] != 1 and groups > 1) or (apart[2] != groups and capacity > 1):
         raise _lib.LiaError(f"{what}: the scales of a head have to be neighbours, strides are {apart}")
     return _lib.LiaCacheView(cache.data_ptr(), scale.data_ptr(), strides[0], strides[1], head, apart[0], apart[1], slots, capacity, _lib.CACHE_INT4, dim)
 
