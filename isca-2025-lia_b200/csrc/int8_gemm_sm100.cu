@@ -44,6 +44,20 @@ template <typename T, int Q_THREADS> __global__ void __launch_bounds__(Q_THREADS
   const T* src = reinterpret_cast<const T*>(a.x) + (long long)blockIdx.x * a.ldx;
   auto load = [&](int v) {                                         // numbers behind the row's end are zeros
     if (v >= vecs) return Raw8<T>{};
+    if constexpr (sizeof(T) == 2) {                                // rows of bf16 on 2-byte boundaries: by words of 4 bytes, of which only a row's first and last could lie outside it
+      if (!a.vec && v > 0 && v * 8 + 8 < a.K) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(src + v * 8);
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+        uint32_t u[5];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = p[i];
+        const bool half = at & 2;
+        u[4] = half ? p[4] : 0u;
+        Raw8<T> r;
+        r.u[0] = half ? make_uint4(__byte_perm(u[0], u[1], 0x5432), __byte_perm(u[1], u[2], 0x5432), __byte_perm(u[2], u[3], 0x5432), __byte_perm(u[3], u[4], 0x5432)) : make_uint4(u[0], u[1], u[2], u[3]);
+        return r;
+      }
+    }
     if (v * 8 + 8 <= a.K) return load8(src + v * 8, a.vec);
     T r[8];
 #pragma unroll
@@ -110,7 +124,8 @@ __device__ __forceinline__ void mma_i8_pair_if(uint32_t one, uint32_t d, uint64_
 
 template <bool FEW, int BN, bool PAIR> struct Shape {
   static constexpr int A_BYTES = TILE * KB, B_BYTES = (PAIR ? BN / 2 : BN) * KB, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGING = FEW ? 0 : 4 * 4096;               // 32 rows of 128 bytes for each epilogue warp
+  static constexpr int OUT_WARPS = FEW ? 4 : 8, THREADS = 128 + 32 * OUT_WARPS;                // warps that take sums to outputs: two for 32 rows of a tile
+  static constexpr int STAGING = FEW ? 0 : OUT_WARPS * 2048;       // 32 rows of 64 bytes for each of them
   static constexpr int STAGES = ((FEW ? 112640 : 228352) - STAGING) / STAGE > 8 ? 8 : ((FEW ? 112640 : 228352) - STAGING) / STAGE;    // (of FEW's, two blocks fit an SM)
   static constexpr int BARS = STAGES * STAGE + STAGING;
   static constexpr int SCALES = (BARS + (2 * STAGES + 5) * 8 + 8 + 15) / 16 * 16, SMEM = SCALES + (FEW ? BN : 2 * BN) * 4 + 1024;   // of the tokens, or of two tiles' channels
@@ -162,8 +177,9 @@ template <bool OUT32> __device__ __forceinline__ void put_one(void* out, size_t 
 }
 
 template <bool FEW, int BN, bool PAIR, bool OUT32>
-__global__ void __launch_bounds__(256, FEW ? 2 : 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Args p) {
   static_assert(!PAIR || (!FEW && BN == 256), "CTA pairs: 256 x 256 tiles");
+  static_assert(FEW || BN >= 64, "two warps share the columns");
   using L = Shape<FEW, BN, PAIR>;
   constexpr int STAGES = L::STAGES;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;             // of a pair the first issues every product and owns the barriers that loads and epilogues arrive on
@@ -192,7 +208,7 @@ __global__ void __launch_bounds__(256, FEW ? 2 : 1) int8_gemm_kernel(const __gri
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull(a), 1);
-      mbar_init(tempty(a), PAIR ? 8 : 4);
+      mbar_init(tempty(a), L::OUT_WARPS * (PAIR ? 2 : 1));
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -304,13 +320,14 @@ __global__ void __launch_bounds__(256, FEW ? 2 : 1) int8_gemm_kernel(const __gri
     }
   } else if (warp >= 4) {
     // ================================================================ sums to outputs
-    const int ew = warp - 4;                                       // TMEM lanes 32 ew .. 32 ew + 31
+    const int ew = warp & 3, half = (warp - 4) >> 2;               // TMEM lanes 32 ew .. 32 ew + 31; of MANY's two warps for them each has every other 32 columns
+    auto out_warps_meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(L::OUT_WARPS * 32) : "memory"); };
     pdl_wait();
     float* scales_s = reinterpret_cast<float*>(smem_gen + L::SCALES);                          // (read one by one between the outputs' stores they cost an L2 round trip each: 128 tokens 30 us)
     if (FEW) {
       const int i = ew * 32 + lane;
       if (i < BN) scales_s[i] = i < p.M ? __ldcg(p.sx + i) : 0.f;
-      epi_bar_sync();
+      out_warps_meet();
     }
     Sched<FEW> s(p, PAIR);
     Work w;
@@ -319,8 +336,8 @@ __global__ void __launch_bounds__(256, FEW ? 2 : 1) int8_gemm_kernel(const __gri
     bool alive = true;
     while (s.next(w)) {
       if (!FEW) {                                                  // the channels' scales, while the sums are on their way; zeros behind the last (the buffer before the last tile's has been read)
-        for (int i = ew * 32 + lane; i < BN; i += 128) scales_s[acc * BN + i] = w.tb * BN + i < p.N ? __ldg(p.sw + w.tb * BN + i) : 0.f;
-        epi_bar_sync();
+        for (int i = threadIdx.x - 128; i < BN; i += L::OUT_WARPS * 32) scales_s[acc * BN + i] = w.tb * BN + i < p.N ? __ldg(p.sw + w.tb * BN + i) : 0.f;
+        out_warps_meet();
       }
       alive = __all_sync(0xffffffffu, alive && wait_for(tfull(acc), acc_phase, dead));
       tcgen05_fence_after();
@@ -353,59 +370,66 @@ __global__ void __launch_bounds__(256, FEW ? 2 : 1) int8_gemm_kernel(const __gri
         // a lane has one token, its columns are channels: through shared memory to whole rows
         const int row0 = (w.ta * (PAIR ? 2 : 1) + (int)rank) * TILE + ew * 32, m = row0 + lane;
         const float sx = m < p.M ? __ldcg(p.sx + m) : 0.f;
-        const uint32_t stg = smem + STAGES * L::STAGE + ew * 4096;
-        constexpr int SLAB = OUT32 ? 32 : 64, PER = OUT32 ? 4 : 8; // columns of 128 bytes, of 16 bytes
+        const uint32_t stg = smem + STAGES * L::STAGE + (warp - 4) * 2048;
+        constexpr int PER = OUT32 ? 4 : 8, COLS = OUT32 ? 16 : 32; // columns of 16 bytes; of 64, which 32 rows of are in shared memory at a time
 #pragma unroll 1
-        for (int c0 = 0; c0 < BN; c0 += SLAB) {
-#pragma unroll
-          for (int half = 0; half < SLAB / 32; ++half) {
-            uint32_t v[32];
-            float f[32];
-            if (alive) {
-              tmem_ld32(taddr + c0 + half * 32, v);
-              tmem_ld_wait();
-            }
-            const float4* sw = reinterpret_cast<const float4*>(scales_s + acc * BN + c0 + half * 32);
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 w4 = sw[j / 4];
-              f[j] = alive ? (float)(int)v[j] * sx * w4.x : NAN;
-              f[j + 1] = alive ? (float)(int)v[j + 1] * sx * w4.y : NAN;
-              f[j + 2] = alive ? (float)(int)v[j + 2] * sx * w4.z : NAN;
-              f[j + 3] = alive ? (float)(int)v[j + 3] * sx * w4.w : NAN;
-            }
-#pragma unroll
-            for (int j = 0; j < 32 / PER; ++j) {                   // each row's chunks turned by the row, so that neither side of the transposition collides
-              const int chunk = half * 4 + j;
-              uint4 q;
-              if constexpr (OUT32) q = make_uint4(__float_as_uint(f[4 * j]), __float_as_uint(f[4 * j + 1]), __float_as_uint(f[4 * j + 2]), __float_as_uint(f[4 * j + 3]));
-              else q = pack8(f + 8 * j);
-              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stg + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
-            }
+        for (int c0 = 32 * half; c0 < BN; c0 += 64) {
+          uint32_t v[32];
+          if (alive) {
+            tmem_ld32(taddr + c0, v);
+            tmem_ld_wait();
+            if (c0 + 64 >= BN) give_back();                        // (by now they are in registers)
           }
-          if (c0 + SLAB >= BN && alive) give_back();
-          else __syncwarp();
+          const float4* sw = reinterpret_cast<const float4*>(scales_s + acc * BN + c0);
 #pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int r = it * 4 + (lane >> 3), chunk = lane & 7;
-            uint4 q;
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(stg + r * 128 + ((chunk ^ (r & 7)) << 4)));
-            const int n = w.tb * BN + c0 + chunk * PER;
-            if (row0 + r >= p.M || n >= p.N) continue;
-            const size_t at = (size_t)(row0 + r) * p.N + n;
-            if (p.wide && n + PER <= p.N) {
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + at * (OUT32 ? 4 : 2)) = q;
-            } else {
-              const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+          for (int j = 0; j < 32; j += 4) {
+            const float4 w4 = sw[j / 4];
+            const float f[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-              for (int i = 0; i < PER; ++i) {
-                if (n + i >= p.N) break;
-                if constexpr (OUT32) reinterpret_cast<uint32_t*>(p.out)[at + i] = u[i];
-                else reinterpret_cast<uint16_t*>(p.out)[at + i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+            for (int e = 0; e < 4; ++e) v[j + e] = __float_as_uint(alive ? (float)(int)v[j + e] * sx * f[e] : NAN);
+          }
+#pragma unroll
+          for (int part = 0; part < 32 / COLS; ++part) {
+#pragma unroll
+            for (int chunk = 0; chunk < 4; ++chunk) {              // each pair of rows' chunks turned by the pair, so that neither side of the transposition collides
+              const uint32_t* u = v + part * COLS + chunk * PER;
+              uint4 q;
+              if constexpr (OUT32) q = make_uint4(u[0], u[1], u[2], u[3]);
+              else q = pack8(reinterpret_cast<const float*>(u));
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stg + lane * 64 + ((chunk ^ (lane >> 1 & 3)) << 4)), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+            }
+            __syncwarp();
+            const int n0 = w.tb * BN + c0 + part * COLS;
+            if (p.wide) {
+#pragma unroll
+              for (int it = 0; it < 4; ++it) {
+                const int r = it * 8 + (lane >> 2), chunk = lane & 3, n = n0 + chunk * PER;
+                uint4 q;
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(stg + r * 64 + ((chunk ^ (r >> 1 & 3)) << 4)));
+                if (row0 + r < p.M && n < p.N) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + ((size_t)(row0 + r) * p.N + n) * (OUT32 ? 4 : 2)) = q;
+              }
+            } else {                                               // rows that begin anywhere: neighbouring lanes, neighbouring numbers (202 x 26373 outputs by fours and eights a lane: 33 us)
+              constexpr int AT_ONCE = 32 / COLS;                   // rows
+              const int e = lane % COLS, rows = min(32, p.M - row0);
+              const bool in = n0 + e < p.N;
+#pragma unroll 8
+              for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+                const int r = r0 + lane / COLS;
+                const uint32_t from = stg + r * 64 + (((e / PER) ^ (r >> 1 & 3)) << 4) + e % PER * (16 / PER);
+                const size_t at = (size_t)(row0 + r) * p.N + n0 + e;
+                if constexpr (OUT32) {
+                  uint32_t x;
+                  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(from));
+                  if (in && r < rows) reinterpret_cast<uint32_t*>(p.out)[at] = x;
+                } else {
+                  uint16_t x;
+                  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(from));
+                  if (in && r < rows) reinterpret_cast<uint16_t*>(p.out)[at] = x;
+                }
               }
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
       acc ^= 1;
@@ -423,26 +447,31 @@ __global__ void __launch_bounds__(256, FEW ? 2 : 1) int8_gemm_kernel(const __gri
     const float* sx_s = reinterpret_cast<const float*>(smem_gen + L::SCALES);
     bool bad = false;
     for (int o = 0; o < p.parts; ++o) bad |= cluster_ld_u32(cluster_place(const_cast<const int*>(dead), o)) != 0u;
-    for (int i = first + (int)threadIdx.x; i < last; i += 256) {
-      const int m = i / (TILE / 4), n = n0 + i % (TILE / 4) * 4;
-      int4 sum = make_int4(0, 0, 0, 0);
+    if (p.wide) {
+      for (int i = first + (int)threadIdx.x; i < last; i += 256) {
+        const int m = i / (TILE / 4), n = n0 + i % (TILE / 4) * 4;
+        int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll 4
-      for (int o = 0; o < p.parts; ++o) {
-        const float4 f = cluster_ld_f4(cluster_place(smem_gen + (size_t)i * 16, o));
-        sum.x += __float_as_int(f.x), sum.y += __float_as_int(f.y), sum.z += __float_as_int(f.z), sum.w += __float_as_int(f.w);
-      }
-      const int v[4] = {sum.x, sum.y, sum.z, sum.w};
-      float y[4];
+        for (int o = 0; o < p.parts; ++o) {
+          const float4 f = cluster_ld_f4(cluster_place(smem_gen + (size_t)i * 16, o));
+          sum.x += __float_as_int(f.x), sum.y += __float_as_int(f.y), sum.z += __float_as_int(f.z), sum.w += __float_as_int(f.w);
+        }
+        if (n >= p.N) continue;                                    // (whole vectors, as rows are)
+        const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+        float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = bad ? NAN : n + j < p.N ? (float)v[j] * sx_s[m] * __ldg(p.sw + n + j) : 0.f;
-      const size_t at = (size_t)m * p.N + n;
-      if (p.wide && n + 4 <= p.N) {
+        for (int j = 0; j < 4; ++j) y[j] = bad ? NAN : (float)v[j] * sx_s[m] * __ldg(p.sw + n + j);
+        const size_t at = (size_t)m * p.N + n;
         if constexpr (OUT32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
         else *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(p.out) + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) put_one<OUT32>(p.out, at + j, y[j]);
+      }
+    } else {                                                       // rows that begin anywhere: one channel a thread
+      for (int i = first * 4 + (int)threadIdx.x; i < last * 4; i += 256) {
+        const int m = i / TILE, n = n0 + i % TILE;
+        int sum = 0;
+#pragma unroll 4
+        for (int o = 0; o < p.parts; ++o) sum += (int)cluster_ld_u32(cluster_place(smem_gen + (size_t)i * 4, o));
+        if (n < p.N) put_one<OUT32>(p.out, (size_t)m * p.N + n, bad ? NAN : (float)sum * sx_s[m] * __ldg(p.sw + n));
       }
     }
   }
@@ -560,8 +589,8 @@ template <bool FEW, int BN, bool PAIR, bool OUT32> int launch(const Plan& pl, co
     LIA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
     if (dev < 64) configured[dev] = true;
   }
-  if (PAIR || pl.parts > 1) LIA_CUDA(lia_launch_cluster_as(early || PAIR, PAIR ? 2 : pl.parts, kernel, dim3(pl.grid), dim3(256), L::SMEM, stream, tmA, tmB, a));
-  else LIA_CUDA(lia_launch_as(early, kernel, dim3(pl.grid), dim3(256), L::SMEM, stream, tmA, tmB, a));
+  if (PAIR || pl.parts > 1) LIA_CUDA(lia_launch_cluster_as(early || PAIR, PAIR ? 2 : pl.parts, kernel, dim3(pl.grid), dim3(L::THREADS), L::SMEM, stream, tmA, tmB, a));
+  else LIA_CUDA(lia_launch_as(early, kernel, dim3(pl.grid), dim3(L::THREADS), L::SMEM, stream, tmA, tmB, a));
   return LIA_OK;
 }
 template <bool OUT32> int launch_plan(const Plan& pl, const CUtensorMap& tmA, const CUtensorMap& tmB, const Args& a, bool early, cudaStream_t stream) {

@@ -154,19 +154,27 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
   for (int d = 0; d < DEPTH; ++d) bring(b0 + warp + d * WARPS, d); // (on their way while the queries are brought)
 
   // ---- queries: rows (token, head) in the order of the products' operands
-  for (int r = warp; r < S::ROWS; r += WARPS) {
-    const bool there = r0 + r < R;
-    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
-    uint2 u = make_uint2(0u, 0u);
-    if (there && lane < DIM / 4) u = *reinterpret_cast<const uint2*>(a.q + (p.row + i) * a.ldq + h * DIM + lane * 4);
-    float f = a.scale * (a.temp != nullptr && there ? a.temp[h] : 1.f) * (a.softcap > 0.f ? 1.f : LOG2E);
+  constexpr int MINE = S::ROWS / WARPS;                            // rows of a warp, asked for together
+  uint2 asked[MINE];
+  float temps[MINE];
+#pragma unroll
+  for (int x = 0; x < MINE; ++x) {
+    const int r = warp + x * WARPS, i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    asked[x] = r0 + r < R && lane < DIM / 4 ? *reinterpret_cast<const uint2*>(a.q + (p.row + i) * a.ldq + h * DIM + lane * 4) : make_uint2(0u, 0u);
+    temps[x] = a.temp != nullptr && r0 + r < R ? a.temp[h] : 1.f;
+  }
+#pragma unroll
+  for (int x = 0; x < MINE; ++x) {
+    const int r = warp + x * WARPS;
+    const uint2 u = asked[x];
+    float f = a.scale * temps[x] * (a.softcap > 0.f ? 1.f : LOG2E);
     const uint32_t top = max(max((u.x & 0x7fffu), (u.x >> 16) & 0x7fffu), max((u.y & 0x7fffu), (u.y >> 16) & 0x7fffu));
     const Down down = down_of(__reduce_max_sync(0xffffffffu, top));
-    float x[4];
-    unpack_bf16x2(u.x, x[0], x[1]);
-    unpack_bf16x2(u.y, x[2], x[3]);
+    float y[4];
+    unpack_bf16x2(u.x, y[0], y[1]);
+    unpack_bf16x2(u.y, y[2], y[3]);
     constexpr float ODD = SMALL ? 0.0625f : 1.f;                   // channels 1, 3, 5, 7 of every eight go with 16 u
-    uint2 w = make_uint2(pack_f16x2(x[0] * down.by, x[1] * down.by * ODD), pack_f16x2(x[2] * down.by, x[3] * down.by * ODD));
+    uint2 w = make_uint2(pack_f16x2(y[0] * down.by, y[1] * down.by * ODD), pack_f16x2(y[2] * down.by, y[3] * down.by * ODD));
     f *= down.back;
     w = in_code_order(w);                                          // of eight channels an even lane has 0 4 1 5, an odd one 2 6 3 7: their operands of two steps
     if constexpr (SMALL) {
