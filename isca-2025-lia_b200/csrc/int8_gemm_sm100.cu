@@ -7,6 +7,8 @@
 //   FEW    (up to 128 tokens; bound by the weights' bytes)  the weights' rows are the product's 128 rows, the tokens its 16 to 128 columns.  A CTA has a tile of 128 channels, or `parts` CTAs that are a
 //          cluster share one along K and add up each other's sums by way of shared memory.  Two CTAs fit an SM, so that one's beginning and end lie under the other's loads, and memory shares itself out
 //          among as many tiles as there are.  Weights are on their way while the tokens are quantised.
+//   a token or two and matrices up to 64 Mi products, whose time is latency: int8_tokens_kernel, on the ordinary cores and in one launch.  Every block makes the tokens' codes for itself, in shared memory,
+//          while its first weights are on their way; a warp has an equal part of the block's channels' codes.
 //   MANY   (bound by the tensor cores)  the tokens' rows are the product's rows: CTA pairs on 256 x 256 tiles (cta_group::2), or one CTA on 128 x 256, 128 or 64 where those would leave SMs idle.
 //
 // Every wait is bounded; a CTA that gives one up makes its tile's outputs NaN and counts itself in lia_moe_timeouts_seen().
@@ -33,6 +35,32 @@ struct QuantArgs {
   float* scale;
   int K, vec;
 };
+// Numbers 8 v .. 8 v + 7 of a row of K; those behind its end are zeros
+template <typename T> __device__ __forceinline__ Raw8<T> load_of_row(const T* src, int v, int K, bool vec) {
+  if (v * 8 >= K) return Raw8<T>{};
+  if constexpr (sizeof(T) == 2) {                                  // rows of bf16 on 2-byte boundaries: by words of 4 bytes, of which only a row's first and last could lie outside it
+    if (!vec && v > 0 && v * 8 + 8 < K) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(src + v * 8);
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+      uint32_t u[5];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = p[i];
+      const bool half = at & 2;
+      u[4] = half ? p[4] : 0u;
+      Raw8<T> r;
+      r.u[0] = half ? make_uint4(__byte_perm(u[0], u[1], 0x5432), __byte_perm(u[1], u[2], 0x5432), __byte_perm(u[2], u[3], 0x5432), __byte_perm(u[3], u[4], 0x5432)) : make_uint4(u[0], u[1], u[2], u[3]);
+      return r;
+    }
+  }
+  if (v * 8 + 8 <= K) return load8(src + v * 8, vec);
+  T r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v * 8 + i < K ? src[v * 8 + i] : (T)0.f;
+  Raw8<T> u;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.u[i] = reinterpret_cast<const uint4*>(r)[i];
+  return u;
+}
 constexpr int Q_HELD = 4;                                          // vectors of eight numbers that a thread holds: rows of 8192 numbers, or 32768, are read once
 
 template <typename T, int Q_THREADS> __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_constant__ QuantArgs a) {
@@ -42,31 +70,7 @@ template <typename T, int Q_THREADS> __global__ void __launch_bounds__(Q_THREADS
   __shared__ uint32_t part[Q_THREADS / 32];
   const int t = threadIdx.x, vecs = (a.K + 7) / 8;
   const T* src = reinterpret_cast<const T*>(a.x) + (long long)blockIdx.x * a.ldx;
-  auto load = [&](int v) {                                         // numbers behind the row's end are zeros
-    if (v >= vecs) return Raw8<T>{};
-    if constexpr (sizeof(T) == 2) {                                // rows of bf16 on 2-byte boundaries: by words of 4 bytes, of which only a row's first and last could lie outside it
-      if (!a.vec && v > 0 && v * 8 + 8 < a.K) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(src + v * 8);
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
-        uint32_t u[5];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = p[i];
-        const bool half = at & 2;
-        u[4] = half ? p[4] : 0u;
-        Raw8<T> r;
-        r.u[0] = half ? make_uint4(__byte_perm(u[0], u[1], 0x5432), __byte_perm(u[1], u[2], 0x5432), __byte_perm(u[2], u[3], 0x5432), __byte_perm(u[3], u[4], 0x5432)) : make_uint4(u[0], u[1], u[2], u[3]);
-        return r;
-      }
-    }
-    if (v * 8 + 8 <= a.K) return load8(src + v * 8, a.vec);
-    T r[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = v * 8 + i < a.K ? src[v * 8 + i] : (T)0.f;
-    Raw8<T> u;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.u[i] = reinterpret_cast<const uint4*>(r)[i];
-    return u;
-  };
+  auto load = [&](int v) { return load_of_row(src, v, a.K, a.vec); };
   Raw8<T> raw[Q_HELD];
 #pragma unroll
   for (int i = 0; i < Q_HELD; ++i) raw[i] = load(t + i * Q_THREADS);
@@ -97,6 +101,166 @@ template <typename T, int Q_THREADS> __global__ void __launch_bounds__(Q_THREADS
   for (int i = 0; i < Q_HELD; ++i) put(t + i * Q_THREADS, raw[i]);
   for (int v = t + Q_HELD * Q_THREADS; v < vecs; v += Q_THREADS) put(v, load(v));
   if (t == 0) a.scale[blockIdx.x] = code.scale;
+}
+
+// ------------------------------------------------------------------ a few tokens
+struct TokenArgs {
+  const void* x;
+  const float* sx;                                                 // of codes that are given
+  const int8_t* w;
+  const float* sw;
+  void* out;
+  long long ldx, ldw;
+  int N, K, vec, rows, steps;                                      // vec: vectors of 16 bytes may be read of x; channels of a block (an even number), blocks of 512 codes of a row
+};
+constexpr int T_WARPS = 16, T_THREADS = T_WARPS * 32, T_STEP = 512;                            // codes of a channel that a warp takes at once, 16 a lane
+constexpr int T_ROWS = 1024, T_CODES = 32768;                       // most channels of a block; most numbers of the tokens
+size_t token_smem(int M, int steps, int rows) { return (size_t)M * steps * T_STEP + (size_t)M * rows * 4; }
+static_assert(T_CODES + 2 * T_STEP + 2 * T_ROWS * 4 <= 47 * 1024, "shared memory without asking for more");
+
+template <typename T, int TOKENS, bool OUT32> __global__ void __launch_bounds__(T_THREADS, 1) int8_tokens_kernel(const __grid_constant__ TokenArgs a) {
+  constexpr int UNITS = 4, HELD = T_CODES / 8 / T_THREADS / TOKENS;             // vectors of eight numbers that a thread has of each token
+  extern __shared__ __align__(16) uint8_t smem_gen[];
+  __shared__ uint32_t part[TOKENS][T_WARPS];
+  __shared__ float sx_s[TOKENS];
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, width = a.steps * T_STEP;
+  const int row0 = blockIdx.x * a.rows, rows = min(a.rows, a.N - row0);
+  int* sums = reinterpret_cast<int*>(smem_gen + TOKENS * width);                               // [rows][TOKENS]
+  // Units of two channels' 512 codes, the block's in a row: a sixteenth of them for each warp
+  const int units = (rows + 1) / 2 * a.steps, first = (int)((long long)units * warp / T_WARPS), last = (int)((long long)units * (warp + 1) / T_WARPS);
+  auto codes_at = [&](int pair, int k, int r) { return a.w + (long long)(row0 + 2 * pair + r) * a.ldw + k * T_STEP + lane * 16; };
+  int pair = first / a.steps, k = first - pair * a.steps;          // of the units that are asked for next
+  int ask = first;
+  for (int u = ask, p = pair, s = k; u < min(last, ask + UNITS); ++u) {                        // to L2, where what comes before may still change them; the loads come behind the wait
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      if (lane % 2 == 0 && 2 * p + r < rows && s * T_STEP + lane * 16 < a.K) asm volatile("prefetch.global.L2 [%0];" ::"l"(codes_at(p, s, r)));
+    if (++s == a.steps) s = 0, ++p;
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  uint4 w[UNITS][2], next[UNITS][2];
+  auto ask_units = [&](uint4 (&to)[UNITS][2]) {
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+      const int left = a.K - k * T_STEP - lane * 16;               // of the row, from this lane's codes on
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        to[j][r] = make_uint4(0u, 0u, 0u, 0u);
+        if (ask + j < last && 2 * pair + r < rows && left > 0) {
+          const int8_t* src = codes_at(pair, k, r);
+          if (left >= 16 || row0 + 2 * pair + r + 1 < a.N) {       // (what lies between two rows is multiplied by zeros)
+            to[j][r] = __ldg(reinterpret_cast<const uint4*>(src));
+          } else {
+            uint32_t q[4] = {0u, 0u, 0u, 0u};
+            for (int i = 0; i < left; ++i) q[i >> 2] |= (uint32_t)(uint8_t)src[i] << (8 * (i & 3));
+            to[j][r] = make_uint4(q[0], q[1], q[2], q[3]);
+          }
+        }
+      }
+      if (++k == a.steps) k = 0, ++pair;
+    }
+    ask += UNITS;
+  };
+  int done = first, now = pair, at = k;                            // the unit that is multiplied next
+  ask_units(w);
+
+  // the tokens' codes, zeros behind their ends
+  for (int i = t; i < a.rows * TOKENS; i += T_THREADS) sums[i] = 0;
+  if constexpr (sizeof(T) == 1) {
+    for (int i = t; i < TOKENS * (width / 16); i += T_THREADS) {
+      const int m = i / (width / 16), c = (i - m * (width / 16)) * 16, left = a.K - c;
+      uint4 q = make_uint4(0u, 0u, 0u, 0u);
+      if (left > 0) {
+        const int8_t* src = static_cast<const int8_t*>(a.x) + (long long)m * a.ldx + c;
+        if (left >= 16) {
+          q = ldg_act(reinterpret_cast<const bf16*>(src));
+        } else {
+          uint32_t b[4] = {0u, 0u, 0u, 0u};
+          for (int e = 0; e < left; ++e) b[e >> 2] |= (uint32_t)(uint8_t)src[e] << (8 * (e & 3));
+          q = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+      }
+      *reinterpret_cast<uint4*>(smem_gen + m * width + c) = q;
+    }
+    if (t < TOKENS) sx_s[t] = __ldcg(a.sx + t);
+  } else {
+    Raw8<T> raw[TOKENS][HELD];
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m)
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) raw[m][i] = load_of_row(static_cast<const T*>(a.x) + m * a.ldx, t + i * T_THREADS, a.K, a.vec);
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m) {
+      uint32_t most = 0u;
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) most = most_of(raw[m][i], most);
+      if constexpr (sizeof(T) == 2) most = max(most & 0xffffu, most >> 16) << 16;
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) part[m][warp] = most;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m) {
+      const Coder<true> code(__uint_as_float(__reduce_max_sync(0xffffffffu, part[m][lane % T_WARPS])));
+      auto put = [&](int v, const Raw8<T>& r) {
+        if (v >= width / 8) return;
+        float f[8];
+        numbers_of(r, f);
+        *reinterpret_cast<uint2*>(smem_gen + m * width + v * 8) = code(f);
+      };
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) put(t + i * T_THREADS, raw[m][i]);
+      if (t == 0) sx_s[m] = code.scale;
+    }
+  }
+  __syncthreads();
+
+  int sum[TOKENS][2];
+#pragma unroll
+  for (int m = 0; m < TOKENS; ++m) sum[m][0] = sum[m][1] = 0;
+  auto multiply = [&](const uint4 (&q)[UNITS][2]) {
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+      if (done >= last) return;
+#pragma unroll
+      for (int m = 0; m < TOKENS; ++m) {
+        const int4 c = *reinterpret_cast<const int4*>(smem_gen + m * width + at * T_STEP + lane * 16);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          sum[m][r] = __dp4a((int)q[j][r].w, c.w, __dp4a((int)q[j][r].z, c.z, __dp4a((int)q[j][r].y, c.y, __dp4a((int)q[j][r].x, c.x, sum[m][r]))));
+      }
+      ++done;
+      ++at;
+      if (at == a.steps || done == last) {                         // the channels' sums, or this warp's part of them
+        int mine = 0;
+#pragma unroll
+        for (int m = 0; m < TOKENS; ++m)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int s = __reduce_add_sync(0xffffffffu, sum[m][r]);
+            if (lane == r * TOKENS + m) mine = s;
+            sum[m][r] = 0;
+          }
+        if (lane < 2 * TOKENS) atomicAdd(sums + 2 * now * TOKENS + lane, mine);                // (whole numbers: in any order)
+      }
+      if (at == a.steps) at = 0, ++now;
+    }
+  };
+  while (done < last) {
+    ask_units(next);
+    multiply(w);
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) w[j][0] = next[j][0], w[j][1] = next[j][1];
+  }
+  __syncthreads();
+  for (int i = t; i < rows * TOKENS; i += T_THREADS) {
+    const int m = i / rows, r = i - m * rows;
+    const float y = (float)sums[r * TOKENS + m] * sx_s[m] * __ldg(a.sw + row0 + r);
+    const size_t o = (size_t)m * a.N + row0 + r;
+    if constexpr (OUT32) static_cast<float*>(a.out)[o] = y;
+    else static_cast<bf16*>(a.out)[o] = __float2bfloat16_rn(y);
+  }
 }
 
 // ------------------------------------------------------------------ products
@@ -623,6 +787,25 @@ int quantize(const void* x, int act_f32, long long ldx, int8_t* codes, long long
   return LIA_OK;
 }
 
+// us with quantisation and tcgen05 | in one launch, bf16 tokens: 1 of 1024 x 1024 5.9 | 4.8, of 2560 x 2560 7.5 | 5.3, of 1000 x 8192 8.4 | 5.8, of 64 x 28672 12.5 | 6.2, of 7168 x 7168 14.0 | 13.3, of
+// 50272 x 2560 26.0 | 25.7, of 28672 x 7168 35.6 | 37.3, of 200000 x 64 21 | 26 (and in two rounds, 200000 x 256, 23 | 26); 2 of 2560 x 2560 7.5 | 5.7, of 1000 x 8192 8.4 | 6.8, of 2048 x 28672 16.7 | 20.1 (every block quantises the tokens);
+// 4 of 2560 x 2560 7.5 | 7.0, of 1000 x 8192 8.5 | 8.5, of 7168 x 7168 14.0 | 16.3.  A call is shorter by a launch and an allocation too.
+bool few_tokens(int M, int N, int K) { return M <= 2 && K >= T_STEP / 2 && (long long)M * K <= T_CODES && (long long)M * N * K <= 1ll << 26 && N <= lia_sm_count() * T_ROWS; }
+
+template <typename T, bool OUT32> int launch_tokens(TokenArgs a, int M, cudaStream_t stream) {
+  const int sms = lia_sm_count();                                  // as many channels for each
+  a.rows = ((a.N + sms - 1) / sms + 1) / 2 * 2;
+  LIA_CUDA(lia_launch(M == 1 ? int8_tokens_kernel<T, 1, OUT32> : int8_tokens_kernel<T, 2, OUT32>, dim3((a.N + a.rows - 1) / a.rows), dim3(T_THREADS), token_smem(M, a.steps, a.rows), stream, a));
+  return LIA_OK;
+}
+template <bool OUT32> int launch_tokens(int x_type, const TokenArgs& a, int M, cudaStream_t stream) {
+  switch (x_type) {
+    case LIA_X_BF16: return launch_tokens<bf16, OUT32>(a, M, stream);
+    case LIA_X_F32: return launch_tokens<float, OUT32>(a, M, stream);
+    default: return launch_tokens<int8_t, OUT32>(a, M, stream);
+  }
+}
+
 }  // namespace
 
 extern "C" int lia_quantize_rows(const void* x, int act_f32, long long ldx, void* codes, long long ldc, float* scale, int M, int K, lia_stream_t stream) {
@@ -635,7 +818,7 @@ extern "C" int lia_quantize_rows(const void* x, int act_f32, long long ldx, void
 
 extern "C" size_t lia_linear_int8_workspace_bytes(int x_type, int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0 || K > MOST_K) return 0;
-  return rooms_of(M, K, x_type == LIA_X_INT8).bytes;
+  return rooms_of(M, K, x_type == LIA_X_INT8 || few_tokens(M, N, K)).bytes;
 }
 
 extern "C" int lia_linear_int8(const void* x, int x_type, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, void* out, int out_f32, int M, int N, int K,
@@ -649,6 +832,11 @@ extern "C" int lia_linear_int8(const void* x, int x_type, long long ldx, const f
   LIA_CHECK_ARG(x && w && w_scale && out && (given == (x_scale != nullptr)), "lia_linear_int8: null pointer, or scales of tokens that are not codes");
   LIA_CHECK_ARG(reinterpret_cast<uintptr_t>(w) % 16 == 0 && ldw % 16 == 0 && (!given || (reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 16 == 0)),
                 "lia_linear_int8: rows of codes have to be whole 16-byte vectors apart");
+  if (few_tokens(M, N, K)) {
+    const int vec = given || (reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (x_type == LIA_X_F32 ? 4 : 8) == 0);
+    const TokenArgs a{x, x_scale, static_cast<const int8_t*>(w), w_scale, out, ldx, ldw, N, K, vec, 0, (K + T_STEP - 1) / T_STEP};
+    return out_f32 ? launch_tokens<true>(x_type, a, M, stream) : launch_tokens<false>(x_type, a, M, stream);
+  }
   const Plan pl = plan_of(M, N, K);
   LIA_CHECK_ARG((long long)pl.tiles_a * pl.k_blocks < (1ll << 31) && (long long)pl.tiles_a * pl.tiles_b < (1ll << 31), "lia_linear_int8: too large (M=%d N=%d K=%d)", M, N, K);
   const Rooms r = rooms_of(M, K, given);

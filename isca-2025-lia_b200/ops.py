@@ -1621,7 +1621,7 @@ def linear_int8(x, w, w_scale, out=None, x_scale=None):
     size = lib.lia_linear_int8_workspace_bytes(kind, M, N, K)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     check(lib.lia_linear_int8(xp, kind, ldx, sp, wp, ldw, wsp, op, _f32(out), M, N, K, _p(ws), size, _stream()), "lia_linear_int8")
-    count_launches(1 if kind == _lib.X_INT8 else 2)
+    count_launches(2 if size else 1)
     return out
 
 

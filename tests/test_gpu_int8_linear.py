@@ -116,9 +116,10 @@ def test_from_activations(ops, act, M):
         assert torch.isnan(y[3]).all() and (y[1] == 0).all() and torch.isfinite(y[4]).all()
 
 
-def test_weights_quantised_right_before(ops):
+@pytest.mark.parametrize("M", [1, 3])
+def test_weights_quantised_right_before(ops, M):
     """A product begins to bring its weights while the tokens are quantised: not before the kernel that wrote them has ended."""
-    N, K, M = 8192, 4096, 3
+    N, K = 8192, 4096
     x = torch.randn(M, K, generator=torch.Generator("cuda").manual_seed(1), device="cuda").to(BF16)
     c, s = ops.quantize_rows(x)
     buffer, sw = torch.empty(N, K, dtype=I8, device="cuda"), torch.empty(N, device="cuda")
@@ -130,7 +131,7 @@ def test_weights_quantised_right_before(ops):
         assert torch.equal(one, want(c, s, buffer, sw, BF16)), i
 
 
-@pytest.mark.parametrize("M", [3, 64, 700])
+@pytest.mark.parametrize("M", [1, 3, 64, 700])
 def test_streams_and_graphs(ops, M):
     """Two streams at once, a captured call with other tokens in it, and two captured graphs that are replayed at the same time: each has its own workspace."""
     N, K = 2560, 2560
@@ -162,6 +163,32 @@ def test_streams_and_graphs(ops, M):
     assert torch.equal(graphs[0][1], want(*ops.quantize_rows(xs[0]), w, sw, BF16)) and torch.equal(graphs[1][1], wants[1])
 
 
+@pytest.mark.parametrize("act", [BF16, F32, I8], ids=["bf16", "f32", "codes"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 256), (2, 1, 255), (2, 3, 257), (1, 300, 511), (2, 1001, 513), (1, 129, 1543), (2, 515, 7000), (1, 7, 32768), (1, 7, 32769), (2, 33, 16384), (2, 33, 16385),
+                                   (1, 200001, 300), (2, 120001, 270), (1, 64, 28673), (2, 2561, 2561), (1, 16384, 4096), (1, 16385, 4096)])
+def test_a_token_or_two(ops, act, M, N, K):
+    """Both sides of the borders of the form in one launch: its last channels' last codes lie at the very end of the weights, tokens are columns of something wider."""
+    ld = (K + 15) // 16 * 16
+    flat = codes(N, K, 2, ld).as_strided((N * ld,), (1,))[:(N - 1) * ld + K].clone()
+    w, sw = flat.as_strided((N, K), (ld, 1)), scales(N, 4)
+    guard = torch.full((M * N + 64,), 77.0, dtype=F32, device="cuda")
+    y = guard[32:32 + M * N].view(M, N)
+    if act == I8:
+        x, sx = codes(M, K, 1, ld + 16), scales(M, 3)
+        ops.linear_int8(x, w, sw, out=y, x_scale=sx)
+    else:
+        x = torch.randn(M, K + 9, generator=torch.Generator("cuda").manual_seed(1), device="cuda").to(act)[:, 5:5 + K]
+        ops.linear_int8(x, w, sw, out=y)
+        x, sx = ops.quantize_rows(x)
+    assert torch.equal(y, want(x, sx, w, sw, F32)) and (guard[:32] == 77).all() and (guard[-32:] == 77).all()
+    assert torch.equal(ops.linear_int8(x, w, sw, x_scale=sx), want(x, sx, w, sw, BF16))
+    if act != I8:
+        bad = torch.randn(M, K, device="cuda").to(act)
+        bad[M - 1, K - 1] = NAN
+        out = ops.linear_int8(bad, w, sw)
+        assert torch.isnan(out[M - 1]).all() and torch.isfinite(out[:M - 1]).all()
+
+
 def test_a_tokens_outputs_do_not_depend_on_the_others(ops):
     N, K = 1536, 2048
     w, sw = ops.quantize_rows(torch.randn(N, K, generator=torch.Generator("cuda").manual_seed(1), device="cuda"))
@@ -171,7 +198,7 @@ def test_a_tokens_outputs_do_not_depend_on_the_others(ops):
         assert torch.equal(ops.linear_int8(x[:n], w, sw), all_rows[:n])
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 2560, 2560), (40, 700, 1000), (128, 300, 4096), (200, 500, 300), (700, 1000, 256)])
+@pytest.mark.parametrize("M,N,K", [(3, 2560, 2560), (40, 700, 1000), (128, 300, 4096), (200, 500, 300), (700, 1000, 256)])
 @pytest.mark.parametrize("given", [False, True])
 def test_waits_that_run_out(nowait, monkeypatch, ops, M, N, K, given):  # noqa: F811
     """With a limit of 0 every wait gives up: the launch ends, every output is NaN and nothing else is written, its blocks are counted; the next launch is right."""
