@@ -151,7 +151,7 @@ const char* tensor_of(const LiaCacheRows& r, int slots, Tensor& t) {
     if (r.pieces != 1) return "a state in pieces";
     t.state = (int)(r.piece_bytes / t.vec);
     t.pos = t.bytes = t.vec;
-  } else if (r.pos_stride == 0) {
+  } else if (r.pos_stride < r.piece_bytes || (r.pieces > 1 && r.piece_stride < r.piece_bytes)) {
     return "slots or rows that share their place";
   }
   const long long row = t.bytes * t.pieces;

@@ -1591,7 +1591,7 @@ def quantize_rows(x, codes=None, scale=None):
     cp, ldc = _rows_of(codes, torch.int8, (M, K), dev, "quantize_rows: codes")
     if M == 1:
         ldc = (K + 7) // 8 * 8                                  # (one row has no next one)
-    check(_lib.load().lia_quantize_rows(xp, _f32(x), max(ldx, K), cp, ldc, _need(scale, F32, (M,), dev, "quantize_rows: scale"), M, K, _stream()), "lia_quantize_rows")
+    check(_lib.load().lia_quantize_rows(xp, _f32(x), ldx, cp, ldc, _need(scale, F32, (M,), dev, "quantize_rows: scale"), M, K, _stream()), "lia_quantize_rows")
     count_launches()
     return codes, scale
 
@@ -1657,7 +1657,7 @@ class CacheSet:
                 pieces *= n
             else:
                 raise _lib.LiaError(f"CacheSet: a row of strides {strides} is not runs of bytes at equal distances")
-        if (self.slots > 1 and strides[0] == 0) or (not state and self.capacity > 1 and strides[1] == 0) or (pieces > 1 and apart < piece) or (state and pieces > 1):
+        if (self.slots > 1 and strides[0] == 0) or (not state and self.capacity > 1 and strides[1] * size < piece) or (pieces > 1 and apart < piece) or (state and pieces > 1):
             raise _lib.LiaError(f"CacheSet: rows that share their place, or a state that is not contiguous: strides {strides}")
         pos = 0 if state else strides[1] * size if self.capacity > 1 else piece
         return _lib.LiaCacheRows(t.data_ptr(), strides[0] * size, pos, apart, piece, pieces, int(state))

@@ -91,24 +91,19 @@ class SlotState:
             raise SlotError(f"requests {held or new_ids!r} already hold slots, or are named twice")
         if len(new_ids) > self.owner.count(None):
             raise SlotError(f"{len(new_ids)} slots are needed, {self.owner.count(None)} are free")
-        n, to = self.length[src], []
-        for s in range(self.n_slots):
-            if self.owner[s] is None and len(to) < len(new_ids):
-                self.owner[s], self.length[s] = new_ids[len(to)], n
-                self.by_id[new_ids[len(to)]] = s
-                to.append(s)
-        if not to or not (self.recurrent or self.positioned):
-            return to
+        n, to = self.length[src], [s for s in range(self.n_slots) if self.owner[s] is None][:len(new_ids)]
         if self.device.type != "cuda":                                    # (host-resident models: tests)
             for s in to:
                 for t in self.recurrent:
                     t[s] = t[src]
                 for t in self.positioned:
                     t[s, :n] = t[src, :n]
-            return to
-        if self._set is None:
-            self._set = ops.CacheSet(self.positioned, self.recurrent)
-        self._set.fork(torch.tensor([(src, s, n) for s in to], dtype=torch.int32, device=self.device), max_count=n)
+        elif to and (self.recurrent or self.positioned):
+            if self._set is None or len(self._set.tensors) < len(self.positioned) + len(self.recurrent):
+                self._set = ops.CacheSet(self.positioned, self.recurrent)
+            self._set.fork(torch.tensor([(src, s, n) for s in to], dtype=torch.int32, device=self.device), max_count=n)
+        for s, r in zip(to, new_ids):
+            self.owner[s], self.length[s], self.by_id[r] = r, n, s
         return to
 
     def free(self, req_id):

@@ -146,7 +146,7 @@ def rows(_lib, **change):
 
 
 @pytest.mark.parametrize("change,message", [({"data": None}, "null"), ({"pieces": 0}, "bytes"), ({"piece_bytes": 0}, "bytes"), ({"piece_bytes": 1 << 31}, "bytes"), ({"slot_stride": -64}, "share"),
-                                            ({"slot_stride": 0}, "share"), ({"pos_stride": 0}, "share"), ({"state": 1, "pieces": 2}, "pieces")])
+                                            ({"slot_stride": 0}, "share"), ({"pos_stride": 0}, "share"), ({"pos_stride": 63}, "share"), ({"pieces": 2, "piece_bytes": 32, "piece_stride": 16}, "share"), ({"state": 1, "pieces": 2}, "pieces")])
 def test_moves_refuse_tensors(lib, change, message):
     L = lib.load()
     assert L.lia_cache_fork(rows(lib, **change), 1, 4, 64, 16, 1, 1, None) == -1 and message in lib.last_error()

@@ -159,7 +159,7 @@ def test_sets_that_are_refused(ops):
     from lia_b200._lib import LiaError
     a = rnd(3, 20, 8)
     for rows, states in (([], []), ([a, rnd(2, 20, 8)], []), ([a, rnd(3, 21, 8)], []), ([a, a.cpu()], []), ([a[:, :, :0]], []), ([rnd(3, 1, 8).expand(3, 20, 8)], []), ([rnd(1, 20, 8).expand(3, 20, 8)], []),
-                         ([rnd(3, 20, 4, 9, 8)[:, :, :, :3, :5]], []), ([a], [rnd(3, 8, 8).transpose(1, 2)]), ([rnd(3, 20, 1).expand(3, 20, 8)], [])):
+                         ([rnd(3, 20, 4, 9, 8)[:, :, :, :3, :5]], []), ([a], [rnd(3, 8, 8).transpose(1, 2)]), ([rnd(3, 20, 1).expand(3, 20, 8)], []), ([rnd(3, 200).as_strided((3, 20, 8), (200, 4, 1))], [])):
         with pytest.raises(LiaError):
             ops.CacheSet(rows, states)
     s = ops.CacheSet([a], [rnd(3, 4)])

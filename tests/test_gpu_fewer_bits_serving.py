@@ -152,6 +152,26 @@ def test_a_fork_goes_on_as_its_request_would(cache_dtype):
         assert eng.slots.slot_of("e") is None and eng.slots.owner.count(None) == 1
 
 
+def test_forks_of_slots_take_tensors_that_come_later_and_are_all_or_none(monkeypatch):
+    from lia_b200.seq_state import SlotState
+    s = SlotState(4, 9, "cuda")
+    a = s.add_rows(16, torch.bfloat16)
+    s.alloc("x")
+    s.reserve(0, 5)
+    a[0] = 1
+    assert s.fork("x", ["y"]) == [1]
+    b = s.add_rows(8, torch.float32)
+    b[0] = 2
+    assert s.fork("x", ["z"]) == [2] and (a[2, :5] == 1).all() and (b[2, :5] == 2).all() and (b[2, 5:] == 0).all() and (b[1] == 0).all()
+
+    def broken(*args, **kw):
+        raise RuntimeError("no launch")
+    monkeypatch.setattr(s._set, "fork", broken)
+    with pytest.raises(RuntimeError, match="no launch"):
+        s.fork("x", ["w"])
+    assert s.owner == ["x", "y", "z", None] and s.length == [5, 5, 5, 0] and s.slot_of("w") is None
+
+
 @pytest.mark.parametrize("requests", [8, 3, 2])
 def test_scores_of_choices(requests):
     """As scores of the prompt with each choice behind it, whose last tokens they are; all slots are free afterwards."""

@@ -72,6 +72,17 @@ def test_tokens_codes_at_the_edges(ops):
     assert ops.quantize_rows(x[:0])[0].shape == (0, 50)
 
 
+def test_rows_that_share_their_place_are_refused(ops):
+    from lia_b200._lib import LiaError
+    x = torch.randn(1, 64, device="cuda")
+    w, sw = ops.quantize_rows(torch.randn(16, 64, device="cuda"))
+    for call in (lambda: ops.quantize_rows(x.expand(5, 64)), lambda: ops.quantize_rows(x.view(64).as_strided((3, 32), (8, 1))), lambda: ops.linear_int8(x.expand(5, 64), w, sw),
+                 lambda: ops.linear_int8(x, w[:1].expand(4, 64), sw[:4])):
+        with pytest.raises(LiaError, match="sizes"):
+            call()
+    assert torch.equal(ops.quantize_rows(x.expand(1, 64))[0], ops.quantize_rows(x)[0])
+
+
 @pytest.mark.parametrize("out", [BF16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("M,N,K", [
     (1, 1, 1), (1, 2560, 2560), (2, 7, 15), (3, 130, 16), (16, 128, 128), (17, 1000, 129), (33, 129, 1000), (64, 4096, 512), (65, 300, 4096), (100, 257, 777), (128, 1024, 1024), (1, 300, 16384),
