@@ -6,8 +6,12 @@
 // 128 1 / 9, and a channel that is ten times the others takes the bits of 31 others instead of 127.
 //
 // Eight lanes have a head: lane q takes the channels 4 q .. 4 q + 3 of every group, which are 64 neighbouring bytes of bf16 activations for the eight, and whose codes are neighbours in the cache (byte4()).  Up
-// to four groups at a time, so that a lane's codes of 128 channels are one 8-byte store.
+// to four groups at a time, so that a lane's codes of 128 channels are one 8-byte store; each lane sees to one group's scale, which the others get by shuffles.
+//
+// 7169 tokens with 8 heads of 128 (29 MB each of keys and values in, 8 MB out; graph replay): store 12.8 us, bound by instructions (20 a number for 32 lanes, three slots in four taken; with 40 registers
+// instead of 32 a thread 13.3, every lane with all groups' scales 15.5); load 10.3, bound by what memory takes of its 29 MB of results (keys and values by the same lanes: 12.8, and the store 13.9).
 #include "cache8.cuh"
+#include "pairs.cuh"
 
 namespace {
 
@@ -63,29 +67,32 @@ template <typename T> __device__ __forceinline__ void numbers_of(const Raw4<T>& 
     for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r.w[i]);
   }
 }
-// The bits of four groups' largest magnitudes, for the eight lanes of a head (as whole numbers NaN is above infinity and that above the rest)
-template <typename T> __device__ __forceinline__ void most_of(const Raw4<T>* raw, uint32_t* most) {
+// Of the four groups' largest magnitudes, each over the eight lanes of a head, the bits of that of group 2 (q / 4) + q % 2 (as whole numbers NaN is above infinity and that above the rest)
+__device__ __forceinline__ int group_of(int q) { return (q >> 2) * 2 + (q & 1); }
+__device__ __forceinline__ int lane_of(int g) { return (g >> 1) * 4 + (g & 1); }
+template <typename T> __device__ __forceinline__ uint32_t most_of(const Raw4<T>* raw, int q) {
+  const bool last = q & 4, odd = q & 1;                            // halves of the lanes give each other what they do not keep
   if constexpr (sizeof(T) == 2) {                                  // two groups of 16 bits at a time
-    uint32_t m[AT_ONCE];
+    uint32_t m[AT_ONCE], two[2];
 #pragma unroll
     for (int g = 0; g < AT_ONCE; ++g) m[g] = __vmaxu2(raw[g].w[0] & 0x7fff7fffu, raw[g].w[1] & 0x7fff7fffu);
 #pragma unroll
-    for (int g = 0; g < AT_ONCE; g += 2) {
-      uint32_t two = __vmaxu2(__byte_perm(m[g], m[g + 1], 0x5410), __byte_perm(m[g], m[g + 1], 0x7632));
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, o));
-      most[g] = two << 16;
-      most[g + 1] = two & 0xffff0000u;
-    }
+    for (int g = 0; g < 2; ++g) two[g] = __vmaxu2(__byte_perm(m[2 * g], m[2 * g + 1], 0x5410), __byte_perm(m[2 * g], m[2 * g + 1], 0x7632));
+    uint32_t mine = __vmaxu2(last ? two[1] : two[0], __shfl_xor_sync(0xffffffffu, last ? two[0] : two[1], 4));
+    mine = __vmaxu2(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+    mine = __vmaxu2(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+    return odd ? mine & 0xffff0000u : mine << 16;
   } else {
+    uint32_t m[AT_ONCE];
 #pragma unroll
     for (int g = 0; g < AT_ONCE; ++g) {
-      most[g] = 0u;
+      m[g] = 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) most[g] = max(most[g], raw[g].w[i] & 0x7fffffffu);
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) most[g] = max(most[g], __shfl_xor_sync(0xffffffffu, most[g], o));
+      for (int i = 0; i < 4; ++i) m[g] = max(m[g], raw[g].w[i] & 0x7fffffffu);
     }
+    const uint32_t even_group = max(last ? m[2] : m[0], __shfl_xor_sync(0xffffffffu, last ? m[0] : m[2], 4)), odd_group = max(last ? m[3] : m[1], __shfl_xor_sync(0xffffffffu, last ? m[1] : m[3], 4));
+    uint32_t mine = max(odd ? odd_group : even_group, __shfl_xor_sync(0xffffffffu, odd ? even_group : odd_group, 1));
+    return max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
   }
 }
 template <typename T> __device__ __forceinline__ void store4(T* p, bool vec, const float* x) {
@@ -143,27 +150,23 @@ __device__ __forceinline__ void get_units(const uint16_t* src, int ng, int n, ui
 
 constexpr float ROUND = 12582912.f;                                // 1.5 * 2^23: what is added to it is rounded to a whole number
 
-// Grid: blocks of heads of k and, behind them, of v
-template <typename T>
-__global__ void __launch_bounds__(THREADS) kv_store_4bit_kernel(const __grid_constant__ Side k, const __grid_constant__ Side v, const int* __restrict__ meta, int M, int G, int blocks, float eps) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const bool is_v = (int)blockIdx.x >= blocks;
-  const Side& s = is_v ? v : k;
-  const Head h = head_of(is_v ? blockIdx.x - blocks : blockIdx.x, meta, M, G);
+template <typename T> __device__ __forceinline__ void store_heads(const Side& s, bool norm, const Head& h, float eps) {
   const int ng = s.c.dim / GROUP4;
   const T* src = reinterpret_cast<const T*>(s.x) + h.row * s.ld + h.g * s.c.dim + h.q * 4;
   Raw4<T> raw[AT_ONCE];
   auto load = [&](int g0) {
+    const int n = h.there ? ng - g0 : 0;
+    if (s.vec && n >= AT_ONCE) {
 #pragma unroll
-    for (int g = 0; g < AT_ONCE; ++g) {
-      raw[g] = Raw4<T>{};
-      if (h.there && g0 + g < ng) raw[g] = load4(src + (g0 + g) * GROUP4, s.vec);
+      for (int g = 0; g < AT_ONCE; ++g) raw[g] = load4(src + (g0 + g) * GROUP4, true);
+    } else {
+#pragma unroll
+      for (int g = 0; g < AT_ONCE; ++g) raw[g] = g < n ? load4(src + (g0 + g) * GROUP4, s.vec) : Raw4<T>{};
     }
   };
   load(0);
   float root = 1.f, inv_root = 1.f;
-  if (s.norm) {
+  if (norm) {
     float sum = 0.f;
     for (int g0 = 0; g0 < ng; g0 += AT_ONCE) {
       if (g0 > 0) load(g0);
@@ -188,51 +191,60 @@ __global__ void __launch_bounds__(THREADS) kv_store_4bit_kernel(const __grid_con
   uint16_t* scales = held ? reinterpret_cast<uint16_t*>(s.c.scale4_at(h.slot, h.g)) + (long long)h.pos * ng : nullptr;
   for (int g0 = 0; g0 < ng; g0 += AT_ONCE) {
     if (g0 > 0) load(g0);
-    uint32_t most[AT_ONCE], units[AT_ONCE], sc[AT_ONCE];
-    most_of(raw, most);
+    // a lane sees to one group's scale (two lanes to the same), which the others get from it
+    float a = __uint_as_float(most_of(raw, h.q));
+    if (norm) a = quotient(a, root, inv_root);                   // (the largest before, divided as it is: rounding keeps order)
+    const bool bad = !(a <= 3.402823466e38f);
+    const __nv_bfloat16 s16 = __float2bfloat16_rn(quotient(fmaxf(a, LEAST), 7.f, 1.f / 7.f));
+    const float scale = __bfloat162float(s16);
+    const float inv = bad ? 0.f : inverse(scale) * (norm ? inv_root : 1.f);                  // (normed, the root is off by more than these two products)
+    uint32_t units[AT_ONCE];
 #pragma unroll
     for (int g = 0; g < AT_ONCE; ++g) {
-      float a = __uint_as_float(most[g]), x[4], c[4];
-      if (s.norm) a = quotient(a, root, inv_root);                 // (the largest before, divided as it is: rounding keeps order)
-      const bool bad = !(a <= 3.402823466e38f);
-      a = bad ? 1.f : fmaxf(a, LEAST);
-      const __nv_bfloat16 s16 = __float2bfloat16_rn(quotient(a, 7.f, 1.f / 7.f));
-      const float scale = __bfloat162float(s16), inv = inverse(scale);
-      sc[g] = bad ? 0x7fc0u : (uint32_t)__bfloat16_as_ushort(s16);
+      const float by = __shfl_sync(0xffffffffu, inv, lane_of(g), LANES);
+      float x[4], c[4];                                            // codes + ROUND, whose lowest bits are the codes
       numbers_of(raw[g], x);
-      if (s.norm) {                                                // (the root is off by more than these two products)
-        const float f = inv_root * inv;
+      if (norm) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = fmaf(x[i], f, ROUND) - ROUND;
+        for (int i = 0; i < 4; i += 2) unpack2(fma2(pack2(x[i], x[i + 1]), both(by), both(ROUND)), c[i], c[i + 1]);
       } else {
+        const float d = __shfl_sync(0xffffffffu, scale, lane_of(g), LANES);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          c[i] = (quotient(x[i], scale, inv) + ROUND) - ROUND;
-          // where rounding the quotient to 24 bits made a tie of it, the exact rest (a code times 8 bits) tells on which side it was; of two numbers of 8 bits it is a tie or far from one
-          if (sizeof(T) == 4) {
-            const float rest = fmaf(-c[i], scale, x[i]);
-            c[i] += fabsf(rest) > 0.5f * scale ? copysignf(1.f, rest) : 0.f;
+        for (int i = 0; i < 4; i += 2) {
+          const f32x2 y = pack2(x[i], x[i + 1]), e = mul2(y, both(by));
+          unpack2(add2(fma2(fma2(both(-d), e, y), both(by), e), both(ROUND)), c[i], c[i + 1]);   // (quotient())
+        }
+        // where rounding the quotient to 24 bits made a tie of it, the exact rest (a code times 8 bits) tells on which side it was; of two numbers of 8 bits it is a tie or far from one
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float rest = fmaf(-(c[i] - ROUND), d, x[i]);
+            c[i] += fabsf(rest) > 0.5f * d ? copysignf(1.f, rest) : 0.f;
           }
         }
       }
-      // four codes + 8 as the lowest 16 bits of a float
-      const float sum = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + (8388608.f + 0x8888);
-      units[g] = bad ? 0x8888u : __float_as_uint(sum) & 0xffffu;
+      uint32_t u = 0x8888u;                                        // four codes + 8
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u += __float_as_uint(c[i]) << (4 * i);
+      units[g] = by == 0.f ? 0x8888u : u & 0xffffu;
     }
     if (!held) continue;
-    const int n = min(AT_ONCE, ng - g0);
+    const int n = min(AT_ONCE, ng - g0), own = group_of(h.q);
     put_units(codes + g0, ng, n, units);
-    if (h.q == 0) put_units(scales + g0, ng, n, sc);
+    if ((h.q & 2) == 0 && own < n) scales[g0 + own] = bad ? 0x7fc0u : __bfloat16_as_ushort(s16);
   }
 }
 
+// Grid: blocks of heads of k and, behind them, of v (each with code of its own: which of two it is costs a lookup for whatever is asked of it)
 template <typename T>
-__global__ void __launch_bounds__(THREADS) kv_load_4bit_kernel(const __grid_constant__ Side k, const __grid_constant__ Side v, const int* __restrict__ meta, int M, int G, int blocks) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 8 : 4) kv_store_4bit_kernel(const __grid_constant__ Side k, const __grid_constant__ Side v, const int* __restrict__ meta, int M, int G, int blocks, float eps) {
   pdl_launch_dependents();
   pdl_wait();
-  const bool is_v = (int)blockIdx.x >= blocks;
-  const Side& s = is_v ? v : k;
-  const Head h = head_of(is_v ? blockIdx.x - blocks : blockIdx.x, meta, M, G);
+  if ((int)blockIdx.x < blocks) store_heads<T>(k, false, head_of(blockIdx.x, meta, M, G), eps);
+  else store_heads<T>(v, v.norm, head_of(blockIdx.x - blocks, meta, M, G), eps);
+}
+
+template <typename T> __device__ __forceinline__ void load_heads(const Side& s, const Head& h) {
   if (!h.there) return;
   const int ng = s.c.dim / GROUP4;
   const bool held = s.c.holds(h.slot, h.pos);
@@ -247,15 +259,33 @@ __global__ void __launch_bounds__(THREADS) kv_load_4bit_kernel(const __grid_cons
       get_units(scales + g0, ng, n, sc);
     }
 #pragma unroll
-    for (int g = 0; g < AT_ONCE; ++g) {
-      if (g >= n) break;
-      const float scale = __uint_as_float(sc[g] << 16);
-      float x[4];
+    for (int g = 0; g < AT_ONCE; g += 2) {                         // two groups' codes at a time, as 128 + n in bf16; a code times a scale has 12 bits, which are rounded once
+      const uint32_t two = u[g] | u[g + 1] << 16;
+      __nv_bfloat162 c[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = (float)((int)(u[g] >> (4 * i) & 15u) - 8) * scale;
-      store4(dst + (g0 + g) * GROUP4, s.vec, x);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = (two >> (4 * i) & 0x000f000fu) | 0x43004300u;
+        c[i] = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w), __float2bfloat162_rn(136.f));
+      }
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        if (g + o >= n) break;
+        const float scale = __uint_as_float(sc[g + o] << 16);
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (o ? __high2float(c[i]) : __low2float(c[i])) * scale;
+        store4(dst + (g0 + g + o) * GROUP4, s.vec, x);
+      }
     }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) kv_load_4bit_kernel(const __grid_constant__ Side k, const __grid_constant__ Side v, const int* __restrict__ meta, int M, int G, int blocks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if ((int)blockIdx.x < blocks) load_heads<T>(k, head_of(blockIdx.x, meta, M, G));
+  else load_heads<T>(v, head_of(blockIdx.x - blocks, meta, M, G));
 }
 
 Side make_side(const void* x, long long ld, int act_f32, const LiaCacheView* view, int norm) {
