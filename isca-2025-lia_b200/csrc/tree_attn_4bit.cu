@@ -199,9 +199,26 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
   }
   __syncthreads();
   uint2 qa[NR == 1 ? S::STEPS : 1];                                // few rows' queries stay in registers, the others' in shared memory
-  if constexpr (PACKED) {                                          // column gq: row gq & 1, in the quarter gq >> 1 of the steps
+  constexpr int PER = 4 / S::KG, VPER = 4 / S::VG;                 // (PACKED) quarters of a group of keys' and of values' channels: 1 or 2
+  uint32_t lower[2], upper[2];                                     // (PACKED) where of a word of two groups' weights those of a column's group go
+  if constexpr (PACKED) {                                          // column gq: row gq & 1, in quarter gq >> 1.  A key's word has the same four channels of two groups: a step has two of them, of either group
+    const int quarter = gq >> 1, group = quarter / PER, vgroup = quarter / VPER;
 #pragma unroll
-    for (int s = 0; s < S::STEPS; ++s) qa[s] = (gq >> 1) == s / (S::STEPS / 4) ? qs[s * 32 + (gq & 1) * 4 + t4] : make_uint2(0u, 0u);
+    for (int w = 0; w < S::STEPS / 2; ++w)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const uint2 u = qs[(group * 2 + st) * 32 + (gq & 1) * 4 + t4];
+        const int pairs = S::KG / 2, four = w / pairs;             // the group's four 2 t4 or 2 t4 + 1
+        const bool mine = group / 2 == w % pairs && (PER == 1 || (quarter & 1) == st);
+        const uint32_t to = !mine ? 0x4444u : four == 0 ? (group & 1 ? 0x1044u : 0x4410u) : (group & 1 ? 0x3244u : 0x4432u);
+        qa[w * 2 + st] = make_uint2(__byte_perm(u.x, 0u, to), __byte_perm(u.y, 0u, to));
+      }
+#pragma unroll
+    for (int h = 0; h < S::VG / 2; ++h) {
+      const bool mine = vgroup / 2 == h && quarter % VPER == 0;
+      lower[h] = !mine ? 0x4444u : vgroup & 1 ? 0x1044u : 0x4410u;
+      upper[h] = !mine ? 0x4444u : vgroup & 1 ? 0x3244u : 0x4432u;
+    }
   } else if constexpr (NR == 1) {
 #pragma unroll
     for (int s = 0; s < S::STEPS; ++s) qa[s] = qs[s * 32 + lane];
@@ -224,11 +241,12 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
 #pragma unroll
       for (int e = 0; e < 2; ++e) from[gr][e] = PACKED ? row_q[e * 4 + t4] : row_q[(t4 * 2 + e) * S::KG + gr];
   }
-  float o[NR][S::MT][4];                                           // [..][0]: a lane's first channel of a pair and row 2 t4, [1]: row 2 t4 + 1, [2], [3]: its second channel
+  constexpr int MT = PACKED ? 2 : S::MT;
+  float o[NR][MT][4];                                              // [..][0]: a lane's first channel of a pair and row 2 t4, [1]: row 2 t4 + 1, [2], [3]: its second channel (PACKED: of group t4 / VPER)
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int n = 0; n < S::MT; ++n)
+    for (int n = 0; n < MT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[r][n][e] = 0.f;
 
@@ -252,17 +270,16 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
     if constexpr (PACKED) {
       float even[4] = {from[0][0], from[0][1], from[0][0], from[0][1]}, odd[4] = {};
 #pragma unroll
-      for (int gr = 0; gr < S::KG; ++gr) {
+      for (int w = 0; w < S::STEPS / 2; ++w) {
         uint32_t codes[2][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) small4x2(codes_of(j, gr), codes[j]);
+        for (int j = 0; j < 2; ++j) small4x2(kr[j][w], codes[j]);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const uint32_t ka[4] = {codes[0][2 * st], codes[1][2 * st], codes[0][2 * st + 1], codes[1][2 * st + 1]};
-          mma_f16(st == 0 ? even : odd, ka, qa[gr * 2 + st].x, qa[gr * 2 + st].y);
+          mma_f16(st == 0 ? even : odd, ka, qa[w * 2 + st].x, qa[w * 2 + st].y);
         }
       }
-      constexpr int PER = 4 / S::KG;                               // quarters of a group
       float kg[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) kg[j] = lds_bf16(at + S::KS_AT + ((gq + j * 8) * S::KG + t4 / PER) * 2);
@@ -329,7 +346,7 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
       lv[j] = lg2(y);
       rv[j] = rcp(y);
       if constexpr (PACKED) {
-        ratio[j][0] = lds_bf16(from_at + t4 / (4 / S::VG) * 2) * rv[j];
+        ratio[j][0] = lds_bf16(from_at + t4 / VPER * 2) * rv[j];
       } else {
         scales4_of<S::VG>(vs4, ratio[j]);
 #pragma unroll
@@ -381,7 +398,7 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
           if (up) m[r][e] = top - LIFT;
           l[r][e] *= keep;
 #pragma unroll
-          for (int n = 0; n < S::MT; ++n) {
+          for (int n = 0; n < MT; ++n) {
             o[r][n][e] *= keep;
             o[r][n][2 + e] *= keep;
           }
@@ -413,16 +430,33 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
     __syncwarp();                                                  // the stage has been read
     bring(b + DEPTH * WARPS, stage);
     stage = stage + 1 == DEPTH ? 0 : stage + 1;
+    if constexpr (PACKED) {
 #pragma unroll
-    for (int gr = 0; gr < S::VG; ++gr) {
-      uint32_t va[2][4];                                           // a lane's four channels of the group, of keys 2 t4 and 2 t4 + 1, and of those 8 on
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) int4x2(__byte_perm(vr[2 * c][gr >> 1], vr[2 * c + 1][gr >> 1], gr & 1 ? 0x7632 : 0x5410), va[c]);
+        for (int h = 0; h < S::VG / 2; ++h) {
+          uint32_t codes[2][4];                                    // of keys 8 j + 2 t4 and the next one: four channels of two groups
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        const uint32_t v4[4] = {va[0][c], va[0][c + 1], va[1][c], va[1][c + 1]};
+          for (int c = 0; c < 2; ++c) int4x2(vr[2 * j + c][h], codes[c]);
+          const uint32_t lo16 = __byte_perm(pb[0][0][j], 0u, lower[h]), hi16 = __byte_perm(pb[0][0][j], 0u, upper[h]);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) mma_f16(o[r][gr * 2 + (c >> 1)], v4, pb[PACKED ? 0 : gr][r][0], pb[PACKED ? 0 : gr][r][1]);
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t v4[4] = {codes[0][2 * n], codes[0][2 * n + 1], codes[1][2 * n], codes[1][2 * n + 1]};
+            mma_f16(o[0][n], v4, lo16, hi16);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int gr = 0; gr < S::VG; ++gr) {
+        uint32_t va[2][4];                                           // a lane's four channels of the group, of keys 2 t4 and 2 t4 + 1, and of those 8 on
+#pragma unroll
+        for (int c = 0; c < 2; ++c) int4x2(__byte_perm(vr[2 * c][gr >> 1], vr[2 * c + 1][gr >> 1], gr & 1 ? 0x7632 : 0x5410), va[c]);
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          const uint32_t v4[4] = {va[0][c], va[0][c + 1], va[1][c], va[1][c + 1]};
+#pragma unroll
+          for (int r = 0; r < NR; ++r) mma_f16(o[r][gr * 2 + (c >> 1)], v4, pb[gr][r][0], pb[gr][r][1]);
+        }
       }
     }
   }
@@ -440,10 +474,14 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
       for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
       const int at = warp * S::ROWS + (PACKED ? e : r * 8 + t4 * 2 + e);
       if (gq == 0 && (!PACKED || t4 == 0)) part[at] = make_float2(m[r][e], x);
+      if constexpr (PACKED) {
+        if (t4 % VPER == 0)
+          *reinterpret_cast<float4*>(os + at * VDIM + t4 / VPER * GROUP4 + gq * 4) = make_float4(o[0][0][e], o[0][0][2 + e], o[0][1][e], o[0][1][2 + e]);
+      } else {
 #pragma unroll
-      for (int n = 0; n < S::MT; ++n)
-        if (!PACKED || t4 == (n >> 1) * (4 / S::VG))               // (of a lane's columns those of the channels' own group)
+        for (int n = 0; n < S::MT; ++n)
           *reinterpret_cast<float2*>(os + at * VDIM + (n >> 1) * GROUP4 + gq * 4 + (n & 1) * 2) = make_float2(o[r][n][e], o[r][n][2 + e]);
+      }
     }
   __syncthreads();
 }
