@@ -5,14 +5,18 @@
 // As over 8 bits the keys are the products' rows and the queries their columns, and a warp takes 16 keys at a time.  What is different: half the bytes leave half the time, so that instructions count.
 //   * Keys, values and scales come to shared memory by cp.async, DEPTH blocks of a warp ahead, and from there as the products want them.
 //   * A key's codes are code + 8 = u in 0 .. 15: four bits in the lowest ten of an fp16 number are the subnormal number u 2^-24 (or 16 u 2^-24, whose query is divided by 16), so that one instruction
-//     makes two operands.  The sums begin with -8 (the queries' sum) instead of 0.  With more than eight rows the 2^10 and the offset are subtracted from 1024 + u instead, as they are of values, whose
-//     offset would be -8 (the weights' sum): that is large beside what many keys' values average out to.
+//     makes two operands.  The sums begin with -8 (the queries' sum) instead of 0.  With more than eight rows the 2^10 and the offset are subtracted from 1024 + u instead, as they are of values with
+//     more than two.
 //   * A value's group scale multiplies its weight, relative to the value's largest scale, which goes into the exponent (tree_attn.cu).
 //   * One or two rows (PACKED; a decoded token of up to two query heads): the eight columns are four quarters of the channels times two rows.  A column's query is nothing but in its quarter, whose
-//     group is one, so that a lane has one scale a key instead of four, and a weight goes into the second product once, not once a group.
+//     group is one, so that a lane has one scale a key instead of four, and a weight goes into the second product once, not once a group.  A word of codes has four channels of two groups, and is taken as
+//     it is: what belongs together along the products' sum are the same channel of two groups, of which a column's query or weight is that of its own group, and nothing for the other.  Values' codes are
+//     subnormal numbers too: the sums of 16 keys begin with -8 (their weights' sum), and are added to what was before (over all keys that would be large beside what they average out to; of 16 it leaves
+//     2^-13 of a weight times its value's scale at most, where a weight's own rounding leaves 2^-11 of a weight times its value).
 //
-// 16 tokens behind 21000 to 30001 positions, 16 heads on 8 (475 MB): 117 us, 4.1 TB/s, 62 % of the copy rate; with the 8-bit kernel's structure 207.  What bounds it: instructions, some 350 a warp for 16
-// keys (488 before), half of them on the integer pipe (59 % busy, issue slots 61 %); a fifth block an SM changes nothing.
+// 16 tokens behind 21000 to 30001 positions, 16 heads on 8 (475 MB): 98 us, 4.9 TB/s, 74 % of the copy rate, the second launch among them; with the 8-bit kernel's structure 207.  What bounds it:
+// instructions, some 290 a warp for 16 keys (488 at first; 342 with values' codes less 1032 instead of subnormal, 110 us), half of them on the integer pipe (51 % busy, issue slots 62 %), and memory next;
+// five or six blocks an SM change nothing (99.5, 100), nor do shorter spans (twice as many 112).
 #include "mma.cuh"
 #include "tree_attn.cuh"
 
@@ -123,6 +127,7 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
     if (b < b1) {
       const uint32_t at = ring + stage * S::STAGE;
       const int last = hi - 1 - (lo + b * 16);                     // of the block: keys behind it are that one again
+      const bf16* src = sp;
       if (last >= 15) {
 #pragma unroll
         for (int n = 0; n < KN; ++n) cp_async16(at + k_to + n * 512, kp + n * 8 * a.k.pos, 16);
@@ -136,8 +141,8 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
           const int i = lane / VCH + n * 8;
           cp_async16(at + 16 * S::KROW + value_at<S::VROW>(i, lane % VCH), vp + (long long)(min(i, last) - lane / VCH) * a.v.pos, 16);
         }
+        src += (min(lane & 15, last) - (lane & 15)) * sgroups;
       }
-      const bf16* src = sp + (min(lane & 15, last) - (lane & 15)) * sgroups;
       if constexpr (S::KG == S::VG) {
         cp_async_small<S::KG * 2>(at + s_to, src);
       } else {
@@ -430,21 +435,30 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
     __syncwarp();                                                  // the stage has been read
     bring(b + DEPTH * WARPS, stage);
     stage = stage + 1 == DEPTH ? 0 : stage + 1;
-    if constexpr (PACKED) {
+    if constexpr (PACKED) {                                        // 16 keys' sums begin with -8 (the weights' sum): of 16 keys that is no more than the products are
+      float sum[2][4] = {};
+      constexpr uint32_t OFFSET[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};     // -8 2^-24, and 16 times that
+      mma_f16(sum[0], OFFSET, pb[0][0][0], pb[0][0][1]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[1][e] = sum[0][e];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int h = 0; h < S::VG / 2; ++h) {
           uint32_t codes[2][4];                                    // of keys 8 j + 2 t4 and the next one: four channels of two groups
 #pragma unroll
-          for (int c = 0; c < 2; ++c) int4x2(vr[2 * j + c][h], codes[c]);
+          for (int c = 0; c < 2; ++c) small4x2(vr[2 * j + c][h], codes[c]);
           const uint32_t lo16 = __byte_perm(pb[0][0][j], 0u, lower[h]), hi16 = __byte_perm(pb[0][0][j], 0u, upper[h]);
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             const uint32_t v4[4] = {codes[0][2 * n], codes[0][2 * n + 1], codes[1][2 * n], codes[1][2 * n + 1]};
-            mma_f16(o[0][n], v4, lo16, hi16);
+            mma_f16(sum[n], v4, lo16, hi16);
           }
         }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][n][e] += sum[n][e];
     } else {
 #pragma unroll
       for (int gr = 0; gr < S::VG; ++gr) {
@@ -476,7 +490,7 @@ template <int DIM, int VDIM, int NR, bool PACKED> __device__ __forceinline__ voi
       if (gq == 0 && (!PACKED || t4 == 0)) part[at] = make_float2(m[r][e], x);
       if constexpr (PACKED) {
         if (t4 % VPER == 0)
-          *reinterpret_cast<float4*>(os + at * VDIM + t4 / VPER * GROUP4 + gq * 4) = make_float4(o[0][0][e], o[0][0][2 + e], o[0][1][e], o[0][1][2 + e]);
+          *reinterpret_cast<float4*>(os + at * VDIM + t4 / VPER * GROUP4 + gq * 4) = make_float4(o[0][0][e] * 0x1p24f, o[0][0][2 + e] * 0x1p20f, o[0][1][e] * 0x1p24f, o[0][1][2 + e] * 0x1p20f);
       } else {
 #pragma unroll
         for (int n = 0; n < S::MT; ++n)

@@ -2,7 +2,10 @@
 
 Tolerances are those of attention over 8-bit caches (tests/test_gpu_tree_attn.py): weights in fp16, 2^-11 of A; with more than 32 rows of a key head values are multiplied by their group's scale in
 fp16 as well, 2^-11 for the factor and 2^-11 for the product.  There keys are multiplied by their group's scale, relative to the key's largest, in the same way: 2^-10 of every product, so that a score
-is off by up to 2^-10 B more."""
+is off by up to 2^-10 B more.
+
+Up to two rows of a key head: the sums of 16 keys, of codes + 8 times weights, begin with -8 times the weights' sum W.  That is 5 products of up to 17 additions, each at least as exact as fp32 cut off
+(2^-23) and none of more than 15 W in codes: 5 * 17 * 2^-23 * 15 W, and over all keys as much of the weighted sum of the channel's scales, where A is the weighted sum of its numbers."""
 import pytest
 import torch
 
@@ -55,6 +58,8 @@ class Case4(Case):
                 x = x.masked_fill(~see, -INF)
                 p = torch.where(see.any(1, keepdim=True), torch.softmax(x, -1), torch.zeros_like(x))
                 o, A = p @ v, p @ v.abs()
+                if max(s[3] for s in self.segs) * (self.H // self.G) <= 2:
+                    A = A + 2.0 ** 11 * 5 * 17 * 15 * 2.0 ** -23 * (p @ self.vs[s, g, :p0 + n].double().nan_to_num().repeat_interleave(32, -1))
                 d = (self.dim * 2.0 ** -24 + (2.0 ** -10 if many else 0)) * B + 2.0 ** -21 * (S + self.softcap) + 2.0 ** -20
                 tol = 2.0 ** -8 * o.abs() + ((3 if many else 1) * 2.0 ** -11 + 2 * d) * A + 1e-30
                 got = out[r:r + n, h * self.vdim:(h + 1) * self.vdim].double()
