@@ -374,8 +374,8 @@ struct Plan {
 int rows_here(int type, long long span) { return type == LIA_CACHE_BF16 && span > 512 ? 16 : 32; }
 long long span_of(int rows, int max_ctx, int window) { return window > 0 && (long long)window + rows < max_ctx ? (long long)window + rows : max_ctx; }
 // Histories of four bits: up to eight rows of a key head in equal spans of all histories together, which no block has more of than another, and a second launch that joins; or so many blocks a history,
-// and a cluster that joins.  us, spans | splits: a token of 16 requests behind 30001 positions, 16 heads on 8, 135 | 145, of requests behind 21000 to 30001 117 | 136, behind 3000 to 30001 85 | 131; of 32
-// behind 8000, 8 heads on 8 (3459 keys a block) 79 | 82; of 64 behind 2000, 32 heads on 8 (1729) 54 | 49; of 16 behind 1901 (411) 22 | 16.
+// and a cluster that joins.  us, spans | splits: a token of 16 requests behind 30001 positions, 16 heads on 8, 111 | 124, of requests behind 21000 to 30001 97 | 116, behind 3000 to 30001 71 | 107; of 32
+// behind 8000, 8 heads on 8 (3459 keys a block) 68 | 69; of 64 behind 2000, 32 heads on 8 (1729) 53 | 49; of 16 behind 1901 (411) 20 | 14.
 constexpr long long SPAN_KEYS = 3000;                              // of a block, from which on
 Plan cut(int nr, long long R, int nseg, int rows, int max_ctx, int G, int window, int type) {
   Plan p{};
