@@ -709,18 +709,23 @@ Plan plan_of(int M, int N, int K) {
   auto tiles = [&](int rows, int cols) { return (long long)((M + rows - 1) / rows) * ((N + cols - 1) / cols); };
   auto rounds = [&](long long n, int workers) { return (n + workers - 1) / workers; };
   long long least = -1;
-  auto offer = [&](int bn, bool pair, long long ns) {
-    if (least >= 0 && ns >= least) return;
-    least = ns;
+  auto offer = [&](int bn, bool pair, long long time) {
+    if (least >= 0 && time >= least) return;
+    least = time;
     p.bn = bn;
     p.pair = pair;
   };
-  // ns of a round for each block of K, and once, fitted to 7 matrices from 1024 x 1024 to 28672 x 7168 at 129 to 4096 tokens.  us by pairs | 256 wide | 128 | 64: 256 tokens of 1024 x 1024 10.4 | 10.0 | 7.8
-  // | 7.2; of 7168 x 7168 26.6 | 30.5 | 22.1 | 27.4; 1000 tokens of it 45 | 52 | 55 | 82; 4096 of 28672 x 7168 521 | 566 | 801 | 1364.
-  offer(256, true, rounds(tiles(2 * TILE, 256), sms / 2) * p.k_blocks * 330 + 5000);
-  offer(256, false, rounds(tiles(TILE, 256), sms) * p.k_blocks * 390 + 4300);
-  offer(128, false, rounds(tiles(TILE, 128), sms) * p.k_blocks * 235 + 3200);
-  offer(64, false, rounds(tiles(TILE, 64), sms) * p.k_blocks * 190 + 2900);
+  // ns: a call's own, and for each round what its blocks of K take or, behind the first one, what its sums take on their way out if that is longer; fitted to 90 shapes (on which what is chosen so takes 0.7 %
+  // more than the best).  us by pairs | 256 wide | 128 | 64, of codes: 256 tokens of 1024 x 1024 7.6 | 7.4 | 5.5 | 4.9, of 7168 x 7168 22 | 21 | 15 | 24; 1000 tokens of it 39 | 40 | 46 | 76; 1150 of
+  // 23176 x 416 28 | 24 | 28 | 37; 4096 of 28672 x 7168 493 | 622 | 765 | 1265.
+  auto ns = [&](long long n, int workers, long long once, int block, int sums) {
+    const long long products = (long long)p.k_blocks * block;
+    return once + products + (rounds(n, workers) - 1) * (products > sums ? products : sums);
+  };
+  offer(256, true, ns(tiles(2 * TILE, 256), sms / 2, 5900, 374, 3900));
+  offer(256, false, ns(tiles(TILE, 256), sms, 6000, 533, 3300));
+  offer(128, false, ns(tiles(TILE, 128), sms, 5000, 342, 2150));
+  offer(64, false, ns(tiles(TILE, 64), sms, 4550, 253, 1600));
   const int rows = p.pair ? 2 * TILE : TILE;
   p.tiles_a = (M + rows - 1) / rows;
   p.tiles_b = (N + p.bn - 1) / p.bn;
