@@ -9,7 +9,8 @@
 //          among as many tiles as there are.  Weights are on their way while the tokens are quantised.
 //   a token or two and matrices up to 64 Mi products, whose time is latency: int8_tokens_kernel, on the ordinary cores and in one launch.  Every block makes the tokens' codes for itself, in shared memory,
 //          while its first weights are on their way; a warp has an equal part of the block's channels' codes.
-//   MANY   (bound by the tensor cores)  the tokens' rows are the product's rows: CTA pairs on 256 x 256 tiles (cta_group::2), or one CTA on 128 x 256, 128 or 64 where those would leave SMs idle.
+//   MANY   (bound by the tensor cores, and what feeds them)  the tokens' rows are the product's rows: a CTA an SM on tiles of 128 x 256, or 128 or 64 where those would leave SMs idle.  (CTA pairs on
+//          256 x 256 tiles, cta_group::2, took 493 us instead of 622 for 4096 tokens of 28672 x 7168, and came to a standstill once in some 20000 launches; why was not found, so they are not here.)
 //
 // Every wait is bounded; a CTA that gives one up makes its tile's outputs NaN and counts itself in lia_moe_timeouts_seen().
 #include <cuda.h>
@@ -280,14 +281,8 @@ __device__ __forceinline__ void mma_i8_if(uint32_t one, uint32_t d, uint64_t a, 
                "r"(accumulate), "r"(one)
                : "memory");
 }
-__device__ __forceinline__ void mma_i8_pair_if(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-               "r"(accumulate), "r"(one)
-               : "memory");
-}
-
-template <bool FEW, int BN, bool PAIR> struct Shape {
-  static constexpr int A_BYTES = TILE * KB, B_BYTES = (PAIR ? BN / 2 : BN) * KB, STAGE = A_BYTES + B_BYTES;
+template <bool FEW, int BN> struct Shape {
+  static constexpr int A_BYTES = TILE * KB, B_BYTES = BN * KB, STAGE = A_BYTES + B_BYTES;
   static constexpr int OUT_WARPS = FEW ? 4 : 8, THREADS = 128 + 32 * OUT_WARPS;                // warps that take sums to outputs: two for 32 rows of a tile
   static constexpr int STAGING = FEW ? 0 : OUT_WARPS * 2048;       // 32 rows of 64 bytes for each of them
   static constexpr int STAGES = ((FEW ? 112640 : 228352) - STAGING) / STAGE > 8 ? 8 : ((FEW ? 112640 : 228352) - STAGING) / STAGE;    // (of FEW's, two blocks fit an SM)
@@ -303,15 +298,15 @@ struct Work {
 template <bool FEW> struct Sched {
   int k_blocks, tiles_a, tiles_b, group;
   unsigned pos, end, step;
-  __device__ __forceinline__ Sched(const Args& p, bool pair) : k_blocks(p.k_blocks), tiles_a(p.tiles_a), tiles_b(p.tiles_b), group(pair ? 8 : 16) {
+  __device__ __forceinline__ explicit Sched(const Args& p) : k_blocks(p.k_blocks), tiles_a(p.tiles_a), tiles_b(p.tiles_b), group(16) {
     if (FEW) {
       const unsigned tile = blockIdx.x / (unsigned)p.parts, part = blockIdx.x - tile * (unsigned)p.parts;
       pos = tile * (unsigned)k_blocks + (unsigned)k_blocks * part / (unsigned)p.parts;         // (k_blocks is 1024 at most, and parts 8)
       end = tile * (unsigned)k_blocks + (unsigned)k_blocks * (part + 1) / (unsigned)p.parts;
       step = 0;
     } else {
-      pos = pair ? blockIdx.x >> 1 : blockIdx.x;
-      step = pair ? gridDim.x >> 1 : gridDim.x;
+      pos = blockIdx.x;
+      step = gridDim.x;
       end = (unsigned)tiles_a * (unsigned)tiles_b;
     }
   }
@@ -340,13 +335,11 @@ template <bool OUT32> __device__ __forceinline__ void put_one(void* out, size_t 
   else reinterpret_cast<bf16*>(out)[at] = __float2bfloat16_rn(y);
 }
 
-template <bool FEW, int BN, bool PAIR, bool OUT32>
-__global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Args p) {
-  static_assert(!PAIR || (!FEW && BN == 256), "CTA pairs: 256 x 256 tiles");
+template <bool FEW, int BN, bool OUT32>
+__global__ void __launch_bounds__(Shape<FEW, BN>::THREADS, FEW ? 2 : 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Args p) {
   static_assert(FEW || BN >= 64, "two warps share the columns");
-  using L = Shape<FEW, BN, PAIR>;
+  using L = Shape<FEW, BN>;
   constexpr int STAGES = L::STAGES;
-  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;             // of a pair the first issues every product and owns the barriers that loads and epilogues arrive on
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem - smem_u32(smem_raw));
@@ -372,23 +365,17 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull(a), 1);
-      mbar_init(tempty(a), L::OUT_WARPS * (PAIR ? 2 : 1));
+      mbar_init(tempty(a), L::OUT_WARPS);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
-    if (PAIR) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_at)), "r"((uint32_t)L::COLS) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_at)), "r"((uint32_t)L::COLS) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_at)), "r"((uint32_t)L::COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tcgen05_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync_all();
   tcgen05_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
   pdl_launch_dependents();                                         // (only weights are touched before pdl_wait)
@@ -399,7 +386,7 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
     if (lane == 0) {
       int early = 0;
       if (FEW) {                                                   // weights, which no kernel writes, before the tokens' codes are there
-        Sched<FEW> s(p, PAIR);
+        Sched<FEW> s(p);
         Work w;
         while (early < STAGES && s.next(w))
           for (int kb = w.kb0; kb < w.kb1 && early < STAGES; ++kb, ++early) {
@@ -408,7 +395,7 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
           }
       }
       pdl_wait();
-      Sched<FEW> s(p, PAIR);
+      Sched<FEW> s(p);
       Work w;
       int stage = 0;
       uint32_t phase = 0;
@@ -420,16 +407,9 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
             tma_load_2d(sb, &tmB, kb * KB, 0, full(stage));
           } else {
             if (!(alive = wait_for(empty(stage), phase ^ 1u, dead))) break;
-            if (PAIR) {
-              const uint32_t fb = mapa_u32(full(stage), 0);
-              if (rank == 0) mbar_expect_tx(full(stage), 2 * L::STAGE);
-              tma_load_2d_pair(sa, &tmA, kb * KB, (w.ta * 2 + (int)rank) * TILE, fb);
-              tma_load_2d_pair(sb, &tmB, kb * KB, w.tb * BN + (int)rank * (BN / 2), fb);
-            } else {
-              mbar_expect_tx(full(stage), L::STAGE);
-              tma_load_2d(sa, &tmA, kb * KB, w.ta * TILE, full(stage));
-              tma_load_2d(sb, &tmB, kb * KB, w.tb * BN, full(stage));
-            }
+            mbar_expect_tx(full(stage), L::STAGE);
+            tma_load_2d(sa, &tmA, kb * KB, w.ta * TILE, full(stage));
+            tma_load_2d(sb, &tmB, kb * KB, w.tb * BN, full(stage));
           }
           ++issued;
           if (++stage == STAGES) {
@@ -440,47 +420,36 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
     }
   } else if (warp == 1) {
     // ================================================================ products
-    if (rank == 0) {
-      const uint32_t one = elect_one();
-      constexpr uint32_t idesc = idesc_i8(PAIR ? 2 * TILE : TILE, BN);
-      Sched<FEW> s(p, PAIR);
-      Work w;
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool alive = true;
-      while (alive && s.next(w)) {
-        if (!(alive = warp_wait(tempty(acc), acc_phase ^ 1u, dead))) break;
+    const uint32_t one = elect_one();
+    constexpr uint32_t idesc = idesc_i8(TILE, BN);
+    Sched<FEW> s(p);
+    Work w;
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool alive = true;
+    while (alive && s.next(w)) {
+      if (!(alive = warp_wait(tempty(acc), acc_phase ^ 1u, dead))) break;
+      tcgen05_fence_after();
+      const uint32_t d = tmem + (uint32_t)(acc * BN);
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        if (!(alive = warp_wait(full(stage), phase, dead))) break;
         tcgen05_fence_after();
-        const uint32_t d = tmem + (uint32_t)(acc * BN);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!(alive = warp_wait(full(stage), phase, dead))) break;
-          tcgen05_fence_after();
-          const uint32_t sa = smem + stage * L::STAGE;
-          const uint64_t da = make_smem_desc(sa), db = make_smem_desc(sa + L::A_BYTES);
+        const uint32_t sa = smem + stage * L::STAGE;
+        const uint64_t da = make_smem_desc(sa), db = make_smem_desc(sa + L::A_BYTES);
 #pragma unroll
-          for (int k = 0; k < KB / 32; ++k) {                      // 32 codes on are 32 bytes inside the swizzled row: + 2 in the address field
-            if (PAIR) mma_i8_pair_if(one, d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb > w.kb0 || k > 0) ? 1u : 0u);
-            else mma_i8_if(one, d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb > w.kb0 || k > 0) ? 1u : 0u);
-          }
-          if (PAIR) {
-            if (one) tcgen05_commit_pair(empty(stage));
-          } else {
-            commit_if(one, empty(stage));
-          }
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        for (int k = 0; k < KB / 32; ++k) {                      // 32 codes on are 32 bytes inside the swizzled row: + 2 in the address field
+          mma_i8_if(one, d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb > w.kb0 || k > 0) ? 1u : 0u);
         }
-        if (!alive) break;
-        if (PAIR) {
-          if (one) tcgen05_commit_pair(tfull(acc));
-        } else {
-          commit_if(one, tfull(acc));
+        commit_if(one, empty(stage));
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
       }
+      if (!alive) break;
+      commit_if(one, tfull(acc));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
     }
   } else if (warp >= 4) {
     // ================================================================ sums to outputs
@@ -493,7 +462,7 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
       if (i < BN) scales_s[i] = i < p.M ? __ldcg(p.sx + i) : 0.f;
       out_warps_meet();
     }
-    Sched<FEW> s(p, PAIR);
+    Sched<FEW> s(p);
     Work w;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -509,10 +478,7 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
       auto give_back = [&] {                                       // the sums are read
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(tempty(acc), 0));
-          else mbar_arrive(tempty(acc));
-        }
+        if (lane == 0) mbar_arrive(tempty(acc));
       };
       if constexpr (FEW) {
         // a lane has one channel, its columns are the tokens: to shared memory where the operands were, [tokens][TILE]
@@ -532,7 +498,7 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
         }
       } else {
         // a lane has one token, its columns are channels: through shared memory to whole rows
-        const int row0 = (w.ta * (PAIR ? 2 : 1) + (int)rank) * TILE + ew * 32, m = row0 + lane;
+        const int row0 = w.ta * TILE + ew * 32, m = row0 + lane;
         const float sx = m < p.M ? __ldcg(p.sx + m) : 0.f;
         const uint32_t stg = smem + STAGES * L::STAGE + (warp - 4) * 2048;
         constexpr int PER = OUT32 ? 4 : 8, COLS = OUT32 ? 16 : 32; // columns of 16 bytes; of 64, which 32 rows of are in shared memory at a time
@@ -642,27 +608,22 @@ __global__ void __launch_bounds__(Shape<FEW, BN, PAIR>::THREADS, FEW ? 2 : 1) in
   if (*dead) {                                                     // loads and products in flight end before shared memory and TMEM are given back
     if (threadIdx.x == 0) {
       atomicAdd_system(p.timeouts, 1);
-      for (int i = 0; i < STAGES && i < issued && rank == 0; ++i) { // (a pair's loads all arrive on the first one's barriers)
+      for (int i = 0; i < STAGES && i < issued; ++i) {
         const int n = issued - 1 - i;
         wait_in_flight(full(n % STAGES), (uint32_t)(n / STAGES) & 1u);
       }
     }
-    if (warp == 1 && rank == 0) {
+    if (warp == 1) {
       const uint32_t one = elect_one();
-      if (PAIR) {
-        if (one) tcgen05_commit_pair(drain);
-      } else {
-        commit_if(one, drain);
-      }
+      commit_if(one, drain);
       wait_in_flight(drain, 0u);
     }
     __syncthreads();
   }
-  if (PAIR || (FEW && p.parts > 1)) cluster_barrier();             // nobody leaves while others may arrive on its barriers, or read its sums
+  if (FEW && p.parts > 1) cluster_barrier();                       // nobody leaves while others may read its sums
   if (warp == 2) {
     tcgen05_fence_after();
-    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
   }
 }
 
@@ -683,7 +644,7 @@ int make_tmap(CUtensorMap* map, const void* base, int rows, int K, long long ld,
 }
 
 struct Plan {
-  bool few, pair;
+  bool few;
   int bn, grid, tiles_a, tiles_b, k_blocks, parts;                 // parts: CTAs of a cluster that share a tile
 };
 Plan plan_of(int M, int N, int K) {
@@ -706,31 +667,26 @@ Plan plan_of(int M, int N, int K) {
     p.grid = p.tiles_a * p.parts;
     return p;
   }
-  auto tiles = [&](int rows, int cols) { return (long long)((M + rows - 1) / rows) * ((N + cols - 1) / cols); };
-  auto rounds = [&](long long n, int workers) { return (n + workers - 1) / workers; };
+  auto tiles = [&](int cols) { return (long long)((M + TILE - 1) / TILE) * ((N + cols - 1) / cols); };
   long long least = -1;
-  auto offer = [&](int bn, bool pair, long long time) {
+  auto offer = [&](int bn, long long time) {
     if (least >= 0 && time >= least) return;
     least = time;
     p.bn = bn;
-    p.pair = pair;
   };
-  // ns: a call's own, and for each round what its blocks of K take or, behind the first one, what its sums take on their way out if that is longer; fitted to 90 shapes (on which what is chosen so takes 0.7 %
-  // more than the best).  us by pairs | 256 wide | 128 | 64, of codes: 256 tokens of 1024 x 1024 7.6 | 7.4 | 5.5 | 4.9, of 7168 x 7168 22 | 21 | 15 | 24; 1000 tokens of it 39 | 40 | 46 | 76; 1150 of
-  // 23176 x 416 28 | 24 | 28 | 37; 4096 of 28672 x 7168 493 | 622 | 765 | 1265.
-  auto ns = [&](long long n, int workers, long long once, int block, int sums) {
+  // ns: a call's own, and for each round what its blocks of K take or, behind the first one, what its sums take on their way out if that is longer; fitted to 90 shapes.  us by tiles 256 wide | 128 | 64,
+  // of codes: 256 tokens of 1024 x 1024 7.4 | 5.5 | 4.9, of 7168 x 7168 21 | 15 | 24; 1000 tokens of it 40 | 46 | 76; 1150 of 23176 x 416 24 | 28 | 37; 4096 of 28672 x 7168 622 | 765 | 1265.
+  auto ns = [&](long long n, long long once, int block, int sums) {
     const long long products = (long long)p.k_blocks * block;
-    return once + products + (rounds(n, workers) - 1) * (products > sums ? products : sums);
+    return once + products + ((n + sms - 1) / sms - 1) * (products > sums ? products : sums);
   };
-  offer(256, true, ns(tiles(2 * TILE, 256), sms / 2, 5900, 374, 3900));
-  offer(256, false, ns(tiles(TILE, 256), sms, 6000, 533, 3300));
-  offer(128, false, ns(tiles(TILE, 128), sms, 5000, 342, 2150));
-  offer(64, false, ns(tiles(TILE, 64), sms, 4550, 253, 1600));
-  const int rows = p.pair ? 2 * TILE : TILE;
-  p.tiles_a = (M + rows - 1) / rows;
+  offer(256, ns(tiles(256), 6000, 533, 3300));
+  offer(128, ns(tiles(128), 5000, 342, 2150));
+  offer(64, ns(tiles(64), 4550, 253, 1600));
+  p.tiles_a = (M + TILE - 1) / TILE;
   p.tiles_b = (N + p.bn - 1) / p.bn;
   const long long units = (long long)p.tiles_a * p.tiles_b;
-  p.grid = p.pair ? 2 * (int)(units < sms / 2 ? units : sms / 2) : (int)(units < sms ? units : sms);
+  p.grid = (int)(units < sms ? units : sms);
   return p;
 }
 // of a workspace: codes and scales of the tokens, unless they are given
@@ -747,10 +703,10 @@ Rooms rooms_of(int M, int K, bool given) {
   return r;
 }
 
-template <bool FEW, int BN, bool PAIR, bool OUT32> int launch(const Plan& pl, const CUtensorMap& tmA, const CUtensorMap& tmB, const Args& a, bool early, cudaStream_t stream) {
-  using L = Shape<FEW, BN, PAIR>;
+template <bool FEW, int BN, bool OUT32> int launch(const Plan& pl, const CUtensorMap& tmA, const CUtensorMap& tmB, const Args& a, bool early, cudaStream_t stream) {
+  using L = Shape<FEW, BN>;
   static_assert(L::SMEM <= (FEW ? 115712 : 232448) && L::STAGES >= 3 && (!FEW || L::STAGES * L::STAGE >= BN * TILE * 4), "shared memory");
-  auto kernel = int8_gemm_kernel<FEW, BN, PAIR, OUT32>;
+  auto kernel = int8_gemm_kernel<FEW, BN, OUT32>;
   static bool configured[64] = {};                                 // per device
   int dev = 0;
   LIA_CUDA(cudaGetDevice(&dev));
@@ -758,24 +714,23 @@ template <bool FEW, int BN, bool PAIR, bool OUT32> int launch(const Plan& pl, co
     LIA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
     if (dev < 64) configured[dev] = true;
   }
-  if (PAIR || pl.parts > 1) LIA_CUDA(lia_launch_cluster_as(early || PAIR, PAIR ? 2 : pl.parts, kernel, dim3(pl.grid), dim3(L::THREADS), L::SMEM, stream, tmA, tmB, a));
+  if (pl.parts > 1) LIA_CUDA(lia_launch_cluster_as(early, pl.parts, kernel, dim3(pl.grid), dim3(L::THREADS), L::SMEM, stream, tmA, tmB, a));
   else LIA_CUDA(lia_launch_as(early, kernel, dim3(pl.grid), dim3(L::THREADS), L::SMEM, stream, tmA, tmB, a));
   return LIA_OK;
 }
 template <bool OUT32> int launch_plan(const Plan& pl, const CUtensorMap& tmA, const CUtensorMap& tmB, const Args& a, bool early, cudaStream_t stream) {
   if (pl.few) {
     switch (pl.bn) {
-      case 16: return launch<true, 16, false, OUT32>(pl, tmA, tmB, a, early, stream);
-      case 32: return launch<true, 32, false, OUT32>(pl, tmA, tmB, a, early, stream);
-      case 64: return launch<true, 64, false, OUT32>(pl, tmA, tmB, a, early, stream);
-      default: return launch<true, 128, false, OUT32>(pl, tmA, tmB, a, early, stream);
+      case 16: return launch<true, 16, OUT32>(pl, tmA, tmB, a, early, stream);
+      case 32: return launch<true, 32, OUT32>(pl, tmA, tmB, a, early, stream);
+      case 64: return launch<true, 64, OUT32>(pl, tmA, tmB, a, early, stream);
+      default: return launch<true, 128, OUT32>(pl, tmA, tmB, a, early, stream);
     }
   }
-  if (pl.pair) return launch<false, 256, true, OUT32>(pl, tmA, tmB, a, early, stream);
   switch (pl.bn) {
-    case 256: return launch<false, 256, false, OUT32>(pl, tmA, tmB, a, early, stream);
-    case 128: return launch<false, 128, false, OUT32>(pl, tmA, tmB, a, early, stream);
-    default: return launch<false, 64, false, OUT32>(pl, tmA, tmB, a, early, stream);
+    case 256: return launch<false, 256, OUT32>(pl, tmA, tmB, a, early, stream);
+    case 128: return launch<false, 128, OUT32>(pl, tmA, tmB, a, early, stream);
+    default: return launch<false, 64, OUT32>(pl, tmA, tmB, a, early, stream);
   }
 }
 
@@ -851,7 +806,7 @@ extern "C" int lia_linear_int8(const void* x, int x_type, long long ldx, const f
   const long long ldc = given ? ldx : r.ldc;
   CUtensorMap tmX, tmW;
   int rc = make_tmap(&tmX, codes, M, K, ldc, pl.few ? pl.bn : TILE);
-  if (rc == LIA_OK) rc = make_tmap(&tmW, w, N, K, ldw, pl.few ? TILE : pl.pair ? pl.bn / 2 : pl.bn);
+  if (rc == LIA_OK) rc = make_tmap(&tmW, w, N, K, ldw, pl.few ? TILE : pl.bn);
   if (rc != LIA_OK) return rc;
   Args a{given ? x_scale : reinterpret_cast<float*>(base + r.scales), w_scale, out, lia_timeout_word(), M, N, pl.k_blocks,
          pl.tiles_a, pl.tiles_b, reinterpret_cast<uintptr_t>(out) % 16 == 0 && (long long)N * (out_f32 ? 4 : 2) % 16 == 0, pl.parts};
