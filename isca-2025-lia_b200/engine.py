@@ -14,7 +14,7 @@ a few microseconds each -- so it is captured as a CUDA graph the second time its
 on: the ids, portions and positions live in one static device buffer that the pinned copy refreshes before every replay;
 the kernels read slots and positions from it, so one graph serves every step of that shape.  "Shape" is the number of
 rows, whether logits are wanted, and the model's ``graph_class(longest history)`` or, where it has one, ``graph_plan(rows, longest history)``: whatever else its launches depend on
-(how many key ranges the attention splits a history into: ``ops.latent_attn_splits``, ``ops.window_attn_split_class``, and over 8-bit caches ``ops.tree_attn_plan``).  The graph replays
+(how many key ranges the attention splits a history into: ``ops.latent_attn_splits``, ``ops.window_attn_split_class``, and over 8- and 4-bit caches ``ops.tree_attn_plan``).  The graph replays
 the very kernels of the eager pass; results are bit-identical.
 
 The reference serves one static batch per generate() call (greedy_search.py:37-460); this is the request-level face the

@@ -289,7 +289,7 @@ class BebulornForCausalLM:
         return tuple(sorted({ops.window_attn_split_class(max_ctx, l.mixer.window) for l in self.layers if isinstance(l.mixer, WindowAttentionMixer)}))
 
     def graph_plan(self, requests, max_ctx):
-        """The same for a pass of ``requests`` single tokens, over whichever caches there are: with 8-bit ones how many blocks share a history goes by the number of requests too."""
+        """The same for a pass of ``requests`` single tokens, over whichever caches there are: with 8- or 4-bit ones how many blocks share a history goes by the number of requests too."""
         if self.cache_dtype is None:
             return self.graph_class(max_ctx)
         plans = {}

@@ -427,7 +427,7 @@ class WindowAttentionMixer:
         if cache_dtype is not None and (cache_dtype not in (torch.int8, torch.float8_e4m3fn, torch.int4) or dtype != BF16 or dim not in (64, 128) or vdim not in (64, 128)):
             raise ValueError(f"caches of 8 bits are int8 or float8_e4m3fn (of 4 int4), for bf16 layers with heads of 64 or 128 channels, not {cache_dtype} for {dtype} with heads of {dim} and {vdim}")
         if cache_dtype is not None and softcap > 1024:
-            raise ValueError(f"caches of 8 bits: scores are capped at 1024 at most, not {softcap}")
+            raise ValueError(f"caches of 8 and 4 bits: scores are capped at 1024 at most, not {softcap}")
         self.cache_dtype = cache_dtype
         if heads % kv_heads:
             raise ValueError(f"{heads} heads do not divide into {kv_heads} key/value heads")
@@ -439,7 +439,7 @@ class WindowAttentionMixer:
         self.out = Linear([w["o"]], dtype, device)
 
     def step_plans(self, requests, max_ctx, seen):
-        """What a decode step of ``requests`` tokens launches over an 8-bit cache by, into ``seen`` by what layers share."""
+        """What a decode step of ``requests`` tokens launches over an 8- or 4-bit cache by, into ``seen`` by what layers share."""
         shape = (self.H, self.G, self.window)
         if shape not in seen:
             seen[shape] = tree_attn_plan(requests, 1, max_ctx, *shape, self.cache_dtype)
