@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(Shape<FEW, BN>::THREADS, FEW ? 2 : 1) int8_gem
         while (early < STAGES && s.next(w))
           for (int kb = w.kb0; kb < w.kb1 && early < STAGES; ++kb, ++early) {
             mbar_expect_tx(full(early), L::STAGE);
-            tma_load_2d(smem + early * L::STAGE, &tmA, kb * KB, w.ta * TILE, full(early));
+            tma_load_block(smem + early * L::STAGE, &tmA, kb, w.ta * TILE, full(early));
           }
       }
       pdl_wait();
@@ -407,12 +407,12 @@ __global__ void __launch_bounds__(Shape<FEW, BN>::THREADS, FEW ? 2 : 1) int8_gem
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           const uint32_t sa = smem + stage * L::STAGE, sb = sa + L::A_BYTES;
           if (FEW && issued < early) {
-            tma_load_2d(sb, &tmB, kb * KB, 0, full(stage));
+            tma_load_block(sb, &tmB, kb, 0, full(stage));
           } else {
             if (!(alive = wait_for(empty(stage), phase ^ 1u, dead))) break;
             mbar_expect_tx(full(stage), L::STAGE);
-            tma_load_2d(sa, &tmA, kb * KB, w.ta * TILE, full(stage));
-            tma_load_2d(sb, &tmB, kb * KB, w.tb * BN, full(stage));
+            tma_load_block(sa, &tmA, kb, w.ta * TILE, full(stage));
+            tma_load_block(sb, &tmB, kb, w.tb * BN, full(stage));
           }
           ++issued;
           if (++stage == STAGES) {
@@ -659,7 +659,6 @@ Plan plan_of(int M, int N, int K) {
     p.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     p.tiles_a = (N + TILE - 1) / TILE;
     p.tiles_b = 1;
-    const long long total = (long long)p.tiles_a * p.k_blocks;
     // Sharing a tile costs a cluster's meeting, 1 to 2 us, and pays as long as the CTAs fit two an SM; eight of them only where the tiles are few and long.  us with 1 | 2 | 4 | 8 parts, 64 tokens:
     // 1024 x 1024 9.0 | 8.2 | 7.4 | 7.2; 2560 x 2560 12.1 | 10.2 | 8.8 | 9.6; 1024 x 8192 22.5 | 15.6 | 11.5 | 10.7; 7168 x 7168 24.2 | 19.1 | 17.0 | 23.6; 12288 x 4096 19.3 | 18.0 | 21.4;
     // 28672 x 7168 41.4 | 46.5.  (As spans of equal length over one CTA an SM, whose shared tiles met by way of global memory, 2560 x 2560 took 18, 28672 x 7168 49.)

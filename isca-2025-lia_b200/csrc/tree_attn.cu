@@ -358,7 +358,36 @@ __global__ void __launch_bounds__(THREADS, blocks_an_sm(KIND, NR)) tree_attn_ker
       for (int n = 0; n < S::MT; ++n) *reinterpret_cast<float2*>(os + at * VDIM + S::channel(n, gq)) = make_float2(o[r][n][e], o[r][n][2 + e]);
     }
   __syncthreads();
-  meet<DIM, VDIM, KIND, S::ROWS>(a, p, r0, R, g, os, part);
+  constexpr int N = VDIM / 32, ROWS = S::ROWS;
+  const long long rows = (long long)a.M * a.H;
+  for (int r = warp; r < ROWS && r0 + r < R; r += WARPS) {
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    float top = NONE, sum = 0.f, y[N] = {};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w * ROWS + r].x);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 x = part[w * ROWS + r];
+      const float f = ex2(x.x - top);
+      sum = fmaf(x.y, f, sum);
+#pragma unroll
+      for (int c = 0; c < N; ++c) y[c] = fmaf(os[(w * ROWS + r) * VDIM + lane * N + c], f, y[c]);
+    }
+    if (a.splits == 1) {
+      put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
+    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read: with all lanes, before one of them writes)
+#pragma unroll
+      for (int c = 0; c < N; ++c) os[r * VDIM + lane * N + c] = y[c];
+      __syncwarp();
+      if (lane == 0) part[r] = make_float2(top, sum);
+    } else {
+      const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;
+#pragma unroll
+      for (int c = 0; c < N; ++c) a.ws[at * VDIM + lane * N + c] = y[c];
+      if (lane == 0) reinterpret_cast<float2*>(a.ws + a.splits * rows * VDIM)[at] = make_float2(top, sum);
+    }
+  }
+  meet_cluster<DIM, VDIM, KIND, ROWS>(a, p, r0, R, g, os, part);
 }
 
 // How a call is cut: rows of a block, blocks of a portion's rows, blocks that share a history

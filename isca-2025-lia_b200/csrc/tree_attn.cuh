@@ -250,40 +250,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {       // of 8 x 8 n
   return y;
 }
 
-// A block's parts, in shared memory as [WARPS][ROWS], to outputs: os the weighted values [..][VDIM], part maximum and sum of weights
-template <int DIM, int VDIM, int KIND, int ROWS> __device__ __forceinline__ void meet(const TreeArgs& a, const Portion& p, int r0, int R, int g, float* os, float2* part) {
+// The blocks that share a history are a cluster: each joins some of the rows, always in the same order
+template <int DIM, int VDIM, int KIND, int ROWS> __device__ __forceinline__ void meet_cluster(const TreeArgs& a, const Portion& p, int r0, int R, int g, float* os, float2* part) {
+  if (a.splits == 1 || a.splits > CLUSTER) return;
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int N = VDIM / 32;
-  const long long rows = (long long)a.M * a.H;
-  for (int r = warp; r < ROWS && r0 + r < R; r += WARPS) {
-    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
-    float top = NONE, sum = 0.f, y[N] = {};
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w * ROWS + r].x);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float2 x = part[w * ROWS + r];
-      const float f = ex2(x.x - top);
-      sum = fmaf(x.y, f, sum);
-#pragma unroll
-      for (int c = 0; c < N; ++c) y[c] = fmaf(os[(w * ROWS + r) * VDIM + lane * N + c], f, y[c]);
-    }
-    if (a.splits == 1) {
-      put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
-    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read: with all lanes, before one of them writes)
-#pragma unroll
-      for (int c = 0; c < N; ++c) os[r * VDIM + lane * N + c] = y[c];
-      __syncwarp();
-      if (lane == 0) part[r] = make_float2(top, sum);
-    } else {
-      const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;
-#pragma unroll
-      for (int c = 0; c < N; ++c) a.ws[at * VDIM + lane * N + c] = y[c];
-      if (lane == 0) reinterpret_cast<float2*>(a.ws + a.splits * rows * VDIM)[at] = make_float2(top, sum);
-    }
-  }
-  if (a.splits == 1 || a.splits > CLUSTER) return;
-  // ---- the blocks that share a history are a cluster: each joins some of the rows, always in the same order
   cluster_barrier();
   for (int r = warp * a.splits + blockIdx.x; r < ROWS && r0 + r < R; r += WARPS * a.splits) {
     const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;

@@ -533,7 +533,40 @@ __global__ void __launch_bounds__(THREADS, tree_attn4_blocks(NR)) tree_attn4_ker
   const int lo = first_key(a, p, near), hi = end_key(a, p, i1), all_lo = first_key(a, p, far), all_hi = min(hi, a.mask != nullptr ? p.p0 : p.p0 + i0 + 1);
   const int nb = (hi - lo + 15) >> 4, b0 = (int)((long long)nb * blockIdx.x / a.splits), b1 = (int)((long long)nb * (blockIdx.x + 1) / a.splits);
   run_piece<DIM, VDIM, NR, PACKED>(a, p, Piece{g, r0, lo, hi, all_lo, all_hi, b0, b1}, sh);
-  meet<DIM, VDIM, LIA_CACHE_INT4, S::ROWS>(a, p, r0, R, g, sh.os, sh.part);
+  // ---- the warps' parts of a row to its output, to shared memory for the cluster, or to the workspace
+  constexpr int N = VDIM / 32, ROWS = S::ROWS, KIND = LIA_CACHE_INT4;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
+  float* os = sh.os;
+  float2* part = sh.part;
+  const long long rows = (long long)a.M * a.H;
+  for (int r = warp; r < ROWS && r0 + r < R; r += WARPS) {
+    const int i = (r0 + r) / a.rep, h = g * a.rep + (r0 + r) - i * a.rep;
+    float top = NONE, sum = 0.f, y[N] = {};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w * ROWS + r].x);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 x = part[w * ROWS + r];
+      const float f = ex2(x.x - top);
+      sum = fmaf(x.y, f, sum);
+#pragma unroll
+      for (int c = 0; c < N; ++c) y[c] = fmaf(os[(w * ROWS + r) * VDIM + lane * N + c], f, y[c]);
+    }
+    if (a.splits == 1) {
+      put_row<DIM, VDIM, KIND>(a, p, i, h, y, sum);
+    } else if (a.splits <= CLUSTER) {                              // (in the place of the first warp's part, which this warp alone has read: with all lanes, before one of them writes)
+#pragma unroll
+      for (int c = 0; c < N; ++c) os[r * VDIM + lane * N + c] = y[c];
+      __syncwarp();
+      if (lane == 0) part[r] = make_float2(top, sum);
+    } else {
+      const long long at = blockIdx.x * rows + (long long)(p.row + i) * a.H + h;
+#pragma unroll
+      for (int c = 0; c < N; ++c) a.ws[at * VDIM + lane * N + c] = y[c];
+      if (lane == 0) reinterpret_cast<float2*>(a.ws + a.splits * rows * VDIM)[at] = make_float2(top, sum);
+    }
+  }
+  meet_cluster<DIM, VDIM, KIND, ROWS>(a, p, r0, R, g, os, part);
 }
 
 // ---- All histories as one list of units of 64 keys (16 for each warp), of which every block of a key head has the same number, whatever the histories' lengths: its span may end one history and begin

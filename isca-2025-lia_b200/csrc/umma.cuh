@@ -81,6 +81,8 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
+// the same of rows of bytes: their bytes 128 block .. 128 block + 127, from row `row` on
+__device__ __forceinline__ void tma_load_block(uint32_t dst, const CUtensorMap* map, int block, int row, uint32_t bar) { tma_load_2d(dst, map, block * 128, row, bar); }
 // ---- CTA-pair (cta_group::2) variants: the two CTAs of a cluster drive ONE 256-row MMA
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

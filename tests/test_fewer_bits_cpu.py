@@ -213,3 +213,14 @@ def test_choices_are_put_together(lib, monkeypatch):
     from lia_b200.seq_state import SlotError
     with pytest.raises(SlotError):
         Engine(Model(), 16, max_requests=1).score_choices([8, 1], choices)
+
+
+def test_costs_of_the_operators():
+    """What the comparison benchmark counts for them: bytes of codes and scales, half the operations of a product in 8 bits (which run at twice the rate)."""
+    from lia_b200 import bench_compare
+    e = lambda *s, dt=BF16: torch.empty(*s, dtype=dt)  # noqa: E731
+    cost = bench_compare._cost
+    assert cost("kv_store_4bit", (e(10, 256), e(10, 128)), {}) == (0.0, 10 * 384 * 2.5625, "mem") and cost("quantize_rows", (e(3, 64, dt=F32),), {}) == (0.0, 3 * (64 * 5 + 4), "mem")
+    assert cost("linear_int8", (e(5, 64), e(7, 64, dt=torch.int8)), {"out": e(5, 7, dt=F32)}) == (5 * 7 * 64, 7 * 64 + 28 + 5 * 64 * 2 + 5 * 7 * 4, "tc")
+    q, cache = e(4, 8 * 64), e(2, 100, 2 * 32, dt=U8)
+    assert cost("tree_attn", (q, cache, cache, None, q, 8, 2, 64, 64), {"_wkeys": 50, "_wctx": 50}) == (2 * 50 * 8 * 128, 2 * 4 * 512 * 2 + 50 * 2 * 72, "tc")
