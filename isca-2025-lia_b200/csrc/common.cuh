@@ -164,8 +164,10 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// clusters: a barrier of all their blocks, and the place in block `rank` that is a block's own at `addr`
+// clusters: a barrier of all their blocks, and the place in block `rank` that is a block's own at `addr`.  Its instructions are a warp's as a whole (.aligned), and what comes before may have been a loop that
+// lanes leave one after the other, so the warp meets first.
 __device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -607,6 +607,7 @@ __global__ void __launch_bounds__(Shape<FEW, BN>::THREADS, FEW ? 2 : 1) int8_gem
         if (n < p.N) put_one<OUT32>(p.out, (size_t)m * p.N + n, bad ? NAN : (float)sum * sx_s[m] * __ldg(p.sw + n));
       }
     }
+    __syncwarp();                                                  // (lanes leave these loops after different rounds, and TMEM is given back by a whole warp)
   }
   if (*dead) {                                                     // loads and products in flight end before shared memory and TMEM are given back
     if (threadIdx.x == 0) {
