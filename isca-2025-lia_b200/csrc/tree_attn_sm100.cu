@@ -20,7 +20,7 @@
 // memory (700 clocks for 64 keys of 8 bits, 1400 of bf16).  A call behind a single position takes 16 us with 256 rows a block, 10 with up to 128: programs are loaded, and what depends on the portion, one
 // behind the other.  A tree of 64 tokens behind 131003 positions, 32 heads on 8: int8 212 us, bf16 205; its products would take 83 at the tensor cores' rate, its bytes 42 and 82.
 // Keys' scales are held 16 at a time (32: 240 us, for registers).
-// 4 bits: a loading lane has eight channels of each of a key's groups, which it brings to fp16 relative to the key's largest scale; what bounds it stays: portions of 1003 and 701 tokens behind 512 and 360, 16
+// 4 bits: a loading lane has eight channels of each of a key's groups, which it brings to fp16 relative to the power of two of the key's largest scale, exactly; what bounds it stays: portions of 1003 and 701 tokens behind 512 and 360, 16
 // heads on 8, bf16 39.9 us, int8 40.5, 4 bits 41.6.
 // The issuing warp's block numbers are made uniform by a shuffle: without, each product took twice its instructions.
 #include "pairs.cuh"
@@ -39,6 +39,7 @@ constexpr int LAUNCH_REGS = 96;
 static_assert(SOFTMAX_REGS >= LAUNCH_REGS && LOADER_REGS <= LAUNCH_REGS && OTHER_REGS <= LAUNCH_REGS && 2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS <= TC_THREADS / 128 * LAUNCH_REGS, "shares");
 constexpr uint32_t VALUES = 256;
 constexpr float LEAST_KEY_SCALE = 0x1p-110f;                       // a 4-bit key's largest scale counts as that at least, so that its inverse is finite
+constexpr uint32_t KEY_UP = 11;                                    // 4-bit keys are brought to fp16 with the power of two of their largest scale as 2^11: codes of -8 to 7 stay below 2^15
 
 template <int DIM, int VDIM, int KIND, bool PAIR>
 struct Tc {
@@ -637,7 +638,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attn_tc_kernel(const __gri
 #pragma unroll
           for (int i = 1; i < C::VG; ++i) vm = max_nan(vm, vg[i]);
           km = max_nan(km, LEAST_KEY_SCALE);
-          const float f = vm * ref_inv, y = max_nan(vm, LEAST_SCALE), k_by = __fdividef(1.f, km);
+          const float f = vm * ref_inv, y = max_nan(vm, LEAST_SCALE);
+          // by powers of two: a scale of 8 bits times a code of 3 (or the sign and none) is 11 bits, which fp16 holds as they are down to 2^-28 of a key's largest scale
+          const uint32_t ke = __float_as_uint(km) & 0x7f800000u;   // (255 where it is not finite, which its groups' numbers stay)
+          const float k_by = __uint_as_float(((254u + KEY_UP) << 23) - ke);
           const bool near = (f >= 0x1p-8f && f < 64.f) || !there4[x];
           const float v_by = near ? ref_inv : __fdividef(1.f, y);
           const uint32_t kw[4] = {kr[x][0].x, kr[x][0].y, kr[x][0].z, kr[x][0].w}, vw[4] = {vr[x][0].x, vr[x][0].y, vr[x][0].z, vr[x][0].w};
@@ -657,7 +661,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attn_tc_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < C::VG; ++i) widen4(at + C::K_BYTES, vw, std::integral_constant<int, C::VG>{}, vg, v_by, i);
           if (kt == 0) {
-            sm.ks[st][k0] = km;
+            sm.ks[st][k0] = __uint_as_float(ke - (KEY_UP << 23));
             const float z = near ? pow2(ref) : y;
             sm.lv[st][k0] = lg2(z);
             sm.rv[st][k0] = __fdividef(1.f, z);
