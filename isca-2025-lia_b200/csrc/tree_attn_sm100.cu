@@ -20,8 +20,8 @@
 // memory (700 clocks for 64 keys of 8 bits, 1400 of bf16).  A call behind a single position takes 16 us with 256 rows a block, 10 with up to 128: programs are loaded, and what depends on the portion, one
 // behind the other.  A tree of 64 tokens behind 131003 positions, 32 heads on 8: int8 212 us, bf16 205; its products would take 83 at the tensor cores' rate, its bytes 42 and 82.
 // Keys' scales are held 16 at a time (32: 240 us, for registers).
-// 4 bits: a loading lane has eight channels of each of a key's groups, which it brings to fp16 relative to the power of two of the key's largest scale, exactly; what bounds it stays: portions of 1003 and 701 tokens behind 512 and 360, 16
-// heads on 8, bf16 39.9 us, int8 40.5, 4 bits 41.6.
+// 4 bits: a loading lane has eight channels of each of a key's and a value's groups, which it brings to fp16 relative to powers of two, exactly; what bounds it stays: portions of 1003 and 701 tokens behind
+// 512 and 360, 16 heads on 8, bf16 39.9 us, int8 40.5, 4 bits 41.6.
 // The issuing warp's block numbers are made uniform by a shuffle: without, each product took twice its instructions.
 #include "pairs.cuh"
 #include "tree_attn.cuh"
@@ -39,6 +39,7 @@ constexpr int LAUNCH_REGS = 96;
 static_assert(SOFTMAX_REGS >= LAUNCH_REGS && LOADER_REGS <= LAUNCH_REGS && OTHER_REGS <= LAUNCH_REGS && 2 * SOFTMAX_REGS + 2 * LOADER_REGS + OTHER_REGS <= TC_THREADS / 128 * LAUNCH_REGS, "shares");
 constexpr uint32_t VALUES = 256;
 constexpr float LEAST_KEY_SCALE = 0x1p-110f;                       // a 4-bit key's largest scale counts as that at least, so that its inverse is finite
+constexpr uint32_t VALUE_UP = 6;                                   // as 4-bit values are with REF's power of two as 2^6, so that scales 64 times REF fit too
 constexpr uint32_t KEY_UP = 11;                                    // 4-bit keys are brought to fp16 with the power of two of their largest scale as 2^11: codes of -8 to 7 stay below 2^15
 
 template <int DIM, int VDIM, int KIND, bool PAIR>
@@ -52,6 +53,7 @@ struct Tc {
   static constexpr int KN = KEYS * KT / LOADERS, VN = KEYS * VT / LOADERS;                       // vectors of a lane
   static constexpr int KG = FOUR ? DIM / GROUP4 : 2, VG = FOUR ? VDIM / GROUP4 : 2;             // scales of a position with 4 bits (else: not used)
   static constexpr int AHEAD = SCALED ? 2 : 1;                      // blocks of 16 or 32 KB on their way from memory (more: more instructions to bring, 5 to 30 % slower with four)
+  static constexpr int UP = FOUR ? VALUE_UP : 0;                   // values are in fp16 as number / 2^(REF - UP)
   static constexpr float LIFT = SCALED ? 7.f : 0.f;                 // weights are 2^(x - maximum + LIFT): below 2^15 in fp16
 };
 struct Tail {
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attn_tc_kernel(const __gri
     float m = -1e30f, l = 0.f;
     bool alive = true;
     int done = 0;                                                  // of the group's blocks
-    const int ref = SCALED ? ref_of(scales) : 0;
+    const int ref = SCALED ? ref_of(scales) - C::UP : 0;
     const float ref_l = (float)ref, ref_inv = pow2(-ref);
     // (a row's first block sees to a maximum; -1e30 stands for none, so that nothing is less than it but -inf)
 #pragma unroll 1
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attn_tc_kernel(const __gri
     for (int x = 0; x < C::AHEAD; ++x) ask(x, x);
     if constexpr (FOUR) ask_ref4<C::VG>(a.v.scale4_at(p.slot, g) + (long long)start * C::VG, n > 0 ? min(hi - start, KEYS) : 0, scales);
     else if constexpr (SCALED) ask_ref(a.v.scale_at(p.slot, g) + start, n > 0 ? min(hi - start, KEYS) : 0, scales);
-    const int ref = SCALED ? ref_of(scales) : 0;
+    const int ref = SCALED ? ref_of(scales) - C::UP : 0;
     const float ref_inv = pow2(-ref);
     bool alive = true;
 #pragma unroll 1
@@ -642,8 +644,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attn_tc_kernel(const __gri
           // by powers of two: a scale of 8 bits times a code of 3 (or the sign and none) is 11 bits, which fp16 holds as they are down to 2^-28 of a key's largest scale
           const uint32_t ke = __float_as_uint(km) & 0x7f800000u;   // (255 where it is not finite, which its groups' numbers stay)
           const float k_by = __uint_as_float(((254u + KEY_UP) << 23) - ke);
-          const bool near = (f >= 0x1p-8f && f < 64.f) || !there4[x];
-          const float v_by = near ? ref_inv : __fdividef(1.f, y);
+          // Values likewise, relative to REF 2^-VALUE_UP where that leaves all groups' scales their bits -- the smallest one's factor is 2^-17 or more; what counts as nothing (LEAST_SCALE) is not asked for --
+          // and relative to the power of two of the position's largest scale where it does not: there down to 2^-23 of that
+          float least = __uint_as_float(0x7f800000u);
+#pragma unroll
+          for (int i = 0; i < C::VG; ++i) least = fminf(least, vg[i] < LEAST_SCALE ? least : vg[i]);
+          const uint32_t ve = __float_as_uint(y) & 0x7f800000u;
+          const bool near = (f >= 0x1p-2f && f < 0x1p12f && least * ref_inv >= 0x1p-17f) || !there4[x];
+          const float v_by = near ? ref_inv : __uint_as_float(((254u + VALUE_UP) << 23) - ve);
           const uint32_t kw[4] = {kr[x][0].x, kr[x][0].y, kr[x][0].z, kr[x][0].w}, vw[4] = {vr[x][0].x, vr[x][0].y, vr[x][0].z, vr[x][0].w};
           auto widen4 = [&](uint32_t to, const uint32_t (&w)[4], auto ng, const float* s, float by, int i) {
             constexpr int NG = decltype(ng)::value;
@@ -662,9 +670,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attn_tc_kernel(const __gri
           for (int i = 0; i < C::VG; ++i) widen4(at + C::K_BYTES, vw, std::integral_constant<int, C::VG>{}, vg, v_by, i);
           if (kt == 0) {
             sm.ks[st][k0] = __uint_as_float(ke - (KEY_UP << 23));
-            const float z = near ? pow2(ref) : y;
-            sm.lv[st][k0] = lg2(z);
-            sm.rv[st][k0] = __fdividef(1.f, z);
+            sm.lv[st][k0] = near ? (float)ref : (float)((int)(ve >> 23) - 127 - (int)VALUE_UP);
+            sm.rv[st][k0] = v_by;                                  // (powers of two)
           }
           const bool odd = __any_sync(0xffffffffu, !near);
           if (lane == 0) reinterpret_cast<uint8_t*>(&sm.odd[st])[warp - 8] = odd;

@@ -6,7 +6,11 @@ tests/test_gpu_tree_attn.py is then, with more than 32 rows too: the output's ow
 
 Weights that are small beside a row's largest: that one is 2^7 to 2^15 in fp16, whose numbers below 2^-14 are 2^-24 apart, so that such a weight is off by 2^-25, which is 2^-32 of the largest at most.  A
 channel of which the largest weights' keys have a code of 0 is made of these: 2^-32 of the row's largest p for every key, times that key's value.  (Scales are within a factor of 64, so that the values' part of
-the weights is one power of two for all.)"""
+the weights is one power of two for all.  Where a test has them further apart, a position's part z of the weights is a power of two within a factor of 2 of its largest scale y: then it is 2^-32 of the row's
+largest p z, over z, for every key: 4 times that with y.)
+
+Groups below 2^-23 of their position's largest scale y: that one's power of two is 2^6 in fp16, so that such a group's scale is below 2^-16 there and is off by up to half of 2^-24 for its factor, times a code
+of 8, and as much for the product: 9 * 2^-25, which is 9 * 2^-31 of y for each of the position's channels in that group."""
 import pytest
 import torch
 
@@ -26,6 +30,8 @@ def ops():
 
 
 class Exact(Case4):
+    apart = False                                                           # values' scales further apart than a factor of 64, each position's weights with its own part
+
     def check(self, out):
         for z, (s, p0, r, n) in enumerate(self.segs):
             see = self.visible(z)
@@ -40,7 +46,11 @@ class Exact(Case4):
                 p = torch.softmax(x.masked_fill(~see, -INF), -1)
                 o, A = p @ v, p @ v.abs()
                 d = self.dim * 2.0 ** -24 * B + 2.0 ** -21 * (S + self.softcap) + 2.0 ** -20
-                tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2 * d + (p0 + n + 32) * 2.0 ** -24) * A + 2.0 ** -32 * p.amax(1, keepdim=True) * (see.double() @ v.abs()) + 1e-30
+                y = 2 * self.vs[s, g, :p0 + n].double().amax(-1) if self.apart else torch.ones(p0 + n, dtype=torch.float64, device="cuda")
+                small = 2.0 ** -32 * (p * y).amax(1, keepdim=True) * (see.double() @ (v.abs() * (4 / y if self.apart else y)[:, None]))
+                groups, most = self.vs[s, g, :p0 + n].double(), self.vs[s, g, :p0 + n].double().amax(-1, keepdim=True)
+                far = p @ torch.where(groups < 2.0 ** -23 * most, 9 * 2.0 ** -31 * most, 0.0).repeat_interleave(32, -1)
+                tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2 * d + (p0 + n + 32) * 2.0 ** -24) * A + small + far + 1e-30
                 off = ((out[r:r + n, h * self.vdim:(h + 1) * self.vdim].double() - o).abs() / tol)
                 assert not torch.isnan(off).any() and off.max() <= 1, (z, h, off.max().item(), off.argmax().item())
 
@@ -91,4 +101,29 @@ def test_codes_of_minus_eight(ops, n):
     c.ks.copy_((c.ks.float() * 0 + 1.9921875).to(BF16))
     c.vs.copy_((c.vs.float() * 0 + 1.9921875).to(BF16))
     c.q *= 0.1
+    c.check(c.run(ops))
+
+
+@pytest.mark.parametrize("n,H,G,softcap", [(40, 4, 2, 0.0), (130, 4, 2, 0.0), (40, 2, 2, 30.0)])
+@pytest.mark.parametrize("up", [5, 12])
+@pytest.mark.parametrize("down", [9, 14, 17, 20])
+def test_small_groups_of_values(ops, n, H, G, softcap, up, down):
+    """A large value among the first 64 positions, whose scale the others' go by as long as they are near it, and a group of channels far below the others: its channels are as exact as theirs."""
+    c = Exact([(0, 300, n), (1, 64, n)], H, G, 128, 128, softcap=softcap)
+    c.apart = up > 6
+    c.vs[:, :, 5, 0] *= 2.0 ** up
+    c.vs[:, :, 5, 2:] *= 2.0 ** up
+    c.vs[:, :, :, 1] *= 2.0 ** -down
+    c.check(c.run(ops))
+
+
+@pytest.mark.parametrize("n", [40, 130])
+def test_groups_of_nothing_beside_others(ops, n):
+    """Groups of zeros have scales near 2^-103 or of 0: the position's other channels, and its rows' sums, are what they are."""
+    c = Exact([(0, 300, n)], 4, 2, 128, 64)
+    c.vs[:, :, ::3, 0] = 2.0 ** -103
+    c.vs[:, :, 1::3, 1] = 0
+    c.vs[:, :, 2::9] = 0
+    c.ks[:, :, ::4, 3] = 2.0 ** -103
+    c.ks[:, :, 1::4, 2] = 0
     c.check(c.run(ops))
