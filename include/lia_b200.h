@@ -674,7 +674,9 @@ int lia_kv_load_8bit(const int* meta, const LiaCacheView* kc, const LiaCacheView
                      lia_stream_t stream);
 
 /* The same with caches of 4 bits, every 32 channels of a head with a scale of their own: scale = a / 7 rounded to fp32 and then to bf16, with a the largest magnitude of the 32 numbers (counted as 2^-100
- * at least); code = rint(x / scale), -7 to 7, of the exact quotient.  A group with an infinity or NaN gets scale NaN and codes 0; the head's other groups do not depend on it.  Heads of up to 1024 channels. */
+ * at least); code = rint(x / scale), -7 to 7, of the exact quotient.  A group with an infinity or NaN gets scale NaN and codes 0; the head's other groups do not depend on it, unless values are normed: then a
+ * NaN leaves its whole head NaN, and an infinity the other groups zeros.  A normed value is the head's number times 1 / root, in fp32, and its code that of fp32 products: the neighbouring one where the quotient is
+ * within some 2^-22 of itself from a border.  Heads of up to 1024 channels. */
 int lia_kv_store_4bit(const void* k, long long ldk, const void* v, long long ldv, int act_f32, const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, int M, int G,
                       float eps, int norm_values, lia_stream_t stream);
 int lia_kv_load_4bit(const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, void* k, long long ldk, void* v, long long ldv, int out_f32, int M, int G,
