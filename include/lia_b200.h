@@ -666,7 +666,8 @@ typedef struct LiaCacheView {
  * the caches do not have is left out.  int8: scale = a / 127, code = rint(127 x / a) with a the largest magnitude of the head's numbers (counted as 2^-100 at least);
  * e4m3: scale = the least power of two with a / scale <= 448, code = x / scale rounded to nearest even
  * (what would read back as 2^128: to the code below).  A head with an infinity or NaN gets scale NaN and codes 0.
- * norm_values: values are first divided by sqrt(mean of their head's squares + eps).  Two rows of one call must not share a place. */
+ * norm_values: values are first divided by sqrt(mean of their head's squares + eps), all of it in fp32: a head whose squares' sum is more than that holds (numbers from some 2^60 on) has an infinite root and is
+ * stored as zeros, and one whose squares are less than it holds (below some 2^-70), without eps, has none and becomes NaN.  Two rows of one call must not share a place. */
 int lia_kv_store_8bit(const void* k, long long ldk, const void* v, long long ldv, int act_f32, const int* meta, const LiaCacheView* kc, const LiaCacheView* vc, int M, int G,
                       float eps, int norm_values, lia_stream_t stream);
 /* The reverse: code * scale of the rows at meta into k [M, G * dim] and v [M, G * vdim]; NaN for a row whose slot or position the caches do not have */
