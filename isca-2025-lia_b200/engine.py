@@ -228,8 +228,8 @@ class Engine:
         self.slots.fork(req_id, new_ids)
 
     def score_choices(self, prompt, choices, top=0):
-        """How likely each of ``choices`` (lists of ids) is behind ``prompt`` (ids): the prompt is processed once and forked to every choice, as many at a time as there are free slots.  Returns a dict
-        per choice as ``score`` does, over all tokens of the choice."""
+        """How likely each of ``choices`` (lists of ids) is behind ``prompt`` (ids): the prompt is processed once and forked to every choice, as many at a time as there are free slots,
+        a pass at a time.  Returns a dict per choice as ``score`` does, over all tokens of the choice."""
         prompt, choices = [int(t) for t in prompt], [[int(t) for t in c] for c in choices]
         if not prompt or any(not c for c in choices):
             raise ValueError("a prompt and its choices have at least one token")
@@ -246,19 +246,31 @@ class Engine:
                 try:
                     if len(prompt) > 1:
                         self.fork(root, keys)
-                    logits = self.step([{"id": k, "tokens": prompt[-1:] + c[:-1], "want": list(range(len(c)))} for k, c in zip(keys, group)])
-                    given = [t for c in group for t in c]
-                    logp, entropy, best, ids = (t.tolist() for t in ops.token_logprobs(logits, torch.tensor(given, dtype=torch.int64, device=self.device), top=top))
-                    self.check()
+                    said = [{"logp": [], "entropy": [], "alternatives": []} for _ in group]
+                    done = [0] * len(group)
+                    while done != [len(c) for c in group]:                     # all that is left or, so that no more logits are held than a pass has rows, as much of each
+                        left = [len(c) - d for c, d in zip(group, done)]
+                        share = max(left) if sum(left) <= self.max_rows else max(1, self.max_rows // sum(n > 0 for n in left))
+                        entries, given, whose = [], [], []
+                        for i, c in enumerate(group):
+                            n = min(left[i], share)
+                            if n:
+                                entries.append({"id": keys[i], "tokens": (prompt[-1:] + c)[done[i]:done[i] + n], "want": list(range(n))})
+                                given += c[done[i]:done[i] + n]
+                                whose += [i] * n
+                                done[i] += n
+                        logits = self.step(entries)
+                        logp, entropy, best, ids = (t.tolist() for t in ops.token_logprobs(logits, torch.tensor(given, dtype=torch.int64, device=self.device), top=top))
+                        self.check()
+                        for r, i in enumerate(whose):
+                            said[i]["logp"].append(logp[r])
+                            said[i]["entropy"].append(entropy[r])
+                            said[i]["alternatives"].append(list(zip(ids[r], best[r])))
+                    out += said
                 finally:
                     for k in keys:
                         if self.slots.slot_of(k) is not None:
                             self.slots.free(k)
-                row = 0
-                for c in group:
-                    rows = range(row, row + len(c))
-                    out.append({"logp": [logp[r] for r in rows], "entropy": [entropy[r] for r in rows], "alternatives": [list(zip(ids[r], best[r])) for r in rows]})
-                    row += len(c)
                 at += len(group)
         finally:
             if self.slots.slot_of(root) is not None:
