@@ -7,6 +7,8 @@
 //             written (up to the i-th place) lies before all that is still to be read, and no two threads share a byte.
 //
 // Bound: fork by memory (every byte is read once and written once for each target), compaction by latency: a few rows in each of hundreds of tensors.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace {
@@ -140,19 +142,27 @@ __global__ void __launch_bounds__(COLUMNS) cache_compact_kernel(const __grid_con
 }
 
 // NULL, or what is wrong with a tensor; else how the kernels take it
-const char* tensor_of(const LiaCacheRows& r, int slots, Tensor& t) {
+const char* tensor_of(const LiaCacheRows& r, int slots, int capacity, Tensor& t) {
   if (!r.data) return "null tensor";
   if (r.pieces <= 0 || r.piece_bytes <= 0 || (long long)r.pieces * r.piece_bytes >= 1ll << 31) return "rows of no or too many bytes";
-  if (r.slot_stride < 0 || r.pos_stride < 0 || r.piece_stride < 0 || (slots > 1 && r.slot_stride == 0)) return "slots or rows that share their place";
+  if (r.state && r.pieces != 1) return "a state in pieces";
+  // each of slots, positions and pieces steps over all that lies closer together
+  struct Step {
+    long long stride, n;
+  } steps[3] = {{r.slot_stride, slots}, {r.pos_stride, r.state ? 1 : capacity}, {r.piece_stride, r.pieces}};
+  std::sort(steps, steps + 3, [](const Step& a, const Step& b) { return a.stride < b.stride; });
+  __int128 span = r.piece_bytes;
+  for (const Step& s : steps) {
+    if (s.n <= 1) continue;
+    if (s.stride < span) return "slots or rows that share their place";
+    span += (__int128)(s.n - 1) * s.stride;
+  }
   t = Tensor{static_cast<uint8_t*>(r.data), r.slot_stride, r.pos_stride, r.piece_stride, r.piece_bytes, r.pieces, 16, 1, 0};
   const uintptr_t bits = reinterpret_cast<uintptr_t>(r.data) | (uintptr_t)r.slot_stride | (r.state ? 0 : (uintptr_t)r.pos_stride) | (r.pieces > 1 ? (uintptr_t)r.piece_stride : 0) | (uintptr_t)r.piece_bytes;
   while (bits % t.vec) t.vec /= 2;
   if (r.state) {                                                   // a slot's bytes as positions of one vector each
-    if (r.pieces != 1) return "a state in pieces";
     t.state = (int)(r.piece_bytes / t.vec);
     t.pos = t.bytes = t.vec;
-  } else if (r.pos_stride < r.piece_bytes || (r.pieces > 1 && r.piece_stride < r.piece_bytes)) {
-    return "slots or rows that share their place";
   }
   const long long row = t.bytes * t.pieces;
   t.per = (int)(row >= CHUNK ? 1 : CHUNK / row);
@@ -170,7 +180,7 @@ extern "C" int lia_cache_fork(const LiaCacheRows* tensors, int n_tensors, int sl
     const int m = n_tensors - t0 < MOST ? n_tensors - t0 : MOST;
     long long chunks = 1;
     for (int i = 0; i < m; ++i) {
-      const char* wrong = tensor_of(tensors[t0 + i], slots, all.t[i]);
+      const char* wrong = tensor_of(tensors[t0 + i], slots, capacity, all.t[i]);
       LIA_CHECK_ARG(!wrong, "lia_cache_fork: %s", wrong);
       const long long positions = all.t[i].state > 0 ? all.t[i].state : max_count < 1 ? 1 : max_count < capacity ? max_count : capacity, need = (positions + all.t[i].per - 1) / all.t[i].per;
       if (need > chunks) chunks = need;
@@ -190,7 +200,7 @@ extern "C" int lia_cache_compact(const LiaCacheRows* tensors, int n_tensors, int
     const int m = n_tensors - t0 < MOST ? n_tensors - t0 : MOST;
     long long columns = 1;
     for (int i = 0; i < m; ++i) {
-      const char* wrong = tensor_of(tensors[t0 + i], slots, all.t[i]);
+      const char* wrong = tensor_of(tensors[t0 + i], slots, capacity, all.t[i]);
       LIA_CHECK_ARG(!wrong, "lia_cache_compact: %s", wrong);
       LIA_CHECK_ARG(!tensors[t0 + i].state, "lia_cache_compact: a state has no positions");
       const long long c = all.t[i].bytes / all.t[i].vec * all.t[i].pieces;

@@ -1657,8 +1657,13 @@ class CacheSet:
                 pieces *= n
             else:
                 raise _lib.LiaError(f"CacheSet: a row of strides {strides} is not runs of bytes at equal distances")
-        if (self.slots > 1 and strides[0] == 0) or (not state and self.capacity > 1 and strides[1] * size < piece) or (pieces > 1 and apart < piece) or (state and pieces > 1):
-            raise _lib.LiaError(f"CacheSet: rows that share their place, or a state that is not contiguous: strides {strides}")
+        if state and pieces > 1:
+            raise _lib.LiaError(f"CacheSet: a state that is not contiguous inside a slot: strides {strides}")
+        span = piece                                                # each of slots, positions and pieces steps over all that lies closer together
+        for n, s in sorted(((n, s) for n, s in ((self.slots, strides[0] * size), (1 if state else self.capacity, 0 if state else strides[1] * size), (pieces, apart)) if n > 1), key=lambda x: x[1]):
+            if s < span:
+                raise _lib.LiaError(f"CacheSet: slots or rows that share their place: shape {list(t.shape)}, strides {strides}")
+            span += (n - 1) * s
         pos = 0 if state else strides[1] * size if self.capacity > 1 else piece
         return _lib.LiaCacheRows(t.data_ptr(), strides[0] * size, pos, apart, piece, pieces, int(state))
 
