@@ -722,7 +722,7 @@ int lia_linear_int8(const void* x, int x_type, long long ldx, const float* x_sca
  * Rows of caches copied to other slots, and moved inside one.
  * ---------------------------------------------------------------------------------------------------------------- */
 /* A tensor of per-request state as bytes: those of (slot, position) are `pieces` runs of piece_bytes at data + slot * slot_stride + position * pos_stride + piece * piece_stride.  state: the tensor has no
- * positions, a slot is piece_bytes (one piece).  Slots, positions and pieces lie inside one another in any order (no two share a byte). */
+ * positions, a slot is piece_bytes (one piece).  Slots, positions and pieces lie inside one another in any order (no two share a byte), and no two tensors of a call share memory. */
 typedef struct LiaCacheRows {
   void* data;
   int64_t slot_stride, pos_stride, piece_stride, piece_bytes;

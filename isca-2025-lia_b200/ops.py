@@ -1631,7 +1631,8 @@ def linear_int8(x, w, w_scale, out=None, x_scale=None):
 class CacheSet:
     """The tensors of per-request state that ``fork`` and ``compact`` work on together (csrc/cache_move.cu): ``rows`` of shape [slots, capacity, ...], of any types and strides as long as what
     follows the positions is whole runs of bytes at equal distances (scales [slots, heads, capacity] are given as ``.transpose(1, 2)``), and ``states`` [slots, ...], contiguous inside a slot.
-    All have the same slots, all rows the same capacity.  The tensors are held, not copied."""
+    All have the same slots, all rows the same capacity, and no two share
+    memory.  The tensors are held, not copied."""
 
     def __init__(self, rows, states=()):
         self.tensors = [*rows, *states]
@@ -1639,6 +1640,8 @@ class CacheSet:
             raise _lib.LiaError("CacheSet: no tensors")
         self.slots, self.capacity, self.states = self.tensors[0].shape[0], rows[0].shape[1] if len(rows) else 1, len(states)
         self.device = self.tensors[0].device
+        if len({t.data_ptr() for t in self.tensors}) < len(self.tensors):
+            raise _lib.LiaError("CacheSet: a tensor twice: what moves inside it would move twice")
         self._rows = (_lib.LiaCacheRows * len(self.tensors))(*[self._of(t, False) for t in rows], *[self._of(t, True) for t in states])
 
     def _of(self, t, state):

@@ -44,6 +44,16 @@ def test_states_that_share_bytes_are_refused(lib):
     assert lib.load().lia_cache_fork(r, 1, 2, 8, 16, 1, 1, None) == -1 and "share" in lib.last_error()
 
 
+def test_a_tensor_twice_is_refused(lib):
+    """Two blocks would move the same rows at their own pace, the second what the first has moved already."""
+    from lia_b200 import ops
+    a, b = torch.zeros(3, 20, 8), torch.zeros(3, 20, 8)
+    ops.CacheSet([a, b])
+    for rows, states in (([a, b, a], []), ([a, a.view(3, 20, 2, 4)], []), ([a], [a])):
+        with pytest.raises(lib.LiaError, match="twice"):
+            ops.CacheSet(rows, states)
+
+
 @pytest.mark.parametrize("t", [torch.zeros(3, 20, 8), torch.zeros(20, 3, 8).transpose(0, 1), torch.zeros(3, 4, 20).transpose(1, 2), torch.zeros(3, 4, 20, 2, dtype=BF16).transpose(1, 2),
                                torch.zeros(4, 20, 3, 8).permute(2, 1, 0, 3), torch.zeros(3, 20, 2, 8)[:, :, 1], torch.zeros(1, 20, 8).expand(1, 20, 8), torch.zeros(3, 1, 4, 8)[:, :, 1:3],
                                torch.zeros(1, 1, 5), torch.zeros(3, 40, 8)[:, ::2], torch.zeros(3, 20)])
