@@ -9,11 +9,12 @@
 //          among as many tiles as there are.  Weights are on their way while the tokens are quantised.
 //   a token or two and matrices up to 64 Mi products, whose time is latency: int8_tokens_kernel, on the ordinary cores and in one launch.  Every block makes the tokens' codes for itself, in shared memory,
 //          while its first weights are on their way; a warp has an equal part of the block's channels' codes.
-//   MANY   (bound by the tensor cores, and what feeds them)  the tokens' rows are the product's rows: a CTA an SM on tiles of 128 x 256, or 128 or 64 where those would leave SMs idle.  (CTA pairs on
-//          256 x 256 tiles, cta_group::2, took 493 us instead of 622 for 4096 tokens of 28672 x 7168, and came to a standstill once in some 20000 launches; why was not found, so they are not here.)
+//   MANY   (bound by the tensor cores, 86 % busy)  the tokens' rows are the product's rows: a CTA an SM on tiles of 128 x 256, or 128 or 64 where those would leave SMs idle.  (CTA pairs on 256 x 256 tiles,
+//          cta_group::2, took 493 us where these took 622 in the same run, and came to a standstill once in some 20000 launches; why was not found, so they are not here.)
 //
-// us (graph replay, bf16 tokens quantised on the way): 1 token of 2560 x 2560 5.1, latency; 64 tokens of 28672 x 7168 41, 5.0 TB/s of weights, 0.78 of the copy rate; 4096 tokens of it 580, 2900 TOP/s,
-// 680 once the power cap lowers the clocks.
+// us: 1 token of 2560 x 2560 5.1, latency; 64 tokens of 28672 x 7168 41, 5.0 TB/s of weights, 0.78 of the copy rate (both bf16, quantised on the way); 4096 tokens of it, of codes, 532 after a rest, 3160 TOP/s,
+// and 620 to 635 at the 1305 to 1372 MHz that the power cap leaves after two seconds of it; bf16 tokens 580, and 662 at 1327 MHz.
+// Quantisation: 28672 rows of 7168 bf16 numbers 114 us, 0.83 of the copy rate (issue slots 87 % busy); 4096 of them 17.7, of fp32 numbers 24.6 (0.91); 64 rows 2.5.
 //
 // Every wait is bounded; a CTA that gives one up makes its tile's outputs NaN and counts itself in lia_moe_timeouts_seen().
 #include <cuda.h>
@@ -678,7 +679,8 @@ Plan plan_of(int M, int N, int K) {
     p.bn = bn;
   };
   // ns: a call's own, and for each round what its blocks of K take or, behind the first one, what its sums take on their way out if that is longer; fitted to 90 shapes.  us by tiles 256 wide | 128 | 64,
-  // of codes: 256 tokens of 1024 x 1024 7.4 | 5.5 | 4.9, of 7168 x 7168 21 | 15 | 24; 1000 tokens of it 40 | 46 | 76; 1150 of 23176 x 416 24 | 28 | 37; 4096 of 28672 x 7168 622 | 765 | 1265.
+  // of codes: 256 tokens of 1024 x 1024 7.4 | 5.5 | 4.9, of 7168 x 7168 21 | 15 | 24; 1000 tokens of it 40 | 46 | 76; 1150 of 23176 x 416 24 | 28 | 37; 4096 of 28672 x 7168 532 | 633 | 1022 after a rest,
+  // 627 at 1340 MHz | 737 at 1425 | 1158 at 1690 under the power cap.
   auto ns = [&](long long n, long long once, int block, int sums) {
     const long long products = (long long)p.k_blocks * block;
     return once + products + ((n + sms - 1) / sms - 1) * (products > sums ? products : sums);
@@ -752,7 +754,7 @@ int quantize(const void* x, int act_f32, long long ldx, int8_t* codes, long long
 
 // us with quantisation and tcgen05 | in one launch, bf16 tokens: 1 of 1024 x 1024 5.9 | 4.8, of 2560 x 2560 7.5 | 5.3, of 1000 x 8192 8.4 | 5.8, of 64 x 28672 12.5 | 6.2, of 7168 x 7168 14.0 | 13.3, of
 // 50272 x 2560 26.0 | 25.7, of 28672 x 7168 35.6 | 37.3, of 200000 x 64 21 | 26 (and in two rounds, 200000 x 256, 23 | 26); 2 of 2560 x 2560 7.5 | 5.7, of 1000 x 8192 8.4 | 6.8, of 2048 x 28672 16.7 | 20.1 (every block quantises the tokens);
-// 4 of 2560 x 2560 7.5 | 7.0, of 1000 x 8192 8.5 | 8.5, of 7168 x 7168 14.0 | 16.3.  A call is shorter by a launch and an allocation too.
+// 4, by a form of it that is not here, of 2560 x 2560 7.5 | 7.0, of 1000 x 8192 8.5 | 8.5, of 7168 x 7168 14.0 | 16.3.  A call is shorter by a launch and an allocation too.
 bool few_tokens(int M, int N, int K) { return M <= 2 && K >= T_STEP / 2 && (long long)M * K <= T_CODES && (long long)M * N * K <= 1ll << 26 && N <= lia_sm_count() * T_ROWS; }
 
 template <typename T, bool OUT32> int launch_tokens(TokenArgs a, int M, cudaStream_t stream) {

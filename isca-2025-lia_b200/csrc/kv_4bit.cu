@@ -8,8 +8,9 @@
 // Eight lanes have a head: lane q takes the channels 4 q .. 4 q + 3 of every group, which are 64 neighbouring bytes of bf16 activations for the eight, and whose codes are neighbours in the cache (byte4()).  Up
 // to four groups at a time, so that a lane's codes of 128 channels are one 8-byte store; each lane sees to one group's scale, which the others get by shuffles.
 //
-// 7169 tokens with 8 heads of 128 (29 MB each of keys and values in, 8 MB out; graph replay): store 12.8 us, bound by instructions (22 a number for 32 lanes, three slots in four taken; with 40 registers
-// instead of 32 a thread 13.3, every lane with all groups' scales 15.5); load 10.3, bound by what memory takes of its 29 MB of results (keys and values by the same lanes: 12.8, and the store 13.9).
+// 7169 tokens with 8 heads of 128 (29 MB each of keys and values in, 8 MB out; ten calls in a graph): store 11.7 us, values normed 12.6, of fp32 numbers 14.7 and 14.2, bound by instructions (22 a number for 32
+// lanes, 78 % of the issue slots; with 40 registers instead of 32 a thread half a microsecond more, every lane with all groups' scales 2.7); load 9.2, to fp32 10.0, instructions too (74 % of the issue slots, memory
+// 8 %: results stay in L2; keys and values by the same lanes: 2.5 more, and the store 1.1).
 #include "cache8.cuh"
 #include "pairs.cuh"
 

@@ -17,6 +17,7 @@
 // 16 tokens behind 21000 to 30001 positions, 16 heads on 8 (475 MB): 98 us, 4.9 TB/s, 74 % of the copy rate, the second launch among them; with the 8-bit kernel's structure 207.  What bounds it:
 // instructions, some 290 a warp for 16 keys (488 at first; 342 with values' codes less 1032 instead of subnormal, 110 us), half of them on the integer pipe (51 % busy, issue slots 62 %), and memory next;
 // five or six blocks an SM change nothing (99.5, 100), nor do shorter spans (twice as many 112).
+// More rows of a key head: the same histories with 4 or 8 rows 123 us, 16 rows 208, 32 rows 342 (issue slots 66, 62 and 50 % busy, 3.2, 2.5 and 1.7 warps a scheduler): scores and weights by rows times groups.
 #include "mma.cuh"
 #include "tree_attn.cuh"
 
